@@ -138,6 +138,29 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [c_int, _I64, _I64, _I64, _I64, _P, _P, _P, _P, c_float, c_float, c_float, c_float, _P],
     ),
+    "gns_adamw_states_step": (
+        c_int,
+        [c_int, _PP, _PP, _PP, _PP, _PP, _PP, _PI64, c_int, c_int, c_int, _PF, _PF, c_float, c_float, c_float, c_float,
+         c_float, c_float, _P, _P],
+    ),
+    "gns_grouped_gemm": (
+        c_int,
+        [c_int, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _I64, _I64, _P, c_int, _P, c_int, _I64, _P],
+    ),
+    "gns_grouped_gemm_reduce_workspace_size": (c_size_t, [_I64]),
+    "gns_grouped_gemm_reduce": (
+        c_int,
+        [c_int, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _P, c_int, _P, c_int, _I64, _I64, _P, c_size_t, _P],
+    ),
+    "gns_layer_norm_forward": (
+        c_int,
+        [c_int, c_int, _I64, _I64, _P, _I64, _P, _P, c_float, _P, _P, _P, _P],
+    ),
+    "gns_layer_norm_backward_workspace_size": (c_size_t, [_I64, _I64]),
+    "gns_layer_norm_backward": (
+        c_int,
+        [c_int, c_int, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, c_size_t, _P],
+    ),
 }
 
 _lock = threading.Lock()

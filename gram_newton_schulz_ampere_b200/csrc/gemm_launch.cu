@@ -388,6 +388,11 @@ int launch_gemm(const GemmArgs& g, cudaStream_t stream) {
 }  // namespace gns
 
 namespace gns {
+int encode_tiles(CUtensorMap* map, int dtype, const void* ptr, int64_t inner, int64_t outer, int64_t batch,
+                 int64_t outer_stride, int64_t batch_stride, int box_outer) {
+  return make_map(map, dtype, ptr, inner, outer, batch, outer_stride, batch_stride, box_outer);
+}
+
 int encode_f16_tiles(CUtensorMap* map, const void* ptr, int64_t inner, int64_t outer, int64_t batch,
                      int64_t outer_stride, int64_t batch_stride, int box_outer) {
   return make_map(map, kF16, ptr, inner, outer, batch, outer_stride, batch_stride, box_outer);
@@ -462,6 +467,10 @@ int gns_device_status(int* status, int clear) {
   rc = gns::small_chain_status(&small, clear);
   if (rc != GNS_OK) return rc;
   if (*status == 0) *status = small;
+  int grouped = 0;
+  rc = gns::grouped_status(&grouped, clear);
+  if (rc != GNS_OK) return rc;
+  if (*status == 0) *status = grouped;
   return GNS_OK;
 }
 

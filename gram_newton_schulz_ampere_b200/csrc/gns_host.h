@@ -99,6 +99,12 @@ int launch_normalize(int x_dtype, int64_t batch, int64_t rows, int64_t cols, con
 // box and 128-byte swizzle (the GEMM's operand maps).
 int encode_f16_tiles(CUtensorMap* map, const void* ptr, int64_t inner, int64_t outer, int64_t batch,
                      int64_t outer_stride, int64_t batch_stride, int box_outer);
+// The same for either 16-bit type.
+int encode_tiles(CUtensorMap* map, int dtype, const void* ptr, int64_t inner, int64_t outer, int64_t batch,
+                 int64_t outer_stride, int64_t batch_stride, int box_outer);
+
+// Status word of the grouped products (0 = ok); optionally cleared.
+int grouped_status(int* status, int clear);
 
 // Fused single-kernel Gram Newton-Schulz chain for matrices whose short side is
 // at most 128 (small_chain.cu). x0 holds the normalised fp16 X and x1 is the

@@ -884,3 +884,344 @@ def lion_step(
             1 if decay is not None else 0, nat.stream_handle(device),
         )
     nat.check(rc, "gns_lion_step")
+
+
+# ------------------------------------------------- AdamW states in 8 or 32 bits
+STATE_BLOCK = 256  # consecutive elements of a tensor that share a scale of the 8-bit states
+
+
+class AdamWStates:
+    """The AdamW moments of a list of parameters, in 32 bits or in 8, and the step over them.
+
+    With ``bits=8`` the moments are ``float8_e4m3fn`` tensors of the parameters' shapes
+    with one fp32 scale for each 256 consecutive elements (``exp_avg_scales``,
+    ``exp_avg_sq_scales``: 1-D, ``ceil(numel / 256)`` entries): an element's value is its
+    e4m3 value times its block's scale. With ``bits=32`` they are fp32 tensors. Moments
+    that are not given start at zero. Parameters are contiguous CUDA tensors of one
+    16- or 32-bit floating type; they and the moments are updated in place.
+
+    Unlike ``adamw_step``, which rounds after every operation as the torch sequence it
+    replaces does, the arithmetic is fp32 throughout with one rounding at the end.
+    """
+
+    def __init__(
+        self,
+        parameters: Sequence[Tensor],
+        bits: int = 8,
+        exp_avgs: Sequence[Tensor] | None = None,
+        exp_avg_sqs: Sequence[Tensor] | None = None,
+        exp_avg_scales: Sequence[Tensor] | None = None,
+        exp_avg_sq_scales: Sequence[Tensor] | None = None,
+    ) -> None:
+        if bits not in (8, 32):
+            raise ValueError(f"bits must be 8 or 32, got {bits}")
+        self.bits = bits
+        self.parameters = list(parameters)
+        if (exp_avgs is None) != (exp_avg_sqs is None):
+            raise ValueError("give both moments or neither")
+        if bits == 8 and exp_avgs is not None and (exp_avg_scales is None or exp_avg_sq_scales is None):
+            raise ValueError("8-bit moments need their scales")
+        if exp_avg_scales is not None and exp_avgs is None:
+            raise ValueError("scales without moments")
+        if bits == 32 and (exp_avg_scales is not None or exp_avg_sq_scales is not None):
+            raise ValueError("32-bit moments have no scales")
+        dtype = torch.float8_e4m3fn if bits == 8 else torch.float32
+        for p in self.parameters:
+            if not p.is_contiguous():
+                raise ValueError("parameters must be contiguous")
+            if p.dtype != self.parameters[0].dtype:
+                raise TypeError("all parameters of one call must share a dtype")
+        self.device = _require_cuda(*self.parameters) if self.parameters else None
+        if self.parameters:
+            nat.dtype_code(self.parameters[0].dtype)
+
+        def moments(given: Sequence[Tensor] | None) -> list[Tensor]:
+            if given is None:
+                return [torch.zeros(p.shape, dtype=dtype, device=p.device) for p in self.parameters]
+            return self._checked(given, dtype, [p.numel() for p in self.parameters], "moments")
+
+        def scales(given: Sequence[Tensor] | None) -> list[Tensor]:
+            counts = [(p.numel() + STATE_BLOCK - 1) // STATE_BLOCK for p in self.parameters]
+            if given is None:
+                return [torch.zeros(n, dtype=torch.float32, device=self.device) for n in counts]
+            return self._checked(given, torch.float32, counts, "scales")
+
+        self.exp_avgs = moments(exp_avgs)
+        self.exp_avg_sqs = moments(exp_avg_sqs)
+        self.exp_avg_scales = scales(exp_avg_scales) if bits == 8 else []
+        self.exp_avg_sq_scales = scales(exp_avg_sq_scales) if bits == 8 else []
+        self._numel = [p.numel() for p in self.parameters]
+        self._states = (
+            _ptr_array(self.exp_avgs), _ptr_array(self.exp_avg_sqs),
+            _ptr_array(self.exp_avg_scales) if bits == 8 else None,
+            _ptr_array(self.exp_avg_sq_scales) if bits == 8 else None,
+        )
+
+    def _checked(self, given: Sequence[Tensor], dtype: torch.dtype, counts: list[int], what: str) -> list[Tensor]:
+        if len(given) != len(counts):
+            raise ValueError("tensor lists must have equal lengths")
+        for t, n in zip(given, counts, strict=True):
+            if t.dtype != dtype:
+                raise TypeError(f"{self.bits}-bit AdamW {what} must be {dtype}, got {t.dtype}")
+            if t.numel() != n:
+                raise ValueError("tensor sizes differ within one parameter")
+            if not t.is_contiguous():
+                raise ValueError("tensors must be contiguous")
+            if t.device != self.device:
+                raise ValueError("all tensors must be on the same CUDA device")
+        return list(given)
+
+    def step(
+        self,
+        gradients: Sequence[Tensor | None],
+        learning_rate: float,
+        beta1: float,
+        beta2: float,
+        epsilon: float,
+        weight_decay: float,
+        step: int | Sequence[float],
+        gradient_scale: Tensor | None = None,
+    ) -> None:
+        """One AdamW step in place. ``step`` is the number of this step, from 1 on (one value,
+        or one for each parameter); a gradient of None leaves its parameter and moments as
+        they are; ``gradient_scale`` is one fp32 value on the device that every gradient is
+        multiplied by (a clipping factor, or the inverse of a loss scale)."""
+        count = len(self.parameters)
+        if len(gradients) != count:
+            raise ValueError("gradients and parameters must have equal lengths")
+        if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0):
+            raise ValueError(f"betas must be in [0, 1), got {(beta1, beta2)}")
+        if not epsilon > 0.0:
+            raise ValueError(f"epsilon must be positive, got {epsilon}")
+        if count == 0:
+            return
+        g_dtype = None
+        numel = (ctypes.c_int64 * count)()
+        pointers = (ctypes.c_void_p * count)()
+        places = (ctypes.c_void_p * count)()
+        for i, (g, p) in enumerate(zip(gradients, self.parameters, strict=True)):
+            if g is None:
+                continue
+            if g_dtype is None:
+                g_dtype = g.dtype
+            elif g.dtype != g_dtype:
+                raise TypeError("all gradients of one call must share a dtype")
+            n = self._numel[i]
+            if g.numel() != n:
+                raise ValueError("gradient and parameter sizes differ")
+            if not (g.is_contiguous() and p.is_contiguous()):
+                raise ValueError("gradients and parameters must be contiguous")
+            if g.device != self.device:
+                raise ValueError("gradients must be on the parameters' device")
+            numel[i] = n
+            pointers[i] = g.data_ptr()
+            places[i] = p.data_ptr()
+        if g_dtype is None:
+            return
+        if gradient_scale is not None:
+            if gradient_scale.dtype != torch.float32 or gradient_scale.numel() != 1:
+                raise ValueError("gradient_scale must be one float32 value")
+            if gradient_scale.device != self.device:
+                raise ValueError("gradient_scale must be on the parameters' device")
+        steps = [step] * count if isinstance(step, (int, float)) else list(step)
+        if len(steps) != count:
+            raise ValueError("step must be one value or one for each parameter")
+        lr_bc1, inv_bc2 = (ctypes.c_float * count)(), (ctypes.c_float * count)()
+        known: dict[float, tuple[float, float]] = {}
+        for i, t in enumerate(steps):
+            if t not in known:
+                if t < 1:
+                    raise ValueError(f"steps count from 1, got {t}")
+                known[t] = (learning_rate / (1 - beta1**t), (1 - beta2**t) ** -0.5)
+            lr_bc1[i], inv_bc2[i] = known[t]
+        lib = nat.load()
+        with torch.cuda.device(self.device):
+            rc = lib.gns_adamw_states_step(
+                count, places, pointers, *self._states, numel, nat.dtype_code(self.parameters[0].dtype),
+                nat.dtype_code(g_dtype), self.bits, lr_bc1, inv_bc2, beta1, 1 - beta1, beta2, 1 - beta2, epsilon,
+                1 - learning_rate * weight_decay, nat.ptr(gradient_scale), nat.stream_handle(self.device),
+            )
+        nat.check(rc, "gns_adamw_states_step")
+
+
+# ------------------------------------------------- products grouped by expert
+def _row_operand(t: Tensor) -> Tensor:
+    """Returns the matrix `t` if a TMA tile load can read its rows (unit column stride,
+    16-byte aligned base and row stride), else a copy whose row pitch is padded to a
+    multiple of 8 elements."""
+    rows, cols = t.shape
+    if (
+        t.data_ptr() % 16 == 0
+        and (t.stride(1) == 1 or cols == 1)
+        and ((t.stride(0) % 8 == 0 and t.stride(0) >= cols) or rows == 1)
+    ):
+        return t
+    view = _padded(1, rows, cols, t.dtype, t.device)[0]
+    view.copy_(t)
+    return view
+
+
+def _group_ends(ends: Tensor, groups: int | None = None) -> Tensor:
+    if ends.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"ends must be int32 or int64, got {ends.dtype}")
+    if ends.ndim != 1 or (groups is not None and ends.numel() != groups):
+        raise ValueError("ends must hold one row number for each group")
+    return ends.contiguous()
+
+
+def grouped_gemm(left: Tensor, right: Tensor, ends: Tensor, out_dtype: torch.dtype | None = None) -> Tensor:
+    """``out[r] = left[r] @ right[e]`` for the rows r of each group e, on tcgen05 tensor cores.
+
+    left [T, k] holds rows sorted by group, right [E, k, n] one matrix for each group (either
+    may have its last two dimensions transposed in memory), both float16 or both bfloat16.
+    ``ends`` [E] (int32 or int64, on the device) are the row numbers where the groups end:
+    group e owns the rows ``ends[e - 1] <= r < ends[e]``. They are read on the device, without
+    a synchronisation, and are clamped to [0, T] and to ascending order. Rows that no group
+    owns (from ``ends[-1]`` on) come out zero. Sums are fp32, rounded once to ``out_dtype``
+    (default: the inputs' type).
+
+    With an expert layer's weights W [E, n, k], the layer is
+    ``grouped_gemm(x, W.transpose(1, 2), ends)``, its gradient for the rows
+    ``grouped_gemm(dy, W, ends)`` and for the weights ``grouped_gemm_reduce(dy, x, ends)``.
+    """
+    device = _require_cuda(left, right, ends)
+    if left.ndim != 2 or right.ndim != 3:
+        raise ValueError("expected left [rows, k] and right [groups, k, n]")
+    if left.dtype != right.dtype or left.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError("left and right must share dtype float16 or bfloat16")
+    if left.shape[1] != right.shape[1]:
+        raise ValueError(f"incompatible shapes {tuple(left.shape)} @ {tuple(right.shape)}")
+    groups, k, n = right.shape
+    rows = left.shape[0]
+    ends = _group_ends(ends, groups)
+    dtype = out_dtype or left.dtype
+    code = nat.dtype_code(dtype)
+    if rows == 0 or n == 0 or k == 0 or groups == 0:
+        return torch.zeros((rows, n), dtype=dtype, device=device)
+    out = torch.empty((rows, n), dtype=dtype, device=device)
+    a = _row_operand(left)
+    if any(size > 1 and stride == 0 for size, stride in zip(right.shape, right.stride(), strict=True)):
+        right = right.contiguous()  # a TMA map has no zero strides
+    b = _aligned_operand(right)
+    lib = nat.load()
+    with torch.cuda.device(device):
+        rc = lib.gns_grouped_gemm(
+            nat.dtype_code(a.dtype), rows, n, k, groups, a.data_ptr(), a.stride(0),
+            b.data_ptr(), b.stride(0), b.stride(1), b.stride(2), ends.data_ptr(), 8 * ends.element_size(),
+            out.data_ptr(), code, out.stride(0), nat.stream_handle(device),
+        )
+    nat.check(rc, "gns_grouped_gemm")
+    return out
+
+
+def grouped_gemm_reduce(left: Tensor, right: Tensor, ends: Tensor, out_dtype: torch.dtype | None = None) -> Tensor:
+    """``out[e] = left[rows of e].T @ right[rows of e]`` for each group of rows, on tcgen05
+    tensor cores: [E, m, n] from left [T, m] and right [T, n], zero for a group without rows.
+    ``ends`` as for ``grouped_gemm``; rows that no group owns have no part in any sum."""
+    device = _require_cuda(left, right, ends)
+    if left.ndim != 2 or right.ndim != 2:
+        raise ValueError("expected left [rows, m] and right [rows, n]")
+    if left.dtype != right.dtype or left.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError("left and right must share dtype float16 or bfloat16")
+    if left.shape[0] != right.shape[0]:
+        raise ValueError(f"left and right have {left.shape[0]} and {right.shape[0]} rows")
+    ends = _group_ends(ends)
+    rows, m = left.shape
+    n = right.shape[1]
+    groups = ends.numel()
+    dtype = out_dtype or left.dtype
+    code = nat.dtype_code(dtype)
+    if rows == 0 or m == 0 or n == 0 or groups == 0:
+        return torch.zeros((groups, m, n), dtype=dtype, device=device)
+    out = torch.empty((groups, m, n), dtype=dtype, device=device)
+    a, b = _row_operand(left), _row_operand(right)
+    lib = nat.load()
+    ws = _workspace(lib.gns_grouped_gemm_reduce_workspace_size(groups), device)
+    with torch.cuda.device(device):
+        rc = lib.gns_grouped_gemm_reduce(
+            nat.dtype_code(a.dtype), rows, m, n, groups, a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0),
+            ends.data_ptr(), 8 * ends.element_size(), out.data_ptr(), code, out.stride(0), out.stride(1),
+            ws.data_ptr(), ws.numel(), nat.stream_handle(device),
+        )
+    nat.check(rc, "gns_grouped_gemm_reduce")
+    return out
+
+
+# ------------------------------------------------------------------ layer norm
+def _norm_rows(t: Tensor, columns: int) -> Tensor:
+    """[rows, columns] view of `t` with unit column stride and rows that do not overlap."""
+    flat = t.reshape(-1, columns)
+    if columns > 1 and flat.stride(1) != 1 or flat.shape[0] > 1 and flat.stride(0) < columns:
+        flat = flat.contiguous()
+    return flat
+
+
+def _norm_check(x: Tensor, weight: Tensor, bias: Tensor | None) -> int:
+    if x.ndim < 1 or weight.ndim != 1 or x.shape[-1] != weight.numel() or weight.numel() == 0:
+        raise ValueError("weight must have one entry for each element of x's last dimension")
+    nat.dtype_code(x.dtype)
+    nat.dtype_code(weight.dtype)
+    if bias is not None:
+        if bias.shape != weight.shape:
+            raise ValueError("weight and bias shapes differ")
+        if bias.dtype != weight.dtype:
+            raise TypeError("weight and bias must share a dtype")
+    return weight.numel()
+
+
+def layer_norm(x: Tensor, weight: Tensor, bias: Tensor | None, epsilon: float) -> tuple[Tensor, Tensor, Tensor]:
+    """Layer norm over the last dimension: ``y = (x - mean) * rstd * weight + bias``.
+
+    Returns y (x's type, contiguous) and the fp32 mean and rstd of each row (x's shape
+    without the last dimension), which ``layer_norm_backward`` takes. The variance is the
+    biased one; all arithmetic is fp32. weight and bias share a floating type of their own;
+    bias may be None."""
+    device = _require_cuda(x, weight, bias)
+    columns = _norm_check(x, weight, bias)
+    flat = _norm_rows(x, columns)
+    rows = flat.shape[0]
+    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    stats = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=device)
+    w = weight.contiguous()
+    b = bias.contiguous() if bias is not None else None
+    lib = nat.load()
+    with torch.cuda.device(device):
+        rc = lib.gns_layer_norm_forward(
+            nat.dtype_code(x.dtype), nat.dtype_code(w.dtype), rows, columns, flat.data_ptr(), flat.stride(0),
+            w.data_ptr(), nat.ptr(b), float(epsilon), y.data_ptr(), stats[0].data_ptr(), stats[1].data_ptr(),
+            nat.stream_handle(device),
+        )
+    nat.check(rc, "gns_layer_norm_forward")
+    return y, stats[0], stats[1]
+
+
+def layer_norm_backward(
+    grad: Tensor, x: Tensor, weight: Tensor, mean: Tensor, rstd: Tensor
+) -> tuple[Tensor, Tensor, Tensor]:
+    """Gradients (dx, dweight, dbias) of ``layer_norm`` from the gradient of y and the mean and
+    rstd that the forward pass returned. dx has x's type, dweight and dbias the weight's;
+    their sums over the rows are fp32, in a fixed order."""
+    device = _require_cuda(grad, x, weight, mean, rstd)
+    columns = _norm_check(x, weight, None)
+    if grad.shape != x.shape:
+        raise ValueError("grad and x shapes differ")
+    if grad.dtype != x.dtype:
+        raise TypeError("grad and x must share a dtype")
+    rows = x.numel() // columns
+    for t in (mean, rstd):
+        if t.dtype != torch.float32 or t.numel() != rows or not t.is_contiguous():
+            raise ValueError("mean and rstd must be contiguous float32 with one entry per row")
+    flat, g = _norm_rows(x, columns), _norm_rows(grad, columns)
+    w = weight.contiguous()
+    dx = torch.empty(x.shape, dtype=x.dtype, device=device)
+    sums = torch.empty((2, columns), dtype=weight.dtype, device=device)
+    lib = nat.load()
+    ws = _workspace(lib.gns_layer_norm_backward_workspace_size(rows, columns), device)
+    with torch.cuda.device(device):
+        rc = lib.gns_layer_norm_backward(
+            nat.dtype_code(x.dtype), nat.dtype_code(w.dtype), rows, columns, g.data_ptr(), g.stride(0),
+            flat.data_ptr(), flat.stride(0), w.data_ptr(), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(),
+            sums[0].data_ptr(), sums[1].data_ptr(), ws.data_ptr(), ws.numel(), nat.stream_handle(device),
+        )
+    nat.check(rc, "gns_layer_norm_backward")
+    return dx, sums[0], sums[1]

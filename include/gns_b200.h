@@ -324,6 +324,77 @@ GNS_API int gns_dion3_apply_rows(int p_dtype, int64_t batch, int64_t rows, int64
                                  const float* squared_norms, float lr, float wd, float lr_adj, float eps,
                                  gns_stream_t stream);
 
+/* --------------------------------------------------- AdamW states in 8 bits
+ * One AdamW step over `count` contiguous tensors, in fp32 arithmetic with one
+ * rounding of the parameter (gns_adamw_step instead rounds after every step, as
+ * the torch sequence it replaces):
+ *   g' = s g;  m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2
+ *   p  = p * decay - lr_bc1[i] * m / (sqrt(v) * inv_bc2[i] + epsilon)
+ * with lr_bc1[i] = lr / (1 - b1^step), inv_bc2[i] = 1 / sqrt(1 - b2^step) and
+ * decay = 1 - lr * weight_decay. s is read from device memory at grad_scale (a
+ * clipping factor, or the inverse of a loss scale), NULL meaning 1.
+ * state_bits 32: exp_avgs and exp_avg_sqs are fp32. state_bits 8: they are e4m3
+ * bytes, and exp_avg_scales[i] / exp_avg_sq_scales[i] hold one fp32 scale for
+ * each 256 consecutive elements of tensor i (the last block may be shorter):
+ * the value of an element is its e4m3 value times its block's scale. Scales are
+ * the block's largest magnitude / 448; values round to nearest, and a second
+ * moment above zero never rounds to zero. A block whose largest magnitude is
+ * at most 1e-30 is held as zeros (a second moment there at the smallest code).
+ * A gradient that is not finite makes its block's states NaN.
+ * Parameters share p_dtype, gradients g_dtype. Tensors with numel 0 are skipped.
+ * No counterpart in the reference. */
+GNS_API int gns_adamw_states_step(int count, void* const* params, const void* const* grads, void* const* exp_avgs,
+                                  void* const* exp_avg_sqs, float* const* exp_avg_scales,
+                                  float* const* exp_avg_sq_scales, const int64_t* numel, int p_dtype, int g_dtype,
+                                  int state_bits, const float* lr_bc1, const float* inv_bc2, float beta1,
+                                  float one_minus_beta1, float beta2, float one_minus_beta2, float epsilon,
+                                  float decay, const float* grad_scale, gns_stream_t stream);
+
+/* ------------------------------------------------ products grouped by expert
+ * Rows are sorted by group: group e owns the rows [ends[e - 1], ends[e]) (from 0
+ * for the first). `ends` is in device memory, 32- or 64-bit integers (ends_bits);
+ * its values are clamped to [0, rows] and to ascending order. left and right
+ * share ab_dtype (F16 or BF16); sums are fp32. At most 1024 groups.
+ *
+ * gns_grouped_gemm: out[r] = left[r] . right[e] for the rows r of group e; rows
+ * past the last end come out zero. left is [rows][k] with unit column stride,
+ * right [group][k][n] with a unit stride along k or along n, out [rows][n] with
+ * unit column stride. Base addresses 16-byte aligned and the other strides
+ * multiples of 16 bytes (a TMA rule; out may have any row stride).
+ *
+ * gns_grouped_gemm_reduce: out[e] = left[rows of e]^T . right[rows of e], zero for
+ * a group without rows. left is [rows][m], right [rows][n], both with unit column
+ * stride and aligned as above; out is [group][m][n] with unit column stride.
+ * No counterpart in the reference (its products are batched, of equal sizes). */
+GNS_API int gns_grouped_gemm(int ab_dtype, int64_t rows, int64_t n, int64_t k, int64_t groups, const void* left,
+                             int64_t left_rstride, const void* right, int64_t right_gstride, int64_t right_rstride,
+                             int64_t right_cstride, const void* ends, int ends_bits, void* out, int out_dtype,
+                             int64_t out_rstride, gns_stream_t stream);
+GNS_API size_t gns_grouped_gemm_reduce_workspace_size(int64_t groups);
+GNS_API int gns_grouped_gemm_reduce(int ab_dtype, int64_t rows, int64_t m, int64_t n, int64_t groups,
+                                    const void* left, int64_t left_rstride, const void* right, int64_t right_rstride,
+                                    const void* ends, int ends_bits, void* out, int out_dtype, int64_t out_gstride,
+                                    int64_t out_rstride, void* workspace, size_t workspace_bytes, gns_stream_t stream);
+
+/* -------------------------------------------------------------- layer norm
+ * y = (x - mean) * rstd * weight + bias over the last dimension of [rows][cols],
+ * rstd = 1 / sqrt(var + eps) with the biased variance; mean and rstd (fp32, one
+ * value per row) are written for the backward pass. x has unit column stride and
+ * x_rstride elements between rows; y is contiguous, of x's type. weight and bias
+ * share w_dtype; bias may be NULL.
+ * Backward: dx (contiguous, x's type), and dweight / dbias (w_dtype), the sums
+ * over all rows of grad * (x - mean) * rstd and of grad, in fp32 and in a fixed
+ * order; dbias may be NULL. rows may be 0 (the sums are then zero).
+ * No counterpart in the reference. */
+GNS_API int gns_layer_norm_forward(int x_dtype, int w_dtype, int64_t rows, int64_t cols, const void* x,
+                                   int64_t x_rstride, const void* weight, const void* bias, float eps, void* y,
+                                   float* mean, float* rstd, gns_stream_t stream);
+GNS_API size_t gns_layer_norm_backward_workspace_size(int64_t rows, int64_t cols);
+GNS_API int gns_layer_norm_backward(int x_dtype, int w_dtype, int64_t rows, int64_t cols, const void* grad,
+                                    int64_t grad_rstride, const void* x, int64_t x_rstride, const void* weight,
+                                    const float* mean, const float* rstd, void* dx, void* dweight, void* dbias,
+                                    void* workspace, size_t workspace_bytes, gns_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
