@@ -221,6 +221,33 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+class on_device:
+    """``torch.cuda.device(index)`` that gives the device's current stream as a handle. It does
+    nothing when `index` is current already, as it is in most calls, and builds no Stream
+    object: together 5-7 us of a small call's host time."""
+
+    __slots__ = ("index", "switch")
+
+    def __init__(self, index: int) -> None:
+        self.index = index
+        self.switch: torch.cuda.device | None = None
+
+    def __enter__(self) -> int:
+        if torch.cuda.current_device() != self.index:
+            self.switch = torch.cuda.device(self.index)
+            self.switch.__enter__()
+        if _raw_stream is not None:
+            return _raw_stream(self.index)
+        return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, *error: object) -> None:
+        if self.switch is not None:
+            self.switch.__exit__(*error)
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

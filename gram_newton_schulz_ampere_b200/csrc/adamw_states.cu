@@ -24,6 +24,8 @@
 // 8-bit states, 22 with 32-bit states.
 #include <cuda_fp8.h>
 
+#include <mutex>
+
 #include "../../include/gns_b200.h"
 #include "gns_common.cuh"
 #include "gns_host.h"
@@ -37,8 +39,11 @@ constexpr float kE4M3Tiny = 0.001953125f;  // 2^-9, the smallest e4m3 value abov
 constexpr float kFlushBelow = 1e-30f;      // a block whose maximum is not above this is held as zeros
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kChunk = 16384;  // elements of a tensor that one CTA steps
+constexpr int kChunkMin = kWarps * kBlockElems;  // elements of a tensor that one CTA steps, at least
+constexpr int kChunkMax = 16 * kChunkMin;        // and at most (a warp's lanes hold its blocks' scales: 32 at most)
 constexpr int kTensors = 128;  // tensors of one launch (8.7 KB of kernel arguments)
+
+constexpr bool sixteen(int dt) { return dt == kF16 || dt == kBF16; }
 
 struct StateArgs {
   void* p[kTensors];
@@ -52,6 +57,7 @@ struct StateArgs {
   float inv_bc2[kTensors];  // 1 / sqrt(1 - b2^t)
   int block_start[kTensors + 1];
   int count;
+  int chunk;  // elements of a tensor that one CTA steps
 };
 
 struct StateScalars {
@@ -79,6 +85,19 @@ __device__ __forceinline__ float sqrt_approx(float x) {
   return r;
 }
 
+__device__ __forceinline__ float reciprocal_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// The larger magnitude; NaN if either is.
+__device__ __forceinline__ float larger(float top, float x) {
+  float r;
+  asm("{\n\t.reg .f32 a;\n\tabs.f32 a, %2;\n\tmax.NaN.f32 %0, %1, a;\n\t}" : "=f"(r) : "f"(top), "f"(x));
+  return r;
+}
+
 __device__ __forceinline__ void unpack8(const uint4& u, int dt, float (&f)[8]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -91,16 +110,32 @@ __device__ __forceinline__ void unpack8(const uint4& u, int dt, float (&f)[8]) {
   }
 }
 
-// 8 consecutive elements; the address is a multiple of 16 bytes.
-__device__ __forceinline__ void load8(const void* base, int64_t i, int dt, float (&f)[8]) {
-  if (dt == kF32) {
-    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(base) + i);
-    const float4 a = q[0], b = q[1];
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  } else {
-    unpack8(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + i), dt, f);
+// 8 consecutive elements of a type as loaded; the address is a multiple of 16 bytes.
+// D < 0: the type is known at run time only.
+template <int D>
+struct Eight {
+  uint4 u[D == kF16 || D == kBF16 ? 1 : 2];
+
+  __device__ __forceinline__ void load(const void* base, int64_t i, int dt) {
+    if (dt == kF32) {
+      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const float*>(base) + i);
+      u[0] = q[0];
+      u[sizeof(u) / sizeof(uint4) - 1] = q[1];
+    } else {
+      u[0] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + i);
+    }
   }
-}
+
+  __device__ __forceinline__ void get(int dt, float (&f)[8]) const {
+    if (dt == kF32) {
+      const uint4 a = u[0], b = u[sizeof(u) / sizeof(uint4) - 1];
+      f[0] = __uint_as_float(a.x); f[1] = __uint_as_float(a.y); f[2] = __uint_as_float(a.z); f[3] = __uint_as_float(a.w);
+      f[4] = __uint_as_float(b.x); f[5] = __uint_as_float(b.y); f[6] = __uint_as_float(b.z); f[7] = __uint_as_float(b.w);
+    } else {
+      unpack8(u[0], dt, f);
+    }
+  }
+};
 
 __device__ __forceinline__ void store8(void* base, int64_t i, int dt, const float (&f)[8]) {
   if (dt == kF32) {
@@ -123,15 +158,15 @@ __device__ __forceinline__ void store8(void* base, int64_t i, int dt, const floa
   *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + i) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-__device__ __forceinline__ void decode8(uint2 codes, float scale, float (&f)[8]) {
+__device__ __forceinline__ void decode8(uint2 codes, float (&f)[8]) {
   const uint32_t w[2] = {codes.x, codes.y};
 #pragma unroll
   for (int h = 0; h < 4; ++h) {
     const __nv_fp8x2_storage_t two = static_cast<__nv_fp8x2_storage_t>(w[h >> 1] >> (16 * (h & 1)));
     const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3);
     const float2 t = __half22float2(__half2(r));
-    f[2 * h] = t.x * scale;
-    f[2 * h + 1] = t.y * scale;
+    f[2 * h] = t.x;
+    f[2 * h + 1] = t.y;
   }
 }
 
@@ -145,64 +180,63 @@ __device__ __forceinline__ uint2 encode8(const float (&f)[8]) {
   return make_uint2(w[0], w[1]);
 }
 
+__device__ __forceinline__ float adamw_update(float p, float m, float v, const StateScalars& k, float lr_bc1,
+                                              float inv_bc2) {
+  const float u = m * reciprocal_approx(fmaf(sqrt_approx(v), inv_bc2, k.epsilon));
+  return fmaf(-lr_bc1, u, p * k.decay);
+}
+
 __device__ __forceinline__ void adamw_math(float g, float& p, float& m, float& v, const StateScalars& k, float scale,
                                            float lr_bc1, float inv_bc2) {
   g *= scale;
   m = fmaf(k.one_minus_beta1, g, m * k.beta1);
   v = fmaf(k.one_minus_beta2, g * g, v * k.beta2);
-  const float u = __fdividef(m, fmaf(sqrt_approx(v), inv_bc2, k.epsilon));
-  p = fmaf(-lr_bc1, u, p * k.decay);
+  p = adamw_update(p, m, v, k, lr_bc1, inv_bc2);
 }
 
 // The largest magnitude of the block, in every lane. Magnitudes order as their
 // bits do, and a NaN is above all of them, so it reaches the scale.
 __device__ __forceinline__ float block_max(const float (&f)[8]) {
-  uint32_t top = 0u;
+  float top = fabsf(f[0]);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
-  return __uint_as_float(__reduce_max_sync(0xffffffffu, top));
+  for (int e = 1; e < 8; ++e) top = larger(top, f[e]);
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top) & 0x7fffffffu));
 }
 
 __device__ __forceinline__ float inverse_scale(float top) {
-  return top <= kFlushBelow ? 0.0f : __fdividef(kE4M3Max, top);
+  return top <= kFlushBelow ? 0.0f : kE4M3Max * reciprocal_approx(top);
 }
 
-// One warp steps one block of 256 elements at `i` whose 8-bit states it decodes,
-// updates and encodes. VEC: lane L holds elements 8 L .. 8 L + 7, all in range and
-// aligned; otherwise lane L holds L, L + 32, ..., with `left` elements in range.
-template <bool VEC>
-__device__ __forceinline__ void step_block(void* p, const void* g, void* m, void* v, float* m_scale, float* v_scale,
-                                           int64_t i, int left, int lane, int p_dt, int g_dt, const StateScalars& k,
-                                           float scale, float lr_bc1, float inv_bc2) {
-  const int64_t block = i / kBlockElems;
-  float pf[8], gf[8], mf[8], vf[8];
-  const float ms = m_scale[block], vs = v_scale[block];
-  uint8_t* mq = static_cast<uint8_t*>(m) + i;
-  uint8_t* vq = static_cast<uint8_t*>(v) + i;
-  if (VEC) {
-    load8(g, i + 8 * lane, g_dt, gf);
-    load8(p, i + 8 * lane, p_dt, pf);
-    const uint2 mc = reinterpret_cast<const uint2*>(mq)[lane];
-    const uint2 vc = reinterpret_cast<const uint2*>(vq)[lane];
-    decode8(mc, ms, mf);
-    decode8(vc, vs, vf);
-  } else {
-    uint2 mc = make_uint2(0u, 0u), vc = make_uint2(0u, 0u);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int at = lane + 32 * e;
-      const bool in = at < left;
-      gf[e] = in ? load_as_float(g, i + at, g_dt) : 0.0f;
-      pf[e] = in ? load_as_float(p, i + at, p_dt) : 0.0f;
-      const uint32_t a = in ? mq[at] : 0u, b = in ? vq[at] : 0u;
-      (e < 4 ? mc.x : mc.y) |= a << (8 * (e & 3));
-      (e < 4 ? vc.x : vc.y) |= b << (8 * (e & 3));
-    }
-    decode8(mc, ms, mf);
-    decode8(vc, vs, vf);
+// Per-launch constants of one tensor.
+struct Step {
+  float g_to_m, g_to_v, lr_bc1, inv_bc2;
+
+  __device__ __forceinline__ Step(const StateArgs& a, const StateScalars& k, int t) {
+    const float scale = k.grad_scale != nullptr ? *k.grad_scale : 1.0f;
+    g_to_m = k.one_minus_beta1 * scale;
+    g_to_v = sqrtf(k.one_minus_beta2) * scale;
+    lr_bc1 = a.lr_bc1[t];
+    inv_bc2 = a.inv_bc2[t];
   }
+};
+
+// New moments and parameter of a lane's 8 elements of a block, the moments' codes and
+// the block's scales (in every lane).
+__device__ __forceinline__ void step_eight(const float (&gf)[8], float (&pf)[8], uint2& mc, uint2& vc, float& ms,
+                                           float& vs, const StateScalars& k, const Step& s) {
+  float mf[8], vf[8];
+  decode8(mc, mf);
+  decode8(vc, vf);
+  // The codes are scaled and decayed by one factor a block, and the gradient's
+  // factors are the launch's: (1 - b1) s for m, sqrt(1 - b2) s before the square for v.
+  const float old_m = ms * k.beta1, old_v = vs * k.beta2;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) adamw_math(gf[e], pf[e], mf[e], vf[e], k, scale, lr_bc1, inv_bc2);
+  for (int e = 0; e < 8; ++e) {
+    const float root = gf[e] * s.g_to_v;
+    mf[e] = fmaf(gf[e], s.g_to_m, mf[e] * old_m);
+    vf[e] = fmaf(root, root, vf[e] * old_v);
+    pf[e] = adamw_update(pf[e], mf[e], vf[e], k, s.lr_bc1, s.inv_bc2);
+  }
   const float m_top = block_max(mf), v_top = block_max(vf);
   const float m_inv = inverse_scale(m_top), v_inv = inverse_scale(v_top);
 #pragma unroll
@@ -211,58 +245,176 @@ __device__ __forceinline__ void step_block(void* p, const void* g, void* m, void
     const float y = vf[e] * v_inv;
     vf[e] = (vf[e] > 0.0f && y < kE4M3Tiny) ? kE4M3Tiny : y;
   }
-  const uint2 mc = encode8(mf), vc = encode8(vf);
-  if (VEC) {
-    store8(p, i + 8 * lane, p_dt, pf);
-    reinterpret_cast<uint2*>(mq)[lane] = mc;
-    reinterpret_cast<uint2*>(vq)[lane] = vc;
-  } else {
+  mc = encode8(mf);
+  vc = encode8(vf);
+  ms = m_top * (1.0f / kE4M3Max);
+  vs = v_top * (1.0f / kE4M3Max);
+}
+
+// A block of `left` elements at `i` without any alignment: lane L holds elements
+// L, L + 32, ...
+__device__ __noinline__ void step_ragged(const StateArgs& args, int t, int64_t i, int left, int p_dt, int g_dt,
+                                         const StateScalars& k) {
+  const int lane = threadIdx.x & 31;
+  void* p = args.p[t];
+  const void* g = args.g[t];
+  uint8_t* m = static_cast<uint8_t*>(args.m[t]);
+  uint8_t* v = static_cast<uint8_t*>(args.v[t]);
+  float* m_scale = args.m_scale[t];
+  float* v_scale = args.v_scale[t];
+  const Step s(args, k, t);
+  float pf[8], gf[8];
+  uint2 mc = make_uint2(0u, 0u), vc = make_uint2(0u, 0u);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int at = lane + 32 * e;
-      if (at >= left) continue;
-      store_from_float(p, i + at, p_dt, pf[e]);
-      mq[at] = static_cast<uint8_t>((e < 4 ? mc.x : mc.y) >> (8 * (e & 3)));
-      vq[at] = static_cast<uint8_t>((e < 4 ? vc.x : vc.y) >> (8 * (e & 3)));
-    }
+  for (int e = 0; e < 8; ++e) {
+    const int at = lane + 32 * e;
+    const bool in = at < left;
+    gf[e] = in ? load_as_float(g, i + at, g_dt) : 0.0f;
+    pf[e] = in ? load_as_float(p, i + at, p_dt) : 0.0f;
+    const uint32_t a = in ? m[i + at] : 0u, b = in ? v[i + at] : 0u;
+    (e < 4 ? mc.x : mc.y) |= a << (8 * (e & 3));
+    (e < 4 ? vc.x : vc.y) |= b << (8 * (e & 3));
+  }
+  const int64_t block = i / kBlockElems;
+  float ms = m_scale[block], vs = v_scale[block];
+  step_eight(gf, pf, mc, vc, ms, vs, k, s);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int at = lane + 32 * e;
+    if (at >= left) continue;
+    store_from_float(p, i + at, p_dt, pf[e]);
+    m[i + at] = static_cast<uint8_t>((e < 4 ? mc.x : mc.y) >> (8 * (e & 3)));
+    v[i + at] = static_cast<uint8_t>((e < 4 ? vc.x : vc.y) >> (8 * (e & 3)));
   }
   if (lane == 0) {
-    m_scale[block] = m_top * (1.0f / kE4M3Max);
-    v_scale[block] = v_top * (1.0f / kE4M3Max);
+    m_scale[block] = ms;
+    v_scale[block] = vs;
   }
 }
 
+__device__ int g_states_status = 0;
+
+// Ring slots of a warp: a block's parameters, gradients and codes.
+constexpr int kSlots = 4;
+
+template <int P, int G>
+struct Slot {
+  static constexpr uint32_t kP = kBlockElems * (sixteen(P) ? 2 : 4);
+  static constexpr uint32_t kG = kBlockElems * (sixteen(G) ? 2 : 4);
+  static constexpr uint32_t kM = kP + kG;
+  static constexpr uint32_t kBytes = kP + kG + 2 * kBlockElems;
+  static constexpr size_t kSmem = static_cast<size_t>(kWarps) * kSlots * kBytes;
+};
+
 // P, G >= 0 fix the types at compile time (the common combinations); -1 takes
 // them from the arguments.
+//
+// Each warp steps consecutive blocks of the chunk. Bulk copies bring them into a
+// ring of its own, four blocks ahead: 48 KB in flight a CTA and 196 KB an SM
+// without a register held for it, and no barrier between warps. Loads into
+// registers kept 41 KB in flight and moved 2.9 TB/s, or 4.5 TB/s with the next
+// block prefetched (323M bf16 elements in 1129 and 717 us). The scales of the
+// warp's blocks are read and written once, a lane for each.
 template <int P, int G>
-__global__ void __launch_bounds__(kThreads) adamw_8bit_kernel(const __grid_constant__ StateArgs args, int p_rt, int g_rt,
-                                                              const StateScalars k) {
+__global__ void __launch_bounds__(kThreads, sixteen(P) && sixteen(G) ? 4 : 2)
+    adamw_8bit_kernel(const __grid_constant__ StateArgs args, int p_rt, int g_rt, const __grid_constant__ StateScalars k) {
+  using S = Slot<P, G>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t full[kWarps][kSlots];
+  __shared__ volatile int abort_flag;
   const int p_dt = P >= 0 ? P : p_rt;
   const int g_dt = G >= 0 ? G : g_rt;
   const int t = owner_of(args, blockIdx.x);
-  const int64_t n = args.numel[t];
-  const int64_t start = static_cast<int64_t>(blockIdx.x - args.block_start[t]) * kChunk;
-  const int64_t end = min(n, start + kChunk);
-  void* p = args.p[t];
-  const void* g = args.g[t];
-  void* m = args.m[t];
-  void* v = args.v[t];
-  float* ms = args.m_scale[t];
-  float* vs = args.v_scale[t];
-  const float lr_bc1 = args.lr_bc1[t], inv_bc2 = args.inv_bc2[t];
-  const float scale = k.grad_scale != nullptr ? *k.grad_scale : 1.0f;
-  const uintptr_t wide = reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g);
-  const uintptr_t half = reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v);
-  const bool vec = wide % 16 == 0 && half % 8 == 0;
-  const int lane = threadIdx.x & 31;
-  for (int64_t i = start + static_cast<int64_t>(threadIdx.x >> 5) * kBlockElems; i < end;
-       i += kWarps * kBlockElems) {
-    if (vec && i + kBlockElems <= end)
-      step_block<true>(p, g, m, v, ms, vs, i, kBlockElems, lane, p_dt, g_dt, k, scale, lr_bc1, inv_bc2);
-    else
-      step_block<false>(p, g, m, v, ms, vs, i, static_cast<int>(min(static_cast<int64_t>(kBlockElems), end - i)), lane,
-                        p_dt, g_dt, k, scale, lr_bc1, inv_bc2);
+  const int64_t start = static_cast<int64_t>(blockIdx.x - args.block_start[t]) * args.chunk;
+  const int count = static_cast<int>(min(args.numel[t] - start, static_cast<int64_t>(args.chunk)));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) abort_flag = 0;
+  if (lane == 0) {
+    for (int i = 0; i < kSlots; ++i) mbar_init(&full[warp][i], 1);
+    fence_barrier_init();
+    fence_proxy_async_smem();
   }
+  __syncthreads();
+  // This warp's blocks of the chunk: [first, first + whole) complete ones, and
+  // perhaps one more that is not.
+  const int share = args.chunk / (kWarps * kBlockElems);
+  const int first = warp * share;
+  const int mine = min(max(count - first * kBlockElems, 0), share * kBlockElems);
+  int whole = mine / kBlockElems;
+  const uintptr_t all = reinterpret_cast<uintptr_t>(args.p[t]) | reinterpret_cast<uintptr_t>(args.g[t]) |
+                        reinterpret_cast<uintptr_t>(args.m[t]) | reinterpret_cast<uintptr_t>(args.v[t]);
+  if (all % 16 != 0) whole = 0;  // the copies need aligned rows: every block goes the ragged way
+  if (whole > 0) {
+    const Step s(args, k, t);
+    const int64_t at0 = start + static_cast<int64_t>(first) * kBlockElems;
+    uint8_t* p = static_cast<uint8_t*>(args.p[t]) + at0 * (p_dt == kF32 ? 4 : 2);
+    const uint8_t* g = static_cast<const uint8_t*>(args.g[t]) + at0 * (g_dt == kF32 ? 4 : 2);
+    uint8_t* m = static_cast<uint8_t*>(args.m[t]) + at0;
+    uint8_t* v = static_cast<uint8_t*>(args.v[t]) + at0;
+    float* m_scale = args.m_scale[t] + at0 / kBlockElems;
+    float* v_scale = args.v_scale[t] + at0 / kBlockElems;
+    const uint32_t p_bytes = kBlockElems * (p_dt == kF32 ? 4 : 2), g_bytes = kBlockElems * (g_dt == kF32 ? 4 : 2);
+    uint8_t* ring = smem + static_cast<uint32_t>(warp * kSlots) * S::kBytes;
+    auto fetch = [&](int i, int st) {
+      uint8_t* slot = ring + static_cast<uint32_t>(st) * S::kBytes;
+      uint64_t* bar = &full[warp][st];
+      mbar_arrive_expect_tx(bar, p_bytes + g_bytes + 2 * kBlockElems);
+      bulk_load(slot, p + static_cast<uint32_t>(i) * p_bytes, p_bytes, bar);
+      bulk_load(slot + S::kP, g + static_cast<uint32_t>(i) * g_bytes, g_bytes, bar);
+      bulk_load(slot + S::kM, m + i * kBlockElems, kBlockElems, bar);
+      bulk_load(slot + S::kM + kBlockElems, v + i * kBlockElems, kBlockElems, bar);
+    };
+    if (lane == 0)
+      for (int i = 0; i < kSlots && i < whole; ++i) fetch(i, i);
+    float my_ms = 0.0f, my_vs = 0.0f;  // of block `lane` of the warp's
+    if (lane < whole) {
+      my_ms = m_scale[lane];
+      my_vs = v_scale[lane];
+    }
+    uint32_t phase = 0;
+    int st = 0;
+    bool ok = true;
+    for (int i = 0; i < whole; ++i) {
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[warp][st], phase, &abort_flag, &g_states_status,
+                                                     kStatusProducerTimeout));
+      if (!ok) break;
+      const uint8_t* slot = ring + static_cast<uint32_t>(st) * S::kBytes;
+      float pf[8], gf[8];
+      Eight<P> pe;
+      Eight<G> ge;
+      pe.load(slot, 8 * lane, p_dt);
+      ge.load(slot + S::kP, 8 * lane, g_dt);
+      uint2 mc = reinterpret_cast<const uint2*>(slot + S::kM)[lane];
+      uint2 vc = reinterpret_cast<const uint2*>(slot + S::kM + kBlockElems)[lane];
+      pe.get(p_dt, pf);
+      ge.get(g_dt, gf);
+      __syncwarp();  // every lane has read the slot: it is filled again
+      if (lane == 0 && i + kSlots < whole) fetch(i + kSlots, st);
+      float ms = __shfl_sync(0xffffffffu, my_ms, i), vs = __shfl_sync(0xffffffffu, my_vs, i);
+      step_eight(gf, pf, mc, vc, ms, vs, k, s);
+      store8(p + static_cast<uint32_t>(i) * p_bytes, 8 * lane, p_dt, pf);
+      reinterpret_cast<uint2*>(m + i * kBlockElems)[lane] = mc;
+      reinterpret_cast<uint2*>(v + i * kBlockElems)[lane] = vc;
+      if (lane == i) {
+        my_ms = ms;
+        my_vs = vs;
+      }
+      if (++st == kSlots) {
+        st = 0;
+        phase ^= 1u;
+      }
+    }
+    if (!ok) {
+      settle_for_ns(2000000ull);  // copies in flight land before the CTA's memory is released
+      return;
+    }
+    if (lane < whole) {
+      m_scale[lane] = my_ms;
+      v_scale[lane] = my_vs;
+    }
+  }
+  for (int i = whole * kBlockElems; i < mine; i += kBlockElems)
+    step_ragged(args, t, start + static_cast<int64_t>(first) * kBlockElems + i, min(kBlockElems, mine - i), p_dt, g_dt, k);
 }
 
 template <int P, int G>
@@ -272,8 +424,8 @@ __global__ void __launch_bounds__(kThreads) adamw_32bit_kernel(const __grid_cons
   const int g_dt = G >= 0 ? G : g_rt;
   const int t = owner_of(args, blockIdx.x);
   const int64_t n = args.numel[t];
-  const int64_t start = static_cast<int64_t>(blockIdx.x - args.block_start[t]) * kChunk;
-  const int64_t end = min(n, start + kChunk);
+  const int64_t start = static_cast<int64_t>(blockIdx.x - args.block_start[t]) * args.chunk;
+  const int64_t end = min(n, start + args.chunk);
   void* p = args.p[t];
   const void* g = args.g[t];
   void* m = args.m[t];
@@ -288,10 +440,17 @@ __global__ void __launch_bounds__(kThreads) adamw_32bit_kernel(const __grid_cons
 #pragma unroll 2
     for (i = start + threadIdx.x * 8; i < vend; i += kThreads * 8) {
       float pf[8], gf[8], mf[8], vf[8];
-      load8(g, i, g_dt, gf);
-      load8(p, i, p_dt, pf);
-      load8(m, i, kF32, mf);
-      load8(v, i, kF32, vf);
+      Eight<P> pe;
+      Eight<G> ge;
+      Eight<kF32> me, ve;
+      ge.load(g, i, g_dt);
+      pe.load(p, i, p_dt);
+      me.load(m, i, kF32);
+      ve.load(v, i, kF32);
+      ge.get(g_dt, gf);
+      pe.get(p_dt, pf);
+      me.get(kF32, mf);
+      ve.get(kF32, vf);
 #pragma unroll
       for (int e = 0; e < 8; ++e) adamw_math(gf[e], pf[e], mf[e], vf[e], k, scale, lr_bc1, inv_bc2);
       store8(p, i, p_dt, pf);
@@ -309,15 +468,44 @@ __global__ void __launch_bounds__(kThreads) adamw_32bit_kernel(const __grid_cons
   }
 }
 
+std::mutex g_mutex;
+bool g_ready[64][8] = {};
+
 template <int P, int G>
-void launch(int bits, int blocks, cudaStream_t st, const StateArgs& a, int p_dt, int g_dt, const StateScalars& k) {
-  if (bits == 8)
-    adamw_8bit_kernel<P, G><<<blocks, kThreads, 0, st>>>(a, p_dt, g_dt, k);
-  else
+int launch(int bits, int blocks, cudaStream_t st, const StateArgs& a, int p_dt, int g_dt, const StateScalars& k, int slot) {
+  if (bits == 8) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+    if (dev < 0 || dev >= 64) return fail(GNS_ERR_DEVICE, "device index out of range");
+    {
+      std::lock_guard<std::mutex> lock(g_mutex);
+      if (!g_ready[dev][slot]) {
+        e = cudaFuncSetAttribute(adamw_8bit_kernel<P, G>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(Slot<P, G>::kSmem));
+        if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(smem)");
+        g_ready[dev][slot] = true;
+      }
+    }
+    adamw_8bit_kernel<P, G><<<blocks, kThreads, Slot<P, G>::kSmem, st>>>(a, p_dt, g_dt, k);
+  } else {
     adamw_32bit_kernel<P, G><<<blocks, kThreads, 0, st>>>(a, p_dt, g_dt, k);
+  }
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? GNS_OK : cuda_fail(e, "adamw states kernel");
 }
 
 }  // namespace
+
+int states_status(int* status, int clear) {
+  cudaError_t e = cudaMemcpyFromSymbol(status, g_states_status, sizeof(int));
+  if (e == cudaSuccess && clear && *status != 0) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_states_status, &zero, sizeof(int));
+  }
+  return e == cudaSuccess ? GNS_OK : cuda_fail(e, "adamw states status");
+}
+
 }  // namespace gns
 
 using namespace gns;
@@ -351,14 +539,21 @@ extern "C" int gns_adamw_states_step(int count, void* const* params, const void*
   if (rc != GNS_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const StateScalars k{beta1, one_minus_beta1, beta2, one_minus_beta2, epsilon, decay, grad_scale};
+  // Long chunks keep a warp's ring going; short ones give every SM work. Elements are
+  // divided into 32 chunks an SM (eight turns of its four CTAs) where there are enough.
+  int64_t total = 0;
+  for (int i = 0; i < count; ++i) total += numel[i];
+  int chunk = kChunkMin;
+  while (chunk < kChunkMax && total / chunk > 32 * static_cast<int64_t>(device_sm_count())) chunk *= 2;
   int i = 0;
   while (i < count) {
     StateArgs a;
     a.count = 0;
+    a.chunk = chunk;
     int64_t blocks = 0;
     for (; i < count && a.count < kTensors; ++i) {
       if (numel[i] == 0) continue;
-      const int64_t nb = (numel[i] + kChunk - 1) / kChunk;
+      const int64_t nb = (numel[i] + chunk - 1) / chunk;
       if (blocks > 0 && blocks + nb > (1ll << 30)) break;  // next launch
       const int j = a.count++;
       a.p[j] = params[i];
@@ -377,17 +572,16 @@ extern "C" int gns_adamw_states_step(int count, void* const* params, const void*
     a.block_start[a.count] = static_cast<int>(blocks);
     const int grid = static_cast<int>(blocks);
     if (p_dtype == kBF16 && g_dtype == kBF16)
-      launch<kBF16, kBF16>(state_bits, grid, st, a, p_dtype, g_dtype, k);
+      rc = launch<kBF16, kBF16>(state_bits, grid, st, a, p_dtype, g_dtype, k, 0);
     else if (p_dtype == kF32 && g_dtype == kF32)
-      launch<kF32, kF32>(state_bits, grid, st, a, p_dtype, g_dtype, k);
+      rc = launch<kF32, kF32>(state_bits, grid, st, a, p_dtype, g_dtype, k, 1);
     else if (p_dtype == kF16 && g_dtype == kF16)
-      launch<kF16, kF16>(state_bits, grid, st, a, p_dtype, g_dtype, k);
+      rc = launch<kF16, kF16>(state_bits, grid, st, a, p_dtype, g_dtype, k, 2);
     else if (p_dtype == kBF16 && g_dtype == kF32)
-      launch<kBF16, kF32>(state_bits, grid, st, a, p_dtype, g_dtype, k);
+      rc = launch<kBF16, kF32>(state_bits, grid, st, a, p_dtype, g_dtype, k, 3);
     else
-      launch<-1, -1>(state_bits, grid, st, a, p_dtype, g_dtype, k);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return cuda_fail(e, "adamw states kernel");
+      rc = launch<-1, -1>(state_bits, grid, st, a, p_dtype, g_dtype, k, 4);
+    if (rc != GNS_OK) return rc;
   }
   return GNS_OK;
 }

@@ -471,6 +471,14 @@ int gns_device_status(int* status, int clear) {
   rc = gns::grouped_status(&grouped, clear);
   if (rc != GNS_OK) return rc;
   if (*status == 0) *status = grouped;
+  int norm_rows = 0;
+  rc = gns::norm_status(&norm_rows, clear);
+  if (rc != GNS_OK) return rc;
+  if (*status == 0) *status = norm_rows;
+  int states = 0;
+  rc = gns::states_status(&states, clear);
+  if (rc != GNS_OK) return rc;
+  if (*status == 0) *status = states;
   return GNS_OK;
 }
 

@@ -105,6 +105,9 @@ int encode_tiles(CUtensorMap* map, int dtype, const void* ptr, int64_t inner, in
 
 // Status word of the grouped products (0 = ok); optionally cleared.
 int grouped_status(int* status, int clear);
+// The same of the layer norm kernels and of the AdamW kernel for 8-bit states.
+int norm_status(int* status, int clear);
+int states_status(int* status, int clear);
 
 // Fused single-kernel Gram Newton-Schulz chain for matrices whose short side is
 // at most 128 (small_chain.cu). x0 holds the normalised fp16 X and x1 is the

@@ -8,13 +8,21 @@
 // A row is held in the registers of TPR threads, 16 elements each, so x (and dy)
 // are read once: the mean is subtracted before the squares are summed, which
 // costs a second reduction but no second read. Rows go to the groups of a
-// persistent grid round robin; the next row's loads are issued before the
-// current row's reduction, so that memory does not wait for the barrier. Each
-// thread keeps the same columns for all its rows: w and b stay in registers, and
-// dw and db are summed there over the rows, written once per CTA and joined by a
-// second kernel in a fixed order (no atomics, the same bits on every run).
+// persistent grid round robin. Each thread keeps the same columns for all its
+// rows: w and b stay in registers, and dw and db are summed there over the rows,
+// written once per CTA and joined by a second kernel in a fixed order (no
+// atomics, the same bits on every run).
+//
+// Rows reach the registers in one of two ways. Aligned rows of more than 512
+// elements come through a ring of rows in shared memory, filled by bulk copies
+// several rows ahead (ring kernels); the bytes in flight do not depend on
+// registers or occupancy. Other rows are loaded directly, the next row before the
+// current row's reduction (direct kernels).
 // Statistics, sums and all arithmetic are fp32; y, dx, dw and db are rounded
 // once, at their stores. Bound by HBM: 2 elements moved forward, 3 backward.
+#include <algorithm>
+#include <mutex>
+
 #include "../../include/gns_b200.h"
 #include "gns_common.cuh"
 #include "gns_host.h"
@@ -45,10 +53,10 @@ struct NormArgs {
 // One thread's 16 elements of a row as loaded. VEC: 16-byte pieces, V elements
 // each, piece j of thread t at element (j TPR + t) V; otherwise element i of
 // thread t is i TPR + t.
-template <int XD, int TPR, bool VEC>
+template <int XD, int TPR, bool VEC, int E = kPer>
 struct Piece {
   static constexpr int kV = XD == kF32 ? 4 : 8;
-  static constexpr int kWords = XD == kF32 ? 16 : 8;
+  static constexpr int kWords = XD == kF32 ? E : E / 2;
   uint32_t w[kWords];
 
   static __device__ __forceinline__ int col(int t, int i) {
@@ -60,7 +68,7 @@ struct Piece {
     const uint8_t* p = static_cast<const uint8_t*>(base) + row * stride * es;
     if (VEC) {
 #pragma unroll
-      for (int j = 0; j < kPer / kV; ++j) {
+      for (int j = 0; j < E / kV; ++j) {
         const int c = (j * TPR + t) * kV;
         uint4 u = make_uint4(0u, 0u, 0u, 0u);
         if (live && c < cols) u = *reinterpret_cast<const uint4*>(p + static_cast<int64_t>(c) * es);
@@ -68,13 +76,13 @@ struct Piece {
       }
     } else if (XD == kF32) {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
+      for (int i = 0; i < E; ++i) {
         const int c = i * TPR + t;
         w[i % kWords] = (live && c < cols) ? reinterpret_cast<const uint32_t*>(p)[c] : 0u;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < kPer; i += 2) {
+      for (int i = 0; i < E; i += 2) {
         const int c = i * TPR + t;
         const uint32_t lo = (live && c < cols) ? reinterpret_cast<const uint16_t*>(p)[c] : 0u;
         const uint32_t hi = (live && c + TPR < cols) ? reinterpret_cast<const uint16_t*>(p)[c + TPR] : 0u;
@@ -91,14 +99,14 @@ struct Piece {
   }
 };
 
-template <int XD, int TPR, bool VEC>
-__device__ __forceinline__ void store_row(void* base, int64_t row, int cols, int t, const float (&v)[kPer]) {
-  using P = Piece<XD, TPR, VEC>;
+template <int XD, int TPR, bool VEC, int E>
+__device__ __forceinline__ void store_row(void* base, int64_t row, int cols, int t, const float (&v)[E]) {
+  using P = Piece<XD, TPR, VEC, E>;
   constexpr int es = XD == kF32 ? 4 : 2;
   uint8_t* p = static_cast<uint8_t*>(base) + row * cols * es;
   if (VEC) {
 #pragma unroll
-    for (int j = 0; j < kPer / P::kV; ++j) {
+    for (int j = 0; j < E / P::kV; ++j) {
       const int c = (j * TPR + t) * P::kV;
       if (c >= cols) continue;
       uint32_t o[4];
@@ -107,10 +115,10 @@ __device__ __forceinline__ void store_row(void* base, int64_t row, int cols, int
         if (XD == kF32) {
           o[q] = __float_as_uint(v[j * P::kV + q]);
         } else if (XD == kBF16) {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(v[(j * P::kV + 2 * q) % kPer], v[(j * P::kV + 2 * q + 1) % kPer]);
+          const __nv_bfloat162 h = __floats2bfloat162_rn(v[(j * P::kV + 2 * q) % E], v[(j * P::kV + 2 * q + 1) % E]);
           o[q] = *reinterpret_cast<const uint32_t*>(&h);
         } else {
-          const __half2 h = __floats2half2_rn(v[(j * P::kV + 2 * q) % kPer], v[(j * P::kV + 2 * q + 1) % kPer]);
+          const __half2 h = __floats2half2_rn(v[(j * P::kV + 2 * q) % E], v[(j * P::kV + 2 * q + 1) % E]);
           o[q] = *reinterpret_cast<const uint32_t*>(&h);
         }
       }
@@ -118,7 +126,7 @@ __device__ __forceinline__ void store_row(void* base, int64_t row, int cols, int
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
+    for (int i = 0; i < E; ++i) {
       const int c = i * TPR + t;
       if (c < cols) store_from_float(p, c, XD, v[i]);
     }
@@ -129,12 +137,12 @@ __device__ __forceinline__ void store_row(void* base, int64_t row, int cols, int
 // `slot` alternates between two buffers, so one barrier per call is enough: a
 // buffer is written again only after the other buffer's barrier, which every
 // reader of it has passed.
-template <int TPR, int THREADS>
+template <int TPR, int THREADS, bool BOTH = true>
 __device__ __forceinline__ float2 group_sum(float a, float b, float2 (*slots)[THREADS / 32], int& slot) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     a += __shfl_xor_sync(0xffffffffu, a, o);
-    b += __shfl_xor_sync(0xffffffffu, b, o);
+    if (BOTH) b += __shfl_xor_sync(0xffffffffu, b, o);
   }
   if (TPR == 32) return make_float2(a, b);
   float2* buf = slots[slot];
@@ -160,7 +168,7 @@ __device__ __forceinline__ float2 group_sum(float a, float b, float2 (*slots)[TH
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       a += __shfl_xor_sync(0xffffffffu, a, o);
-      b += __shfl_xor_sync(0xffffffffu, b, o);
+      if (BOTH) b += __shfl_xor_sync(0xffffffffu, b, o);
     }
   }
   return make_float2(a, b);
@@ -204,22 +212,55 @@ __global__ void __launch_bounds__(threads_of<TPR>()) norm_forward_kernel(const N
       sum += v[i];
     }
     next.load(a.x, row + step, a.x_stride, t, a.cols, row + step < a.rows);
-    const float mu = group_sum<TPR, kThreads>(sum, 0.0f, slots, slot).x * inv_n;
+    const float mu = group_sum<TPR, kThreads, false>(sum, 0.0f, slots, slot).x * inv_n;
     float sq = 0.0f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       v[i] -= mu;
       if (P::col(t, i) < a.cols) sq = fmaf(v[i], v[i], sq);
     }
-    const float var = group_sum<TPR, kThreads>(sq, 0.0f, slots, slot).x * inv_n;
+    const float var = group_sum<TPR, kThreads, false>(sq, 0.0f, slots, slot).x * inv_n;
     const float r = rsqrtf(var + a.eps);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) v[i] = fmaf(v[i] * r, w[i], b[i]);
     if (live) {
-      store_row<XD, TPR, VEC>(a.y, row, a.cols, t, v);
+      store_row<XD, TPR, VEC, kPer>(a.y, row, a.cols, t, v);
       if (t == 0) {
         a.mean[row] = mu;
         a.rstd[row] = r;
+      }
+    }
+  }
+}
+
+// A CTA's column sums: its groups' are joined in `joined` (kThreads kPer floats,
+// unused with one group), in a fixed order.
+template <int TPR, class P>
+__device__ __forceinline__ void write_partial(const NormArgs& a, const float (&dw)[kPer], const float (&db)[kPer],
+                                              float* joined, int t, int group) {
+  constexpr int kGroups = threads_of<TPR>() / TPR;
+  float* out = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    if (kGroups > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) joined[(group * kPer + i) * TPR + t] = which ? db[i] : dw[i];
+      __syncthreads();
+      if (group == 0) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          float sum = 0.0f;
+          for (int q = 0; q < kGroups; ++q) sum += joined[(q * kPer + i) * TPR + t];
+          const int c = P::col(t, i);
+          if (c < a.cols) out[which * a.cols + c] = sum;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int c = P::col(t, i);
+        if (c < a.cols) out[which * a.cols + c] = which ? db[i] : dw[i];
       }
     }
   }
@@ -273,33 +314,266 @@ __global__ void __launch_bounds__(threads_of<TPR>()) norm_backward_kernel(const 
     const float c1 = c.x * inv_n, c2 = c.y * inv_n;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) g[i] = (g[i] - fmaf(h[i], c1, c2)) * r;
-    if (live) store_row<XD, TPR, VEC>(a.y, row, a.cols, t, g);
+    if (live) store_row<XD, TPR, VEC, kPer>(a.y, row, a.cols, t, g);
   }
-  float* out = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
+  write_partial<TPR, P>(a, dw, db, joined, t, group);
+}
+
+// ------------------------------------------------------------- ring kernels
+__device__ int g_norm_status = 0;
+
+constexpr int kMaxStages = 8;
+
+// Ring of row slots: a stage holds one row of each group (and of dy behind it).
+struct Ring {
+  uint64_t* full;             // one barrier per stage, an arrival per group
+  volatile int* abort_flag;
+  uint8_t* rows;              // [stage][group][tensors][row]
+  int stages, stage = 0;
+  uint32_t phase = 0;
+  uint32_t row_bytes, stage_bytes;
+
+  __device__ __forceinline__ Ring(uint8_t* smem, int stages_, int groups, int tensors, uint32_t bytes)
+      : full(reinterpret_cast<uint64_t*>(smem)),
+        abort_flag(reinterpret_cast<volatile int*>(smem + 8 * kMaxStages)),
+        rows(smem + 128),
+        stages(stages_),
+        row_bytes(bytes),
+        stage_bytes(bytes * static_cast<uint32_t>(tensors * groups)) {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < stages; ++i) mbar_init(&full[i], static_cast<uint32_t>(groups));
+      *abort_flag = 0;
+      fence_barrier_init();
+      fence_proxy_async_smem();
+    }
+    __syncthreads();
+  }
+
+  __device__ __forceinline__ uint8_t* slot(int st, int group, int tensors) {
+    return rows + st * stage_bytes + static_cast<uint32_t>(group * tensors) * row_bytes;
+  }
+
+  // A wait that runs out sets the status word and lets the loop go on with what the
+  // slot holds, so that the CTA's barriers stay matched; every later wait returns at
+  // once.
+  __device__ __forceinline__ void wait() {
+    mbar_wait_bounded(&full[stage], phase, abort_flag, &g_norm_status, kStatusProducerTimeout);
+  }
+
+  __device__ __forceinline__ void advance() {
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+
+  // After an aborted wait, copies in flight get time to land before the CTA ends.
+  __device__ __forceinline__ void finish() {
+    __syncthreads();
+    if (*abort_flag) settle_for_ns(2000000ull);
+  }
+};
+
+// One row of each tensor into a stage, by one thread of each group.
+template <int XD, int TENSORS>
+__device__ __forceinline__ void fetch(Ring& ring, int st, int group, const NormArgs& a, int64_t row) {
+  constexpr int es = XD == kF32 ? 4 : 2;
+  if (row >= a.rows) {
+    mbar_arrive(&ring.full[st]);
+    return;
+  }
+  uint8_t* slot = ring.slot(st, group, TENSORS);
+  mbar_arrive_expect_tx(&ring.full[st], TENSORS * ring.row_bytes);
+  bulk_load(slot, static_cast<const uint8_t*>(a.x) + row * a.x_stride * es, ring.row_bytes, &ring.full[st]);
+  if (TENSORS == 2)
+    bulk_load(slot + ring.row_bytes, static_cast<const uint8_t*>(a.dy) + row * a.dy_stride * es, ring.row_bytes,
+              &ring.full[st]);
+}
+
+// Elements of a row per thread in the forward ring kernel: a reduction over a row
+// costs each thread the same whatever it holds, so 32 elements halve its share
+// (with 16, two reductions of two values and 256 threads for 4096 columns, the
+// kernel issued 20 instructions an element and took 57 us for 16384 bf16 rows).
+constexpr int kFwdPer = 32;
+
+__device__ __forceinline__ float warp_total(float v) {
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    if (kGroups > 1) {
-      __syncthreads();
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Mean and variance of a row take one barrier: each warp finds the sum and the
+// squared deviations from its own mean, S_w and Q_w, and over the warps
+//   mu = sum S_w / n,   n var = sum Q_w + n_w (S_w / n_w - mu)^2,
+// which loses nothing to cancellation, unlike sums of squares.
+template <int XD, int TPR>
+__global__ void __launch_bounds__(threads_of<TPR>()) norm_forward_ring_kernel(const NormArgs a, int stages) {
+  constexpr int kThreads = threads_of<TPR>();
+  constexpr int kGroups = kThreads / TPR;
+  constexpr int kW = TPR / 32;
+  constexpr int E = kFwdPer;
+  using P = Piece<XD, TPR, true, E>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float2 slots[2][kThreads / 32];  // S_w, Q_w
+  __shared__ float2 sizes[kThreads / 32];     // n_w, 1 / n_w
+  int slot = 0;
+  const int t = threadIdx.x % TPR;
+  const int group = threadIdx.x / TPR;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int mine = 0;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) joined[(group * kPer + i) * TPR + t] = which ? db[i] : dw[i];
-      __syncthreads();
-      if (group == 0) {
+  for (int i = 0; i < E; i += P::kV) mine += P::col(t, i) < a.cols ? P::kV : 0;
+  const float n_w = warp_total(static_cast<float>(mine));
+  const float inv_w = n_w > 0.0f ? 1.0f / n_w : 0.0f;
+  if (lane == 0) sizes[warp] = make_float2(n_w, inv_w);
+  Ring ring(smem, stages, kGroups, 1, static_cast<uint32_t>(a.cols) * (XD == kF32 ? 4 : 2));
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * kGroups;
+  if (t == 0)
+    for (int i = 0; i < stages; ++i) fetch<XD, 1>(ring, i, group, a, base + group + i * step);
+  float w[E], b[E];
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          float sum = 0.0f;
-          for (int q = 0; q < kGroups; ++q) sum += joined[(q * kPer + i) * TPR + t];
-          const int c = P::col(t, i);
-          if (c < a.cols) out[which * a.cols + c] = sum;
-        }
+  for (int i = 0; i < E; ++i) {
+    const int c = P::col(t, i);
+    w[i] = c < a.cols ? load_as_float(a.w, c, a.w_dt) : 0.0f;
+    b[i] = (a.b != nullptr && c < a.cols) ? load_as_float(a.b, c, a.w_dt) : 0.0f;
+  }
+  const float inv_n = 1.0f / static_cast<float>(a.cols);
+  for (int64_t first = base; first < a.rows; first += step) {
+    const int64_t row = first + group;
+    ring.wait();
+    P p;
+    p.load(ring.slot(ring.stage, group, 1), 0, 0, t, a.cols, true);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) sum += p.get(i);
+    sum = warp_total(sum);
+    const float mean_w = sum * inv_w;
+    float sq = 0.0f;
+#pragma unroll
+    for (int i = 0; i < E; i += P::kV) {
+      if (P::col(t, i) >= a.cols) continue;
+#pragma unroll
+      for (int q = 0; q < P::kV; ++q) {
+        const float d = p.get(i + q) - mean_w;
+        sq = fmaf(d, d, sq);
       }
-    } else {
+    }
+    sq = warp_total(sq);
+    float mu = mean_w, var = sq;
+    if (kW > 1) {
+      float2* buf = slots[slot];
+      slot ^= 1;
+      if (lane == 0) buf[warp] = make_float2(sum, sq);
+      __syncthreads();
+      const int w0 = group * kW;
+      float total = 0.0f, rest = 0.0f;
+      if (kW <= 8) {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int c = P::col(t, i);
-        if (c < a.cols) out[which * a.cols + c] = which ? db[i] : dw[i];
+        for (int q = 0; q < kW; ++q) total += buf[w0 + q].x;
+        mu = total * inv_n;
+#pragma unroll
+        for (int q = 0; q < kW; ++q) {
+          const float d = fmaf(buf[w0 + q].x, sizes[w0 + q].y, -mu);
+          rest += fmaf(d * d, sizes[w0 + q].x, buf[w0 + q].y);
+        }
+      } else {
+        // 16 partial sums: one per lane, joined by shuffles.
+        const bool has = lane < kW;
+        const float2 one = has ? buf[w0 + lane] : make_float2(0.0f, 0.0f);
+        const float2 size = has ? sizes[w0 + lane] : make_float2(0.0f, 0.0f);
+        mu = warp_total(one.x) * inv_n;
+        const float d = fmaf(one.x, size.y, -mu);
+        rest = warp_total(fmaf(d * d, size.x, one.y));
+      }
+      var = rest;
+    } else {
+      __syncwarp();
+    }
+    // Every thread of the group has read the slot: it is filled again.
+    if (t == 0) fetch<XD, 1>(ring, ring.stage, group, a, row + stages * step);
+    ring.advance();
+    const float r = rsqrtf(fmaf(var, inv_n, a.eps));
+    const float shift = -mu * r;
+    if (row < a.rows) {
+      float v[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) v[i] = fmaf(fmaf(p.get(i), r, shift), w[i], b[i]);
+      store_row<XD, TPR, true, E>(a.y, row, a.cols, t, v);
+      if (t == 0) {
+        a.mean[row] = mu;
+        a.rstd[row] = r;
       }
     }
   }
+  ring.finish();
+}
+
+template <int XD, int TPR>
+__global__ void __launch_bounds__(threads_of<TPR>()) norm_backward_ring_kernel(const NormArgs a, int stages) {
+  constexpr int kThreads = threads_of<TPR>();
+  constexpr int kGroups = kThreads / TPR;
+  using P = Piece<XD, TPR, true>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float2 slots[2][kThreads / 32];
+  int slot = 0;
+  const int t = threadIdx.x % TPR;
+  const int group = threadIdx.x / TPR;
+  Ring ring(smem, stages, kGroups, 2, static_cast<uint32_t>(a.cols) * (XD == kF32 ? 4 : 2));
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * kGroups;
+  if (t == 0)
+    for (int i = 0; i < stages; ++i) fetch<XD, 2>(ring, i, group, a, base + group + i * step);
+  float w[kPer], dw[kPer], db[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int c = P::col(t, i);
+    w[i] = c < a.cols ? load_as_float(a.w, c, a.w_dt) : 0.0f;
+    dw[i] = 0.0f;
+    db[i] = 0.0f;
+  }
+  const float inv_n = 1.0f / static_cast<float>(a.cols);
+  // A row's mean and rstd are loaded a turn ahead, as their rows are.
+  float next_mu = 0.0f, next_r = 0.0f;
+  if (base + group < a.rows) {
+    next_mu = a.mean[base + group];
+    next_r = a.rstd[base + group];
+  }
+  for (int64_t first = base; first < a.rows; first += step) {
+    const int64_t row = first + group;
+    const bool live = row < a.rows;
+    const float mu = next_mu, r = live ? next_r : 0.0f;
+    if (row + step < a.rows) {
+      next_mu = a.mean[row + step];
+      next_r = a.rstd[row + step];
+    }
+    ring.wait();
+    const uint8_t* at = ring.slot(ring.stage, group, 2);
+    P px, pg;
+    px.load(at, 0, 0, t, a.cols, live);
+    pg.load(at + ring.row_bytes, 0, 0, t, a.cols, live);
+    float h[kPer], g[kPer];
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      g[i] = pg.get(i);
+      h[i] = (px.get(i) - mu) * r;
+      dw[i] = fmaf(g[i], h[i], dw[i]);
+      db[i] += g[i];
+      g[i] *= w[i];
+      s1 = fmaf(g[i], h[i], s1);
+      s2 += g[i];
+    }
+    const float2 c = group_sum<TPR, kThreads>(s1, s2, slots, slot);
+    if (t == 0) fetch<XD, 2>(ring, ring.stage, group, a, row + stages * step);
+    ring.advance();
+    const float c1 = c.x * inv_n, c2 = c.y * inv_n;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) g[i] = (g[i] - fmaf(h[i], c1, c2)) * r;
+    if (live) store_row<XD, TPR, true, kPer>(a.y, row, a.cols, t, g);
+  }
+  ring.finish();
+  write_partial<TPR, P>(a, dw, db, reinterpret_cast<float*>(ring.rows), t, group);
 }
 
 // Rows too wide for the registers of a CTA: a CTA per row, read again for each pass.
@@ -395,57 +669,124 @@ __global__ void __launch_bounds__(32 * kJoinRows) norm_join_kernel(const float* 
     store_from_float(db, c - cols, dt, s);
 }
 
-// Threads of a row: the fewest that hold it at 16 elements each, a warp at least.
-int threads_per_row(int64_t cols) {
+// Threads of a row: the fewest that hold it at `per` elements each, a warp at least.
+int threads_per_row(int64_t cols, int per) {
   int t = 32;
-  while (t < kMaxTPR && static_cast<int64_t>(t) * kPer < cols) t *= 2;
+  while (t < kMaxTPR && static_cast<int64_t>(t) * per < cols) t *= 2;
   return t;
 }
 
-bool is_wide(int64_t cols) { return cols > static_cast<int64_t>(kMaxTPR) * kPer; }
+// How a call runs: `stages` > 0, the ring kernels; else the direct kernels, or the
+// wide ones for rows that no CTA's registers hold.
+struct Plan {
+  bool wide;
+  int stages, grid, tpr;
+  size_t smem;
+};
 
-// CTAs of the persistent grids: enough for two thirds of an SM's threads, and no
-// more than there are rows for.
-int norm_grid(int64_t rows, int64_t cols) {
-  const int tpr = threads_per_row(cols);
+// Shared memory for rings on an SM, and the stages that one is given at most. Each
+// CTA's share is divided into stages; below two there is nothing to overlap.
+constexpr int kRingBytes = 200 * 1024;
+
+Plan plan_norm(bool backward, bool vec, int x_dt, int64_t rows, int64_t cols) {
+  Plan p{};
+  const bool ring = vec && cols > 32 * kPer && cols <= static_cast<int64_t>(kMaxTPR) * kPer;
+  const int tpr = threads_per_row(cols, ring && !backward ? kFwdPer : kPer);
   const int threads = tpr < 256 ? 256 : tpr;
-  const int64_t turns = (rows + threads / tpr - 1) / (threads / tpr);
-  const int64_t most = static_cast<int64_t>(device_sm_count()) * (threads >= 1024 ? 1 : 768 / threads);
-  return static_cast<int>(turns < most ? turns : most);
+  const int groups = threads / tpr;
+  const int64_t turns = (rows + groups - 1) / groups;
+  const int sms = device_sm_count();
+  p.tpr = tpr;
+  if (ring) {
+    const int ctas = threads > 256 ? 1 : 2;  // per SM: what the registers allow
+    const int64_t stage = cols * dtype_size(x_dt) * groups * (backward ? 2 : 1);
+    const int64_t stages = kRingBytes / ctas / stage;
+    if (stages >= 2) {
+      p.stages = static_cast<int>(stages < kMaxStages ? stages : kMaxStages);
+      p.grid = static_cast<int>(turns < static_cast<int64_t>(sms) * ctas ? turns : static_cast<int64_t>(sms) * ctas);
+      p.smem = 128 + static_cast<size_t>(stage) * p.stages;
+      // The backward pass joins its groups' sums in the ring's memory.
+      if (backward && groups > 1 && p.smem < 128 + sizeof(float) * threads * kPer) p.smem = 128 + sizeof(float) * threads * kPer;
+      return p;
+    }
+  }
+  p.tpr = threads_per_row(cols, kPer);
+  p.wide = p.tpr == kMaxTPR;
+  if (p.wide) {
+    const int64_t most = 2 * static_cast<int64_t>(sms);
+    p.grid = static_cast<int>(rows < most ? rows : most);
+  } else {
+    const int direct = p.tpr < 256 ? 256 : p.tpr;
+    const int64_t needed = (rows + direct / p.tpr - 1) / (direct / p.tpr);
+    const int64_t most = static_cast<int64_t>(sms) * (768 / direct);
+    p.grid = static_cast<int>(needed < most ? needed : most);
+  }
+  return p;
 }
 
-int backward_parts(int64_t rows, int64_t cols) {
-  if (!is_wide(cols)) return norm_grid(rows, cols);
-  return static_cast<int>(rows < 64 ? rows : 64);
+// Partial sums of a backward pass: one of each CTA, or of each of 64 sets of rows.
+int backward_parts(const Plan& p, int64_t rows) { return p.wide ? static_cast<int>(rows < 64 ? rows : 64) : p.grid; }
+
+std::mutex g_mutex;
+bool g_ready[64][64] = {};
+
+template <int XD, int TPR>
+int launch_ring(bool backward, const Plan& p, int slot, cudaStream_t st, const NormArgs& a) {
+  // The forward kernel's 32 elements a thread need no more than 512 threads, and the
+  // backward kernel's 16 no fewer than 64.
+  auto kernel = backward ? norm_backward_ring_kernel<XD, (TPR < 64 ? 64 : TPR)> : norm_forward_ring_kernel<XD, (TPR > 512 ? 512 : TPR)>;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  if (dev < 0 || dev >= 64) return fail(GNS_ERR_DEVICE, "device index out of range");
+  {
+    std::lock_guard<std::mutex> lock(g_mutex);
+    bool& ready = g_ready[dev][slot + (backward ? 32 : 0)];
+    if (!ready) {
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes + 1024);
+      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(smem)");
+      ready = true;
+    }
+  }
+  kernel<<<p.grid, threads_of<TPR>(), p.smem, st>>>(a, p.stages);
+  return GNS_OK;
 }
 
 template <int XD, int TPR, bool VEC>
-void launch_norm(bool backward, int grid, cudaStream_t st, const NormArgs& a) {
+int launch_direct(bool backward, const Plan& p, cudaStream_t st, const NormArgs& a) {
   if (backward)
-    norm_backward_kernel<XD, TPR, VEC><<<grid, threads_of<TPR>(), 0, st>>>(a);
+    norm_backward_kernel<XD, TPR, VEC><<<p.grid, threads_of<TPR>(), 0, st>>>(a);
   else
-    norm_forward_kernel<XD, TPR, VEC><<<grid, threads_of<TPR>(), 0, st>>>(a);
+    norm_forward_kernel<XD, TPR, VEC><<<p.grid, threads_of<TPR>(), 0, st>>>(a);
+  return GNS_OK;
 }
 
-template <int XD, bool VEC>
-void launch_rows(bool backward, int grid, cudaStream_t st, const NormArgs& a) {
-  switch (threads_per_row(a.cols)) {
-    case 32: return launch_norm<XD, 32, VEC>(backward, grid, st, a);
-    case 64: return launch_norm<XD, 64, VEC>(backward, grid, st, a);
-    case 128: return launch_norm<XD, 128, VEC>(backward, grid, st, a);
-    case 256: return launch_norm<XD, 256, VEC>(backward, grid, st, a);
-    case 512: return launch_norm<XD, 512, VEC>(backward, grid, st, a);
-    default: return launch_norm<XD, 1024, VEC>(backward, grid, st, a);
+template <int XD>
+int launch_type(bool backward, bool vec, const Plan& p, cudaStream_t st, const NormArgs& a) {
+  if (p.stages > 0) {
+    switch (p.tpr) {
+      case 32: return launch_ring<XD, 32>(backward, p, 8 * XD + 5, st, a);
+      case 64: return launch_ring<XD, 64>(backward, p, 8 * XD, st, a);
+      case 128: return launch_ring<XD, 128>(backward, p, 8 * XD + 1, st, a);
+      case 256: return launch_ring<XD, 256>(backward, p, 8 * XD + 2, st, a);
+      case 512: return launch_ring<XD, 512>(backward, p, 8 * XD + 3, st, a);
+      default: return launch_ring<XD, 1024>(backward, p, 8 * XD + 4, st, a);
+    }
+  }
+  if (vec && p.tpr == 32) return launch_direct<XD, 32, true>(backward, p, st, a);
+  switch (p.tpr) {
+    case 32: return launch_direct<XD, 32, false>(backward, p, st, a);
+    case 64: return launch_direct<XD, 64, false>(backward, p, st, a);
+    case 128: return launch_direct<XD, 128, false>(backward, p, st, a);
+    case 256: return launch_direct<XD, 256, false>(backward, p, st, a);
+    default: return launch_direct<XD, 512, false>(backward, p, st, a);
   }
 }
 
-void launch_any(bool backward, bool vec, int x_dt, int grid, cudaStream_t st, const NormArgs& a) {
-  if (x_dt == kBF16)
-    vec ? launch_rows<kBF16, true>(backward, grid, st, a) : launch_rows<kBF16, false>(backward, grid, st, a);
-  else if (x_dt == kF16)
-    vec ? launch_rows<kF16, true>(backward, grid, st, a) : launch_rows<kF16, false>(backward, grid, st, a);
-  else
-    vec ? launch_rows<kF32, true>(backward, grid, st, a) : launch_rows<kF32, false>(backward, grid, st, a);
+int launch_any(bool backward, bool vec, int x_dt, const Plan& p, cudaStream_t st, const NormArgs& a) {
+  if (x_dt == kBF16) return launch_type<kBF16>(backward, vec, p, st, a);
+  if (x_dt == kF16) return launch_type<kF16>(backward, vec, p, st, a);
+  return launch_type<kF32>(backward, vec, p, st, a);
 }
 
 // Rows that 16-byte pieces can be read from: every piece aligned and none past the end.
@@ -463,6 +804,16 @@ int check_norm(int x_dtype, int w_dtype, int64_t rows, int64_t cols, int64_t str
 }
 
 }  // namespace
+
+int norm_status(int* status, int clear) {
+  cudaError_t e = cudaMemcpyFromSymbol(status, g_norm_status, sizeof(int));
+  if (e == cudaSuccess && clear && *status != 0) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_norm_status, &zero, sizeof(int));
+  }
+  return e == cudaSuccess ? GNS_OK : cuda_fail(e, "layer norm status");
+}
+
 }  // namespace gns
 
 using namespace gns;
@@ -493,20 +844,24 @@ int gns_layer_norm_forward(int x_dtype, int w_dtype, int64_t rows, int64_t cols,
   a.cols = static_cast<int>(cols);
   a.w_dt = w_dtype;
   a.eps = eps;
-  if (is_wide(cols)) {
-    const int64_t most = 2 * static_cast<int64_t>(device_sm_count());
-    norm_forward_wide_kernel<<<static_cast<int>(rows < most ? rows : most), kWideThreads, 0, st>>>(a, x_dtype);
-  } else {
-    const bool vec = rows_vector(x, x_rstride, cols, x_dtype) && rows_vector(y, cols, cols, x_dtype);
-    launch_any(false, vec, x_dtype, norm_grid(rows, cols), st, a);
-  }
+  const bool vec = rows_vector(x, x_rstride, cols, x_dtype) && rows_vector(y, cols, cols, x_dtype);
+  const Plan plan = plan_norm(false, vec, x_dtype, rows, cols);
+  if (plan.wide)
+    norm_forward_wide_kernel<<<plan.grid, kWideThreads, 0, st>>>(a, x_dtype);
+  else
+    rc = launch_any(false, vec, x_dtype, plan, st, a);
+  if (rc != GNS_OK) return rc;
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? GNS_OK : cuda_fail(e, "layer norm forward kernel");
 }
 
 size_t gns_layer_norm_backward_workspace_size(int64_t rows, int64_t cols) {
   if (rows < 1 || cols < 1) return 0;
-  return static_cast<size_t>(backward_parts(rows, cols)) * 2 * static_cast<size_t>(cols) * sizeof(float);
+  // The most that any type and alignment takes.
+  int parts = 0;
+  for (int dt : {kF16, kF32})
+    for (bool vec : {false, true}) parts = std::max(parts, backward_parts(plan_norm(true, vec, dt, rows, cols), rows));
+  return static_cast<size_t>(parts) * 2 * static_cast<size_t>(cols) * sizeof(float);
 }
 
 int gns_layer_norm_backward(int x_dtype, int w_dtype, int64_t rows, int64_t cols, const void* grad, int64_t grad_rstride,
@@ -541,17 +896,18 @@ int gns_layer_norm_backward(int x_dtype, int w_dtype, int64_t rows, int64_t cols
   a.rows = rows;
   a.cols = static_cast<int>(cols);
   a.w_dt = w_dtype;
-  a.parts = rows > 0 ? backward_parts(rows, cols) : 0;
   if (rows > 0) {
-    if (is_wide(cols)) {
-      const int64_t most = 2 * static_cast<int64_t>(device_sm_count());
-      norm_backward_wide_kernel<<<static_cast<int>(rows < most ? rows : most), kWideThreads, 0, st>>>(a, x_dtype);
+    const bool vec = rows_vector(x, x_rstride, cols, x_dtype) && rows_vector(grad, grad_rstride, cols, x_dtype) &&
+                     rows_vector(dx, cols, cols, x_dtype);
+    const Plan plan = plan_norm(true, vec, x_dtype, rows, cols);
+    a.parts = backward_parts(plan, rows);
+    if (plan.wide) {
+      norm_backward_wide_kernel<<<plan.grid, kWideThreads, 0, st>>>(a, x_dtype);
       const dim3 grid(static_cast<unsigned>((cols + kColThreads - 1) / kColThreads), static_cast<unsigned>(a.parts));
       norm_columns_wide_kernel<<<grid, kColThreads, 0, st>>>(a, x_dtype);
     } else {
-      const bool vec = rows_vector(x, x_rstride, cols, x_dtype) && rows_vector(grad, grad_rstride, cols, x_dtype) &&
-                       rows_vector(dx, cols, cols, x_dtype);
-      launch_any(true, vec, x_dtype, a.parts, st, a);
+      rc = launch_any(true, vec, x_dtype, plan, st, a);
+      if (rc != GNS_OK) return rc;
     }
   }
   const int join = static_cast<int>((2 * cols + 31) / 32);

@@ -12,6 +12,7 @@ import contextlib
 import ctypes
 import os
 from collections.abc import Iterator, Sequence
+from typing import cast
 
 import torch
 from torch import Tensor
@@ -993,55 +994,56 @@ class AdamWStates:
             raise ValueError(f"betas must be in [0, 1), got {(beta1, beta2)}")
         if not epsilon > 0.0:
             raise ValueError(f"epsilon must be positive, got {epsilon}")
-        if count == 0:
+        present = [i for i, g in enumerate(gradients) if g is not None]
+        if not present:
             return
-        g_dtype = None
-        numel = (ctypes.c_int64 * count)()
-        pointers = (ctypes.c_void_p * count)()
-        places = (ctypes.c_void_p * count)()
-        for i, (g, p) in enumerate(zip(gradients, self.parameters, strict=True)):
-            if g is None:
-                continue
-            if g_dtype is None:
-                g_dtype = g.dtype
-            elif g.dtype != g_dtype:
-                raise TypeError("all gradients of one call must share a dtype")
-            n = self._numel[i]
-            if g.numel() != n:
-                raise ValueError("gradient and parameter sizes differ")
-            if not (g.is_contiguous() and p.is_contiguous()):
-                raise ValueError("gradients and parameters must be contiguous")
-            if g.device != self.device:
-                raise ValueError("gradients must be on the parameters' device")
-            numel[i] = n
-            pointers[i] = g.data_ptr()
-            places[i] = p.data_ptr()
-        if g_dtype is None:
-            return
+        whole = len(present) == count
+        given = cast(Sequence[Tensor], gradients) if whole else [cast(Tensor, gradients[i]) for i in present]
+        places = self.parameters if whole else [self.parameters[i] for i in present]
+        g_dtype = given[0].dtype
+        if any(g.dtype != g_dtype for g in given):
+            raise TypeError("all gradients of one call must share a dtype")
+        numel = [g.numel() for g in given]
+        if numel != (self._numel if whole else [self._numel[i] for i in present]):
+            raise ValueError("gradient and parameter sizes differ")
+        if not (all(map(Tensor.is_contiguous, given)) and all(map(Tensor.is_contiguous, places))):
+            raise ValueError("gradients and parameters must be contiguous")
+        index = cast(torch.device, self.device).index
+        if any(g.get_device() != index for g in given) or any(p.get_device() != index for p in places):
+            raise ValueError("gradients must be on the parameters' device")
         if gradient_scale is not None:
             if gradient_scale.dtype != torch.float32 or gradient_scale.numel() != 1:
                 raise ValueError("gradient_scale must be one float32 value")
-            if gradient_scale.device != self.device:
+            if gradient_scale.get_device() != index:
                 raise ValueError("gradient_scale must be on the parameters' device")
-        steps = [step] * count if isinstance(step, (int, float)) else list(step)
-        if len(steps) != count:
-            raise ValueError("step must be one value or one for each parameter")
-        lr_bc1, inv_bc2 = (ctypes.c_float * count)(), (ctypes.c_float * count)()
-        known: dict[float, tuple[float, float]] = {}
-        for i, t in enumerate(steps):
-            if t not in known:
-                if t < 1:
-                    raise ValueError(f"steps count from 1, got {t}")
-                known[t] = (learning_rate / (1 - beta1**t), (1 - beta2**t) ** -0.5)
-            lr_bc1[i], inv_bc2[i] = known[t]
+        floats = ctypes.c_float * len(present)
+        if isinstance(step, (int, float)):
+            lr_bc1, inv_bc2 = self._bias_corrections(step, learning_rate, beta1, beta2)
+            corrections = floats(*[lr_bc1] * len(present)), floats(*[inv_bc2] * len(present))
+        else:
+            if len(step) != count:
+                raise ValueError("step must be one value or one for each parameter")
+            pairs = [self._bias_corrections(step[i], learning_rate, beta1, beta2) for i in present]
+            corrections = floats(*[a for a, _ in pairs]), floats(*[b for _, b in pairs])
+        states = self._states
+        if not whole:
+            roles = (self.exp_avgs, self.exp_avg_sqs, self.exp_avg_scales, self.exp_avg_sq_scales)
+            states = tuple(_ptr_array([role[i] for i in present]) if role else None for role in roles)
         lib = nat.load()
-        with torch.cuda.device(self.device):
+        with nat.on_device(index) as stream:
             rc = lib.gns_adamw_states_step(
-                count, places, pointers, *self._states, numel, nat.dtype_code(self.parameters[0].dtype),
-                nat.dtype_code(g_dtype), self.bits, lr_bc1, inv_bc2, beta1, 1 - beta1, beta2, 1 - beta2, epsilon,
-                1 - learning_rate * weight_decay, nat.ptr(gradient_scale), nat.stream_handle(self.device),
+                len(present), _ptr_array(places), _ptr_array(given), *states, (ctypes.c_int64 * len(present))(*numel),
+                nat.dtype_code(places[0].dtype), nat.dtype_code(g_dtype), self.bits, *corrections,
+                beta1, 1 - beta1, beta2, 1 - beta2, epsilon, 1 - learning_rate * weight_decay,
+                nat.ptr(gradient_scale), stream,
             )
         nat.check(rc, "gns_adamw_states_step")
+
+    @staticmethod
+    def _bias_corrections(step: float, learning_rate: float, beta1: float, beta2: float) -> tuple[float, float]:
+        if step < 1:
+            raise ValueError(f"steps count from 1, got {step}")
+        return learning_rate / (1 - beta1**step), (1 - beta2**step) ** -0.5
 
 
 # ------------------------------------------------- products grouped by expert
@@ -1104,11 +1106,11 @@ def grouped_gemm(left: Tensor, right: Tensor, ends: Tensor, out_dtype: torch.dty
         right = right.contiguous()  # a TMA map has no zero strides
     b = _aligned_operand(right)
     lib = nat.load()
-    with torch.cuda.device(device):
+    with nat.on_device(device.index) as stream:
         rc = lib.gns_grouped_gemm(
             nat.dtype_code(a.dtype), rows, n, k, groups, a.data_ptr(), a.stride(0),
             b.data_ptr(), b.stride(0), b.stride(1), b.stride(2), ends.data_ptr(), 8 * ends.element_size(),
-            out.data_ptr(), code, out.stride(0), nat.stream_handle(device),
+            out.data_ptr(), code, out.stride(0), stream,
         )
     nat.check(rc, "gns_grouped_gemm")
     return out
@@ -1137,11 +1139,11 @@ def grouped_gemm_reduce(left: Tensor, right: Tensor, ends: Tensor, out_dtype: to
     a, b = _row_operand(left), _row_operand(right)
     lib = nat.load()
     ws = _workspace(lib.gns_grouped_gemm_reduce_workspace_size(groups), device)
-    with torch.cuda.device(device):
+    with nat.on_device(device.index) as stream:
         rc = lib.gns_grouped_gemm_reduce(
             nat.dtype_code(a.dtype), rows, m, n, groups, a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0),
             ends.data_ptr(), 8 * ends.element_size(), out.data_ptr(), code, out.stride(0), out.stride(1),
-            ws.data_ptr(), ws.numel(), nat.stream_handle(device),
+            ws.data_ptr(), ws.numel(), stream,
         )
     nat.check(rc, "gns_grouped_gemm_reduce")
     return out
@@ -1150,7 +1152,7 @@ def grouped_gemm_reduce(left: Tensor, right: Tensor, ends: Tensor, out_dtype: to
 # ------------------------------------------------------------------ layer norm
 def _norm_rows(t: Tensor, columns: int) -> Tensor:
     """[rows, columns] view of `t` with unit column stride and rows that do not overlap."""
-    flat = t.reshape(-1, columns)
+    flat = t if t.ndim == 2 else t.reshape(-1, columns)
     if columns > 1 and flat.stride(1) != 1 or flat.shape[0] > 1 and flat.stride(0) < columns:
         flat = flat.contiguous()
     return flat
@@ -1180,19 +1182,20 @@ def layer_norm(x: Tensor, weight: Tensor, bias: Tensor | None, epsilon: float) -
     columns = _norm_check(x, weight, bias)
     flat = _norm_rows(x, columns)
     rows = flat.shape[0]
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
-    stats = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=device)
+    rstd = torch.empty_like(mean)
     w = weight.contiguous()
     b = bias.contiguous() if bias is not None else None
     lib = nat.load()
-    with torch.cuda.device(device):
+    with nat.on_device(device.index) as stream:
         rc = lib.gns_layer_norm_forward(
             nat.dtype_code(x.dtype), nat.dtype_code(w.dtype), rows, columns, flat.data_ptr(), flat.stride(0),
-            w.data_ptr(), nat.ptr(b), float(epsilon), y.data_ptr(), stats[0].data_ptr(), stats[1].data_ptr(),
-            nat.stream_handle(device),
+            w.data_ptr(), nat.ptr(b), float(epsilon), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+            stream,
         )
     nat.check(rc, "gns_layer_norm_forward")
-    return y, stats[0], stats[1]
+    return y, mean, rstd
 
 
 def layer_norm_backward(
@@ -1213,15 +1216,15 @@ def layer_norm_backward(
             raise ValueError("mean and rstd must be contiguous float32 with one entry per row")
     flat, g = _norm_rows(x, columns), _norm_rows(grad, columns)
     w = weight.contiguous()
-    dx = torch.empty(x.shape, dtype=x.dtype, device=device)
-    sums = torch.empty((2, columns), dtype=weight.dtype, device=device)
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    dweight, dbias = torch.empty_like(w), torch.empty_like(w)
     lib = nat.load()
     ws = _workspace(lib.gns_layer_norm_backward_workspace_size(rows, columns), device)
-    with torch.cuda.device(device):
+    with nat.on_device(device.index) as stream:
         rc = lib.gns_layer_norm_backward(
             nat.dtype_code(x.dtype), nat.dtype_code(w.dtype), rows, columns, g.data_ptr(), g.stride(0),
             flat.data_ptr(), flat.stride(0), w.data_ptr(), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(),
-            sums[0].data_ptr(), sums[1].data_ptr(), ws.data_ptr(), ws.numel(), nat.stream_handle(device),
+            dweight.data_ptr(), dbias.data_ptr(), ws.data_ptr(), ws.numel(), stream,
         )
     nat.check(rc, "gns_layer_norm_backward")
-    return dx, sums[0], sums[1]
+    return dx, dweight, dbias
