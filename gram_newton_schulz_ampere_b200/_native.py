@@ -147,10 +147,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [c_int, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _I64, _I64, _P, c_int, _P, c_int, _I64, _P],
     ),
-    "gns_grouped_gemm_reduce_workspace_size": (c_size_t, [_I64]),
     "gns_grouped_gemm_reduce": (
         c_int,
-        [c_int, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _P, c_int, _P, c_int, _I64, _I64, _P, c_size_t, _P],
+        [c_int, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _P, c_int, _P, c_int, _I64, _I64, _P],
     ),
     "gns_layer_norm_forward": (
         c_int,

@@ -203,21 +203,19 @@ __device__ __forceinline__ float block_max(const float (&f)[8]) {
   return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top) & 0x7fffffffu));
 }
 
+// 448 / top for the codes of a block; 0 for a block that is held as zeros. Correctly
+// rounded, as the moments are: a code that is rounded the other way moves by 6%, so
+// all that leads to it is kept free of choices.
 __device__ __forceinline__ float inverse_scale(float top) {
-  return top <= kFlushBelow ? 0.0f : kE4M3Max * reciprocal_approx(top);
+  return top <= kFlushBelow ? 0.0f : __fmul_rn(kE4M3Max, __frcp_rn(top));
 }
 
 // Per-launch constants of one tensor.
 struct Step {
-  float g_to_m, g_to_v, lr_bc1, inv_bc2;
+  float scale, lr_bc1, inv_bc2;
 
-  __device__ __forceinline__ Step(const StateArgs& a, const StateScalars& k, int t) {
-    const float scale = k.grad_scale != nullptr ? *k.grad_scale : 1.0f;
-    g_to_m = k.one_minus_beta1 * scale;
-    g_to_v = sqrtf(k.one_minus_beta2) * scale;
-    lr_bc1 = a.lr_bc1[t];
-    inv_bc2 = a.inv_bc2[t];
-  }
+  __device__ __forceinline__ Step(const StateArgs& a, const StateScalars& k, int t)
+      : scale(k.grad_scale != nullptr ? *k.grad_scale : 1.0f), lr_bc1(a.lr_bc1[t]), inv_bc2(a.inv_bc2[t]) {}
 };
 
 // New moments and parameter of a lane's 8 elements of a block, the moments' codes and
@@ -227,18 +225,18 @@ __device__ __forceinline__ void step_eight(const float (&gf)[8], float (&pf)[8],
   float mf[8], vf[8];
   decode8(mc, mf);
   decode8(vc, vf);
-  // The codes are scaled and decayed by one factor a block, and the gradient's
-  // factors are the launch's: (1 - b1) s for m, sqrt(1 - b2) s before the square for v.
-  const float old_m = ms * k.beta1, old_v = vs * k.beta2;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float root = gf[e] * s.g_to_v;
-    mf[e] = fmaf(gf[e], s.g_to_m, mf[e] * old_m);
-    vf[e] = fmaf(root, root, vf[e] * old_v);
+    // Every product and sum of the moments is rounded by itself (no fma).
+    const float g = gf[e] * s.scale;
+    mf[e] = __fadd_rn(__fmul_rn(__fmul_rn(mf[e], ms), k.beta1), __fmul_rn(g, k.one_minus_beta1));
+    vf[e] = __fadd_rn(__fmul_rn(__fmul_rn(vf[e], vs), k.beta2), __fmul_rn(__fmul_rn(g, g), k.one_minus_beta2));
     pf[e] = adamw_update(pf[e], mf[e], vf[e], k, s.lr_bc1, s.inv_bc2);
   }
   const float m_top = block_max(mf), v_top = block_max(vf);
-  const float m_inv = inverse_scale(m_top), v_inv = inverse_scale(v_top);
+  // One lane in two works out the inverse for m, the other for v.
+  const float inverse = inverse_scale((threadIdx.x & 1) ? v_top : m_top);
+  const float m_inv = __shfl_sync(0xffffffffu, inverse, 0), v_inv = __shfl_sync(0xffffffffu, inverse, 1);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     mf[e] *= m_inv;

@@ -22,11 +22,14 @@
 // fill other columns of the accumulator, which are not stored.
 //
 // Reduced product: the rows are the contraction, so rows of other groups must not
-// enter. Each group gets its own tensor maps (written by a small kernel) whose row
-// extent ends with the group; TMA fills zeros behind it.
+// enter. A group's last 64 rows may reach into the next group: only the 16-row steps
+// with rows of the group are multiplied, and the foreign rows of the last step are
+// zeroed in shared memory (in both operands: a NaN times zero is a NaN) by a warp
+// of its own between the loads and the MMA.
 //
 // Sums are fp32 in TMEM, rounded once at the store. Every wait is bounded.
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 #include <string>
 
@@ -90,6 +93,86 @@ __device__ __forceinline__ Cut cut_group(int rows, int tile, int unit) {
   return {(rows + size - 1) / size, size};
 }
 
+// The groups as a CTA works through them, in shared memory: place i holds group
+// order[i], whose tiles follow first_tile[i]. Groups with costly tiles come first.
+// The tiles are dealt to the CTAs of a persistent grid in turn, so the sums of the
+// shares differ by less than one tile, and the tiles of the last, partial turn are
+// the cheap ones. (In the groups' own order the busiest CTA pair of a ragged batch
+// had about a quarter more than the mean.)
+struct Table {
+  int* first_row;   // [count + 1], by group
+  int* first_tile;  // [count + 1], by place
+  uint16_t* order;  // [count], by place
+  static constexpr uint32_t kBytes = 2 * (kMaxGroups + 1) * 4 + kMaxGroups * 2;
+
+  __device__ __forceinline__ explicit Table(uint8_t* at)
+      : first_row(reinterpret_cast<int*>(at)),
+        first_tile(first_row + kMaxGroups + 1),
+        order(reinterpret_cast<uint16_t*>(first_tile + kMaxGroups + 1)) {}
+};
+
+// One warp fills the table. cost(rows) is the cost of a group's tiles, in [0, 31];
+// tiles(rows) their number. A counting sort: the groups of each cost are counted,
+// then placed behind the costlier ones. `counts` is 32 integers of shared memory.
+template <class Cost, class Tiles>
+__device__ __forceinline__ void fill_table(const Table& table, int* counts, const Groups& groups, int lane, Cost cost,
+                                           Tiles tiles) {
+  counts[lane] = 0;
+  __syncwarp();
+  int carry = 0;
+  for (int base = 0; base < groups.count; base += 32) {
+    const int e = base + lane;
+    int begin, end;
+    group_rows(groups, e, lane, carry, begin, end);
+    if (e < groups.count) table.first_row[e] = begin;
+    const int c = e < groups.count ? cost(end - begin) : 32;
+    const uint32_t same = __match_any_sync(0xffffffffu, c);
+    if (c < 32 && lane == __ffs(same) - 1) counts[c] += __popc(same);
+    __syncwarp();
+  }
+  if (lane == 0) table.first_row[groups.count] = carry;
+  // Place of the next group of cost `lane`: behind all costlier ones.
+  const int with_cost = counts[lane];
+  int place = with_cost;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int other = __shfl_down_sync(0xffffffffu, place, o);
+    if (lane + o < 32) place += other;
+  }
+  counts[lane] = place - with_cost;
+  __syncwarp();
+  for (int base = 0; base < groups.count; base += 32) {
+    const int e = base + lane;
+    const int c = e < groups.count ? cost(table.first_row[e + 1] - table.first_row[e]) : 32;
+    const uint32_t same = __match_any_sync(0xffffffffu, c);
+    const int at = c < 32 ? counts[c] : 0;
+    __syncwarp();
+    if (c < 32) {
+      table.order[at + __popc(same & ((1u << lane) - 1u))] = static_cast<uint16_t>(e);
+      if (lane == __ffs(same) - 1) counts[c] = at + __popc(same);
+    }
+    __syncwarp();
+  }
+  int before = 0;
+  for (int base = 0; base < groups.count; base += 32) {
+    const int i = base + lane;
+    int n = 0;
+    if (i < groups.count) {
+      const int e = table.order[i];
+      n = tiles(table.first_row[e + 1] - table.first_row[e]);
+    }
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += other;
+    }
+    if (i < groups.count) table.first_tile[i] = before + sum - n;
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  if (lane == 0) table.first_tile[groups.count] = before;
+}
+
 struct Output {
   void* d;
   int64_t ldd, bstride;
@@ -150,23 +233,26 @@ struct Barriers {
   uint64_t* empty;
   uint64_t* tfull;
   uint64_t* tempty;
+  uint64_t* tail;  // reduced product: a stage whose rows end inside it has landed in this CTA
   uint32_t* tmem_slot;
   volatile int* abort_flag;
-  static constexpr uint32_t kBytes = (2 * S + 4) * 8 + 16;
+  static constexpr uint32_t kBytes = (3 * S + 4) * 8 + 8;
 
   __device__ __forceinline__ explicit Barriers(uint8_t* at) {
     full = reinterpret_cast<uint64_t*>(at);
     empty = full + S;
     tfull = full + 2 * S;
     tempty = full + 2 * S + 2;
-    tmem_slot = reinterpret_cast<uint32_t*>(full + 2 * S + 4);
+    tail = full + 2 * S + 4;
+    tmem_slot = reinterpret_cast<uint32_t*>(tail + S);
     abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   }
 
-  __device__ __forceinline__ void init() {
+  __device__ __forceinline__ void init(uint32_t full_arrivals) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], full_arrivals);
       mbar_init(&empty[s], 1);
+      mbar_init(&tail[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
@@ -189,8 +275,9 @@ __device__ __forceinline__ void meet() {
 // Set-up common to both kernels: barriers, TMEM, and the wait for the stream's
 // previous kernel. Returns the TMEM base.
 template <int S, bool PAIR>
-__device__ __forceinline__ uint32_t set_up(const Barriers<S, PAIR>& bar, int warp, uint32_t tmem_cols) {
-  if (threadIdx.x == 0) const_cast<Barriers<S, PAIR>&>(bar).init();
+__device__ __forceinline__ uint32_t set_up(const Barriers<S, PAIR>& bar, int warp, uint32_t tmem_cols,
+                                           uint32_t full_arrivals = 1) {
+  if (threadIdx.x == 0) const_cast<Barriers<S, PAIR>&>(bar).init(full_arrivals);
   if (warp == 1) {
     if (PAIR) {
       tmem_alloc_pair(bar.tmem_slot, tmem_cols);
@@ -206,6 +293,21 @@ __device__ __forceinline__ uint32_t set_up(const Barriers<S, PAIR>& bar, int war
   pdl_launch_dependents();
   pdl_wait_predecessor();
   return *bar.tmem_slot;
+}
+
+// The producer's end: it waits until every stage it filled has been released. In a
+// pair the releases of CTA 1's stages are arrivals that CTA 0's MMAs send when they
+// complete; none may be on its way when the CTA leaves and its shared memory goes to
+// another.
+template <int S, bool PAIR>
+__device__ __forceinline__ void drain(const Barriers<S, PAIR>& bar, int st, uint32_t ph, bool ok) {
+  for (int i = 0; i < S && ok; ++i) {
+    ok = mbar_wait_bounded(&bar.empty[st], ph ^ 1u, bar.abort_flag, &g_grouped_status, kStatusProducerTimeout);
+    if (++st == S) {
+      st = 0;
+      ph ^= 1u;
+    }
+  }
 }
 
 // Teardown: all roles meet; after an abort, copies and MMAs in flight get time to
@@ -232,18 +334,29 @@ struct RowsShape {
   int n, k_blocks, feature_tiles;
 };
 
+// Maps of the row operand with boxes of 32, 64, 96 and 128 rows: a part of any
+// width comes with one copy a stage (several small boxes instead cost up to 8%).
+struct RowMaps {
+  CUtensorMap box[4];
+};
+
+// A tile's rows lie in one or two units of at most 256 columns of the accumulator,
+// and the unit buffers are used in turn. TOK = 512: both units of a tile share the
+// loads of the expert's columns.
 template <int TOK, bool OUT_F32, bool PAIR>
 struct RowsConfig {
-  static constexpr int kStages = (PAIR ? 6 : 8) - (OUT_F32 ? 1 : 0);
-  static constexpr int kFeatures = PAIR ? 2 * kBM : kBM;   // features of a tile
-  static constexpr int kTokRows = PAIR ? TOK / 2 : TOK;    // rows that one CTA loads, at most
-  static constexpr int kUnit = PAIR ? 32 : 16;             // granularity of N
-  static constexpr uint32_t kTokBytes = kTokRows * kBK * 2;
-  static constexpr uint32_t kStageBytes = kMBytes + kTokBytes;
+  static constexpr int kUnits = TOK > 256 ? 2 : 1;
+  static constexpr int kUnitCols = TOK / kUnits;
+  static constexpr int kFeatures = PAIR ? 2 * kBM : kBM;             // features of a tile
+  static constexpr int kUnitRows = PAIR ? kUnitCols / 2 : kUnitCols;  // rows of a unit that one CTA loads, at most
+  static constexpr int kGrain = PAIR ? 32 : 16;                       // granularity of N
+  static constexpr uint32_t kUnitBytes = kUnitRows * kBK * 2;
+  static constexpr uint32_t kStageBytes = kMBytes + kUnits * kUnitBytes;
+  static constexpr int kStages = 6 * 32768 / kStageBytes - (OUT_F32 ? 1 : 0);
   static constexpr uint32_t kSlotBytes = 32 * (OUT_F32 ? 128 : 64);
-  static constexpr uint32_t kTmemCols = 2 * TOK;
-  static constexpr size_t kSmemBytes = 1024 + kStages * kStageBytes + kEpiWarps * kSlotBytes +
-                                       2 * (kMaxGroups + 1) * 4 + 8 + Barriers<kStages, PAIR>::kBytes;
+  static constexpr uint32_t kTmemCols = 2 * kUnitCols;
+  static constexpr size_t kSmemBytes = 1024 + kStages * kStageBytes + kEpiWarps * kSlotBytes + Table::kBytes +
+                                       Barriers<kStages, PAIR>::kBytes;
 };
 
 // A tile: `rows` rows from `row0` of group e, feature tile `f`.
@@ -251,14 +364,14 @@ struct RowsTile {
   int e, row0, rows, f;
 };
 
-template <int TOK, int UNIT>
-__device__ __forceinline__ RowsTile rows_tile(const int* first_tile, const int* first_row, int t, int& e) {
-  while (t >= first_tile[e + 1]) ++e;
-  const int begin = first_row[e], rows = first_row[e + 1] - begin;
-  const Cut cut = cut_group(rows, TOK, UNIT);
-  const int l = t - first_tile[e];
+template <int TOK, int GRAIN>
+__device__ __forceinline__ RowsTile rows_tile(const Table& table, int t, int& place) {
+  while (t >= table.first_tile[place + 1]) ++place;
   RowsTile tile;
-  tile.e = e;
+  tile.e = table.order[place];
+  const int begin = table.first_row[tile.e], rows = table.first_row[tile.e + 1] - begin;
+  const Cut cut = cut_group(rows, TOK, GRAIN);
+  const int l = t - table.first_tile[place];
   tile.f = l / cut.parts;  // a group's row parts are neighbours: they share the expert's columns in L2
   const int part = l - tile.f * cut.parts;
   tile.row0 = begin + part * cut.size;
@@ -266,11 +379,24 @@ __device__ __forceinline__ RowsTile rows_tile(const int* first_tile, const int* 
   return tile;
 }
 
+// Rows of the tile's first unit: all of them if a unit holds them, else half (an
+// MMA of a narrow remainder would wait for its other operand's shared memory reads).
+template <class Cfg>
+__device__ __forceinline__ int first_unit(const RowsTile& tile) {
+  if (tile.rows <= Cfg::kUnitCols) return tile.rows;
+  return ((tile.rows + 1) / 2 + Cfg::kGrain - 1) / Cfg::kGrain * Cfg::kGrain;
+}
+
+// N of the MMA for `rows` rows.
+template <class Cfg>
+__device__ __forceinline__ int mma_width(int rows) {
+  return (rows + Cfg::kGrain - 1) / Cfg::kGrain * Cfg::kGrain;
+}
+
 template <bool F_MN, int TOK, bool OUT_F32, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
-    grouped_rows_kernel(const __grid_constant__ CUtensorMap map_right, const __grid_constant__ CUtensorMap map_full,
-                        const __grid_constant__ CUtensorMap map_part, const Groups groups, const RowsShape shape,
-                        const Output out, const int ab_bf16) {
+    grouped_rows_kernel(const __grid_constant__ CUtensorMap map_right, const __grid_constant__ RowMaps map_rows,
+                        const Groups groups, const RowsShape shape, const Output out, const int ab_bf16) {
   using Cfg = RowsConfig<TOK, OUT_F32, PAIR>;
   constexpr int S = Cfg::kStages;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
@@ -285,54 +411,40 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem_n = smem + S * kMBytes;
   uint8_t* smem_epi = smem + S * Cfg::kStageBytes;
   const Barriers<S, PAIR> bar(smem_epi + kEpiWarps * Cfg::kSlotBytes);
-  int* first_tile = reinterpret_cast<int*>(smem_epi + kEpiWarps * Cfg::kSlotBytes + Barriers<S, PAIR>::kBytes);
-  int* first_row = first_tile + kMaxGroups + 1;
+  const Table table(smem_epi + kEpiWarps * Cfg::kSlotBytes + Barriers<S, PAIR>::kBytes);
 
   const uint32_t tmem_base = set_up<S, PAIR>(bar, warp, Cfg::kTmemCols);
 
-  // Tiles and rows before each group.
-  if (warp == 0) {
-    int row_carry = 0, tile_carry = 0;
-    for (int base = 0; base < groups.count; base += 32) {
-      const int e = base + lane;
-      int begin, end;
-      group_rows(groups, e, lane, row_carry, begin, end);
-      const int tiles = cut_group(end - begin, TOK, Cfg::kUnit).parts * shape.feature_tiles;
-      int sum = tiles;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int other = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += other;
-      }
-      if (e < groups.count) {
-        first_row[e] = begin;
-        first_tile[e] = tile_carry + sum - tiles;
-      }
-      tile_carry += __shfl_sync(0xffffffffu, sum, 31);
-    }
-    if (lane == 0) {
-      first_row[groups.count] = row_carry;
-      first_tile[groups.count] = tile_carry;
-    }
-  }
+  // A tile's cost is its rows.
+  if (warp == 0)
+    fill_table(
+        table, reinterpret_cast<int*>(smem_epi), groups, lane,
+        [](int rows) { return (cut_group(rows, TOK, Cfg::kGrain).size * 31) / TOK; },
+        [&](int rows) { return cut_group(rows, TOK, Cfg::kGrain).parts * shape.feature_tiles; });
   __syncthreads();
-  const int tiles = first_tile[groups.count];
+  const int tiles = table.first_tile[groups.count];
 
   if (warp == 0) {
     if (lane == 0) {
-      int st = 0, e = 0;
+      int st = 0, place = 0;
       uint32_t ph = 0;
       bool ok = true;
       const uint32_t full0 = PAIR ? cluster_addr(&bar.full[0], 0) : 0u;
       for (int t = tile_begin; t < tiles && ok; t += tile_step) {
-        const RowsTile tile = rows_tile<TOK, Cfg::kUnit>(first_tile, first_row, t, e);
-        const int width = (tile.rows + Cfg::kUnit - 1) / Cfg::kUnit * Cfg::kUnit;  // N of the MMA
-        const int mine = PAIR ? width / 2 : width;                                  // rows this CTA loads
-        const int row0 = tile.row0 + static_cast<int>(rank) * mine;
+        const RowsTile tile = rows_tile<TOK, Cfg::kGrain>(table, t, place);
         const int f0 = tile.f * Cfg::kFeatures + static_cast<int>(rank) * kBM;
-        const bool whole = mine == Cfg::kTokRows;
-        const int boxes = (mine + 31) / 32;
-        const uint32_t bytes = kMBytes + (whole ? Cfg::kTokBytes : static_cast<uint32_t>(boxes) * 32u * kBK * 2u);
+        const int split = first_unit<Cfg>(tile);
+        // This CTA's rows of each unit, and the smallest box that holds them.
+        int row[2], box[2];
+        uint32_t bytes = kMBytes;
+#pragma unroll
+        for (int u = 0; u < Cfg::kUnits; ++u) {
+          const int width = mma_width<Cfg>(u == 0 ? split : tile.rows - split);
+          const int mine = PAIR ? width / 2 : width;
+          row[u] = tile.row0 + u * split + static_cast<int>(rank) * mine;
+          box[u] = (mine + 31) / 32;
+          bytes += static_cast<uint32_t>(box[u]) * 32u * kBK * 2u;
+        }
         for (int kb = 0; kb < shape.k_blocks; ++kb) {
           if (!mbar_wait_bounded(&bar.empty[st], ph ^ 1u, bar.abort_flag, &g_grouped_status, kStatusProducerTimeout)) {
             ok = false;
@@ -340,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           const int k0 = kb * kBK;
           uint8_t* sm = smem_m + st * kMBytes;
-          uint8_t* sn = smem_n + st * Cfg::kTokBytes;
+          uint8_t* sn = smem_n + st * Cfg::kUnits * Cfg::kUnitBytes;
           if (PAIR) {
             if (rank == 0) mbar_arrive_expect_tx(&bar.full[st], 2 * bytes);
             const uint32_t fb = full0 + static_cast<uint32_t>(st) * 8u;
@@ -350,10 +462,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int c = 0; c < kBM / 64; ++c) tma_load_3d_pair(sm + c * 8192, &map_right, fb, f0 + 64 * c, k0, tile.e);
             }
-            if (whole)
-              tma_load_3d_pair(sn, &map_full, fb, k0, row0, 0);
-            else
-              for (int c = 0; c < boxes; ++c) tma_load_3d_pair(sn + c * 4096, &map_part, fb, k0, row0 + 32 * c, 0);
+#pragma unroll
+            for (int u = 0; u < Cfg::kUnits; ++u)
+              if (box[u] > 0)
+                tma_load_3d_pair(sn + u * Cfg::kUnitBytes, &map_rows.box[box[u] - 1], fb, k0, row[u], 0);
           } else {
             mbar_arrive_expect_tx(&bar.full[st], bytes);
             if (!F_MN) {
@@ -362,10 +474,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int c = 0; c < kBM / 64; ++c) tma_load_3d(sm + c * 8192, &map_right, &bar.full[st], f0 + 64 * c, k0, tile.e);
             }
-            if (whole)
-              tma_load_3d(sn, &map_full, &bar.full[st], k0, row0, 0);
-            else
-              for (int c = 0; c < boxes; ++c) tma_load_3d(sn + c * 4096, &map_part, &bar.full[st], k0, row0 + 32 * c, 0);
+#pragma unroll
+            for (int u = 0; u < Cfg::kUnits; ++u)
+              if (box[u] > 0)
+                tma_load_3d(sn + u * Cfg::kUnitBytes, &map_rows.box[box[u] - 1], &bar.full[st], k0, row[u], 0);
           }
           if (++st == S) {
             st = 0;
@@ -373,6 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
+      drain<S, PAIR>(bar, st, ph, ok);
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
@@ -382,16 +495,35 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t empty1 = PAIR ? cluster_addr(&bar.empty[0], 1) : 0u;
       const uint32_t tfull0 = PAIR ? cluster_addr(&bar.tfull[0], 0) : 0u;
       const uint32_t tfull1 = PAIR ? cluster_addr(&bar.tfull[0], 1) : 0u;
-      int st = 0, e = 0, acc = 0;
+      auto hand_over = [&](int b) {
+        if (PAIR) {
+          tc_commit_pair(tfull0 + static_cast<uint32_t>(b) * 8u);
+          tc_commit_pair(tfull1 + static_cast<uint32_t>(b) * 8u);
+        } else {
+          tc_commit(&bar.tfull[b]);
+        }
+      };
+      int st = 0, place = 0, acc = 0;
       uint32_t ph = 0, acc_ph = 0;
       bool ok = true;
       for (int t = tile_begin; t < tiles && ok; t += tile_step) {
-        const RowsTile tile = rows_tile<TOK, Cfg::kUnit>(first_tile, first_row, t, e);
-        const int width = (tile.rows + Cfg::kUnit - 1) / Cfg::kUnit * Cfg::kUnit;
-        const uint32_t idesc = make_idesc_f16(ab_bf16, F_MN ? 1 : 0, 0, Cfg::kFeatures, width);
-        if (!mbar_wait_bounded(&bar.tempty[acc], acc_ph ^ 1u, bar.abort_flag, &g_grouped_status, kStatusMmaTimeout)) break;
+        const RowsTile tile = rows_tile<TOK, Cfg::kGrain>(table, t, place);
+        const int split = first_unit<Cfg>(tile);
+        int units = 0, buffer[2];
+        uint32_t idesc[2];
+#pragma unroll
+        for (int u = 0; u < Cfg::kUnits; ++u) {
+          const int width = mma_width<Cfg>(u == 0 ? split : tile.rows - split);
+          if (width == 0 || !ok) continue;
+          idesc[u] = make_idesc_f16(ab_bf16, F_MN ? 1 : 0, 0, Cfg::kFeatures, width);
+          ok = mbar_wait_bounded(&bar.tempty[acc], acc_ph ^ 1u, bar.abort_flag, &g_grouped_status, kStatusMmaTimeout);
+          buffer[u] = acc;
+          units = u + 1;
+          acc ^= 1;
+          if (acc == 0) acc_ph ^= 1u;
+        }
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * TOK);
         for (int kb = 0; kb < shape.k_blocks; ++kb) {
           if (!mbar_wait_bounded(&bar.full[st], ph, bar.abort_flag, &g_grouped_status, kStatusMmaTimeout)) {
             ok = false;
@@ -399,14 +531,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           tc_fence_after();
           const uint64_t m0 = (F_MN ? desc_t : desc_k) + ((smem_u32(smem_m + st * kMBytes) >> 4) & 0x3FFFu);
-          const uint64_t n0 = desc_k + ((smem_u32(smem_n + st * Cfg::kTokBytes) >> 4) & 0x3FFFu);
 #pragma unroll
-          for (int kk = 0; kk < kBK / 16; ++kk) {
-            const uint32_t more = (kb > 0 || kk > 0) ? 1u : 0u;
-            if (PAIR)
-              tc_mma_f16_pair(d_tmem, m0 + kk * (F_MN ? 128u : 2u), n0 + kk * 2u, idesc, more);
-            else
-              tc_mma_f16(d_tmem, m0 + kk * (F_MN ? 128u : 2u), n0 + kk * 2u, idesc, more);
+          for (int u = 0; u < Cfg::kUnits; ++u) {
+            if (u > 0 && u >= units) continue;
+            const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(buffer[u] * Cfg::kUnitCols);
+            const uint64_t n0 =
+                desc_k + ((smem_u32(smem_n + (st * Cfg::kUnits + u) * Cfg::kUnitBytes) >> 4) & 0x3FFFu);
+#pragma unroll
+            for (int kk = 0; kk < kBK / 16; ++kk) {
+              const uint32_t more = (kb > 0 || kk > 0) ? 1u : 0u;
+              if (PAIR)
+                tc_mma_f16_pair(d_tmem, m0 + kk * (F_MN ? 128u : 2u), n0 + kk * 2u, idesc[u], more);
+              else
+                tc_mma_f16(d_tmem, m0 + kk * (F_MN ? 128u : 2u), n0 + kk * 2u, idesc[u], more);
+            }
+            // The first unit of two is handed over as soon as its last products are issued.
+            if (u + 1 < Cfg::kUnits && u + 1 < units && kb + 1 == shape.k_blocks) hand_over(buffer[u]);
           }
           if (PAIR) {
             tc_commit_pair(empty0 + static_cast<uint32_t>(st) * 8u);
@@ -419,15 +559,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             ph ^= 1u;
           }
         }
-        if (!ok) break;
-        if (PAIR) {
-          tc_commit_pair(tfull0 + static_cast<uint32_t>(acc) * 8u);
-          tc_commit_pair(tfull1 + static_cast<uint32_t>(acc) * 8u);
-        } else {
-          tc_commit(&bar.tfull[acc]);
-        }
-        acc ^= 1;
-        if (acc == 0) acc_ph ^= 1u;
+        // Last of the tile's commits, so that a CTA whose epilogue has seen it has seen
+        // every earlier arrival on its barriers.
+        if (ok) hand_over(buffer[units - 1]);
       }
     }
   } else {
@@ -436,42 +570,49 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int half = ew >> 2;      // even (0) or odd (1) blocks of 32 rows
     uint8_t* slot = smem_epi + ew * Cfg::kSlotBytes;
     const uint32_t tempty0 = PAIR ? cluster_addr(&bar.tempty[0], 0) : 0u;
-    int e = 0, acc = 0;
+    int place = 0, acc = 0;
     uint32_t acc_ph = 0;
-    for (int t = tile_begin; t < tiles; t += tile_step) {
-      const RowsTile tile = rows_tile<TOK, Cfg::kUnit>(first_tile, first_row, t, e);
-      if (!mbar_wait_bounded(&bar.tfull[acc], acc_ph, bar.abort_flag, &g_grouped_status, kStatusEpilogueTimeout)) break;
-      __syncwarp();
-      tc_fence_after();
+    bool ok = true;
+    for (int t = tile_begin; t < tiles && ok; t += tile_step) {
+      const RowsTile tile = rows_tile<TOK, Cfg::kGrain>(table, t, place);
       const int f0 = tile.f * Cfg::kFeatures + static_cast<int>(rank) * kBM + quarter * 32;
-      const uint32_t at = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * TOK);
+      const int split = first_unit<Cfg>(tile);
+      for (int first = 0; first < tile.rows; first += split) {
+        ok = mbar_wait_bounded(&bar.tfull[acc], acc_ph, bar.abort_flag, &g_grouped_status, kStatusEpilogueTimeout);
+        if (!ok) break;
+        __syncwarp();
+        tc_fence_after();
+        const uint32_t at =
+            tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * Cfg::kUnitCols);
+        const int rows = first == 0 ? split : tile.rows - split;
 #pragma unroll 1
-      for (int c = 32 * half; c < tile.rows && f0 < shape.n; c += 64) {
-        float v[32];
+        for (int c = 32 * half; c < rows && f0 < shape.n; c += 64) {
+          float v[32];
+          __syncwarp();
+          tmem_load_32cols(at + c, v);
+          XRow<OUT_F32> x;
+          round_row<OUT_F32>(v, out.bf16, x);
+          // Lane = feature, value = row of the output: the block is turned in its slot.
+          stage_write_col<OUT_F32>(slot, lane, x);
+          __syncwarp();
+          store_rows<OUT_F32>(slot, out, static_cast<int64_t>(tile.row0 + first + c) * out.ldd + f0, min(32, rows - c),
+                              shape.n - f0, lane);
+          __syncwarp();
+        }
+        tc_fence_before();
         __syncwarp();
-        tmem_load_32cols(at + c, v);
-        XRow<OUT_F32> x;
-        round_row<OUT_F32>(v, out.bf16, x);
-        // Lane = feature, value = row of the output: the block is turned in its slot.
-        stage_write_col<OUT_F32>(slot, lane, x);
-        __syncwarp();
-        store_rows<OUT_F32>(slot, out, static_cast<int64_t>(tile.row0 + c) * out.ldd + f0, min(32, tile.rows - c),
-                            shape.n - f0, lane);
-        __syncwarp();
+        if (lane == 0) {
+          if (PAIR)
+            mbar_arrive_cluster(tempty0 + static_cast<uint32_t>(acc) * 8u);
+          else
+            mbar_arrive(&bar.tempty[acc]);
+        }
+        acc ^= 1;
+        if (acc == 0) acc_ph ^= 1u;
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (PAIR)
-          mbar_arrive_cluster(tempty0 + static_cast<uint32_t>(acc) * 8u);
-        else
-          mbar_arrive(&bar.tempty[acc]);
-      }
-      acc ^= 1;
-      if (acc == 0) acc_ph ^= 1u;
     }
     // Rows that no group owns.
-    for (int r = first_row[groups.count] + static_cast<int>(blockIdx.x) * kEpiWarps + ew; r < groups.rows;
+    for (int r = table.first_row[groups.count] + static_cast<int>(blockIdx.x) * kEpiWarps + ew; r < groups.rows;
          r += static_cast<int>(gridDim.x) * kEpiWarps) {
       const int64_t base = static_cast<int64_t>(r) * out.ldd;
       for (int c = lane; c < shape.n; c += 32) {
@@ -502,46 +643,38 @@ struct ReduceConfig {
   static constexpr uint32_t kSlotBytes = 32 * (OUT_F32 ? 128 : 64);
   static constexpr uint32_t kTmemCols = 2 * kReduceN;
   static constexpr size_t kSmemBytes =
-      1024 + kStages * kStageBytes + kEpiWarps * kSlotBytes + (kMaxGroups + 1) * 4 + 4 + Barriers<kStages, PAIR>::kBytes;
+      1024 + kStages * kStageBytes + kEpiWarps * kSlotBytes + Table::kBytes + Barriers<kStages, PAIR>::kBytes;
 };
 
-// The tensor maps of a group's rows of both operands, from maps of the whole
-// operands: base address at the group's first row, row extent to its last.
-// One warp; maps [count][2] of 128 bytes each.
-__global__ void __launch_bounds__(32) group_maps_kernel(const __grid_constant__ CUtensorMap left,
-                                                        const __grid_constant__ CUtensorMap right, const Groups groups,
-                                                        const void* left_base, const void* right_base,
-                                                        int64_t left_pitch, int64_t right_pitch, CUtensorMap* maps) {
-  pdl_launch_dependents();
-  const int lane = threadIdx.x;
-  int carry = 0;
-  for (int base = 0; base < groups.count; base += 32) {
-    const int e = base + lane;
-    int begin, end;
-    group_rows(groups, e, lane, carry, begin, end);
-    if (e >= groups.count || end == begin) continue;  // no map is read for an empty group
-    for (int which = 0; which < 2; ++which) {
-      CUtensorMap* to = maps + 2 * e + which;
-      const uint4* from = reinterpret_cast<const uint4*>(which ? &right : &left);
-#pragma unroll
-      for (int q = 0; q < 8; ++q) reinterpret_cast<uint4*>(to)[q] = from[q];
-      const uint64_t address = reinterpret_cast<uint64_t>(which ? right_base : left_base) +
-                               static_cast<uint64_t>(begin) * static_cast<uint64_t>(which ? right_pitch : left_pitch);
-      asm volatile("tensormap.replace.tile.global_address.global.b1024.b64 [%0], %1;" ::"l"(to), "l"(address) : "memory");
-      asm volatile("tensormap.replace.tile.global_dim.global.b1024.b32 [%0], 1, %1;" ::"l"(to), "r"(end - begin) : "memory");
-    }
-  }
-  asm volatile("fence.proxy.tensormap::generic.release.gpu;" ::: "memory");
-}
+constexpr int kReduceThreads = kThreads + 32;  // and the warp that zeroes foreign rows
 
-__device__ __forceinline__ void acquire_map(const CUtensorMap* map) {
-  asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(map) : "memory");
+// The order of a tile's blocks of 64 rows. A last block with foreign rows needs the
+// zeroing warp, about 800 clocks after it has landed. So it is loaded up to two
+// blocks ahead of its turn: the ring holds (.., last, a, b), the MMAs take
+// (.., a, b, last). (Taken in the ring's order, its wait was exposed in every
+// tile: 275 against 249 us for 64 groups of 500 rows, 1024 x 4096.)
+struct Blocks {
+  int rows, count, ahead;
+
+  __device__ __forceinline__ explicit Blocks(int rows_)
+      : rows(rows_), count((rows_ + kBK - 1) / kBK), ahead(rows_ % 16 == 0 ? 0 : min(2, count - 1)) {}
+  // Place in the tile's stretch of the ring of the last block.
+  __device__ __forceinline__ int last_place() const { return count - 1 - ahead; }
+  // The block that is loaded at ring place `at`.
+  __device__ __forceinline__ int block_at(int at) const {
+    return at < last_place() ? at : (at == last_place() ? count - 1 : at - 1);
+  }
+};
+
+// Arrives on another CTA's barrier after this thread's writes to shared memory.
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t bar_cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
 }
 
 template <bool OUT_F32, bool PAIR>
-__global__ void __launch_bounds__(kThreads, 1)
-    grouped_reduce_kernel(const CUtensorMap* __restrict__ maps, const Groups groups, const ReduceShape shape,
-                          const Output out, const int ab_bf16) {
+__global__ void __launch_bounds__(kReduceThreads, 1)
+    grouped_reduce_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ CUtensorMap map_r,
+                          const Groups groups, const ReduceShape shape, const Output out, const int ab_bf16) {
   using Cfg = ReduceConfig<OUT_F32, PAIR>;
   constexpr int S = Cfg::kStages;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
@@ -556,62 +689,69 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem_n = smem + S * kMBytes;
   uint8_t* smem_epi = smem + S * Cfg::kStageBytes;
   const Barriers<S, PAIR> bar(smem_epi + kEpiWarps * Cfg::kSlotBytes);
-  int* first_row = reinterpret_cast<int*>(smem_epi + kEpiWarps * Cfg::kSlotBytes + Barriers<S, PAIR>::kBytes);
+  const Table table(smem_epi + kEpiWarps * Cfg::kSlotBytes + Barriers<S, PAIR>::kBytes);
 
-  const uint32_t tmem_base = set_up<S, PAIR>(bar, warp, Cfg::kTmemCols);
+  // A stage is full when each CTA has arrived and the bytes are there: those of
+  // both CTAs count on CTA 0's barrier, or, for a stage whose foreign rows are to be
+  // zeroed, each CTA's on its own tail barrier, and the zeroing warps arrive.
+  const uint32_t tmem_base = set_up<S, PAIR>(bar, warp, Cfg::kTmemCols, PAIR ? 2 : 1);
+  // A tile's cost is its group's rows, in 31sts of a group twice as large as the mean.
+  const int per_group = shape.tiles_m * shape.tiles_n;
   if (warp == 0) {
-    int carry = 0;
-    for (int base = 0; base < groups.count; base += 32) {
-      int begin, end;
-      group_rows(groups, base + lane, lane, carry, begin, end);
-      if (base + lane < groups.count) first_row[base + lane] = begin;
-    }
-    if (lane == 0) first_row[groups.count] = carry;
+    const float unit = 31.0f * groups.count / (2.0f * groups.rows);
+    fill_table(
+        table, reinterpret_cast<int*>(smem_epi), groups, lane, [&](int rows) { return min(31, static_cast<int>(rows * unit)); },
+        [&](int) { return per_group; });
   }
   __syncthreads();
-  const int per_group = shape.tiles_m * shape.tiles_n;
   const int tiles = per_group * groups.count;
 
   if (warp == 0) {
     if (lane == 0) {
-      int st = 0, have = -1;
+      int st = 0;
       uint32_t ph = 0;
       bool ok = true;
       const uint32_t full0 = PAIR ? cluster_addr(&bar.full[0], 0) : 0u;
+      const uint32_t tail_own = PAIR ? cluster_addr(&bar.tail[0], rank) : 0u;
       for (int t = tile_begin; t < tiles && ok; t += tile_step) {
-        const int e = t / per_group, l = t - e * per_group;
-        const int k_blocks = (first_row[e + 1] - first_row[e] + kBK - 1) / kBK;
-        if (k_blocks == 0) continue;
-        const CUtensorMap* map_l = maps + 2 * e;
-        const CUtensorMap* map_r = map_l + 1;
-        if (e != have) {
-          acquire_map(map_l);
-          acquire_map(map_r);
-          have = e;
-        }
+        const int place = t / per_group, l = t - place * per_group;
+        const int e = table.order[place];
+        const int begin = table.first_row[e], rows = table.first_row[e + 1] - begin;
         const int i = l / shape.tiles_n, j = l - i * shape.tiles_n;
         const int m0 = i * Cfg::kTileM + static_cast<int>(rank) * kBM;
         const int n0 = j * kReduceN + static_cast<int>(rank) * Cfg::kNRows;
-        for (int kb = 0; kb < k_blocks; ++kb) {
+        const Blocks blocks(rows);
+        for (int at = 0; at < blocks.count; ++at) {
           if (!mbar_wait_bounded(&bar.empty[st], ph ^ 1u, bar.abort_flag, &g_grouped_status, kStatusProducerTimeout)) {
             ok = false;
             break;
           }
           uint8_t* sm = smem_m + st * kMBytes;
           uint8_t* sn = smem_n + st * Cfg::kNBytes;
+          const int kb = blocks.block_at(at);
+          const int row = begin + kb * kBK;
+          const bool whole = kb + 1 < blocks.count || rows % 16 == 0;  // no foreign rows in a 16-row step
+          if (!whole) mbar_arrive_expect_tx(&bar.tail[st], Cfg::kStageBytes);
           if (PAIR) {
-            if (rank == 0) mbar_arrive_expect_tx(&bar.full[st], 2 * Cfg::kStageBytes);
-            const uint32_t fb = full0 + static_cast<uint32_t>(st) * 8u;
+            uint32_t fb = tail_own + static_cast<uint32_t>(st) * 8u;
+            if (whole) {
+              fb = full0 + static_cast<uint32_t>(st) * 8u;
+              if (rank == 0)
+                mbar_arrive_expect_tx(&bar.full[st], 2 * Cfg::kStageBytes);
+              else
+                mbar_arrive_cluster(fb);
+            }
 #pragma unroll
-            for (int c = 0; c < kBM / 64; ++c) tma_load_3d_pair(sm + c * 8192, map_l, fb, m0 + 64 * c, kb * kBK, 0);
+            for (int c = 0; c < kBM / 64; ++c) tma_load_3d_pair(sm + c * 8192, &map_l, fb, m0 + 64 * c, row, 0);
 #pragma unroll
-            for (int c = 0; c < Cfg::kNRows / 64; ++c) tma_load_3d_pair(sn + c * 8192, map_r, fb, n0 + 64 * c, kb * kBK, 0);
+            for (int c = 0; c < Cfg::kNRows / 64; ++c) tma_load_3d_pair(sn + c * 8192, &map_r, fb, n0 + 64 * c, row, 0);
           } else {
-            mbar_arrive_expect_tx(&bar.full[st], Cfg::kStageBytes);
+            uint64_t* landed = whole ? &bar.full[st] : &bar.tail[st];
+            if (whole) mbar_arrive_expect_tx(landed, Cfg::kStageBytes);
 #pragma unroll
-            for (int c = 0; c < kBM / 64; ++c) tma_load_3d(sm + c * 8192, map_l, &bar.full[st], m0 + 64 * c, kb * kBK, 0);
+            for (int c = 0; c < kBM / 64; ++c) tma_load_3d(sm + c * 8192, &map_l, landed, m0 + 64 * c, row, 0);
 #pragma unroll
-            for (int c = 0; c < Cfg::kNRows / 64; ++c) tma_load_3d(sn + c * 8192, map_r, &bar.full[st], n0 + 64 * c, kb * kBK, 0);
+            for (int c = 0; c < Cfg::kNRows / 64; ++c) tma_load_3d(sn + c * 8192, &map_r, landed, n0 + 64 * c, row, 0);
           }
           if (++st == S) {
             st = 0;
@@ -619,6 +759,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
+      drain<S, PAIR>(bar, st, ph, ok);
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
@@ -632,39 +773,69 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t ph = 0, acc_ph = 0;
       bool ok = true;
       for (int t = tile_begin; t < tiles && ok; t += tile_step) {
-        const int e = t / per_group;
-        const int rows = first_row[e + 1] - first_row[e];
-        const int k_blocks = (rows + kBK - 1) / kBK;
-        if (k_blocks == 0) continue;
+        const int e = table.order[t / per_group];
+        const int rows = table.first_row[e + 1] - table.first_row[e];
+        if (rows == 0) continue;
         if (!mbar_wait_bounded(&bar.tempty[acc], acc_ph ^ 1u, bar.abort_flag, &g_grouped_status, kStatusMmaTimeout)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kReduceN);
-        for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!mbar_wait_bounded(&bar.full[st], ph, bar.abort_flag, &g_grouped_status, kStatusMmaTimeout)) {
-            ok = false;
-            break;
-          }
+        const Blocks blocks(rows);
+        // Steps of the ring's current stage into the accumulator; `steps` 16-row steps.
+        auto multiply = [&](int at, uint32_t at_ph, int steps, uint32_t more) {
+          if (!mbar_wait_bounded(&bar.full[at], at_ph, bar.abort_flag, &g_grouped_status, kStatusMmaTimeout)) return false;
           tc_fence_after();
-          const uint64_t m0 = desc_t + ((smem_u32(smem_m + st * kMBytes) >> 4) & 0x3FFFu);
-          const uint64_t n0 = desc_t + ((smem_u32(smem_n + st * Cfg::kNBytes) >> 4) & 0x3FFFu);
-#pragma unroll
-          for (int kk = 0; kk < kBK / 16; ++kk) {
-            const uint32_t more = (kb > 0 || kk > 0) ? 1u : 0u;
+          const uint64_t m0 = desc_t + ((smem_u32(smem_m + at * kMBytes) >> 4) & 0x3FFFu);
+          const uint64_t n0 = desc_t + ((smem_u32(smem_n + at * Cfg::kNBytes) >> 4) & 0x3FFFu);
+          auto step = [&](int kk, uint32_t add) {
             if (PAIR)
-              tc_mma_f16_pair(d_tmem, m0 + kk * 128u, n0 + kk * 128u, idesc, more);
+              tc_mma_f16_pair(d_tmem, m0 + kk * 128u, n0 + kk * 128u, idesc, add);
             else
-              tc_mma_f16(d_tmem, m0 + kk * 128u, n0 + kk * 128u, idesc, more);
+              tc_mma_f16(d_tmem, m0 + kk * 128u, n0 + kk * 128u, idesc, add);
+          };
+          step(0, more);
+          if (steps == kBK / 16) {
+#pragma unroll
+            for (int kk = 1; kk < kBK / 16; ++kk) step(kk, 1u);
+          } else {
+            for (int kk = 1; kk < steps; ++kk) step(kk, 1u);
           }
           if (PAIR) {
-            tc_commit_pair(empty0 + static_cast<uint32_t>(st) * 8u);
-            tc_commit_pair(empty1 + static_cast<uint32_t>(st) * 8u);
+            tc_commit_pair(empty0 + static_cast<uint32_t>(at) * 8u);
+            tc_commit_pair(empty1 + static_cast<uint32_t>(at) * 8u);
           } else {
-            tc_commit(&bar.empty[st]);
+            tc_commit(&bar.empty[at]);
           }
+          return true;
+        };
+        auto advance = [&]() {
           if (++st == S) {
             st = 0;
             ph ^= 1u;
           }
+        };
+        // The whole blocks in the ring's order, past the last one, which follows them.
+        const int whole = blocks.count - (rows % kBK == 0 ? 0 : 1);
+        const int skip = whole < blocks.count ? blocks.last_place() : -1;
+        int last = 0;
+        uint32_t last_ph = 0u, more = 0u;
+        for (int i = 0; i < whole; ++i) {
+          if (i == skip) {
+            last = st;
+            last_ph = ph;
+            advance();
+          }
+          ok = multiply(st, ph, kBK / 16, more);
+          if (!ok) break;
+          more = 1u;
+          advance();
+        }
+        if (ok && whole < blocks.count) {
+          if (skip >= whole) {
+            last = st;
+            last_ph = ph;
+            advance();
+          }
+          ok = multiply(last, last_ph, (rows % kBK + 15) / 16, more);
         }
         if (!ok) break;
         if (PAIR) {
@@ -677,6 +848,44 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (acc == 0) acc_ph ^= 1u;
       }
     }
+  } else if (warp == kReduceThreads / 32 - 1) {
+    // Zeroes the foreign rows of a group's last 16-row step. Row r of a 64 x 64 box is
+    // bytes [128 r, 128 r + 128) of it (the swizzle stays within a row).
+    const uint32_t full0 = PAIR ? cluster_addr(&bar.full[0], 0) : 0u;
+    int st = 0;
+    uint32_t phases = 0;  // bit s: parity of the next use of tail[s]
+    for (int t = tile_begin; t < tiles; t += tile_step) {
+      const int e = table.order[t / per_group];
+      const int rows = table.first_row[e + 1] - table.first_row[e];
+      const Blocks blocks(rows);
+      const int last = (st + blocks.last_place()) % S;
+      st = (st + blocks.count) % S;
+      if (rows % 16 == 0) continue;
+      const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bar.tail[last], (phases >> last) & 1u, bar.abort_flag,
+                                                                &g_grouped_status, kStatusProducerTimeout));
+      if (!ok) break;
+      phases ^= 1u << last;
+      // Four rows at a time, eight lanes each, from the first row of the last step on.
+      const int step_row = rows % kBK / 16 * 16;
+      constexpr int kBoxes = (kBM + Cfg::kNRows) / 64;
+#pragma unroll
+      for (int box = 0; box < kBoxes; ++box) {
+        uint8_t* at = (box < kBM / 64 ? smem_m + last * kMBytes + box * 8192
+                                      : smem_n + last * Cfg::kNBytes + (box - kBM / 64) * 8192) +
+                      step_row * 128 + lane * 16;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (4 * q + lane / 8 >= rows % 16) *reinterpret_cast<uint4*>(at + q * 512) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      fence_proxy_async_smem();  // the zeros are written before the MMA reads them
+      __syncwarp();
+      if (lane == 0) {
+        if (PAIR)
+          mbar_arrive_release_cluster(full0 + static_cast<uint32_t>(last) * 8u);
+        else
+          mbar_arrive(&bar.full[last]);
+      }
+    }
   } else {
     const int ew = warp - 2;
     const int quarter = warp & 3;
@@ -686,12 +895,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     int acc = 0;
     uint32_t acc_ph = 0;
     for (int t = tile_begin; t < tiles; t += tile_step) {
-      const int e = t / per_group, l = t - e * per_group;
+      const int place = t / per_group, l = t - place * per_group;
+      const int e = table.order[place];
       const int i = l / shape.tiles_n, j = l - i * shape.tiles_n;
       const int r0 = i * Cfg::kTileM + static_cast<int>(rank) * kBM + quarter * 32;
       const int live = min(32, shape.m - r0);
       const int64_t base = e * out.bstride + static_cast<int64_t>(r0) * out.ldd;
-      const bool empty = first_row[e + 1] == first_row[e];
+      const bool empty = table.first_row[e + 1] == table.first_row[e];
       if (!empty) {
         if (!mbar_wait_bounded(&bar.tfull[acc], acc_ph, bar.abort_flag, &g_grouped_status, kStatusEpilogueTimeout)) break;
         __syncwarp();
@@ -740,14 +950,15 @@ int g_resident[kDevices][kSlots] = {};  // co-resident CTAs (or CTAs of pairs) o
 
 // Launches a persistent grid of at most `wanted` CTAs (or pairs) of `kernel`.
 template <bool PAIR, typename... Params, typename... Args>
-int launch_persistent(void (*kernel)(Params...), int slot, size_t smem, int64_t wanted, cudaStream_t stream, Args... args) {
+int launch_persistent(void (*kernel)(Params...), int threads, int slot, size_t smem, int64_t wanted, cudaStream_t stream,
+                      Args... args) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
   if (dev < 0 || dev >= kDevices) return fail(GNS_ERR_DEVICE, "device index out of range");
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2];
-  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -783,7 +994,8 @@ int launch_persistent(void (*kernel)(Params...), int slot, size_t smem, int64_t 
 }
 
 struct RowsCall {
-  CUtensorMap right, full, part;
+  CUtensorMap right;
+  RowMaps maps;
   Groups groups;
   RowsShape shape;
   Output out;
@@ -795,9 +1007,9 @@ template <bool F_MN, int TOK, bool OUT_F32, bool PAIR>
 int launch_rows(RowsCall& c, int slot, cudaStream_t stream) {
   using Cfg = RowsConfig<TOK, OUT_F32, PAIR>;
   c.shape.feature_tiles = (c.shape.n + Cfg::kFeatures - 1) / Cfg::kFeatures;
-  return launch_persistent<PAIR>(grouped_rows_kernel<F_MN, TOK, OUT_F32, PAIR>, slot, Cfg::kSmemBytes,
-                                 c.row_tiles * c.shape.feature_tiles, stream, c.right, c.full, c.part, c.groups,
-                                 c.shape, c.out, c.bf16);
+  return launch_persistent<PAIR>(grouped_rows_kernel<F_MN, TOK, OUT_F32, PAIR>, kThreads, slot, Cfg::kSmemBytes,
+                                 c.row_tiles * c.shape.feature_tiles, stream, c.right, c.maps, c.groups, c.shape, c.out,
+                                 c.bf16);
 }
 
 template <int TOK, bool PAIR>
@@ -808,6 +1020,39 @@ int launch_rows_any(bool mn, bool f32, RowsCall& c, int slot, cudaStream_t strea
   }
   if (f32) return launch_rows<false, TOK, true, PAIR>(c, slot + 1, stream);
   return launch_rows<false, TOK, false, PAIR>(c, slot, stream);
+}
+
+// Rows of a tile: 64 or 128 (a CTA, 128 features), 256 or 512 (a pair, 256 features).
+// The time of a call goes in turns of all SMs, so the choice is the one with the
+// least turns times the cost of its tile. The groups' sizes are not known here: T
+// rows in E groups make about T / tile + E / 2 parts, one for each group at least.
+// Costs of a tile, measured with one turn and with many: 1, 1.08, 1.3 (64, 128,
+// 256). Microseconds measured for 64 / 128 / 256, ragged groups of g rows on average:
+//   5 x (1000 x 1501)   g = 96: 13.8 / 15.0 / 18.6   g = 128: 19.4 / 15.5 / 20.0
+//   8 x (2048 x 2048)   g = 48: 30.3 / 22.3 / 23.7   g = 96: 28.4 / 31.7 / 25.1
+//   64 x (1024 x 4096)  g = 32: 107 / 107 / 111      g = 128: 209 / 135 / 123
+// Tiles of 512 rows load the features half as often, but both accumulators belong
+// to one tile, so the epilogue does not overlap the next one: for long products of
+// large groups only (256 against 512: 8 groups of 2048 rows, 4096 x 14336, 1441
+// and 1390 us; 64 of 1024, 4096 x 1024: 455 and 413; but 64 of 640, 1024 x 4096:
+// 350 and 383, and 8 of 1024 with few tiles, 4096 x 4096: 211 and 218).
+int rows_tile_choice(int64_t rows, int64_t n, int64_t k, int64_t groups) {
+  const int sms = device_sm_count();
+  const double t = static_cast<double>(rows), e = static_cast<double>(groups);
+  if (rows >= 1024 * groups && k >= 2048 && (t / 512) * static_cast<double>((n + 255) / 256) >= 6.0 * (sms / 2)) return 512;
+  int best = 64;
+  double least = 0.0;
+  for (int tile : {64, 128, 256}) {
+    const int features = tile == 256 ? 256 : 128, workers = tile == 256 ? sms / 2 : sms;
+    const double parts = std::max(std::min(e, t), t / tile + e / 2);
+    const double turns = std::ceil(parts * static_cast<double>((n + features - 1) / features) / workers);
+    const double cost = turns * (tile == 64 ? 1.0 : (tile == 128 ? 1.08 : 1.3));
+    if (tile == 64 || cost < least) {
+      best = tile;
+      least = cost;
+    }
+  }
+  return best;
 }
 
 int check_groups(int ab_dtype, int ends_bits, int64_t groups, int64_t rows, int64_t a, int64_t b, int d_dtype) {
@@ -824,8 +1069,6 @@ bool aligned_rows(const void* d, int64_t ldd, int64_t bstride, int dtype) {
   const int es = dtype_size(dtype);
   return reinterpret_cast<uintptr_t>(d) % 16 == 0 && (ldd * es) % 16 == 0 && (bstride * es) % 16 == 0;
 }
-
-size_t reduce_workspace(int64_t groups) { return 128 + static_cast<size_t>(groups) * 2 * sizeof(CUtensorMap); }
 
 }  // namespace
 
@@ -862,41 +1105,37 @@ int gns_grouped_gemm(int ab_dtype, int64_t rows, int64_t n, int64_t k, int64_t g
   rc = check_device();
   if (rc != GNS_OK) return rc;
   RowsCall c{};
-  // Groups of up to 64 rows on average are bound by reading the experts' matrices:
-  // narrow row tiles leave the shared memory to more stages of them.
-  const bool small = rows <= 64 * groups;
-  const int box = small ? 64 : 128;
   rc = k_major ? encode_tiles(&c.right, ab_dtype, right, k, n, groups, right_cstride, right_gstride, kBM)
                : encode_tiles(&c.right, ab_dtype, right, n, k, groups, right_rstride, right_gstride, 64);
-  if (rc == GNS_OK) rc = encode_tiles(&c.full, ab_dtype, left, k, rows, 1, left_rstride, 0, box);
-  if (rc == GNS_OK) rc = encode_tiles(&c.part, ab_dtype, left, k, rows, 1, left_rstride, 0, 32);
+  for (int i = 0; i < 4 && rc == GNS_OK; ++i)
+    rc = encode_tiles(&c.maps.box[i], ab_dtype, left, k, rows, 1, left_rstride, 0, 32 * (i + 1));
   if (rc != GNS_OK) return rc;
   c.groups = {ends, ends_bits == 64 ? 1 : 0, static_cast<int>(groups), static_cast<int>(rows)};
   c.shape.n = static_cast<int>(n);
   c.shape.k_blocks = static_cast<int>((k + kBK - 1) / kBK);
   c.out = {out, out_rstride, 0, out_dtype == kBF16 ? 1 : 0, aligned_rows(out, out_rstride, 0, out_dtype) ? 1 : 0};
   c.bf16 = ab_dtype == kBF16 ? 1 : 0;
-  c.row_tiles = rows / (small ? 32 : 128) + std::min(groups, rows);
+  c.row_tiles = rows / 32 + std::min(groups, rows);
   if (c.row_tiles * ((n + kBM - 1) / kBM) > (1ll << 30)) return fail(GNS_ERR_UNSUPPORTED, "too many tiles");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (small) return launch_rows_any<64, false>(!k_major, out_dtype == kF32, c, 0, st);
-  return launch_rows_any<256, true>(!k_major, out_dtype == kF32, c, 4, st);
+  const int tile = rows_tile_choice(rows, n, k, groups);
+  const bool f32 = out_dtype == kF32;
+  if (tile == 64) return launch_rows_any<64, false>(!k_major, f32, c, 0, st);
+  if (tile == 128) return launch_rows_any<128, false>(!k_major, f32, c, 4, st);
+  if (tile == 256) return launch_rows_any<256, true>(!k_major, f32, c, 8, st);
+  return launch_rows_any<512, true>(!k_major, f32, c, 12, st);
 }
-
-size_t gns_grouped_gemm_reduce_workspace_size(int64_t groups) { return groups < 1 ? 0 : reduce_workspace(groups); }
 
 int gns_grouped_gemm_reduce(int ab_dtype, int64_t rows, int64_t m, int64_t n, int64_t groups, const void* left,
                             int64_t left_rstride, const void* right, int64_t right_rstride, const void* ends,
                             int ends_bits, void* out, int out_dtype, int64_t out_gstride, int64_t out_rstride,
-                            void* workspace, size_t workspace_bytes, gns_stream_t stream) {
+                            gns_stream_t stream) {
   clear_error();
   int rc = check_groups(ab_dtype, ends_bits, groups, rows, m, n, out_dtype);
   if (rc != GNS_OK) return rc;
   if (groups == 0 || m == 0 || n == 0) return GNS_OK;
   if (rows == 0) return fail(GNS_ERR_UNSUPPORTED, "a reduced product needs rows");
   if (left == nullptr || right == nullptr || ends == nullptr || out == nullptr) return fail(GNS_ERR_ARGUMENT, "null tensor");
-  if (workspace == nullptr || workspace_bytes < reduce_workspace(groups))
-    return fail(GNS_ERR_WORKSPACE, "grouped reduction workspace too small");
   const bool pair = m > kBM;
   const int64_t tiles_m = (m + (pair ? 2 * kBM : kBM) - 1) / (pair ? 2 * kBM : kBM);
   const int64_t tiles_n = (n + kReduceN - 1) / kReduceN;
@@ -908,11 +1147,7 @@ int gns_grouped_gemm_reduce(int ab_dtype, int64_t rows, int64_t m, int64_t n, in
   if (rc == GNS_OK) rc = encode_tiles(&map_r, ab_dtype, right, n, rows, 1, right_rstride, 0, 64);
   if (rc != GNS_OK) return rc;
   const Groups g{ends, ends_bits == 64 ? 1 : 0, static_cast<int>(groups), static_cast<int>(rows)};
-  auto* maps = reinterpret_cast<CUtensorMap*>((reinterpret_cast<uintptr_t>(workspace) + 127) & ~uintptr_t(127));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  group_maps_kernel<<<1, 32, 0, st>>>(map_l, map_r, g, left, right, left_rstride * 2, right_rstride * 2, maps);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, "group maps kernel");
   const ReduceShape shape{static_cast<int>(m), static_cast<int>(n), static_cast<int>(tiles_m), static_cast<int>(tiles_n)};
   const Output o{out, out_rstride, out_gstride, out_dtype == kBF16 ? 1 : 0,
                  aligned_rows(out, out_rstride, out_gstride, out_dtype) ? 1 : 0};
@@ -920,16 +1155,16 @@ int gns_grouped_gemm_reduce(int ab_dtype, int64_t rows, int64_t m, int64_t n, in
   const int64_t tiles = tiles_m * tiles_n * groups;
   if (pair) {
     if (out_dtype == kF32)
-      return launch_persistent<true>(grouped_reduce_kernel<true, true>, 8, ReduceConfig<true, true>::kSmemBytes, tiles, st,
-                                     static_cast<const CUtensorMap*>(maps), g, shape, o, bf16);
-    return launch_persistent<true>(grouped_reduce_kernel<false, true>, 9, ReduceConfig<false, true>::kSmemBytes, tiles, st,
-                                   static_cast<const CUtensorMap*>(maps), g, shape, o, bf16);
+      return launch_persistent<true>(grouped_reduce_kernel<true, true>, kReduceThreads, 16, ReduceConfig<true, true>::kSmemBytes, tiles, st,
+                                     map_l, map_r, g, shape, o, bf16);
+    return launch_persistent<true>(grouped_reduce_kernel<false, true>, kReduceThreads, 17, ReduceConfig<false, true>::kSmemBytes, tiles, st,
+                                   map_l, map_r, g, shape, o, bf16);
   }
   if (out_dtype == kF32)
-    return launch_persistent<false>(grouped_reduce_kernel<true, false>, 10, ReduceConfig<true, false>::kSmemBytes, tiles, st,
-                                    static_cast<const CUtensorMap*>(maps), g, shape, o, bf16);
-  return launch_persistent<false>(grouped_reduce_kernel<false, false>, 11, ReduceConfig<false, false>::kSmemBytes, tiles, st,
-                                  static_cast<const CUtensorMap*>(maps), g, shape, o, bf16);
+    return launch_persistent<false>(grouped_reduce_kernel<true, false>, kReduceThreads, 18, ReduceConfig<true, false>::kSmemBytes, tiles, st,
+                                    map_l, map_r, g, shape, o, bf16);
+  return launch_persistent<false>(grouped_reduce_kernel<false, false>, kReduceThreads, 19, ReduceConfig<false, false>::kSmemBytes, tiles, st,
+                                  map_l, map_r, g, shape, o, bf16);
 }
 
 }  // extern "C"

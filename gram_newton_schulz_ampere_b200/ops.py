@@ -1138,12 +1138,10 @@ def grouped_gemm_reduce(left: Tensor, right: Tensor, ends: Tensor, out_dtype: to
     out = torch.empty((groups, m, n), dtype=dtype, device=device)
     a, b = _row_operand(left), _row_operand(right)
     lib = nat.load()
-    ws = _workspace(lib.gns_grouped_gemm_reduce_workspace_size(groups), device)
     with nat.on_device(device.index) as stream:
         rc = lib.gns_grouped_gemm_reduce(
             nat.dtype_code(a.dtype), rows, m, n, groups, a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0),
-            ends.data_ptr(), 8 * ends.element_size(), out.data_ptr(), code, out.stride(0), out.stride(1),
-            ws.data_ptr(), ws.numel(), stream,
+            ends.data_ptr(), 8 * ends.element_size(), out.data_ptr(), code, out.stride(0), out.stride(1), stream,
         )
     nat.check(rc, "gns_grouped_gemm_reduce")
     return out

@@ -370,11 +370,10 @@ GNS_API int gns_grouped_gemm(int ab_dtype, int64_t rows, int64_t n, int64_t k, i
                              int64_t left_rstride, const void* right, int64_t right_gstride, int64_t right_rstride,
                              int64_t right_cstride, const void* ends, int ends_bits, void* out, int out_dtype,
                              int64_t out_rstride, gns_stream_t stream);
-GNS_API size_t gns_grouped_gemm_reduce_workspace_size(int64_t groups);
 GNS_API int gns_grouped_gemm_reduce(int ab_dtype, int64_t rows, int64_t m, int64_t n, int64_t groups,
                                     const void* left, int64_t left_rstride, const void* right, int64_t right_rstride,
                                     const void* ends, int ends_bits, void* out, int out_dtype, int64_t out_gstride,
-                                    int64_t out_rstride, void* workspace, size_t workspace_bytes, gns_stream_t stream);
+                                    int64_t out_rstride, gns_stream_t stream);
 
 /* -------------------------------------------------------------- layer norm
  * y = (x - mean) * rstd * weight + bias over the last dimension of [rows][cols],
