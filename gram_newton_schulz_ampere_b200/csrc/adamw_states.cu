@@ -91,6 +91,32 @@ __device__ __forceinline__ float reciprocal_approx(float x) {
   return r;
 }
 
+// Two fp32 values worked on by one instruction, each rounded as a scalar one would.
+struct Pair {
+  uint64_t bits;
+
+  __device__ __forceinline__ Pair() {}
+  __device__ __forceinline__ Pair(float x, float y) {
+    asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(x), "f"(y));
+  }
+  __device__ __forceinline__ explicit Pair(float both) : Pair(both, both) {}
+  __device__ __forceinline__ void get(float& x, float& y) const {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(bits));
+  }
+};
+
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+  return r;
+}
+
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+  return r;
+}
+
 // The larger magnitude; NaN if either is.
 __device__ __forceinline__ float larger(float top, float x) {
   float r;
@@ -225,23 +251,38 @@ __device__ __forceinline__ void step_eight(const float (&gf)[8], float (&pf)[8],
   float mf[8], vf[8];
   decode8(mc, mf);
   decode8(vc, vf);
+  // Every product and sum of the moments is rounded by itself (no fma). Elements go two
+  // to an instruction: one at a time, the kernel issued 38 instructions an element and
+  // took 544 us for 323M bf16 elements.
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    // Every product and sum of the moments is rounded by itself (no fma).
-    const float g = gf[e] * s.scale;
-    mf[e] = __fadd_rn(__fmul_rn(__fmul_rn(mf[e], ms), k.beta1), __fmul_rn(g, k.one_minus_beta1));
-    vf[e] = __fadd_rn(__fmul_rn(__fmul_rn(vf[e], vs), k.beta2), __fmul_rn(__fmul_rn(g, g), k.one_minus_beta2));
-    pf[e] = adamw_update(pf[e], mf[e], vf[e], k, s.lr_bc1, s.inv_bc2);
+  for (int e = 0; e < 8; e += 2) {
+    const Pair g = mul2(Pair(gf[e], gf[e + 1]), Pair(s.scale));
+    // (The sums are scalar: a paired add of two products is fused with one of them.)
+    float m0, m1, v0, v1;
+    mul2(mul2(Pair(mf[e], mf[e + 1]), Pair(ms)), Pair(k.beta1)).get(mf[e], mf[e + 1]);
+    mul2(g, Pair(k.one_minus_beta1)).get(m0, m1);
+    mul2(mul2(Pair(vf[e], vf[e + 1]), Pair(vs)), Pair(k.beta2)).get(vf[e], vf[e + 1]);
+    mul2(mul2(g, g), Pair(k.one_minus_beta2)).get(v0, v1);
+    mf[e] = __fadd_rn(mf[e], m0);
+    mf[e + 1] = __fadd_rn(mf[e + 1], m1);
+    vf[e] = __fadd_rn(vf[e], v0);
+    vf[e + 1] = __fadd_rn(vf[e + 1], v1);
+    float d0, d1;
+    fma2(Pair(sqrt_approx(vf[e]), sqrt_approx(vf[e + 1])), Pair(s.inv_bc2), Pair(k.epsilon)).get(d0, d1);
+    const Pair u = mul2(Pair(mf[e], mf[e + 1]), Pair(reciprocal_approx(d0), reciprocal_approx(d1)));
+    fma2(Pair(-s.lr_bc1), u, mul2(Pair(pf[e], pf[e + 1]), Pair(k.decay))).get(pf[e], pf[e + 1]);
   }
   const float m_top = block_max(mf), v_top = block_max(vf);
   // One lane in two works out the inverse for m, the other for v.
   const float inverse = inverse_scale((threadIdx.x & 1) ? v_top : m_top);
   const float m_inv = __shfl_sync(0xffffffffu, inverse, 0), v_inv = __shfl_sync(0xffffffffu, inverse, 1);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    mf[e] *= m_inv;
-    const float y = vf[e] * v_inv;
-    vf[e] = (vf[e] > 0.0f && y < kE4M3Tiny) ? kE4M3Tiny : y;
+  for (int e = 0; e < 8; e += 2) {
+    mul2(Pair(mf[e], mf[e + 1]), Pair(m_inv)).get(mf[e], mf[e + 1]);
+    float y0, y1;
+    mul2(Pair(vf[e], vf[e + 1]), Pair(v_inv)).get(y0, y1);
+    vf[e] = (vf[e] > 0.0f && y0 < kE4M3Tiny) ? kE4M3Tiny : y0;
+    vf[e + 1] = (vf[e + 1] > 0.0f && y1 < kE4M3Tiny) ? kE4M3Tiny : y1;
   }
   mc = encode8(mf);
   vc = encode8(vf);
