@@ -20,7 +20,9 @@ and every rank applies every update (muon.py:399-476); both leave every rank
 with the same bits, but here the update pass and the update writes of the
 momentum kernel shrink to the owned 1/W share.
 AdamW and Lion groups (vectors and scalars) are one fused multi-tensor kernel
-per dtype combination. Under DistributedDataParallel, ``momentum_comm_hook()``
+per dtype combination. An AdamW group with ``"state_bits": 8`` (or 32) holds its
+moments in 8 bits (or fp32) whatever the parameters' type and steps in fp32
+arithmetic (``ops.AdamWStates``; no counterpart in the reference). Under DistributedDataParallel, ``momentum_comm_hook()``
 moves stage 1 into the backward pass: each gradient bucket's momentum runs as
 soon as its all-reduce has landed.
 """
@@ -70,6 +72,7 @@ from gram_newton_schulz_ampere_b200.optimizer_types import (
 NS_SETTINGS = ("ns_algorithm", "ns_epsilon", "ns_backend", "ns_coefficients", "gram_newton_schulz_reset_iterations")
 ALGORITHMS = frozenset({"muon", "dion3", "adamw", "lion"})
 ADJUSTMENTS = frozenset({"spectral_norm", "rms_norm"})
+ADAMW_STATES = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
 
 
 def orthogonalization_flops(shape: tuple[int, ...]) -> float:
@@ -200,6 +203,7 @@ class Muon(Optimizer):
 
     def load_state_dict(self, state_dict: StateDict) -> None:
         super().load_state_dict(state_dict)
+        self._restore_adamw_states(state_dict)
         first = self.param_groups[0]
         self.ns_algorithm = cast(NewtonSchulzAlgorithm, first.get("ns_algorithm", self.ns_algorithm))
         self.ns_epsilon = cast(float, first.get("ns_epsilon", self.ns_epsilon))
@@ -220,6 +224,18 @@ class Muon(Optimizer):
             self.initialize_parameter_group_state(group)
         self.validate_cuda_configuration()
         self.configure_newton_schulz()
+
+    def _restore_adamw_states(self, state_dict: StateDict) -> None:
+        """Moments, scales and step counts of the groups with ``state_bits`` as they were saved,
+        in tensors of their own: torch's loading casts every state tensor to its parameter's
+        type, which would round them, and shares those that need no cast with the source."""
+        for group, saved in zip(self.param_groups, state_dict["param_groups"], strict=True):
+            if group["algorithm"] != "adamw" or group.get("state_bits") is None:
+                continue
+            for parameter, key in zip(cast(list[Tensor], group["params"]), saved["params"], strict=True):
+                for name, value in state_dict["state"].get(key, {}).items():
+                    if name in ADAMW_STATES or name == "step":
+                        self.state[parameter][name] = value.detach().to(parameter.device, copy=True)
 
     def add_param_group(self, param_group: ParameterGroupInput) -> None:
         group_count = len(self.param_groups)
@@ -307,6 +323,14 @@ class Muon(Optimizer):
                     "Orthogonal optimizer groups require matrix parameters. Put scalar "
                     f"and vector parameters in an adamw or lion group. Invalid shapes: {bad}"
                 )
+        state_bits = group.get("state_bits")
+        if state_bits is not None:
+            if state_bits not in (8, 32):
+                raise ValueError(f"state_bits must be 8, 32 or None, got {state_bits}")
+            if algorithm != "adamw":
+                raise ValueError("state_bits is a setting of adamw groups")
+            if any(isinstance(p, DTensor) for p in cast(list[Tensor], group["params"])):
+                raise ValueError("state_bits requires parameters that are not DTensors")
         self.validate_nonnegative_group_scalar(group, "lr")
         self.validate_nonnegative_group_scalar(group, "weight_decay")
         momentum = group["momentum"]
@@ -360,6 +384,13 @@ class Muon(Optimizer):
             elif algorithm == "adamw":
                 if "step" not in state:
                     state["step"] = torch.zeros((), dtype=torch.float32, device=local_tensor(parameter).device)
+                if group.get("state_bits") is not None:
+                    if "exp_avg" not in state:
+                        fresh = ops.AdamWStates([parameter.detach().contiguous()], cast(int, group["state_bits"]))
+                        names = ADAMW_STATES if fresh.bits == 8 else ADAMW_STATES[:2]
+                        roles = (fresh.exp_avgs, fresh.exp_avg_sqs, fresh.exp_avg_scales, fresh.exp_avg_sq_scales)
+                        state.update({name: role[0] for name, role in zip(names, roles)})
+                    continue
                 if "exp_avg" not in state:
                     state["exp_avg"] = torch.zeros_like(parameter)
                 if "exp_avg_sq" not in state:
@@ -804,6 +835,8 @@ class Muon(Optimizer):
         read-back after the first step (``_host_step_values``; the reference reads
         each one back), and the bias corrections are formed on the host in double
         precision exactly as the reference forms them."""
+        if group.get("state_bits") is not None:
+            return self._step_adamw_states(group)
         lr = float(cast(LearningRate, group["lr"]))
         wd = float(cast(LearningRate, group["weight_decay"]))
         beta1, beta2 = cast(tuple[float, float], group["betas"])
@@ -845,6 +878,36 @@ class Muon(Optimizer):
                 avg_sqs.append(_contiguous_in_place(v, writeback))
                 grads.append(g.contiguous())
             ops.adamw_step(params, grads, avgs, avg_sqs, lr_bc1, inv_bc2, beta1, beta2, epsilon, decay)
+            for original, copy in writeback:
+                original.copy_(copy)
+
+    def _step_adamw_states(self, group: ParameterGroup) -> None:
+        """``step_adamw_group`` for a group whose moments are held in 8 or 32 bits."""
+        beta1, beta2 = cast(tuple[float, float], group["betas"])
+        bits = cast(int, group["state_bits"])
+        members: dict[tuple, list[tuple[Tensor, Tensor, dict[str, Tensor]]]] = {}
+        for parameter in cast(list[Tensor], group["params"]):
+            if parameter.grad is None:
+                continue
+            gradient = resolve_gradient(parameter)
+            self.reject_sparse_or_complex_gradient(gradient)
+            members.setdefault((parameter.dtype, gradient.dtype, parameter.device), []).append(
+                (parameter, gradient, self.state[parameter])
+            )
+        for entries in members.values():
+            steps = [state["step"] for _, _, state in entries]
+            values = self._host_step_values(steps)
+            torch._foreach_add_(steps, 1)
+            writeback: list[tuple[Tensor, Tensor]] = []
+            held = {name: [state[name] for _, _, state in entries] for name in ADAMW_STATES if name in entries[0][2]}
+            states = ops.AdamWStates(
+                [_contiguous_in_place(p.detach(), writeback) for p, _, _ in entries], bits,
+                held["exp_avg"], held["exp_avg_sq"], held.get("exp_avg_scale"), held.get("exp_avg_sq_scale"),
+            )
+            states.step(
+                [g.contiguous() for _, g, _ in entries], float(cast(LearningRate, group["lr"])), beta1, beta2,
+                cast(float, group["epsilon"]), float(cast(LearningRate, group["weight_decay"])), values,
+            )
             for original, copy in writeback:
                 original.copy_(copy)
 
