@@ -221,6 +221,7 @@ def stream_handle(device: torch.device) -> int:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 class on_device:
@@ -235,7 +236,7 @@ class on_device:
         self.switch: torch.cuda.device | None = None
 
     def __enter__(self) -> int:
-        if torch.cuda.current_device() != self.index:
+        if _current_device() != self.index:
             self.switch = torch.cuda.device(self.index)
             self.switch.__enter__()
         if _raw_stream is not None:

@@ -1105,9 +1105,10 @@ int gns_grouped_gemm(int ab_dtype, int64_t rows, int64_t n, int64_t k, int64_t g
   rc = check_device();
   if (rc != GNS_OK) return rc;
   RowsCall c{};
+  const int tile = rows_tile_choice(rows, n, k, groups);
   rc = k_major ? encode_tiles(&c.right, ab_dtype, right, k, n, groups, right_cstride, right_gstride, kBM)
                : encode_tiles(&c.right, ab_dtype, right, n, k, groups, right_rstride, right_gstride, 64);
-  for (int i = 0; i < 4 && rc == GNS_OK; ++i)
+  for (int i = 0; i < (tile == 64 ? 2 : 4) && rc == GNS_OK; ++i)
     rc = encode_tiles(&c.maps.box[i], ab_dtype, left, k, rows, 1, left_rstride, 0, 32 * (i + 1));
   if (rc != GNS_OK) return rc;
   c.groups = {ends, ends_bits == 64 ? 1 : 0, static_cast<int>(groups), static_cast<int>(rows)};
@@ -1115,10 +1116,9 @@ int gns_grouped_gemm(int ab_dtype, int64_t rows, int64_t n, int64_t k, int64_t g
   c.shape.k_blocks = static_cast<int>((k + kBK - 1) / kBK);
   c.out = {out, out_rstride, 0, out_dtype == kBF16 ? 1 : 0, aligned_rows(out, out_rstride, 0, out_dtype) ? 1 : 0};
   c.bf16 = ab_dtype == kBF16 ? 1 : 0;
-  c.row_tiles = rows / 32 + std::min(groups, rows);
+  c.row_tiles = rows / (tile == 64 ? 32 : 64) + std::min(groups, rows);
   if (c.row_tiles * ((n + kBM - 1) / kBM) > (1ll << 30)) return fail(GNS_ERR_UNSUPPORTED, "too many tiles");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int tile = rows_tile_choice(rows, n, k, groups);
   const bool f32 = out_dtype == kF32;
   if (tile == 64) return launch_rows_any<64, false>(!k_major, f32, c, 0, st);
   if (tile == 128) return launch_rows_any<128, false>(!k_major, f32, c, 4, st);

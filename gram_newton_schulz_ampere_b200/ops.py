@@ -76,6 +76,24 @@ def _require_cuda(*tensors: Tensor | None) -> torch.device:
     return device
 
 
+def _device_index(*tensors: Tensor | None) -> int:
+    """``_require_cuda`` for the calls whose host time counts: the device's index."""
+    index = -1
+    for t in tensors:
+        if t is None:
+            continue
+        here = t.get_device()
+        if here < 0:
+            raise ValueError("gram_newton_schulz_ampere_b200 kernels require CUDA tensors")
+        if index < 0:
+            index = here
+        elif here != index:
+            raise ValueError("all tensors must be on the same CUDA device")
+    if index < 0:
+        raise ValueError("no tensor given")
+    return index
+
+
 def _workspace(nbytes: int, device: torch.device) -> Tensor:
     return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
 
@@ -952,6 +970,7 @@ class AdamWStates:
         self.exp_avg_scales = scales(exp_avg_scales) if bits == 8 else []
         self.exp_avg_sq_scales = scales(exp_avg_sq_scales) if bits == 8 else []
         self._numel = [p.numel() for p in self.parameters]
+        self._sizes = (ctypes.c_int64 * max(len(self._numel), 1))(*self._numel)
         self._states = (
             _ptr_array(self.exp_avgs), _ptr_array(self.exp_avg_sqs),
             _ptr_array(self.exp_avg_scales) if bits == 8 else None,
@@ -994,14 +1013,14 @@ class AdamWStates:
             raise ValueError(f"betas must be in [0, 1), got {(beta1, beta2)}")
         if not epsilon > 0.0:
             raise ValueError(f"epsilon must be positive, got {epsilon}")
-        present = [i for i, g in enumerate(gradients) if g is not None]
+        whole = not any(g is None for g in gradients)
+        present = range(count) if whole else [i for i, g in enumerate(gradients) if g is not None]
         if not present:
             return
-        whole = len(present) == count
         given = cast(Sequence[Tensor], gradients) if whole else [cast(Tensor, gradients[i]) for i in present]
         places = self.parameters if whole else [self.parameters[i] for i in present]
         g_dtype = given[0].dtype
-        if any(g.dtype != g_dtype for g in given):
+        if len({g.dtype for g in given}) > 1:
             raise TypeError("all gradients of one call must share a dtype")
         numel = [g.numel() for g in given]
         if numel != (self._numel if whole else [self._numel[i] for i in present]):
@@ -1009,30 +1028,31 @@ class AdamWStates:
         if not (all(map(Tensor.is_contiguous, given)) and all(map(Tensor.is_contiguous, places))):
             raise ValueError("gradients and parameters must be contiguous")
         index = cast(torch.device, self.device).index
-        if any(g.get_device() != index for g in given) or any(p.get_device() != index for p in places):
+        if {t.get_device() for t in (*given, *places)} != {index}:
             raise ValueError("gradients must be on the parameters' device")
         if gradient_scale is not None:
             if gradient_scale.dtype != torch.float32 or gradient_scale.numel() != 1:
                 raise ValueError("gradient_scale must be one float32 value")
             if gradient_scale.get_device() != index:
                 raise ValueError("gradient_scale must be on the parameters' device")
-        floats = ctypes.c_float * len(present)
+        floats = ctypes.c_float * len(given)
         if isinstance(step, (int, float)):
             lr_bc1, inv_bc2 = self._bias_corrections(step, learning_rate, beta1, beta2)
-            corrections = floats(*[lr_bc1] * len(present)), floats(*[inv_bc2] * len(present))
+            corrections = floats(*[lr_bc1] * len(given)), floats(*[inv_bc2] * len(given))
         else:
             if len(step) != count:
                 raise ValueError("step must be one value or one for each parameter")
             pairs = [self._bias_corrections(step[i], learning_rate, beta1, beta2) for i in present]
             corrections = floats(*[a for a, _ in pairs]), floats(*[b for _, b in pairs])
-        states = self._states
+        states, sizes = self._states, self._sizes
         if not whole:
+            sizes = (ctypes.c_int64 * len(given))(*numel)
             roles = (self.exp_avgs, self.exp_avg_sqs, self.exp_avg_scales, self.exp_avg_sq_scales)
             states = tuple(_ptr_array([role[i] for i in present]) if role else None for role in roles)
         lib = nat.load()
         with nat.on_device(index) as stream:
             rc = lib.gns_adamw_states_step(
-                len(present), _ptr_array(places), _ptr_array(given), *states, (ctypes.c_int64 * len(present))(*numel),
+                len(given), _ptr_array(places), _ptr_array(given), *states, sizes,
                 nat.dtype_code(places[0].dtype), nat.dtype_code(g_dtype), self.bits, *corrections,
                 beta1, 1 - beta1, beta2, 1 - beta2, epsilon, 1 - learning_rate * weight_decay,
                 nat.ptr(gradient_scale), stream,
@@ -1086,7 +1106,7 @@ def grouped_gemm(left: Tensor, right: Tensor, ends: Tensor, out_dtype: torch.dty
     ``grouped_gemm(x, W.transpose(1, 2), ends)``, its gradient for the rows
     ``grouped_gemm(dy, W, ends)`` and for the weights ``grouped_gemm_reduce(dy, x, ends)``.
     """
-    device = _require_cuda(left, right, ends)
+    index = _device_index(left, right, ends)
     if left.ndim != 2 or right.ndim != 3:
         raise ValueError("expected left [rows, k] and right [groups, k, n]")
     if left.dtype != right.dtype or left.dtype not in (torch.float16, torch.bfloat16):
@@ -1099,14 +1119,14 @@ def grouped_gemm(left: Tensor, right: Tensor, ends: Tensor, out_dtype: torch.dty
     dtype = out_dtype or left.dtype
     code = nat.dtype_code(dtype)
     if rows == 0 or n == 0 or k == 0 or groups == 0:
-        return torch.zeros((rows, n), dtype=dtype, device=device)
-    out = torch.empty((rows, n), dtype=dtype, device=device)
+        return torch.zeros((rows, n), dtype=dtype, device=left.device)
+    out = torch.empty((rows, n), dtype=dtype, device=left.device)
     a = _row_operand(left)
-    if any(size > 1 and stride == 0 for size, stride in zip(right.shape, right.stride(), strict=True)):
+    if 0 in right.stride():
         right = right.contiguous()  # a TMA map has no zero strides
     b = _aligned_operand(right)
     lib = nat.load()
-    with nat.on_device(device.index) as stream:
+    with nat.on_device(index) as stream:
         rc = lib.gns_grouped_gemm(
             nat.dtype_code(a.dtype), rows, n, k, groups, a.data_ptr(), a.stride(0),
             b.data_ptr(), b.stride(0), b.stride(1), b.stride(2), ends.data_ptr(), 8 * ends.element_size(),
@@ -1120,7 +1140,7 @@ def grouped_gemm_reduce(left: Tensor, right: Tensor, ends: Tensor, out_dtype: to
     """``out[e] = left[rows of e].T @ right[rows of e]`` for each group of rows, on tcgen05
     tensor cores: [E, m, n] from left [T, m] and right [T, n], zero for a group without rows.
     ``ends`` as for ``grouped_gemm``; rows that no group owns have no part in any sum."""
-    device = _require_cuda(left, right, ends)
+    index = _device_index(left, right, ends)
     if left.ndim != 2 or right.ndim != 2:
         raise ValueError("expected left [rows, m] and right [rows, n]")
     if left.dtype != right.dtype or left.dtype not in (torch.float16, torch.bfloat16):
@@ -1134,11 +1154,11 @@ def grouped_gemm_reduce(left: Tensor, right: Tensor, ends: Tensor, out_dtype: to
     dtype = out_dtype or left.dtype
     code = nat.dtype_code(dtype)
     if rows == 0 or m == 0 or n == 0 or groups == 0:
-        return torch.zeros((groups, m, n), dtype=dtype, device=device)
-    out = torch.empty((groups, m, n), dtype=dtype, device=device)
+        return torch.zeros((groups, m, n), dtype=dtype, device=left.device)
+    out = torch.empty((groups, m, n), dtype=dtype, device=left.device)
     a, b = _row_operand(left), _row_operand(right)
     lib = nat.load()
-    with nat.on_device(device.index) as stream:
+    with nat.on_device(index) as stream:
         rc = lib.gns_grouped_gemm_reduce(
             nat.dtype_code(a.dtype), rows, m, n, groups, a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0),
             ends.data_ptr(), 8 * ends.element_size(), out.data_ptr(), code, out.stride(0), out.stride(1), stream,
@@ -1176,17 +1196,17 @@ def layer_norm(x: Tensor, weight: Tensor, bias: Tensor | None, epsilon: float) -
     without the last dimension), which ``layer_norm_backward`` takes. The variance is the
     biased one; all arithmetic is fp32. weight and bias share a floating type of their own;
     bias may be None."""
-    device = _require_cuda(x, weight, bias)
+    index = _device_index(x, weight, bias)
     columns = _norm_check(x, weight, bias)
     flat = _norm_rows(x, columns)
     rows = flat.shape[0]
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=device)
+    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
     rstd = torch.empty_like(mean)
     w = weight.contiguous()
     b = bias.contiguous() if bias is not None else None
     lib = nat.load()
-    with nat.on_device(device.index) as stream:
+    with nat.on_device(index) as stream:
         rc = lib.gns_layer_norm_forward(
             nat.dtype_code(x.dtype), nat.dtype_code(w.dtype), rows, columns, flat.data_ptr(), flat.stride(0),
             w.data_ptr(), nat.ptr(b), float(epsilon), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
@@ -1202,7 +1222,7 @@ def layer_norm_backward(
     """Gradients (dx, dweight, dbias) of ``layer_norm`` from the gradient of y and the mean and
     rstd that the forward pass returned. dx has x's type, dweight and dbias the weight's;
     their sums over the rows are fp32, in a fixed order."""
-    device = _require_cuda(grad, x, weight, mean, rstd)
+    index = _device_index(grad, x, weight, mean, rstd)
     columns = _norm_check(x, weight, None)
     if grad.shape != x.shape:
         raise ValueError("grad and x shapes differ")
@@ -1217,8 +1237,8 @@ def layer_norm_backward(
     dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     dweight, dbias = torch.empty_like(w), torch.empty_like(w)
     lib = nat.load()
-    ws = _workspace(lib.gns_layer_norm_backward_workspace_size(rows, columns), device)
-    with nat.on_device(device.index) as stream:
+    ws = _workspace(lib.gns_layer_norm_backward_workspace_size(rows, columns), x.device)
+    with nat.on_device(index) as stream:
         rc = lib.gns_layer_norm_backward(
             nat.dtype_code(x.dtype), nat.dtype_code(w.dtype), rows, columns, g.data_ptr(), g.stride(0),
             flat.data_ptr(), flat.stride(0), w.data_ptr(), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(),
