@@ -61,14 +61,10 @@ __device__ __forceinline__ int64_t group_end(const Groups& g, int e) {
   return g.ends64 ? static_cast<const int64_t*>(g.ends)[e] : static_cast<int64_t>(static_cast<const int32_t*>(g.ends)[e]);
 }
 
-// Row range of group e = base + lane for the 32 lanes of a warp: ends clamped to
-// [0, rows] and to the largest end before them (`carry`, updated for the next 32).
-__device__ __forceinline__ void group_rows(const Groups& g, int e, int lane, int& carry, int& begin, int& end) {
-  end = 0;
-  if (e < g.count) {
-    const int64_t v = group_end(g, e);
-    end = static_cast<int>(v < 0 ? 0 : (v > g.rows ? g.rows : v));
-  }
+// Row ranges of the 32 groups of a warp's lanes: ends clamped to [0, rows] and to the
+// largest end before them (`carry`, updated for the next 32).
+__device__ __forceinline__ void group_rows(int64_t value, int rows, int lane, int& carry, int& begin, int& end) {
+  end = static_cast<int>(value < 0 ? 0 : (value > rows ? rows : value));
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int other = __shfl_up_sync(0xffffffffu, end, o);
@@ -80,6 +76,15 @@ __device__ __forceinline__ void group_rows(const Groups& g, int e, int lane, int
   carry = __shfl_sync(0xffffffffu, end, 31);
 }
 
+__device__ __forceinline__ int inclusive_sum(int v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int other = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += other;
+  }
+  return v;
+}
+
 // A group of `rows` rows is cut into `parts` parts of `size` rows (the last may be
 // shorter): as few as the tile allows, equal up to the MMA's granularity.
 struct Cut {
@@ -87,90 +92,116 @@ struct Cut {
 };
 
 __device__ __forceinline__ Cut cut_group(int rows, int tile, int unit) {
-  if (rows == 0) return {0, unit};
-  const int least = (rows + tile - 1) / tile;
-  const int size = ((rows + least - 1) / least + unit - 1) / unit * unit;
-  return {(rows + size - 1) / size, size};
+  if (rows <= tile) return {rows > 0 ? 1 : 0, (rows + unit - 1) / unit * unit};
+  const unsigned least = (rows + tile - 1) / tile;
+  const int size = static_cast<int>((rows + least - 1) / least + unit - 1) / unit * unit;
+  return {static_cast<int>(static_cast<unsigned>(rows + size - 1) / static_cast<unsigned>(size)), size};
 }
 
 // The groups as a CTA works through them, in shared memory: place i holds group
-// order[i], whose tiles follow first_tile[i]. Groups with costly tiles come first.
-// The tiles are dealt to the CTAs of a persistent grid in turn, so the sums of the
-// shares differ by less than one tile, and the tiles of the last, partial turn are
-// the cheap ones. (In the groups' own order the busiest CTA pair of a ragged batch
-// had about a quarter more than the mean.)
+// order[i], whose tiles follow first_tile[i]. Where the tiles take more than one turn
+// of the persistent grid, groups with costly tiles come first. The tiles are dealt to
+// the CTAs in turn, so the sums of the shares then differ by less than one tile, and
+// the tiles of the last, partial turn are the cheap ones. (In the groups' own order
+// the busiest CTA pair of a ragged batch had about a quarter more than the mean.)
 struct Table {
   int* first_row;   // [count + 1], by group
   int* first_tile;  // [count + 1], by place
+  int* parts;       // [count], by group
+  uint16_t* size;   // [count], by group: rows of a part
   uint16_t* order;  // [count], by place
-  static constexpr uint32_t kBytes = 2 * (kMaxGroups + 1) * 4 + kMaxGroups * 2;
+  int* counts;      // [32]: scratch of the sort
+  static constexpr uint32_t kBytes = 2 * (kMaxGroups + 1) * 4 + kMaxGroups * 8 + 32 * 4;
 
   __device__ __forceinline__ explicit Table(uint8_t* at)
       : first_row(reinterpret_cast<int*>(at)),
         first_tile(first_row + kMaxGroups + 1),
-        order(reinterpret_cast<uint16_t*>(first_tile + kMaxGroups + 1)) {}
+        parts(first_tile + kMaxGroups + 1),
+        size(reinterpret_cast<uint16_t*>(parts + kMaxGroups)),
+        order(size + kMaxGroups),
+        counts(reinterpret_cast<int*>(order + kMaxGroups)) {}
+
+  __device__ __forceinline__ int rows(int e) const { return first_row[e + 1] - first_row[e]; }
 };
 
-// One warp fills the table. cost(rows) is the cost of a group's tiles, in [0, 31];
-// tiles(rows) their number. A counting sort: the groups of each cost are counted,
-// then placed behind the costlier ones. `counts` is 32 integers of shared memory.
-template <class Cost, class Tiles>
-__device__ __forceinline__ void fill_table(const Table& table, int* counts, const Groups& groups, int lane, Cost cost,
-                                           Tiles tiles) {
-  counts[lane] = 0;
+// One warp fills the table. cut(rows) gives a group's parts, each of `per_part` tiles,
+// and their size; cost(rows, size) the cost of its tiles, in [0, 31].
+template <class CutFn, class Cost>
+__device__ __forceinline__ void fill_table(const Table& table, const Groups& groups, int lane, int workers,
+                                           int per_part, CutFn cut, Cost cost) {
+  constexpr int kAhead = 4;  // ends that a lane loads at once
+  int carry = 0, before = 0;
+  for (int base = 0; base < groups.count; base += 32 * kAhead) {
+    int64_t value[kAhead];
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {
+      const int e = base + 32 * q + lane;
+      value[q] = e < groups.count ? group_end(groups, e) : 0;
+    }
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {
+      const int e = base + 32 * q + lane;
+      if (e - lane >= groups.count) break;
+      int begin, end;
+      group_rows(value[q], groups.rows, lane, carry, begin, end);
+      const Cut c = cut(end - begin);
+      const int tiles = e < groups.count ? c.parts * per_part : 0;
+      const int sum = inclusive_sum(tiles, lane);
+      if (e < groups.count) {
+        table.first_row[e] = begin;
+        table.parts[e] = c.parts;
+        table.size[e] = static_cast<uint16_t>(c.size);
+        table.order[e] = static_cast<uint16_t>(e);
+        table.first_tile[e] = before + sum - tiles;
+      }
+      before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+  }
+  if (lane == 0) {
+    table.first_row[groups.count] = carry;
+    table.first_tile[groups.count] = before;
+  }
+  table.counts[lane] = 0;
   __syncwarp();
-  int carry = 0;
+  if (before <= workers) return;
+  // A counting sort: the groups of each cost are counted, then placed behind the
+  // costlier ones.
   for (int base = 0; base < groups.count; base += 32) {
     const int e = base + lane;
-    int begin, end;
-    group_rows(groups, e, lane, carry, begin, end);
-    if (e < groups.count) table.first_row[e] = begin;
-    const int c = e < groups.count ? cost(end - begin) : 32;
+    const int c = e < groups.count ? cost(table.rows(e), table.size[e]) : 32;
     const uint32_t same = __match_any_sync(0xffffffffu, c);
-    if (c < 32 && lane == __ffs(same) - 1) counts[c] += __popc(same);
+    if (c < 32 && lane == __ffs(same) - 1) table.counts[c] += __popc(same);
     __syncwarp();
   }
-  if (lane == 0) table.first_row[groups.count] = carry;
-  // Place of the next group of cost `lane`: behind all costlier ones.
-  const int with_cost = counts[lane];
+  const int with_cost = table.counts[lane];
   int place = with_cost;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int other = __shfl_down_sync(0xffffffffu, place, o);
     if (lane + o < 32) place += other;
   }
-  counts[lane] = place - with_cost;
+  table.counts[lane] = place - with_cost;  // the costlier groups
   __syncwarp();
   for (int base = 0; base < groups.count; base += 32) {
     const int e = base + lane;
-    const int c = e < groups.count ? cost(table.first_row[e + 1] - table.first_row[e]) : 32;
+    const int c = e < groups.count ? cost(table.rows(e), table.size[e]) : 32;
     const uint32_t same = __match_any_sync(0xffffffffu, c);
-    const int at = c < 32 ? counts[c] : 0;
+    const int at = c < 32 ? table.counts[c] : 0;
     __syncwarp();
     if (c < 32) {
       table.order[at + __popc(same & ((1u << lane) - 1u))] = static_cast<uint16_t>(e);
-      if (lane == __ffs(same) - 1) counts[c] = at + __popc(same);
+      if (lane == __ffs(same) - 1) table.counts[c] = at + __popc(same);
     }
     __syncwarp();
   }
-  int before = 0;
+  before = 0;
   for (int base = 0; base < groups.count; base += 32) {
     const int i = base + lane;
-    int n = 0;
-    if (i < groups.count) {
-      const int e = table.order[i];
-      n = tiles(table.first_row[e + 1] - table.first_row[e]);
-    }
-    int sum = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int other = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += other;
-    }
-    if (i < groups.count) table.first_tile[i] = before + sum - n;
+    const int tiles = i < groups.count ? table.parts[table.order[i]] * per_part : 0;
+    const int sum = inclusive_sum(tiles, lane);
+    if (i < groups.count) table.first_tile[i] = before + sum - tiles;
     before += __shfl_sync(0xffffffffu, sum, 31);
   }
-  if (lane == 0) table.first_tile[groups.count] = before;
 }
 
 struct Output {
@@ -364,18 +395,26 @@ struct RowsTile {
   int e, row0, rows, f;
 };
 
-template <int TOK, int GRAIN>
-__device__ __forceinline__ RowsTile rows_tile(const Table& table, int t, int& place) {
-  while (t >= table.first_tile[place + 1]) ++place;
+__device__ __forceinline__ RowsTile rows_tile(const Table& table, int count, int t, int& place) {
+  // Mostly the next tile is of the same place or the next one; else it is searched for.
+  if (t >= table.first_tile[place + 1] && t >= table.first_tile[++place + 1]) {
+    int hi = count - 1;
+    while (place < hi) {
+      const int mid = (place + hi + 1) >> 1;
+      if (table.first_tile[mid] <= t)
+        place = mid;
+      else
+        hi = mid - 1;
+    }
+  }
   RowsTile tile;
   tile.e = table.order[place];
-  const int begin = table.first_row[tile.e], rows = table.first_row[tile.e + 1] - begin;
-  const Cut cut = cut_group(rows, TOK, GRAIN);
+  const int parts = table.parts[tile.e], size = table.size[tile.e];
   const int l = t - table.first_tile[place];
-  tile.f = l / cut.parts;  // a group's row parts are neighbours: they share the expert's columns in L2
-  const int part = l - tile.f * cut.parts;
-  tile.row0 = begin + part * cut.size;
-  tile.rows = min(cut.size, rows - part * cut.size);
+  tile.f = l / parts;  // a group's row parts are neighbours: they share the expert's columns in L2
+  const int part = l - tile.f * parts;
+  tile.row0 = table.first_row[tile.e] + part * size;
+  tile.rows = min(size, table.first_row[tile.e + 1] - tile.row0);
   return tile;
 }
 
@@ -413,14 +452,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   const Barriers<S, PAIR> bar(smem_epi + kEpiWarps * Cfg::kSlotBytes);
   const Table table(smem_epi + kEpiWarps * Cfg::kSlotBytes + Barriers<S, PAIR>::kBytes);
 
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&map_right);
+    for (int i = 0; i < Cfg::kUnitRows / 32; ++i) tma_prefetch_desc(&map_rows.box[i]);
+  }
   const uint32_t tmem_base = set_up<S, PAIR>(bar, warp, Cfg::kTmemCols);
 
   // A tile's cost is its rows.
   if (warp == 0)
     fill_table(
-        table, reinterpret_cast<int*>(smem_epi), groups, lane,
-        [](int rows) { return (cut_group(rows, TOK, Cfg::kGrain).size * 31) / TOK; },
-        [&](int rows) { return cut_group(rows, TOK, Cfg::kGrain).parts * shape.feature_tiles; });
+        table, groups, lane, tile_step, shape.feature_tiles, [](int rows) { return cut_group(rows, TOK, Cfg::kGrain); },
+        [](int, int size) { return size * 31 / TOK; });
   __syncthreads();
   const int tiles = table.first_tile[groups.count];
 
@@ -431,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       const uint32_t full0 = PAIR ? cluster_addr(&bar.full[0], 0) : 0u;
       for (int t = tile_begin; t < tiles && ok; t += tile_step) {
-        const RowsTile tile = rows_tile<TOK, Cfg::kGrain>(table, t, place);
+        const RowsTile tile = rows_tile(table, groups.count, t, place);
         const int f0 = tile.f * Cfg::kFeatures + static_cast<int>(rank) * kBM;
         const int split = first_unit<Cfg>(tile);
         // This CTA's rows of each unit, and the smallest box that holds them.
@@ -507,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t ph = 0, acc_ph = 0;
       bool ok = true;
       for (int t = tile_begin; t < tiles && ok; t += tile_step) {
-        const RowsTile tile = rows_tile<TOK, Cfg::kGrain>(table, t, place);
+        const RowsTile tile = rows_tile(table, groups.count, t, place);
         const int split = first_unit<Cfg>(tile);
         int units = 0, buffer[2];
         uint32_t idesc[2];
@@ -574,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t acc_ph = 0;
     bool ok = true;
     for (int t = tile_begin; t < tiles && ok; t += tile_step) {
-      const RowsTile tile = rows_tile<TOK, Cfg::kGrain>(table, t, place);
+      const RowsTile tile = rows_tile(table, groups.count, t, place);
       const int f0 = tile.f * Cfg::kFeatures + static_cast<int>(rank) * kBM + quarter * 32;
       const int split = first_unit<Cfg>(tile);
       for (int first = 0; first < tile.rows; first += split) {
@@ -694,14 +736,18 @@ __global__ void __launch_bounds__(kReduceThreads, 1)
   // A stage is full when each CTA has arrived and the bytes are there: those of
   // both CTAs count on CTA 0's barrier, or, for a stage whose foreign rows are to be
   // zeroed, each CTA's on its own tail barrier, and the zeroing warps arrive.
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&map_l);
+    tma_prefetch_desc(&map_r);
+  }
   const uint32_t tmem_base = set_up<S, PAIR>(bar, warp, Cfg::kTmemCols, PAIR ? 2 : 1);
   // A tile's cost is its group's rows, in 31sts of a group twice as large as the mean.
   const int per_group = shape.tiles_m * shape.tiles_n;
   if (warp == 0) {
     const float unit = 31.0f * groups.count / (2.0f * groups.rows);
     fill_table(
-        table, reinterpret_cast<int*>(smem_epi), groups, lane, [&](int rows) { return min(31, static_cast<int>(rows * unit)); },
-        [&](int) { return per_group; });
+        table, groups, lane, tile_step, per_group, [](int) { return Cut{1, 0}; },
+        [&](int rows, int) { return min(31, static_cast<int>(rows * unit)); });
   }
   __syncthreads();
   const int tiles = per_group * groups.count;
