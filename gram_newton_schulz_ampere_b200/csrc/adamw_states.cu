@@ -253,7 +253,7 @@ __device__ __forceinline__ void step_eight(const float (&gf)[8], float (&pf)[8],
   decode8(vc, vf);
   // Every product and sum of the moments is rounded by itself (no fma). Elements go two
   // to an instruction: one at a time, the kernel issued 38 instructions an element and
-  // took 544 us for 323M bf16 elements.
+  // took 5% longer.
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
     const Pair g = mul2(Pair(gf[e], gf[e + 1]), Pair(s.scale));
@@ -290,44 +290,58 @@ __device__ __forceinline__ void step_eight(const float (&gf)[8], float (&pf)[8],
   vs = v_top * (1.0f / kE4M3Max);
 }
 
-// A block of `left` elements at `i` without any alignment: lane L holds elements
-// L, L + 32, ...
+// A lane's elements L, L + 32, ... of a block, wherever it starts: from `base` on, in
+// global or shared memory.
+__device__ __forceinline__ void gather8(const void* base, int lane, int left, int dt, float (&f)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = lane + 32 * e < left ? load_as_float(base, lane + 32 * e, dt) : 0.0f;
+}
+
+__device__ __forceinline__ uint2 gather_codes(const uint8_t* base, int lane, int left) {
+  uint2 c = make_uint2(0u, 0u);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t b = lane + 32 * e < left ? base[lane + 32 * e] : 0u;
+    (e < 4 ? c.x : c.y) |= b << (8 * (e & 3));
+  }
+  return c;
+}
+
+__device__ __forceinline__ void scatter8(void* base, int lane, int left, int dt, const float (&f)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (lane + 32 * e < left) store_from_float(base, lane + 32 * e, dt, f[e]);
+}
+
+__device__ __forceinline__ void scatter_codes(uint8_t* base, int lane, int left, uint2 c) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (lane + 32 * e < left) base[lane + 32 * e] = static_cast<uint8_t>((e < 4 ? c.x : c.y) >> (8 * (e & 3)));
+}
+
+// The last, incomplete block of a tensor: `left` elements at `i`.
 __device__ __noinline__ void step_ragged(const StateArgs& args, int t, int64_t i, int left, int p_dt, int g_dt,
                                          const StateScalars& k) {
   const int lane = threadIdx.x & 31;
-  void* p = args.p[t];
-  const void* g = args.g[t];
-  uint8_t* m = static_cast<uint8_t*>(args.m[t]);
-  uint8_t* v = static_cast<uint8_t*>(args.v[t]);
-  float* m_scale = args.m_scale[t];
-  float* v_scale = args.v_scale[t];
+  uint8_t* p = static_cast<uint8_t*>(args.p[t]) + i * (p_dt == kF32 ? 4 : 2);
+  const uint8_t* g = static_cast<const uint8_t*>(args.g[t]) + i * (g_dt == kF32 ? 4 : 2);
+  uint8_t* m = static_cast<uint8_t*>(args.m[t]) + i;
+  uint8_t* v = static_cast<uint8_t*>(args.v[t]) + i;
+  float* m_scale = args.m_scale[t] + i / kBlockElems;
+  float* v_scale = args.v_scale[t] + i / kBlockElems;
   const Step s(args, k, t);
   float pf[8], gf[8];
-  uint2 mc = make_uint2(0u, 0u), vc = make_uint2(0u, 0u);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int at = lane + 32 * e;
-    const bool in = at < left;
-    gf[e] = in ? load_as_float(g, i + at, g_dt) : 0.0f;
-    pf[e] = in ? load_as_float(p, i + at, p_dt) : 0.0f;
-    const uint32_t a = in ? m[i + at] : 0u, b = in ? v[i + at] : 0u;
-    (e < 4 ? mc.x : mc.y) |= a << (8 * (e & 3));
-    (e < 4 ? vc.x : vc.y) |= b << (8 * (e & 3));
-  }
-  const int64_t block = i / kBlockElems;
-  float ms = m_scale[block], vs = v_scale[block];
+  gather8(p, lane, left, p_dt, pf);
+  gather8(g, lane, left, g_dt, gf);
+  uint2 mc = gather_codes(m, lane, left), vc = gather_codes(v, lane, left);
+  float ms = *m_scale, vs = *v_scale;
   step_eight(gf, pf, mc, vc, ms, vs, k, s);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int at = lane + 32 * e;
-    if (at >= left) continue;
-    store_from_float(p, i + at, p_dt, pf[e]);
-    m[i + at] = static_cast<uint8_t>((e < 4 ? mc.x : mc.y) >> (8 * (e & 3)));
-    v[i + at] = static_cast<uint8_t>((e < 4 ? vc.x : vc.y) >> (8 * (e & 3)));
-  }
+  scatter8(p, lane, left, p_dt, pf);
+  scatter_codes(m, lane, left, mc);
+  scatter_codes(v, lane, left, vc);
   if (lane == 0) {
-    m_scale[block] = ms;
-    v_scale[block] = vs;
+    *m_scale = ms;
+    *v_scale = vs;
   }
 }
 
@@ -336,12 +350,12 @@ __device__ int g_states_status = 0;
 // Ring slots of a warp: a block's parameters, gradients and codes.
 constexpr int kSlots = 4;
 
-template <int P, int G>
+template <int P, int G, bool ALIGNED>
 struct Slot {
   static constexpr uint32_t kP = kBlockElems * (sixteen(P) ? 2 : 4);
   static constexpr uint32_t kG = kBlockElems * (sixteen(G) ? 2 : 4);
-  static constexpr uint32_t kM = kP + kG;
-  static constexpr uint32_t kBytes = kP + kG + 2 * kBlockElems;
+  static constexpr uint32_t kSpare = ALIGNED ? 0 : 16;  // for what a copy starts ahead of its row
+  static constexpr uint32_t kBytes = kP + kG + 2 * kBlockElems + 4 * kSpare;
   static constexpr size_t kSmem = static_cast<size_t>(kWarps) * kSlots * kBytes;
 };
 
@@ -349,15 +363,21 @@ struct Slot {
 // them from the arguments.
 //
 // Each warp steps consecutive blocks of the chunk. Bulk copies bring them into a
-// ring of its own, four blocks ahead: 48 KB in flight a CTA and 196 KB an SM
+// ring of its own, four blocks ahead: 48 KB in flight a CTA and 147 KB an SM
 // without a register held for it, and no barrier between warps. Loads into
 // registers kept 41 KB in flight and moved 2.9 TB/s, or 4.5 TB/s with the next
-// block prefetched (323M bf16 elements in 1129 and 717 us). The scales of the
-// warp's blocks are read and written once, a lane for each.
-template <int P, int G>
-__global__ void __launch_bounds__(kThreads, sixteen(P) && sixteen(G) ? 4 : 2)
+// block prefetched; the ring moves 6.3 TB/s, 0.98 of the measured copy rate (323M
+// bf16 elements in 1129, 717 and 515 us; four CTAs an SM at 64 registers instead of
+// three: 553). The scales of the warp's blocks are read and written once, a lane
+// for each.
+//
+// ALIGNED: all rows start on multiples of 16 bytes. Otherwise the copies start at the
+// multiples before and the lanes take single elements (a launch of its own: one
+// kernel for both was 1.4 times as slow on aligned tensors).
+template <int P, int G, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads, sixteen(P) && sixteen(G) ? 3 : 2)
     adamw_8bit_kernel(const __grid_constant__ StateArgs args, int p_rt, int g_rt, const __grid_constant__ StateScalars k) {
-  using S = Slot<P, G>;
+  using S = Slot<P, G, ALIGNED>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[kWarps][kSlots];
   __shared__ volatile int abort_flag;
@@ -379,10 +399,7 @@ __global__ void __launch_bounds__(kThreads, sixteen(P) && sixteen(G) ? 4 : 2)
   const int share = args.chunk / (kWarps * kBlockElems);
   const int first = warp * share;
   const int mine = min(max(count - first * kBlockElems, 0), share * kBlockElems);
-  int whole = mine / kBlockElems;
-  const uintptr_t all = reinterpret_cast<uintptr_t>(args.p[t]) | reinterpret_cast<uintptr_t>(args.g[t]) |
-                        reinterpret_cast<uintptr_t>(args.m[t]) | reinterpret_cast<uintptr_t>(args.v[t]);
-  if (all % 16 != 0) whole = 0;  // the copies need aligned rows: every block goes the ragged way
+  const int whole = mine / kBlockElems;
   if (whole > 0) {
     const Step s(args, k, t);
     const int64_t at0 = start + static_cast<int64_t>(first) * kBlockElems;
@@ -393,15 +410,26 @@ __global__ void __launch_bounds__(kThreads, sixteen(P) && sixteen(G) ? 4 : 2)
     float* m_scale = args.m_scale[t] + at0 / kBlockElems;
     float* v_scale = args.v_scale[t] + at0 / kBlockElems;
     const uint32_t p_bytes = kBlockElems * (p_dt == kF32 ? 4 : 2), g_bytes = kBlockElems * (g_dt == kF32 ? 4 : 2);
+    // Bytes of each behind a multiple of 16, the same for all blocks. A copy starts at
+    // that multiple and takes 16 bytes more: every 16 that it reads hold a byte of the block.
+    const uint32_t p_off = ALIGNED ? 0u : reinterpret_cast<uintptr_t>(p) & 15u;
+    const uint32_t g_off = ALIGNED ? 0u : reinterpret_cast<uintptr_t>(g) & 15u;
+    const uint32_t m_off = ALIGNED ? 0u : reinterpret_cast<uintptr_t>(m) & 15u;
+    const uint32_t v_off = ALIGNED ? 0u : reinterpret_cast<uintptr_t>(v) & 15u;
     uint8_t* ring = smem + static_cast<uint32_t>(warp * kSlots) * S::kBytes;
+    // g, m, v and the next slot behind p.
+    constexpr uint32_t at_g = S::kP + S::kSpare, at_m = at_g + S::kG + S::kSpare;
+    constexpr uint32_t at_v = at_m + kBlockElems + S::kSpare;
     auto fetch = [&](int i, int st) {
       uint8_t* slot = ring + static_cast<uint32_t>(st) * S::kBytes;
       uint64_t* bar = &full[warp][st];
-      mbar_arrive_expect_tx(bar, p_bytes + g_bytes + 2 * kBlockElems);
-      bulk_load(slot, p + static_cast<uint32_t>(i) * p_bytes, p_bytes, bar);
-      bulk_load(slot + S::kP, g + static_cast<uint32_t>(i) * g_bytes, g_bytes, bar);
-      bulk_load(slot + S::kM, m + i * kBlockElems, kBlockElems, bar);
-      bulk_load(slot + S::kM + kBlockElems, v + i * kBlockElems, kBlockElems, bar);
+      const uint32_t pn = p_bytes + (p_off ? 16u : 0u), gn = g_bytes + (g_off ? 16u : 0u);
+      const uint32_t mn = kBlockElems + (m_off ? 16u : 0u), vn = kBlockElems + (v_off ? 16u : 0u);
+      mbar_arrive_expect_tx(bar, pn + gn + mn + vn);
+      bulk_load(slot, p - p_off + static_cast<uint32_t>(i) * p_bytes, pn, bar);
+      bulk_load(slot + at_g, g - g_off + static_cast<uint32_t>(i) * g_bytes, gn, bar);
+      bulk_load(slot + at_m, m - m_off + i * kBlockElems, mn, bar);
+      bulk_load(slot + at_v, v - v_off + i * kBlockElems, vn, bar);
     };
     if (lane == 0)
       for (int i = 0; i < kSlots && i < whole; ++i) fetch(i, i);
@@ -419,21 +447,36 @@ __global__ void __launch_bounds__(kThreads, sixteen(P) && sixteen(G) ? 4 : 2)
       if (!ok) break;
       const uint8_t* slot = ring + static_cast<uint32_t>(st) * S::kBytes;
       float pf[8], gf[8];
-      Eight<P> pe;
-      Eight<G> ge;
-      pe.load(slot, 8 * lane, p_dt);
-      ge.load(slot + S::kP, 8 * lane, g_dt);
-      uint2 mc = reinterpret_cast<const uint2*>(slot + S::kM)[lane];
-      uint2 vc = reinterpret_cast<const uint2*>(slot + S::kM + kBlockElems)[lane];
-      pe.get(p_dt, pf);
-      ge.get(g_dt, gf);
+      uint2 mc, vc;
+      if (ALIGNED) {  // lane L: elements 8 L .. 8 L + 7
+        Eight<P> pe;
+        Eight<G> ge;
+        pe.load(slot, 8 * lane, p_dt);
+        ge.load(slot + at_g, 8 * lane, g_dt);
+        mc = reinterpret_cast<const uint2*>(slot + at_m)[lane];
+        vc = reinterpret_cast<const uint2*>(slot + at_v)[lane];
+        pe.get(p_dt, pf);
+        ge.get(g_dt, gf);
+      } else {  // lane L: elements L, L + 32, ..
+        gather8(slot + p_off, lane, kBlockElems, p_dt, pf);
+        gather8(slot + at_g + g_off, lane, kBlockElems, g_dt, gf);
+        mc = gather_codes(slot + at_m + m_off, lane, kBlockElems);
+        vc = gather_codes(slot + at_v + v_off, lane, kBlockElems);
+      }
       __syncwarp();  // every lane has read the slot: it is filled again
       if (lane == 0 && i + kSlots < whole) fetch(i + kSlots, st);
       float ms = __shfl_sync(0xffffffffu, my_ms, i), vs = __shfl_sync(0xffffffffu, my_vs, i);
       step_eight(gf, pf, mc, vc, ms, vs, k, s);
-      store8(p + static_cast<uint32_t>(i) * p_bytes, 8 * lane, p_dt, pf);
-      reinterpret_cast<uint2*>(m + i * kBlockElems)[lane] = mc;
-      reinterpret_cast<uint2*>(v + i * kBlockElems)[lane] = vc;
+      uint8_t* to = p + static_cast<uint32_t>(i) * p_bytes;
+      if (ALIGNED) {
+        store8(to, 8 * lane, p_dt, pf);
+        reinterpret_cast<uint2*>(m + i * kBlockElems)[lane] = mc;
+        reinterpret_cast<uint2*>(v + i * kBlockElems)[lane] = vc;
+      } else {
+        scatter8(to, lane, kBlockElems, p_dt, pf);
+        scatter_codes(m + i * kBlockElems, lane, kBlockElems, mc);
+        scatter_codes(v + i * kBlockElems, lane, kBlockElems, vc);
+      }
       if (lane == i) {
         my_ms = ms;
         my_vs = vs;
@@ -508,28 +551,39 @@ __global__ void __launch_bounds__(kThreads) adamw_32bit_kernel(const __grid_cons
 }
 
 std::mutex g_mutex;
-bool g_ready[64][8] = {};
+bool g_ready[64][16] = {};
+
+template <int P, int G, bool ALIGNED>
+int launch_8bit(int blocks, cudaStream_t st, const StateArgs& a, int p_dt, int g_dt, const StateScalars& k, int slot) {
+  constexpr size_t smem = Slot<P, G, ALIGNED>::kSmem;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  if (dev < 0 || dev >= 64) return fail(GNS_ERR_DEVICE, "device index out of range");
+  {
+    std::lock_guard<std::mutex> lock(g_mutex);
+    if (!g_ready[dev][slot]) {
+      e = cudaFuncSetAttribute(adamw_8bit_kernel<P, G, ALIGNED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(smem));
+      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(smem)");
+      g_ready[dev][slot] = true;
+    }
+  }
+  adamw_8bit_kernel<P, G, ALIGNED><<<blocks, kThreads, smem, st>>>(a, p_dt, g_dt, k);
+  return GNS_OK;
+}
 
 template <int P, int G>
-int launch(int bits, int blocks, cudaStream_t st, const StateArgs& a, int p_dt, int g_dt, const StateScalars& k, int slot) {
-  if (bits == 8) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
-    if (dev < 0 || dev >= 64) return fail(GNS_ERR_DEVICE, "device index out of range");
-    {
-      std::lock_guard<std::mutex> lock(g_mutex);
-      if (!g_ready[dev][slot]) {
-        e = cudaFuncSetAttribute(adamw_8bit_kernel<P, G>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 static_cast<int>(Slot<P, G>::kSmem));
-        if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(smem)");
-        g_ready[dev][slot] = true;
-      }
-    }
-    adamw_8bit_kernel<P, G><<<blocks, kThreads, Slot<P, G>::kSmem, st>>>(a, p_dt, g_dt, k);
-  } else {
+int launch(int bits, bool aligned, int blocks, cudaStream_t st, const StateArgs& a, int p_dt, int g_dt,
+           const StateScalars& k, int slot) {
+  int rc = GNS_OK;
+  if (bits == 32)
     adamw_32bit_kernel<P, G><<<blocks, kThreads, 0, st>>>(a, p_dt, g_dt, k);
-  }
+  else if (aligned)
+    rc = launch_8bit<P, G, true>(blocks, st, a, p_dt, g_dt, k, 2 * slot);
+  else
+    rc = launch_8bit<P, G, false>(blocks, st, a, p_dt, g_dt, k, 2 * slot + 1);
+  if (rc != GNS_OK) return rc;
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? GNS_OK : cuda_fail(e, "adamw states kernel");
 }
@@ -579,48 +633,56 @@ extern "C" int gns_adamw_states_step(int count, void* const* params, const void*
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const StateScalars k{beta1, one_minus_beta1, beta2, one_minus_beta2, epsilon, decay, grad_scale};
   // Long chunks keep a warp's ring going; short ones give every SM work. Elements are
-  // divided into 32 chunks an SM (eight turns of its four CTAs) where there are enough.
+  // divided into 32 chunks an SM (about eleven turns of its three CTAs) where there are enough.
   int64_t total = 0;
   for (int i = 0; i < count; ++i) total += numel[i];
   int chunk = kChunkMin;
   while (chunk < kChunkMax && total / chunk > 32 * static_cast<int64_t>(device_sm_count())) chunk *= 2;
-  int i = 0;
-  while (i < count) {
-    StateArgs a;
-    a.count = 0;
-    a.chunk = chunk;
-    int64_t blocks = 0;
-    for (; i < count && a.count < kTensors; ++i) {
-      if (numel[i] == 0) continue;
-      const int64_t nb = (numel[i] + chunk - 1) / chunk;
-      if (blocks > 0 && blocks + nb > (1ll << 30)) break;  // next launch
-      const int j = a.count++;
-      a.p[j] = params[i];
-      a.g[j] = grads[i];
-      a.m[j] = exp_avgs[i];
-      a.v[j] = exp_avg_sqs[i];
-      a.m_scale[j] = state_bits == 8 ? exp_avg_scales[i] : nullptr;
-      a.v_scale[j] = state_bits == 8 ? exp_avg_sq_scales[i] : nullptr;
-      a.numel[j] = numel[i];
-      a.lr_bc1[j] = lr_bc1[i];
-      a.inv_bc2[j] = inv_bc2[i];
-      a.block_start[j] = static_cast<int>(blocks);
-      blocks += nb;
+  // 8-bit states: the tensors whose rows all start on 16 bytes, then the others.
+  auto is_aligned = [&](int i) {
+    const uintptr_t all = reinterpret_cast<uintptr_t>(params[i]) | reinterpret_cast<uintptr_t>(grads[i]) |
+                          reinterpret_cast<uintptr_t>(exp_avgs[i]) | reinterpret_cast<uintptr_t>(exp_avg_sqs[i]);
+    return state_bits == 32 || all % 16 == 0;
+  };
+  for (bool aligned : {true, false}) {
+    int i = 0;
+    while (i < count) {
+      StateArgs a;
+      a.count = 0;
+      a.chunk = chunk;
+      int64_t blocks = 0;
+      for (; i < count && a.count < kTensors; ++i) {
+        if (numel[i] == 0 || is_aligned(i) != aligned) continue;
+        const int64_t nb = (numel[i] + chunk - 1) / chunk;
+        if (blocks > 0 && blocks + nb > (1ll << 30)) break;  // next launch
+        const int j = a.count++;
+        a.p[j] = params[i];
+        a.g[j] = grads[i];
+        a.m[j] = exp_avgs[i];
+        a.v[j] = exp_avg_sqs[i];
+        a.m_scale[j] = state_bits == 8 ? exp_avg_scales[i] : nullptr;
+        a.v_scale[j] = state_bits == 8 ? exp_avg_sq_scales[i] : nullptr;
+        a.numel[j] = numel[i];
+        a.lr_bc1[j] = lr_bc1[i];
+        a.inv_bc2[j] = inv_bc2[i];
+        a.block_start[j] = static_cast<int>(blocks);
+        blocks += nb;
+      }
+      if (a.count == 0) break;
+      a.block_start[a.count] = static_cast<int>(blocks);
+      const int grid = static_cast<int>(blocks);
+      if (p_dtype == kBF16 && g_dtype == kBF16)
+        rc = launch<kBF16, kBF16>(state_bits, aligned, grid, st, a, p_dtype, g_dtype, k, 0);
+      else if (p_dtype == kF32 && g_dtype == kF32)
+        rc = launch<kF32, kF32>(state_bits, aligned, grid, st, a, p_dtype, g_dtype, k, 1);
+      else if (p_dtype == kF16 && g_dtype == kF16)
+        rc = launch<kF16, kF16>(state_bits, aligned, grid, st, a, p_dtype, g_dtype, k, 2);
+      else if (p_dtype == kBF16 && g_dtype == kF32)
+        rc = launch<kBF16, kF32>(state_bits, aligned, grid, st, a, p_dtype, g_dtype, k, 3);
+      else
+        rc = launch<-1, -1>(state_bits, aligned, grid, st, a, p_dtype, g_dtype, k, 4);
+      if (rc != GNS_OK) return rc;
     }
-    if (a.count == 0) break;
-    a.block_start[a.count] = static_cast<int>(blocks);
-    const int grid = static_cast<int>(blocks);
-    if (p_dtype == kBF16 && g_dtype == kBF16)
-      rc = launch<kBF16, kBF16>(state_bits, grid, st, a, p_dtype, g_dtype, k, 0);
-    else if (p_dtype == kF32 && g_dtype == kF32)
-      rc = launch<kF32, kF32>(state_bits, grid, st, a, p_dtype, g_dtype, k, 1);
-    else if (p_dtype == kF16 && g_dtype == kF16)
-      rc = launch<kF16, kF16>(state_bits, grid, st, a, p_dtype, g_dtype, k, 2);
-    else if (p_dtype == kBF16 && g_dtype == kF32)
-      rc = launch<kBF16, kF32>(state_bits, grid, st, a, p_dtype, g_dtype, k, 3);
-    else
-      rc = launch<-1, -1>(state_bits, grid, st, a, p_dtype, g_dtype, k, 4);
-    if (rc != GNS_OK) return rc;
   }
   return GNS_OK;
 }
