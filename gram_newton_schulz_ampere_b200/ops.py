@@ -1067,20 +1067,62 @@ class AdamWStates:
 
 
 # ------------------------------------------------- products grouped by expert
-def _row_operand(t: Tensor) -> Tensor:
+def _aligned_copy(t: Tensor, batch: int, rows: int, cols: int, batch_stride: int, row_stride: int) -> tuple[Tensor, int]:
+    """A buffer with a copy of the rows [batch, rows, cols] that start at `t`'s first element, with
+    unit column stride, and its row pitch, a multiple of 8 elements."""
+    pitch = (cols + 7) // 8 * 8
+    buffer = torch.empty(batch * rows * pitch, dtype=t.dtype, device=t.device)
+    lib = nat.load()
+    with nat.on_device(t.get_device()) as stream:
+        rc = lib.gns_align_rows(batch, rows, cols, t.data_ptr(), batch_stride, row_stride, buffer.data_ptr(),
+                                rows * pitch, pitch, stream)
+    nat.check(rc, "gns_align_rows")
+    return buffer, pitch
+
+
+def row_operand(t: Tensor) -> Tensor:
     """Returns the matrix `t` if a TMA tile load can read its rows (unit column stride,
     16-byte aligned base and row stride), else a copy whose row pitch is padded to a
-    multiple of 8 elements."""
+    multiple of 8 elements. The grouped products make such a copy themselves; a caller
+    that passes a matrix to several of them saves the others with this."""
     rows, cols = t.shape
-    if (
-        t.data_ptr() % 16 == 0
-        and (t.stride(1) == 1 or cols == 1)
-        and ((t.stride(0) % 8 == 0 and t.stride(0) >= cols) or rows == 1)
-    ):
-        return t
-    view = _padded(1, rows, cols, t.dtype, t.device)[0]
-    view.copy_(t)
-    return view
+    held, _, pitch = _row_layout(t)
+    return t if held is t else held.as_strided((rows, cols), (pitch, 1))
+
+
+def _row_layout(t: Tensor) -> tuple[Tensor, int, int]:
+    """(owner, address, row stride) of the matrix `t` or of a copy of it that TMA can read."""
+    rows, cols = t.shape
+    sr, sc = t.stride()
+    place = t.data_ptr()
+    if place % 16 == 0 and (sc == 1 or cols == 1) and ((sr % 8 == 0 and sr >= cols) or rows == 1):
+        return t, place, sr
+    if sc != 1 and cols > 1:
+        t, sr = t.contiguous(), cols
+    copy, pitch = _aligned_copy(t, 1, rows, cols, 0, sr)
+    return copy, copy.data_ptr(), pitch
+
+
+def _group_layout(t: Tensor) -> tuple[Tensor, int, int, int, int]:
+    """(owner, address, strides) of one matrix per group [groups, k, n], stored by rows or by
+    columns, or of a copy of it, in the same order, that TMA can read."""
+    groups, k, n = t.shape
+    sg, sk, sn = t.stride()
+    place = t.data_ptr()
+    sound = place % 16 == 0 and ((sg % 8 == 0 and sg != 0) or groups == 1)
+    by_rows, by_columns = sn == 1 or n == 1, sk == 1 or k == 1
+    if sound and by_rows and ((sk % 8 == 0 and sk >= n) or k == 1):
+        return t, place, sg, sk, 1
+    if sound and by_columns and ((sn % 8 == 0 and sn >= k) or n == 1):
+        return t, place, sg, 1, sn
+    if not (by_rows or by_columns):
+        t = t.contiguous()
+        sg, sk, sn, by_rows = k * n, n, 1, True
+    if by_rows:
+        copy, pitch = _aligned_copy(t, groups, k, n, sg, sk)
+        return copy, copy.data_ptr(), k * pitch, pitch, 1
+    copy, pitch = _aligned_copy(t, groups, n, k, sg, sn)
+    return copy, copy.data_ptr(), n * pitch, 1, pitch
 
 
 def _group_ends(ends: Tensor, groups: int | None = None) -> Tensor:
@@ -1121,16 +1163,13 @@ def grouped_gemm(left: Tensor, right: Tensor, ends: Tensor, out_dtype: torch.dty
     if rows == 0 or n == 0 or k == 0 or groups == 0:
         return torch.zeros((rows, n), dtype=dtype, device=left.device)
     out = torch.empty((rows, n), dtype=dtype, device=left.device)
-    a = _row_operand(left)
-    if 0 in right.stride():
-        right = right.contiguous()  # a TMA map has no zero strides
-    b = _aligned_operand(right)
+    left_held, left_at, left_pitch = _row_layout(left)
+    right_held, *right_layout = _group_layout(right)
     lib = nat.load()
     with nat.on_device(index) as stream:
         rc = lib.gns_grouped_gemm(
-            nat.dtype_code(a.dtype), rows, n, k, groups, a.data_ptr(), a.stride(0),
-            b.data_ptr(), b.stride(0), b.stride(1), b.stride(2), ends.data_ptr(), 8 * ends.element_size(),
-            out.data_ptr(), code, out.stride(0), stream,
+            nat.dtype_code(left.dtype), rows, n, k, groups, left_at, left_pitch, *right_layout,
+            ends.data_ptr(), 8 * ends.element_size(), out.data_ptr(), code, n, stream,
         )
     nat.check(rc, "gns_grouped_gemm")
     return out
@@ -1156,12 +1195,13 @@ def grouped_gemm_reduce(left: Tensor, right: Tensor, ends: Tensor, out_dtype: to
     if rows == 0 or m == 0 or n == 0 or groups == 0:
         return torch.zeros((groups, m, n), dtype=dtype, device=left.device)
     out = torch.empty((groups, m, n), dtype=dtype, device=left.device)
-    a, b = _row_operand(left), _row_operand(right)
+    left_held, left_at, left_pitch = _row_layout(left)
+    right_held, right_at, right_pitch = _row_layout(right)
     lib = nat.load()
     with nat.on_device(index) as stream:
         rc = lib.gns_grouped_gemm_reduce(
-            nat.dtype_code(a.dtype), rows, m, n, groups, a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0),
-            ends.data_ptr(), 8 * ends.element_size(), out.data_ptr(), code, out.stride(0), out.stride(1), stream,
+            nat.dtype_code(left.dtype), rows, m, n, groups, left_at, left_pitch, right_at, right_pitch,
+            ends.data_ptr(), 8 * ends.element_size(), out.data_ptr(), code, m * n, n, stream,
         )
     nat.check(rc, "gns_grouped_gemm_reduce")
     return out

@@ -52,6 +52,7 @@ class _GroupedLinear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad: Tensor):  # type: ignore[no-untyped-def]
         x, weight, ends = ctx.saved_tensors
+        grad = ops.row_operand(grad)  # a copy for TMA, if one is needed, is made once
         dx = ops.grouped_gemm(grad, weight, ends) if ctx.needs_input_grad[0] else None
         dweight = ops.grouped_gemm_reduce(grad, x, ends) if ctx.needs_input_grad[1] else None
         return dx, dweight, None

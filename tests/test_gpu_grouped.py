@@ -220,3 +220,22 @@ def test_refusals(cuda_device):
         ops.grouped_gemm(left, right, ends, torch.float64)
     with pytest.raises(RuntimeError, match="1024 groups"):
         ops.grouped_gemm(left, right[:1].expand(1025, 16, 8), torch.zeros(1025, device=cuda_device, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(1, 1, 1), (1, 3, 7), (2, 5, 8), (3, 17, 65), (1, 200, 1023), (4, 9, 16)])
+@pytest.mark.parametrize("offset", [0, 1, 2, 3, 5, 7])
+def test_rows_are_copied_as_they_are(cuda_device, batch, rows, cols, offset):
+    """Slices that start on any element, with any row pitch, and transposed ones."""
+    size = batch * rows * (cols + 3) + offset
+    flat = torch.arange(size, device=cuda_device).to(torch.int16).view(torch.bfloat16)
+    source = flat[offset:].view(batch, rows, cols + 3)[:, :, :cols]
+    copy, place, pitch = ops._row_layout(source[-1])
+    assert pitch % 8 == 0 and place % 16 == 0 or rows == 1
+    assert torch.equal(ops.row_operand(source[-1]).view(torch.int16), source[-1].view(torch.int16))
+    copy, place, *strides = ops._group_layout(source)
+    assert torch.equal(copy.as_strided(source.shape, strides).contiguous().view(torch.int16),
+                       source.contiguous().view(torch.int16))
+    turned = source.transpose(1, 2)
+    copy, place, *strides = ops._group_layout(turned)
+    assert torch.equal(copy.as_strided(turned.shape, strides).contiguous().view(torch.int16),
+                       turned.contiguous().view(torch.int16))
