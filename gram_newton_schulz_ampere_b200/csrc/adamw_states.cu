@@ -91,32 +91,6 @@ __device__ __forceinline__ float reciprocal_approx(float x) {
   return r;
 }
 
-// Two fp32 values worked on by one instruction, each rounded as a scalar one would.
-struct Pair {
-  uint64_t bits;
-
-  __device__ __forceinline__ Pair() {}
-  __device__ __forceinline__ Pair(float x, float y) {
-    asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(x), "f"(y));
-  }
-  __device__ __forceinline__ explicit Pair(float both) : Pair(both, both) {}
-  __device__ __forceinline__ void get(float& x, float& y) const {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(bits));
-  }
-};
-
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
-  Pair r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
-  return r;
-}
-
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-  Pair r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
-  return r;
-}
-
 // The larger magnitude; NaN if either is.
 __device__ __forceinline__ float larger(float top, float x) {
   float r;

@@ -360,6 +360,40 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(int ab_bf16, int a_mn_majo
          ((static_cast<uint32_t>(m) >> 4) << 24);
 }
 
+// ------------------------------------------------------- paired fp32
+// Two fp32 values worked on by one instruction, each rounded as a scalar one would
+// (an add of a product may be fused with it).
+struct Pair {
+  uint64_t bits;
+
+  __device__ __forceinline__ Pair() {}
+  __device__ __forceinline__ Pair(float x, float y) {
+    asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(x), "f"(y));
+  }
+  __device__ __forceinline__ explicit Pair(float both) : Pair(both, both) {}
+  __device__ __forceinline__ void get(float& x, float& y) const {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(bits));
+  }
+};
+
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+  return r;
+}
+
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+  return r;
+}
+
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+  return r;
+}
+
 // ------------------------------------------------------------ conversions
 __device__ __forceinline__ float load_as_float(const void* base, int64_t idx, int dtype) {
   if (dtype == kF32) return static_cast<const float*>(base)[idx];
