@@ -147,7 +147,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [c_int, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _I64, _I64, _P, c_int, _P, c_int, _I64, _P],
     ),
-    "gns_align_rows": (c_int, [_I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P]),
+    "gns_align_rows": (c_int, [_I64, _I64, _I64, _P, _I64, _I64, _P, c_int, _P, _I64, _I64, _P]),
     "gns_grouped_gemm_reduce": (
         c_int,
         [c_int, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _P, c_int, _P, c_int, _I64, _I64, _P],

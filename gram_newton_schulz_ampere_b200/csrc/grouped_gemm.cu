@@ -993,14 +993,15 @@ __global__ void __launch_bounds__(kReduceThreads, 1)
 // Copies 16-bit rows that start anywhere into rows that start on 16 bytes, the rows
 // that TMA can read. A thread writes 16 bytes: it reads the two aligned 16-byte words
 // that hold them (the second only if the row reaches into it) and shifts. Bound by
-// HBM; a strided copy by single elements moved 1.2 TB/s (32 x 2048 x 1025).
+// HBM; a strided copy by single elements moved 1.2 TB/s (32 x 2048 x 1025). With
+// `ends`, matrices of groups without rows are left out: nothing reads them.
 constexpr int kPadThreads = 256;
 constexpr int kPadItems = 4;  // of a thread
 
 __global__ void __launch_bounds__(kPadThreads) pad_rows_kernel(const uint16_t* src, int64_t src_bstride,
                                                                int64_t src_rstride, uint16_t* dst, int64_t dst_bstride,
                                                                int64_t dst_rstride, uint32_t rows, uint32_t cols,
-                                                               uint32_t words, int64_t items) {
+                                                               uint32_t words, int64_t items, const Groups groups) {
   uint4 lo[kPadItems], hi[kPadItems];
   uint32_t shift[kPadItems];
   uint16_t* to[kPadItems];
@@ -1013,6 +1014,11 @@ __global__ void __launch_bounds__(kPadThreads) pad_rows_kernel(const uint16_t* s
     const int64_t line = item / words;
     const uint32_t word = static_cast<uint32_t>(item - line * words);
     const int64_t b = line / rows, r = line - b * rows;
+    // (Whatever the ends are, a group with rows ends behind the one before it.)
+    if (groups.ends != nullptr) {
+      const int e = static_cast<int>(b);
+      if (group_end(groups, e) <= (e > 0 ? group_end(groups, e - 1) : 0)) continue;
+    }
     const uintptr_t row = reinterpret_cast<uintptr_t>(src + b * src_bstride + r * src_rstride);
     const uintptr_t at = row + word * 16u, end = row + static_cast<uintptr_t>(cols) * 2u;
     const uint4* from = reinterpret_cast<const uint4*>(at & ~uintptr_t(15));
@@ -1226,11 +1232,14 @@ int gns_grouped_gemm(int ab_dtype, int64_t rows, int64_t n, int64_t k, int64_t g
 }
 
 int gns_align_rows(int64_t batch, int64_t rows, int64_t cols, const void* src, int64_t src_bstride, int64_t src_rstride,
-                   void* dst, int64_t dst_bstride, int64_t dst_rstride, gns_stream_t stream) {
+                   const void* ends, int ends_bits, void* dst, int64_t dst_bstride, int64_t dst_rstride,
+                   gns_stream_t stream) {
   clear_error();
+  if (ends != nullptr && ends_bits != 32 && ends_bits != 64) return fail(GNS_ERR_ARGUMENT, "ends must have 32 or 64 bits");
   if (batch < 0 || rows < 0 || cols < 0) return fail(GNS_ERR_ARGUMENT, "negative dimension");
   if (batch == 0 || rows == 0 || cols == 0) return GNS_OK;
-  if (rows > (1ll << 31) || cols > (1ll << 31)) return fail(GNS_ERR_UNSUPPORTED, "dimension beyond kernel limits");
+  if (rows > (1ll << 31) || cols > (1ll << 31) || batch > (1ll << 30))
+    return fail(GNS_ERR_UNSUPPORTED, "dimension beyond kernel limits");
   if (src == nullptr || dst == nullptr) return fail(GNS_ERR_ARGUMENT, "null tensor");
   const int64_t words = (cols + 7) / 8;
   if (reinterpret_cast<uintptr_t>(src) % 2 != 0) return fail(GNS_ERR_LAYOUT, "source must be aligned to its elements");
@@ -1243,7 +1252,8 @@ int gns_align_rows(int64_t batch, int64_t rows, int64_t cols, const void* src, i
   if (blocks > (1ll << 31) - 1) return fail(GNS_ERR_UNSUPPORTED, "too many rows");
   pad_rows_kernel<<<static_cast<unsigned>(blocks), kPadThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
       static_cast<const uint16_t*>(src), src_bstride, src_rstride, static_cast<uint16_t*>(dst), dst_bstride, dst_rstride,
-      static_cast<uint32_t>(rows), static_cast<uint32_t>(cols), static_cast<uint32_t>(words), items);
+      static_cast<uint32_t>(rows), static_cast<uint32_t>(cols), static_cast<uint32_t>(words), items,
+      Groups{ends, ends_bits == 64 ? 1 : 0, static_cast<int>(batch), 0});
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? GNS_OK : cuda_fail(e, "align rows kernel");
 }

@@ -45,6 +45,8 @@ struct NormArgs {
   float* mean;
   float* rstd;
   float* partial;  // [CTA][2][cols]: sums of dy h and of dy
+  void* dw;        // not null: the grid is one CTA, which writes dw and db (may be null) itself
+  void* db;
   int64_t rows;
   int cols, w_dt, parts;
   float eps;
@@ -239,7 +241,14 @@ template <int TPR, class P>
 __device__ __forceinline__ void write_partial(const NormArgs& a, const float (&dw)[kPer], const float (&db)[kPer],
                                               float* joined, int t, int group) {
   constexpr int kGroups = threads_of<TPR>() / TPR;
-  float* out = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
+  auto put = [&](int which, int c, float sum) {
+    if (a.dw == nullptr)
+      a.partial[(static_cast<int64_t>(blockIdx.x) * 2 + which) * a.cols + c] = sum;
+    else if (which == 0)
+      store_from_float(a.dw, c, a.w_dt, sum);
+    else if (a.db != nullptr)
+      store_from_float(a.db, c, a.w_dt, sum);
+  };
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     if (kGroups > 1) {
@@ -253,14 +262,14 @@ __device__ __forceinline__ void write_partial(const NormArgs& a, const float (&d
           float sum = 0.0f;
           for (int q = 0; q < kGroups; ++q) sum += joined[(q * kPer + i) * TPR + t];
           const int c = P::col(t, i);
-          if (c < a.cols) out[which * a.cols + c] = sum;
+          if (c < a.cols) put(which, c, sum);
         }
       }
     } else {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int c = P::col(t, i);
-        if (c < a.cols) out[which * a.cols + c] = which ? db[i] : dw[i];
+        if (c < a.cols) put(which, c, which ? db[i] : dw[i]);
       }
     }
   }
@@ -739,6 +748,15 @@ Plan plan_norm(bool backward, bool vec, int x_dt, int64_t rows, int64_t cols) {
   return p;
 }
 
+// A backward pass of up to four turns runs in one CTA, which writes the weight's and
+// bias's gradients itself: one launch less, against turns of about a microsecond.
+constexpr int kLoneTurns = 4;
+
+bool is_lone(const Plan& p, int64_t rows) {
+  const int groups = (p.tpr < 256 ? 256 : p.tpr) / p.tpr;
+  return !p.wide && rows <= static_cast<int64_t>(kLoneTurns) * groups;
+}
+
 // Partial sums of a backward pass: one of each CTA, or of each of 64 sets of rows.
 int backward_parts(const Plan& p, int64_t rows) { return p.wide ? static_cast<int>(rows < 64 ? rows : 64) : p.grid; }
 
@@ -875,7 +893,10 @@ size_t gns_layer_norm_backward_workspace_size(int64_t rows, int64_t cols) {
   // The most that any type and alignment takes.
   int parts = 0;
   for (int dt : {kF16, kF32})
-    for (bool vec : {false, true}) parts = std::max(parts, backward_parts(plan_norm(true, vec, dt, rows, cols), rows));
+    for (bool vec : {false, true}) {
+      const Plan p = plan_norm(true, vec, dt, rows, cols);
+      if (!is_lone(p, rows)) parts = std::max(parts, backward_parts(p, rows));
+    }
   return static_cast<size_t>(parts) * 2 * static_cast<size_t>(cols) * sizeof(float);
 }
 
@@ -891,9 +912,10 @@ int gns_layer_norm_backward(int x_dtype, int w_dtype, int64_t rows, int64_t cols
   if (rows > 0 && (grad == nullptr || x == nullptr || weight == nullptr || mean == nullptr || rstd == nullptr ||
                    dx == nullptr))
     return fail(GNS_ERR_ARGUMENT, "null tensor");
-  if (workspace_bytes < gns_layer_norm_backward_workspace_size(rows, cols) || (rows > 0 && workspace == nullptr))
+  const size_t needed = gns_layer_norm_backward_workspace_size(rows, cols);
+  if (workspace_bytes < needed || (needed > 0 && workspace == nullptr))
     return fail(GNS_ERR_WORKSPACE, "layer norm backward workspace too small");
-  if (rows > 0 && reinterpret_cast<uintptr_t>(workspace) % 4 != 0)
+  if (needed > 0 && reinterpret_cast<uintptr_t>(workspace) % 4 != 0)
     return fail(GNS_ERR_WORKSPACE, "layer norm backward workspace must be aligned to 4 bytes");
   rc = check_device();
   if (rc != GNS_OK) return rc;
@@ -914,7 +936,12 @@ int gns_layer_norm_backward(int x_dtype, int w_dtype, int64_t rows, int64_t cols
   if (rows > 0) {
     const bool vec = rows_vector(x, x_rstride, cols, x_dtype) && rows_vector(grad, grad_rstride, cols, x_dtype) &&
                      rows_vector(dx, cols, cols, x_dtype);
-    const Plan plan = plan_norm(true, vec, x_dtype, rows, cols);
+    Plan plan = plan_norm(true, vec, x_dtype, rows, cols);
+    if (is_lone(plan, rows)) {
+      plan.grid = 1;
+      a.dw = dweight;
+      a.db = dbias;
+    }
     a.parts = backward_parts(plan, rows);
     if (plan.wide) {
       norm_backward_wide_kernel<<<plan.grid, kWideThreads, 0, st>>>(a, x_dtype);
@@ -924,6 +951,10 @@ int gns_layer_norm_backward(int x_dtype, int w_dtype, int64_t rows, int64_t cols
       rc = launch_any(true, vec, x_dtype, plan, st, a);
       if (rc != GNS_OK) return rc;
     }
+  }
+  if (a.dw != nullptr) {
+    const cudaError_t lone = cudaGetLastError();
+    return lone == cudaSuccess ? GNS_OK : cuda_fail(lone, "layer norm backward kernel");
   }
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];

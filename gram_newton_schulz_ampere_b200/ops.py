@@ -8,6 +8,7 @@ rejected and a missing native library raises.
 
 from __future__ import annotations
 
+import array
 import contextlib
 import ctypes
 import os
@@ -909,6 +910,12 @@ def lion_step(
 STATE_BLOCK = 256  # consecutive elements of a tensor that share a scale of the 8-bit states
 
 
+def _pointers(tensors: Sequence[Tensor]) -> ctypes.Array:
+    """``_ptr_array`` of many tensors, at a quarter of its cost for each."""
+    places = array.array("Q", [t.data_ptr() for t in tensors])
+    return (ctypes.c_void_p * len(places)).from_buffer(places)
+
+
 class AdamWStates:
     """The AdamW moments of a list of parameters, in 32 bits or in 8, and the step over them.
 
@@ -1013,7 +1020,7 @@ class AdamWStates:
             raise ValueError(f"betas must be in [0, 1), got {(beta1, beta2)}")
         if not epsilon > 0.0:
             raise ValueError(f"epsilon must be positive, got {epsilon}")
-        whole = not any(g is None for g in gradients)
+        whole = all(map(torch.is_tensor, gradients))
         present = range(count) if whole else [i for i, g in enumerate(gradients) if g is not None]
         if not present:
             return
@@ -1022,13 +1029,13 @@ class AdamWStates:
         g_dtype = given[0].dtype
         if len({g.dtype for g in given}) > 1:
             raise TypeError("all gradients of one call must share a dtype")
-        numel = [g.numel() for g in given]
+        numel = list(map(Tensor.numel, given))
         if numel != (self._numel if whole else [self._numel[i] for i in present]):
             raise ValueError("gradient and parameter sizes differ")
         if not (all(map(Tensor.is_contiguous, given)) and all(map(Tensor.is_contiguous, places))):
             raise ValueError("gradients and parameters must be contiguous")
         index = cast(torch.device, self.device).index
-        if {t.get_device() for t in (*given, *places)} != {index}:
+        if set(map(Tensor.get_device, given)) != {index} or set(map(Tensor.get_device, places)) != {index}:
             raise ValueError("gradients must be on the parameters' device")
         if gradient_scale is not None:
             if gradient_scale.dtype != torch.float32 or gradient_scale.numel() != 1:
@@ -1052,7 +1059,7 @@ class AdamWStates:
         lib = nat.load()
         with nat.on_device(index) as stream:
             rc = lib.gns_adamw_states_step(
-                len(given), _ptr_array(places), _ptr_array(given), *states, sizes,
+                len(given), _pointers(places), _pointers(given), *states, sizes,
                 nat.dtype_code(places[0].dtype), nat.dtype_code(g_dtype), self.bits, *corrections,
                 beta1, 1 - beta1, beta2, 1 - beta2, epsilon, 1 - learning_rate * weight_decay,
                 nat.ptr(gradient_scale), stream,
@@ -1067,15 +1074,19 @@ class AdamWStates:
 
 
 # ------------------------------------------------- products grouped by expert
-def _aligned_copy(t: Tensor, batch: int, rows: int, cols: int, batch_stride: int, row_stride: int) -> tuple[Tensor, int]:
+def _aligned_copy(
+    t: Tensor, batch: int, rows: int, cols: int, batch_stride: int, row_stride: int, ends: Tensor | None = None
+) -> tuple[Tensor, int]:
     """A buffer with a copy of the rows [batch, rows, cols] that start at `t`'s first element, with
-    unit column stride, and its row pitch, a multiple of 8 elements."""
+    unit column stride, and its row pitch, a multiple of 8 elements. With ``ends``, without
+    the matrices of groups that have no rows."""
     pitch = (cols + 7) // 8 * 8
     buffer = torch.empty(batch * rows * pitch, dtype=t.dtype, device=t.device)
     lib = nat.load()
     with nat.on_device(t.get_device()) as stream:
-        rc = lib.gns_align_rows(batch, rows, cols, t.data_ptr(), batch_stride, row_stride, buffer.data_ptr(),
-                                rows * pitch, pitch, stream)
+        rc = lib.gns_align_rows(batch, rows, cols, t.data_ptr(), batch_stride, row_stride, nat.ptr(ends),
+                                0 if ends is None else 8 * ends.element_size(), buffer.data_ptr(), rows * pitch,
+                                pitch, stream)
     nat.check(rc, "gns_align_rows")
     return buffer, pitch
 
@@ -1103,7 +1114,7 @@ def _row_layout(t: Tensor) -> tuple[Tensor, int, int]:
     return copy, copy.data_ptr(), pitch
 
 
-def _group_layout(t: Tensor) -> tuple[Tensor, int, int, int, int]:
+def _group_layout(t: Tensor, ends: Tensor | None = None) -> tuple[Tensor, int, int, int, int]:
     """(owner, address, strides) of one matrix per group [groups, k, n], stored by rows or by
     columns, or of a copy of it, in the same order, that TMA can read."""
     groups, k, n = t.shape
@@ -1119,9 +1130,9 @@ def _group_layout(t: Tensor) -> tuple[Tensor, int, int, int, int]:
         t = t.contiguous()
         sg, sk, sn, by_rows = k * n, n, 1, True
     if by_rows:
-        copy, pitch = _aligned_copy(t, groups, k, n, sg, sk)
+        copy, pitch = _aligned_copy(t, groups, k, n, sg, sk, ends)
         return copy, copy.data_ptr(), k * pitch, pitch, 1
-    copy, pitch = _aligned_copy(t, groups, n, k, sg, sn)
+    copy, pitch = _aligned_copy(t, groups, n, k, sg, sn, ends)
     return copy, copy.data_ptr(), n * pitch, 1, pitch
 
 
@@ -1162,9 +1173,9 @@ def grouped_gemm(left: Tensor, right: Tensor, ends: Tensor, out_dtype: torch.dty
     code = nat.dtype_code(dtype)
     if rows == 0 or n == 0 or k == 0 or groups == 0:
         return torch.zeros((rows, n), dtype=dtype, device=left.device)
-    out = torch.empty((rows, n), dtype=dtype, device=left.device)
+    out = left.new_empty((rows, n), dtype=dtype)
     left_held, left_at, left_pitch = _row_layout(left)
-    right_held, *right_layout = _group_layout(right)
+    right_held, *right_layout = _group_layout(right, ends)
     lib = nat.load()
     with nat.on_device(index) as stream:
         rc = lib.gns_grouped_gemm(
@@ -1194,7 +1205,7 @@ def grouped_gemm_reduce(left: Tensor, right: Tensor, ends: Tensor, out_dtype: to
     code = nat.dtype_code(dtype)
     if rows == 0 or m == 0 or n == 0 or groups == 0:
         return torch.zeros((groups, m, n), dtype=dtype, device=left.device)
-    out = torch.empty((groups, m, n), dtype=dtype, device=left.device)
+    out = left.new_empty((groups, m, n), dtype=dtype)
     left_held, left_at, left_pitch = _row_layout(left)
     right_held, right_at, right_pitch = _row_layout(right)
     lib = nat.load()
@@ -1241,7 +1252,7 @@ def layer_norm(x: Tensor, weight: Tensor, bias: Tensor | None, epsilon: float) -
     flat = _norm_rows(x, columns)
     rows = flat.shape[0]
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
     rstd = torch.empty_like(mean)
     w = weight.contiguous()
     b = bias.contiguous() if bias is not None else None
@@ -1277,12 +1288,13 @@ def layer_norm_backward(
     dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     dweight, dbias = torch.empty_like(w), torch.empty_like(w)
     lib = nat.load()
-    ws = _workspace(lib.gns_layer_norm_backward_workspace_size(rows, columns), x.device)
+    nbytes = lib.gns_layer_norm_backward_workspace_size(rows, columns)
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     with nat.on_device(index) as stream:
         rc = lib.gns_layer_norm_backward(
             nat.dtype_code(x.dtype), nat.dtype_code(w.dtype), rows, columns, g.data_ptr(), g.stride(0),
             flat.data_ptr(), flat.stride(0), w.data_ptr(), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(),
-            dweight.data_ptr(), dbias.data_ptr(), ws.data_ptr(), ws.numel(), stream,
+            dweight.data_ptr(), dbias.data_ptr(), nat.ptr(ws), nbytes, stream,
         )
     nat.check(rc, "gns_layer_norm_backward")
     return dx, dweight, dbias

@@ -373,10 +373,11 @@ GNS_API int gns_grouped_gemm(int ab_dtype, int64_t rows, int64_t n, int64_t k, i
 /* Copies [batch][rows][cols] of a 16-bit type with unit column stride, wherever its
  * rows start, to rows that start on 16 bytes (dst and its strides in 16-byte
  * multiples, a row of dst holding cols rounded up to 8): operands that the TMA rule
- * excludes. */
+ * excludes. With `ends` (one for each of the batch, else NULL), matrices of groups
+ * without rows are not copied. */
 GNS_API int gns_align_rows(int64_t batch, int64_t rows, int64_t cols, const void* src, int64_t src_bstride,
-                           int64_t src_rstride, void* dst, int64_t dst_bstride, int64_t dst_rstride,
-                           gns_stream_t stream);
+                           int64_t src_rstride, const void* ends, int ends_bits, void* dst, int64_t dst_bstride,
+                           int64_t dst_rstride, gns_stream_t stream);
 GNS_API int gns_grouped_gemm_reduce(int ab_dtype, int64_t rows, int64_t m, int64_t n, int64_t groups,
                                     const void* left, int64_t left_rstride, const void* right, int64_t right_rstride,
                                     const void* ends, int ends_bits, void* out, int out_dtype, int64_t out_gstride,
