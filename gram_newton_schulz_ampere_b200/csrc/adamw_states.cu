@@ -35,7 +35,6 @@ namespace {
 
 constexpr int kBlockElems = 256;   // elements that share a scale: 8 for each lane of a warp
 constexpr float kE4M3Max = 448.0f;
-constexpr float kE4M3Tiny = 0.001953125f;  // 2^-9, the smallest e4m3 value above zero
 constexpr float kFlushBelow = 1e-30f;      // a block whose maximum is not above this is held as zeros
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
@@ -91,10 +90,10 @@ __device__ __forceinline__ float reciprocal_approx(float x) {
   return r;
 }
 
-// The larger magnitude; NaN if either is.
-__device__ __forceinline__ float larger(float top, float x) {
+// The largest magnitude of three; NaN if any is.
+__device__ __forceinline__ float largest(float a, float b, float c) {
   float r;
-  asm("{\n\t.reg .f32 a;\n\tabs.f32 a, %2;\n\tmax.NaN.f32 %0, %1, a;\n\t}" : "=f"(r) : "f"(top), "f"(x));
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -197,9 +196,7 @@ __device__ __forceinline__ void adamw_math(float g, float& p, float& m, float& v
 // The largest magnitude of the block, in every lane. Magnitudes order as their
 // bits do, and a NaN is above all of them, so it reaches the scale.
 __device__ __forceinline__ float block_max(const float (&f)[8]) {
-  float top = fabsf(f[0]);
-#pragma unroll
-  for (int e = 1; e < 8; ++e) top = larger(top, f[e]);
+  const float top = largest(largest(f[0], f[1], f[2]), largest(f[3], f[4], f[5]), largest(f[6], f[7], 0.0f));
   return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top) & 0x7fffffffu));
 }
 
@@ -217,6 +214,8 @@ struct Step {
   __device__ __forceinline__ Step(const StateArgs& a, const StateScalars& k, int t)
       : scale(k.grad_scale != nullptr ? *k.grad_scale : 1.0f), lr_bc1(a.lr_bc1[t]), inv_bc2(a.inv_bc2[t]) {}
 };
+
+__device__ __forceinline__ bool has_zero_byte(uint32_t w) { return ((w - 0x01010101u) & ~w & 0x80808080u) != 0u; }
 
 // New moments and parameter of a lane's 8 elements of a block, the moments' codes and
 // the block's scales (in every lane).
@@ -250,16 +249,25 @@ __device__ __forceinline__ void step_eight(const float (&gf)[8], float (&pf)[8],
   // One lane in two works out the inverse for m, the other for v.
   const float inverse = inverse_scale((threadIdx.x & 1) ? v_top : m_top);
   const float m_inv = __shfl_sync(0xffffffffu, inverse, 0), v_inv = __shfl_sync(0xffffffffu, inverse, 1);
+  float yf[8];
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
     mul2(Pair(mf[e], mf[e + 1]), Pair(m_inv)).get(mf[e], mf[e + 1]);
-    float y0, y1;
-    mul2(Pair(vf[e], vf[e + 1]), Pair(v_inv)).get(y0, y1);
-    vf[e] = (vf[e] > 0.0f && y0 < kE4M3Tiny) ? kE4M3Tiny : y0;
-    vf[e + 1] = (vf[e + 1] > 0.0f && y1 < kE4M3Tiny) ? kE4M3Tiny : y1;
+    Pair y = mul2(Pair(vf[e], vf[e + 1]), Pair(v_inv));
+    y.get(yf[e], yf[e + 1]);
   }
   mc = encode8(mf);
-  vc = encode8(vf);
+  vc = encode8(yf);
+  // Codes of zero are rare: only where there is one is it seen to that its second
+  // moment is zero.
+  if (has_zero_byte(vc.x) || has_zero_byte(vc.y)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      uint32_t& w = e < 4 ? vc.x : vc.y;
+      const uint32_t byte = 0xffu << (8 * (e & 3));
+      if (vf[e] > 0.0f && (w & byte) == 0u) w |= 1u << (8 * (e & 3));
+    }
+  }
   ms = m_top * (1.0f / kE4M3Max);
   vs = v_top * (1.0f / kE4M3Max);
 }
