@@ -209,6 +209,7 @@ struct Output {
   int64_t ldd, bstride;
   int bf16;  // 16-bit outputs: 1 = bf16, 0 = fp16
   int vec;   // base, row and group strides are multiples of 16 bytes
+  int linear;  // reduced product: rows and groups follow one another without gaps
 };
 
 // One whole 32 x 32 block of a staging slot to rows [r0, r0 + live) of the output.
@@ -241,6 +242,15 @@ __device__ __forceinline__ void store_rows(const uint8_t* slot, const Output& ou
     else
       static_cast<uint16_t*>(out.d)[i] = *reinterpret_cast<const uint16_t*>(slot + stage_off<false>(r, 2u * lane));
   }
+}
+
+// Zeros in `bytes` bytes (an even number) from p on, by thread `id` of `threads`.
+__device__ __forceinline__ void zero_fill(uint8_t* p, int64_t bytes, int id, int threads) {
+  const int64_t head = min(bytes, static_cast<int64_t>((16u - (reinterpret_cast<uintptr_t>(p) & 15u)) & 15u));
+  const int64_t words = (bytes - head) / 16;
+  for (int64_t i = 2 * id; i < head; i += 2 * threads) *reinterpret_cast<uint16_t*>(p + i) = 0;
+  for (int64_t i = id; i < words; i += threads) *reinterpret_cast<uint4*>(p + head + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
+  for (int64_t i = head + 16 * words + 2 * id; i < bytes; i += 2 * threads) *reinterpret_cast<uint16_t*>(p + i) = 0;
 }
 
 // A lane's 32 accumulators rounded to the output type.
@@ -948,6 +958,18 @@ __global__ void __launch_bounds__(kReduceThreads, 1)
       const int live = min(32, shape.m - r0);
       const int64_t base = e * out.bstride + static_cast<int64_t>(r0) * out.ldd;
       const bool empty = table.first_row[e + 1] == table.first_row[e];
+      if (empty && out.linear) {
+        // A group without rows: each of its tiles fills an equal stretch of the matrix
+        // (as tiles of unaligned rows, element by element, 65 matrices of 216 x 7201 took
+        // 5 times their floor).
+        constexpr int es = OUT_F32 ? 4 : 2;
+        const int64_t all = static_cast<int64_t>(shape.m) * shape.n;
+        const int64_t share = ((all + per_group - 1) / per_group + 63) / 64 * 64;
+        const int64_t from = min(all, l * share), to = min(all, from + share);
+        zero_fill(static_cast<uint8_t*>(out.d) + (e * out.bstride + from) * es, (to - from) * es,
+                  (static_cast<int>(rank) * kEpiWarps + ew) * 32 + lane, (PAIR ? 2 : 1) * kEpiWarps * 32);
+        continue;
+      }
       if (!empty) {
         if (!mbar_wait_bounded(&bar.tfull[acc], acc_ph, bar.abort_flag, &g_grouped_status, kStatusEpilogueTimeout)) break;
         __syncwarp();
@@ -1219,7 +1241,7 @@ int gns_grouped_gemm(int ab_dtype, int64_t rows, int64_t n, int64_t k, int64_t g
   c.groups = {ends, ends_bits == 64 ? 1 : 0, static_cast<int>(groups), static_cast<int>(rows)};
   c.shape.n = static_cast<int>(n);
   c.shape.k_blocks = static_cast<int>((k + kBK - 1) / kBK);
-  c.out = {out, out_rstride, 0, out_dtype == kBF16 ? 1 : 0, aligned_rows(out, out_rstride, 0, out_dtype) ? 1 : 0};
+  c.out = {out, out_rstride, 0, out_dtype == kBF16 ? 1 : 0, aligned_rows(out, out_rstride, 0, out_dtype) ? 1 : 0, 0};
   c.bf16 = ab_dtype == kBF16 ? 1 : 0;
   c.row_tiles = rows / (tile == 64 ? 32 : 64) + std::min(groups, rows);
   if (c.row_tiles * ((n + kBM - 1) / kBM) > (1ll << 30)) return fail(GNS_ERR_UNSUPPORTED, "too many tiles");
@@ -1282,7 +1304,8 @@ int gns_grouped_gemm_reduce(int ab_dtype, int64_t rows, int64_t m, int64_t n, in
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const ReduceShape shape{static_cast<int>(m), static_cast<int>(n), static_cast<int>(tiles_m), static_cast<int>(tiles_n)};
   const Output o{out, out_rstride, out_gstride, out_dtype == kBF16 ? 1 : 0,
-                 aligned_rows(out, out_rstride, out_gstride, out_dtype) ? 1 : 0};
+                 aligned_rows(out, out_rstride, out_gstride, out_dtype) ? 1 : 0,
+                 out_rstride == n && out_gstride == m * n ? 1 : 0};
   const int bf16 = ab_dtype == kBF16 ? 1 : 0;
   const int64_t tiles = tiles_m * tiles_n * groups;
   if (pair) {

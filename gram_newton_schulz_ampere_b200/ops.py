@@ -912,7 +912,7 @@ STATE_BLOCK = 256  # consecutive elements of a tensor that share a scale of the 
 
 def _pointers(tensors: Sequence[Tensor]) -> ctypes.Array:
     """``_ptr_array`` of many tensors, at a quarter of its cost for each."""
-    places = array.array("Q", [t.data_ptr() for t in tensors])
+    places = array.array("Q", map(Tensor.data_ptr, tensors))
     return (ctypes.c_void_p * len(places)).from_buffer(places)
 
 
@@ -1020,14 +1020,19 @@ class AdamWStates:
             raise ValueError(f"betas must be in [0, 1), got {(beta1, beta2)}")
         if not epsilon > 0.0:
             raise ValueError(f"epsilon must be positive, got {epsilon}")
-        whole = all(map(torch.is_tensor, gradients))
+        try:
+            dtypes = {cast(Tensor, g).dtype for g in gradients}
+            whole = True
+        except AttributeError:  # None among them
+            whole = False
+            dtypes = {g.dtype for g in gradients if g is not None}
         present = range(count) if whole else [i for i, g in enumerate(gradients) if g is not None]
         if not present:
             return
         given = cast(Sequence[Tensor], gradients) if whole else [cast(Tensor, gradients[i]) for i in present]
         places = self.parameters if whole else [self.parameters[i] for i in present]
         g_dtype = given[0].dtype
-        if len({g.dtype for g in given}) > 1:
+        if len(dtypes) > 1:
             raise TypeError("all gradients of one call must share a dtype")
         numel = list(map(Tensor.numel, given))
         if numel != (self._numel if whole else [self._numel[i] for i in present]):
@@ -1045,12 +1050,14 @@ class AdamWStates:
         floats = ctypes.c_float * len(given)
         if isinstance(step, (int, float)):
             lr_bc1, inv_bc2 = self._bias_corrections(step, learning_rate, beta1, beta2)
-            corrections = floats(*[lr_bc1] * len(given)), floats(*[inv_bc2] * len(given))
+            corrections = tuple(
+                floats.from_buffer(array.array("f", [value]) * len(given)) for value in (lr_bc1, inv_bc2)
+            )
         else:
             if len(step) != count:
                 raise ValueError("step must be one value or one for each parameter")
             pairs = [self._bias_corrections(step[i], learning_rate, beta1, beta2) for i in present]
-            corrections = floats(*[a for a, _ in pairs]), floats(*[b for _, b in pairs])
+            corrections = tuple(floats.from_buffer(array.array("f", values)) for values in zip(*pairs))
         states, sizes = self._states, self._sizes
         if not whole:
             sizes = (ctypes.c_int64 * len(given))(*numel)
