@@ -1022,32 +1022,29 @@ constexpr int kPadItems = 4;  // of a thread
 
 __global__ void __launch_bounds__(kPadThreads) pad_rows_kernel(const uint16_t* src, int64_t src_bstride,
                                                                int64_t src_rstride, uint16_t* dst, int64_t dst_bstride,
-                                                               int64_t dst_rstride, uint32_t rows, uint32_t cols,
-                                                               uint32_t words, int64_t items, const Groups groups) {
+                                                               int64_t dst_rstride, uint32_t cols, uint32_t words,
+                                                               uint32_t items, const Groups groups) {
+  // A CTA works on one matrix. (Whatever the ends are, a group with rows ends behind
+  // the one before it.)
+  const int e = static_cast<int>(blockIdx.y);
+  if (groups.ends != nullptr && group_end(groups, e) <= (e > 0 ? group_end(groups, e - 1) : 0)) return;
   uint4 lo[kPadItems], hi[kPadItems];
   uint32_t shift[kPadItems];
   uint16_t* to[kPadItems];
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kPadThreads * kPadItems) + threadIdx.x;
+  const uint32_t first = blockIdx.x * (kPadThreads * kPadItems) + threadIdx.x;
 #pragma unroll
   for (int q = 0; q < kPadItems; ++q) {
-    const int64_t item = first + q * kPadThreads;
+    const uint32_t item = first + q * kPadThreads;
     to[q] = nullptr;
     if (item >= items) continue;
-    const int64_t line = item / words;
-    const uint32_t word = static_cast<uint32_t>(item - line * words);
-    const int64_t b = line / rows, r = line - b * rows;
-    // (Whatever the ends are, a group with rows ends behind the one before it.)
-    if (groups.ends != nullptr) {
-      const int e = static_cast<int>(b);
-      if (group_end(groups, e) <= (e > 0 ? group_end(groups, e - 1) : 0)) continue;
-    }
-    const uintptr_t row = reinterpret_cast<uintptr_t>(src + b * src_bstride + r * src_rstride);
+    const uint32_t r = item / words, word = item - r * words;
+    const uintptr_t row = reinterpret_cast<uintptr_t>(src + e * src_bstride + r * src_rstride);
     const uintptr_t at = row + word * 16u, end = row + static_cast<uintptr_t>(cols) * 2u;
     const uint4* from = reinterpret_cast<const uint4*>(at & ~uintptr_t(15));
     lo[q] = from[0];
     hi[q] = reinterpret_cast<uintptr_t>(from + 1) < end ? from[1] : make_uint4(0u, 0u, 0u, 0u);
     shift[q] = static_cast<uint32_t>(at & 15u);
-    to[q] = dst + b * dst_bstride + r * dst_rstride + word * 8u;
+    to[q] = dst + e * dst_bstride + r * dst_rstride + word * 8u;
   }
 #pragma unroll
   for (int q = 0; q < kPadItems; ++q) {
@@ -1258,10 +1255,10 @@ int gns_align_rows(int64_t batch, int64_t rows, int64_t cols, const void* src, i
                    gns_stream_t stream) {
   clear_error();
   if (ends != nullptr && ends_bits != 32 && ends_bits != 64) return fail(GNS_ERR_ARGUMENT, "ends must have 32 or 64 bits");
+  if (ends != nullptr && batch > kMaxGroups) return fail(GNS_ERR_UNSUPPORTED, "at most 1024 groups are supported");
   if (batch < 0 || rows < 0 || cols < 0) return fail(GNS_ERR_ARGUMENT, "negative dimension");
   if (batch == 0 || rows == 0 || cols == 0) return GNS_OK;
-  if (rows > (1ll << 31) || cols > (1ll << 31) || batch > (1ll << 30))
-    return fail(GNS_ERR_UNSUPPORTED, "dimension beyond kernel limits");
+  if (cols > (1ll << 30)) return fail(GNS_ERR_UNSUPPORTED, "dimension beyond kernel limits");
   if (src == nullptr || dst == nullptr) return fail(GNS_ERR_ARGUMENT, "null tensor");
   const int64_t words = (cols + 7) / 8;
   if (reinterpret_cast<uintptr_t>(src) % 2 != 0) return fail(GNS_ERR_LAYOUT, "source must be aligned to its elements");
@@ -1269,13 +1266,22 @@ int gns_align_rows(int64_t batch, int64_t rows, int64_t cols, const void* src, i
     return fail(GNS_ERR_LAYOUT, "destination rows must start on 16 bytes and hold whole 16-byte words");
   int rc = check_device();
   if (rc != GNS_OK) return rc;
-  const int64_t items = batch * rows * words;
-  const int64_t blocks = (items + kPadThreads * kPadItems - 1) / (kPadThreads * kPadItems);
-  if (blocks > (1ll << 31) - 1) return fail(GNS_ERR_UNSUPPORTED, "too many rows");
-  pad_rows_kernel<<<static_cast<unsigned>(blocks), kPadThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint16_t*>(src), src_bstride, src_rstride, static_cast<uint16_t*>(dst), dst_bstride, dst_rstride,
-      static_cast<uint32_t>(rows), static_cast<uint32_t>(cols), static_cast<uint32_t>(words), items,
-      Groups{ends, ends_bits == 64 ? 1 : 0, static_cast<int>(batch), 0});
+  // Up to 65535 matrices and 2^30 words of each a launch.
+  const auto* from = static_cast<const uint16_t*>(src);
+  auto* to = static_cast<uint16_t*>(dst);
+  const int64_t most_rows = std::max<int64_t>(1, (1ll << 30) / words);
+  for (int64_t b0 = 0; b0 < batch; b0 += 65535) {
+    const int64_t nb = std::min<int64_t>(batch - b0, 65535);
+    for (int64_t r0 = 0; r0 < rows; r0 += most_rows) {
+      const int64_t items = std::min(rows - r0, most_rows) * words;
+      const dim3 grid(static_cast<unsigned>((items + kPadThreads * kPadItems - 1) / (kPadThreads * kPadItems)),
+                      static_cast<unsigned>(nb));
+      pad_rows_kernel<<<grid, kPadThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+          from + b0 * src_bstride + r0 * src_rstride, src_bstride, src_rstride, to + b0 * dst_bstride + r0 * dst_rstride,
+          dst_bstride, dst_rstride, static_cast<uint32_t>(cols), static_cast<uint32_t>(words), static_cast<uint32_t>(items),
+          Groups{ends, ends_bits == 64 ? 1 : 0, static_cast<int>(nb), 0});
+    }
+  }
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? GNS_OK : cuda_fail(e, "align rows kernel");
 }
