@@ -27,6 +27,10 @@
 // zeroed in shared memory (in both operands: a NaN times zero is a NaN) by a warp
 // of its own between the loads and the MMA.
 //
+// Few tiles with a long contraction: a cluster of up to 8 CTAs shares a tile, each
+// with a part of the contraction, and adds up the fp32 partial sums out of the CTAs'
+// shared memory in the order of the parts.
+//
 // Sums are fp32 in TMEM, rounded once at the store. Every wait is bounded.
 #include <algorithm>
 #include <cmath>
@@ -305,9 +309,9 @@ struct Barriers {
   }
 };
 
-template <bool PAIR>
+template <bool CLUSTER>
 __device__ __forceinline__ void meet() {
-  if (PAIR)
+  if (CLUSTER)
     cluster_sync_all();
   else
     __syncthreads();
@@ -315,7 +319,7 @@ __device__ __forceinline__ void meet() {
 
 // Set-up common to both kernels: barriers, TMEM, and the wait for the stream's
 // previous kernel. Returns the TMEM base.
-template <int S, bool PAIR>
+template <int S, bool PAIR, bool CLUSTER = PAIR>
 __device__ __forceinline__ uint32_t set_up(const Barriers<S, PAIR>& bar, int warp, uint32_t tmem_cols,
                                            uint32_t full_arrivals = 1) {
   if (threadIdx.x == 0) const_cast<Barriers<S, PAIR>&>(bar).init(full_arrivals);
@@ -329,7 +333,7 @@ __device__ __forceinline__ uint32_t set_up(const Barriers<S, PAIR>& bar, int war
     }
   }
   tc_fence_before();
-  meet<PAIR>();
+  meet<CLUSTER>();
   tc_fence_after();
   pdl_launch_dependents();
   pdl_wait_predecessor();
@@ -353,13 +357,13 @@ __device__ __forceinline__ void drain(const Barriers<S, PAIR>& bar, int st, uint
 
 // Teardown: all roles meet; after an abort, copies and MMAs in flight get time to
 // land before TMEM and shared memory are released.
-template <int S, bool PAIR>
+template <int S, bool PAIR, bool CLUSTER = PAIR>
 __device__ __forceinline__ void tear_down(const Barriers<S, PAIR>& bar, int warp, uint32_t tmem_base,
                                           uint32_t tmem_cols) {
   tc_fence_before();
-  meet<PAIR>();
+  meet<CLUSTER>();
   if (*bar.abort_flag) settle_for_ns(2000000ull);
-  meet<PAIR>();
+  meet<CLUSTER>();
   tc_fence_after();
   if (warp == 1) {
     __syncwarp();
@@ -384,8 +388,12 @@ struct RowMaps {
 // A tile's rows lie in one or two units of at most 256 columns of the accumulator,
 // and the unit buffers are used in turn. TOK = 512: both units of a tile share the
 // loads of the expert's columns.
-template <int TOK, bool OUT_F32, bool PAIR>
+//
+// SPLIT: a tile belongs to a cluster of 2, 4 or 8 CTAs, each of which multiplies an
+// equal share of the contraction (the join below).
+template <int TOK, bool OUT_F32, bool PAIR, bool SPLIT>
 struct RowsConfig {
+  static_assert(!SPLIT || (TOK == 64 && !PAIR), "a split tile has one block of 32 x 32 accumulators a warp");
   static constexpr int kUnits = TOK > 256 ? 2 : 1;
   static constexpr int kUnitCols = TOK / kUnits;
   static constexpr int kFeatures = PAIR ? 2 * kBM : kBM;             // features of a tile
@@ -393,11 +401,12 @@ struct RowsConfig {
   static constexpr int kGrain = PAIR ? 32 : 16;                       // granularity of N
   static constexpr uint32_t kUnitBytes = kUnitRows * kBK * 2;
   static constexpr uint32_t kStageBytes = kMBytes + kUnits * kUnitBytes;
-  static constexpr int kStages = 6 * 32768 / kStageBytes - (OUT_F32 ? 1 : 0);
-  static constexpr uint32_t kSlotBytes = 32 * (OUT_F32 ? 128 : 64);
+  static constexpr int kStages = 6 * 32768 / kStageBytes - (OUT_F32 || SPLIT ? 1 : 0);
+  static constexpr uint32_t kSlotBytes = 32 * (OUT_F32 || SPLIT ? 128 : 64);
+  static constexpr uint32_t kJoinBytes = SPLIT ? 2 * kEpiWarps * 8 : 0;
   static constexpr uint32_t kTmemCols = 2 * kUnitCols;
   static constexpr size_t kSmemBytes = 1024 + kStages * kStageBytes + kEpiWarps * kSlotBytes + Table::kBytes +
-                                       Barriers<kStages, PAIR>::kBytes;
+                                       Barriers<kStages, PAIR>::kBytes + kJoinBytes;
 };
 
 // A tile: `rows` rows from `row0` of group e, feature tile `f`.
@@ -442,15 +451,94 @@ __device__ __forceinline__ int mma_width(int rows) {
   return (rows + Cfg::kGrain - 1) / Cfg::kGrain * Cfg::kGrain;
 }
 
-template <bool F_MN, int TOK, bool OUT_F32, bool PAIR>
+// The join of a split tile, by one warp of each CTA of the cluster: the same 32 x 32
+// block of all partial accumulators. The warp leaves its own in its slot (fp32, row =
+// row of the output), tells the others, and adds up every size-th stretch of four rows
+// from all slots, always in the order of the CTAs. `there` counts the CTAs whose
+// partial is in place, `read` those that have read this CTA's.
+struct Join {
+  uint64_t* there;
+  uint64_t* read;
+  uint32_t phase, rank, size;
+
+  __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) const {
+    return __all_sync(0xffffffffu,
+                      mbar_wait_bounded<true>(bar, parity, abort_flag, &g_grouped_status, kStatusEpilogueTimeout));
+  }
+
+  // After every lane's accesses of the slots.
+  __device__ __forceinline__ void tell(uint64_t* bar, int lane) const {
+    __syncwarp();
+    if (lane < static_cast<int>(size)) mbar_arrive_release_cluster(cluster_addr(bar, static_cast<uint32_t>(lane)));
+  }
+
+  // Sums are told as read before they are stored: a release waits for earlier stores.
+  template <bool OUT_F32>
+  __device__ __forceinline__ void add_up(const uint8_t* slot, const Output& out, int64_t at, int live, int cols_left,
+                                         int lane) const {
+    const int piece = lane % 8, first = 4 * static_cast<int>(rank) + lane / 8, step = 4 * static_cast<int>(size);
+    float4 sum[4];  // a cluster has two CTAs at least
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      sum[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const int r = first + q * step;
+      if (r >= live) continue;
+      const uint32_t off = stage_off<true>(static_cast<uint32_t>(r), 16u * piece);
+#pragma unroll 4
+      for (uint32_t c = 0; c < size; ++c) {
+        float4 p;
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(p.x), "=f"(p.y), "=f"(p.z), "=f"(p.w)
+                     : "r"(cluster_addr(slot, c) + off)
+                     : "memory");
+        sum[q] = make_float4(sum[q].x + p.x, sum[q].y + p.y, sum[q].z + p.z, sum[q].w + p.w);
+      }
+    }
+    tell(read, lane);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int r = first + q * step;
+      if (r >= live) continue;
+      const int64_t i = at + r * out.ldd + 4 * piece;
+      const int left = cols_left - 4 * piece;
+      const float v[4] = {sum[q].x, sum[q].y, sum[q].z, sum[q].w};
+      if (OUT_F32) {
+        float* d = static_cast<float*>(out.d) + i;
+        if (out.vec && left >= 4) {
+          *reinterpret_cast<float4*>(d) = sum[q];
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (k < left) d[k] = v[k];
+        }
+      } else {
+        uint16_t* d = static_cast<uint16_t*>(out.d) + i;
+        if (out.vec && left >= 4) {
+          *reinterpret_cast<uint2*>(d) = make_uint2(pack_pair(v[0], v[1], out.bf16), pack_pair(v[2], v[3], out.bf16));
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (k < left) d[k] = float_to_half_bits(v[k], out.bf16);
+        }
+      }
+    }
+  }
+};
+
+template <bool F_MN, int TOK, bool OUT_F32, bool PAIR, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
     grouped_rows_kernel(const __grid_constant__ CUtensorMap map_right, const __grid_constant__ RowMaps map_rows,
                         const Groups groups, const RowsShape shape, const Output out, const int ab_bf16) {
-  using Cfg = RowsConfig<TOK, OUT_F32, PAIR>;
+  using Cfg = RowsConfig<TOK, OUT_F32, PAIR, SPLIT>;
   constexpr int S = Cfg::kStages;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
-  const int tile_begin = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
-  const int tile_step = PAIR ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
+  const int ctas = PAIR ? 2 : (SPLIT ? static_cast<int>(cluster_nctarank()) : 1);  // of a tile
+  const int tile_begin = static_cast<int>(blockIdx.x) / ctas;
+  const int tile_step = static_cast<int>(gridDim.x) / ctas;
+  // This CTA's share of the contraction.
+  const int share = SPLIT ? static_cast<int>(cluster_ctarank()) : 0;
+  const int kb_begin = SPLIT ? share * shape.k_blocks / ctas : 0;
+  const int kb_end = SPLIT ? (share + 1) * shape.k_blocks / ctas : shape.k_blocks;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
 
@@ -460,13 +548,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem_n = smem + S * kMBytes;
   uint8_t* smem_epi = smem + S * Cfg::kStageBytes;
   const Barriers<S, PAIR> bar(smem_epi + kEpiWarps * Cfg::kSlotBytes);
-  const Table table(smem_epi + kEpiWarps * Cfg::kSlotBytes + Barriers<S, PAIR>::kBytes);
+  uint64_t* join = reinterpret_cast<uint64_t*>(smem_epi + kEpiWarps * Cfg::kSlotBytes + Barriers<S, PAIR>::kBytes);
+  const Table table(smem_epi + kEpiWarps * Cfg::kSlotBytes + Barriers<S, PAIR>::kBytes + Cfg::kJoinBytes);
 
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&map_right);
     for (int i = 0; i < Cfg::kUnitRows / 32; ++i) tma_prefetch_desc(&map_rows.box[i]);
+    if (SPLIT)
+      for (int i = 0; i < 2 * kEpiWarps; ++i) mbar_init(&join[i], static_cast<uint32_t>(ctas));
   }
-  const uint32_t tmem_base = set_up<S, PAIR>(bar, warp, Cfg::kTmemCols);
+  const uint32_t tmem_base = set_up<S, PAIR, PAIR || SPLIT>(bar, warp, Cfg::kTmemCols);
 
   // A tile's cost is its rows.
   if (warp == 0)
@@ -497,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           box[u] = (mine + 31) / 32;
           bytes += static_cast<uint32_t>(box[u]) * 32u * kBK * 2u;
         }
-        for (int kb = 0; kb < shape.k_blocks; ++kb) {
+        for (int kb = kb_begin; kb < kb_end; ++kb) {
           if (!mbar_wait_bounded(&bar.empty[st], ph ^ 1u, bar.abort_flag, &g_grouped_status, kStatusProducerTimeout)) {
             ok = false;
             break;
@@ -576,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!ok) break;
         tc_fence_after();
-        for (int kb = 0; kb < shape.k_blocks; ++kb) {
+        for (int kb = kb_begin; kb < kb_end; ++kb) {
           if (!mbar_wait_bounded(&bar.full[st], ph, bar.abort_flag, &g_grouped_status, kStatusMmaTimeout)) {
             ok = false;
             break;
@@ -591,14 +682,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 desc_k + ((smem_u32(smem_n + (st * Cfg::kUnits + u) * Cfg::kUnitBytes) >> 4) & 0x3FFFu);
 #pragma unroll
             for (int kk = 0; kk < kBK / 16; ++kk) {
-              const uint32_t more = (kb > 0 || kk > 0) ? 1u : 0u;
+              const uint32_t more = (kb > kb_begin || kk > 0) ? 1u : 0u;
               if (PAIR)
                 tc_mma_f16_pair(d_tmem, m0 + kk * (F_MN ? 128u : 2u), n0 + kk * 2u, idesc[u], more);
               else
                 tc_mma_f16(d_tmem, m0 + kk * (F_MN ? 128u : 2u), n0 + kk * 2u, idesc[u], more);
             }
             // The first unit of two is handed over as soon as its last products are issued.
-            if (u + 1 < Cfg::kUnits && u + 1 < units && kb + 1 == shape.k_blocks) hand_over(buffer[u]);
+            if (u + 1 < Cfg::kUnits && u + 1 < units && kb + 1 == kb_end) hand_over(buffer[u]);
           }
           if (PAIR) {
             tc_commit_pair(empty0 + static_cast<uint32_t>(st) * 8u);
@@ -625,6 +716,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int place = 0, acc = 0;
     uint32_t acc_ph = 0;
     bool ok = true;
+    Join parts{join + ew, join + kEpiWarps + ew, 0u, static_cast<uint32_t>(share), static_cast<uint32_t>(ctas)};
     for (int t = tile_begin; t < tiles && ok; t += tile_step) {
       const RowsTile tile = rows_tile(table, groups.count, t, place);
       const int f0 = tile.f * Cfg::kFeatures + static_cast<int>(rank) * kBM + quarter * 32;
@@ -637,8 +729,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t at =
             tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * Cfg::kUnitCols);
         const int rows = first == 0 ? split : tile.rows - split;
+        const bool joins = SPLIT && 32 * half < rows && f0 < shape.n;  // the same in all CTAs of the cluster
+        if (joins) {
+          float v[32];
+          __syncwarp();
+          tmem_load_32cols(at + 32 * half, v);
+          ok = parts.wait(parts.read, parts.phase ^ 1u, bar.abort_flag);  // of the tile before
+          if (!ok) break;
+          XRow<true> x;
+          round_row<true>(v, out.bf16, x);
+          stage_write_col<true>(slot, lane, x);
+          parts.tell(parts.there, lane);
+        }
 #pragma unroll 1
-        for (int c = 32 * half; c < rows && f0 < shape.n; c += 64) {
+        for (int c = 32 * half; c < rows && f0 < shape.n && !SPLIT; c += 64) {
           float v[32];
           __syncwarp();
           tmem_load_32cols(at + c, v);
@@ -659,10 +763,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           else
             mbar_arrive(&bar.tempty[acc]);
         }
+        if (joins) {
+          ok = parts.wait(parts.there, parts.phase, bar.abort_flag);
+          if (!ok) break;
+          parts.template add_up<OUT_F32>(slot, out, static_cast<int64_t>(tile.row0 + 32 * half) * out.ldd + f0,
+                                         min(32, rows - 32 * half), shape.n - f0, lane);
+          parts.phase ^= 1u;
+        }
         acc ^= 1;
         if (acc == 0) acc_ph ^= 1u;
       }
     }
+    // No CTA leaves while another reads its slots.
+    if (SPLIT && ok) parts.wait(parts.read, parts.phase ^ 1u, bar.abort_flag);
     // Rows that no group owns.
     for (int r = table.first_row[groups.count] + static_cast<int>(blockIdx.x) * kEpiWarps + ew; r < groups.rows;
          r += static_cast<int>(gridDim.x) * kEpiWarps) {
@@ -675,7 +788,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   }
-  tear_down<S, PAIR>(bar, warp, tmem_base, Cfg::kTmemCols);
+  tear_down<S, PAIR, PAIR || SPLIT>(bar, warp, tmem_base, Cfg::kTmemCols);
 }
 
 // ---------------------------------------------------------- reduced product
@@ -717,11 +830,6 @@ struct Blocks {
     return at < last_place() ? at : (at == last_place() ? count - 1 : at - 1);
   }
 };
-
-// Arrives on another CTA's barrier after this thread's writes to shared memory.
-__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t bar_cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
-}
 
 template <bool OUT_F32, bool PAIR>
 __global__ void __launch_bounds__(kReduceThreads, 1)
@@ -1070,12 +1178,12 @@ __global__ void __launch_bounds__(kPadThreads) pad_rows_kernel(const uint16_t* s
 // -------------------------------------------------------------------- launch
 std::mutex g_mutex;
 constexpr int kDevices = 64, kSlots = 32;
-int g_resident[kDevices][kSlots] = {};  // co-resident CTAs (or CTAs of pairs) of an instantiation
+int g_resident[kDevices][kSlots] = {};  // co-resident clusters of an instantiation
 
-// Launches a persistent grid of at most `wanted` CTAs (or pairs) of `kernel`.
-template <bool PAIR, typename... Params, typename... Args>
-int launch_persistent(void (*kernel)(Params...), int threads, int slot, size_t smem, int64_t wanted, cudaStream_t stream,
-                      Args... args) {
+// Launches a persistent grid of at most `wanted` clusters of `kernel`, of `cluster` CTAs each.
+template <typename... Params, typename... Args>
+int launch_persistent(void (*kernel)(Params...), int cluster, int threads, int slot, size_t smem, int64_t wanted,
+                      cudaStream_t stream, Args... args) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
@@ -1088,11 +1196,11 @@ int launch_persistent(void (*kernel)(Params...), int threads, int slot, size_t s
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = PAIR ? 2 : 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   int resident = 0;
   {
     std::lock_guard<std::mutex> lock(g_mutex);
@@ -1101,17 +1209,17 @@ int launch_persistent(void (*kernel)(Params...), int threads, int slot, size_t s
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
       if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(smem)");
       resident = device_sm_count();
-      if (PAIR) {
-        cfg.gridDim = dim3(static_cast<unsigned>(2 * (resident / 2)), 1, 1);
+      if (cluster > 1) {
+        cfg.gridDim = dim3(static_cast<unsigned>(resident / cluster * cluster), 1, 1);
         e = cudaOccupancyMaxActiveClusters(&resident, kernel, &cfg);
         if (e != cudaSuccess) return cuda_fail(e, "cudaOccupancyMaxActiveClusters");
-        if (resident < 1) return fail(GNS_ERR_UNSUPPORTED, "no CTA pair of the grouped product fits on an SM pair");
+        if (resident < 1) return fail(GNS_ERR_UNSUPPORTED, "no cluster of the grouped product fits on the device");
       }
       g_resident[dev][slot] = resident;
     }
   }
   const int64_t units = std::max<int64_t>(1, std::min<int64_t>(wanted, resident));
-  cfg.gridDim = dim3(static_cast<unsigned>(PAIR ? 2 * units : units), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(cluster * units), 1, 1);
   e = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? GNS_OK : cuda_fail(e, "grouped product launch");
@@ -1125,25 +1233,26 @@ struct RowsCall {
   Output out;
   int bf16;
   int64_t row_tiles;  // at most
+  int split;          // CTAs that share a tile's contraction
 };
 
-template <bool F_MN, int TOK, bool OUT_F32, bool PAIR>
+template <bool F_MN, int TOK, bool OUT_F32, bool PAIR, bool SPLIT>
 int launch_rows(RowsCall& c, int slot, cudaStream_t stream) {
-  using Cfg = RowsConfig<TOK, OUT_F32, PAIR>;
+  using Cfg = RowsConfig<TOK, OUT_F32, PAIR, SPLIT>;
   c.shape.feature_tiles = (c.shape.n + Cfg::kFeatures - 1) / Cfg::kFeatures;
-  return launch_persistent<PAIR>(grouped_rows_kernel<F_MN, TOK, OUT_F32, PAIR>, kThreads, slot, Cfg::kSmemBytes,
-                                 c.row_tiles * c.shape.feature_tiles, stream, c.right, c.maps, c.groups, c.shape, c.out,
-                                 c.bf16);
+  return launch_persistent(grouped_rows_kernel<F_MN, TOK, OUT_F32, PAIR, SPLIT>, SPLIT ? c.split : (PAIR ? 2 : 1), kThreads,
+                           slot, Cfg::kSmemBytes, c.row_tiles * c.shape.feature_tiles, stream, c.right, c.maps, c.groups,
+                           c.shape, c.out, c.bf16);
 }
 
-template <int TOK, bool PAIR>
+template <int TOK, bool PAIR, bool SPLIT = false>
 int launch_rows_any(bool mn, bool f32, RowsCall& c, int slot, cudaStream_t stream) {
   if (mn) {
-    if (f32) return launch_rows<true, TOK, true, PAIR>(c, slot + 3, stream);
-    return launch_rows<true, TOK, false, PAIR>(c, slot + 2, stream);
+    if (f32) return launch_rows<true, TOK, true, PAIR, SPLIT>(c, slot + 3, stream);
+    return launch_rows<true, TOK, false, PAIR, SPLIT>(c, slot + 2, stream);
   }
-  if (f32) return launch_rows<false, TOK, true, PAIR>(c, slot + 1, stream);
-  return launch_rows<false, TOK, false, PAIR>(c, slot, stream);
+  if (f32) return launch_rows<false, TOK, true, PAIR, SPLIT>(c, slot + 1, stream);
+  return launch_rows<false, TOK, false, PAIR, SPLIT>(c, slot, stream);
 }
 
 // Rows of a tile: 64 or 128 (a CTA, 128 features), 256 or 512 (a pair, 256 features).
@@ -1173,6 +1282,36 @@ int rows_tile_choice(int64_t rows, int64_t n, int64_t k, int64_t groups) {
     const double cost = turns * (tile == 64 ? 1.0 : (tile == 128 ? 1.08 : 1.3));
     if (tile == 64 || cost < least) {
       best = tile;
+      least = cost;
+    }
+  }
+  return best;
+}
+
+// CTAs that share a tile of 64 rows: 1, 2, 4 or 8. Where tiles are fewer than SMs, or
+// a last turn has few of them, the contraction is cut. The unit is a block of 64 of
+// the contraction (0.28 us of a CTA): a turn of a split tile costs its share and 2
+// blocks, 12 at least (the join of the tile before must be through: 3 us), and the
+// last join 4 more. Clusters of 4 and 8 leave some SMs of a GPC unused. Microseconds
+// measured for 1 / 2 / 4 / 8 (bf16, rows of the call in all):
+//   1 row, 1 x (8192 x 1024)      40.4 / 23.2 / 14.4 / 10.5
+//   1 row, 1 x (4096 x 4096)      22.7 / 15.0 / 12.3 / 15.2
+//   8 rows, 8 x (1024 x 4096)     17.4 / 20.3 / 28.1 / 53.1
+//   98 rows, 10 x (8192 x 2048)   91.4 / 75.1 / 61.4 / 68.7
+//   34 rows, 25 x (8192 x 512)    44.5 / 52.6 / 48.3 / 46.7
+//   192 rows, 64 x (4096 x 1024)  98.0 / 89.7 / 97.3 / 140
+int rows_split(int64_t rows, int64_t n, int64_t k_blocks, int64_t groups) {
+  const double t = static_cast<double>(rows), e = static_cast<double>(groups), depth = static_cast<double>(k_blocks);
+  const double tiles = std::max(std::min(e, t), t / 64 + e / 2) * static_cast<double>((n + kBM - 1) / kBM);
+  const int sms = device_sm_count();
+  int best = 1;
+  double least = std::ceil(tiles / sms) * depth;
+  for (int split : {2, 4, 8}) {
+    const int clusters = (split == 2 ? sms : sms * 9 / 10) / split;
+    if (clusters < 1 || k_blocks < split) break;
+    const double cost = std::ceil(tiles / clusters) * std::max(depth / split + 2.0, 12.0) + 4.0;
+    if (cost < least) {
+      best = split;
       least = cost;
     }
   }
@@ -1244,6 +1383,8 @@ int gns_grouped_gemm(int ab_dtype, int64_t rows, int64_t n, int64_t k, int64_t g
   if (c.row_tiles * ((n + kBM - 1) / kBM) > (1ll << 30)) return fail(GNS_ERR_UNSUPPORTED, "too many tiles");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool f32 = out_dtype == kF32;
+  c.split = tile == 64 ? rows_split(rows, n, c.shape.k_blocks, groups) : 1;
+  if (c.split > 1) return launch_rows_any<64, false, true>(!k_major, f32, c, c.split == 2 ? 20 : (c.split == 4 ? 24 : 28), st);
   if (tile == 64) return launch_rows_any<64, false>(!k_major, f32, c, 0, st);
   if (tile == 128) return launch_rows_any<128, false>(!k_major, f32, c, 4, st);
   if (tile == 256) return launch_rows_any<256, true>(!k_major, f32, c, 8, st);
@@ -1316,15 +1457,15 @@ int gns_grouped_gemm_reduce(int ab_dtype, int64_t rows, int64_t m, int64_t n, in
   const int64_t tiles = tiles_m * tiles_n * groups;
   if (pair) {
     if (out_dtype == kF32)
-      return launch_persistent<true>(grouped_reduce_kernel<true, true>, kReduceThreads, 16, ReduceConfig<true, true>::kSmemBytes, tiles, st,
+      return launch_persistent(grouped_reduce_kernel<true, true>, 2, kReduceThreads, 16, ReduceConfig<true, true>::kSmemBytes, tiles, st,
                                      map_l, map_r, g, shape, o, bf16);
-    return launch_persistent<true>(grouped_reduce_kernel<false, true>, kReduceThreads, 17, ReduceConfig<false, true>::kSmemBytes, tiles, st,
+    return launch_persistent(grouped_reduce_kernel<false, true>, 2, kReduceThreads, 17, ReduceConfig<false, true>::kSmemBytes, tiles, st,
                                    map_l, map_r, g, shape, o, bf16);
   }
   if (out_dtype == kF32)
-    return launch_persistent<false>(grouped_reduce_kernel<true, false>, kReduceThreads, 18, ReduceConfig<true, false>::kSmemBytes, tiles, st,
+    return launch_persistent(grouped_reduce_kernel<true, false>, 1, kReduceThreads, 18, ReduceConfig<true, false>::kSmemBytes, tiles, st,
                                     map_l, map_r, g, shape, o, bf16);
-  return launch_persistent<false>(grouped_reduce_kernel<false, false>, kReduceThreads, 19, ReduceConfig<false, false>::kSmemBytes, tiles, st,
+  return launch_persistent(grouped_reduce_kernel<false, false>, 1, kReduceThreads, 19, ReduceConfig<false, false>::kSmemBytes, tiles, st,
                                   map_l, map_r, g, shape, o, bf16);
 }
 

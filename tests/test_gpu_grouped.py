@@ -90,6 +90,28 @@ def test_rows_product_odd_sizes(cuda_device, k, n, transposed):
     assert_close(ops.grouped_gemm(left, right, ends_of(counts, cuda_device)), exact, magnitude, k)
 
 
+@pytest.mark.parametrize("counts", [[1], [0, 5, 0, 33, 2], [64, 1, 40], [9] * 30, [100, 7]])
+@pytest.mark.parametrize("k,n", [(520, 8), (1000, 328), (2048, 136), (8192, 512), (2051, 133)])
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+def test_rows_product_long_contractions(cuda_device, counts, k, n, transposed, out_dtype):
+    """Few rows and a long contraction: tiles that several CTAs share."""
+    gen = torch.Generator(device=cuda_device).manual_seed(17)
+    rows = sum(counts) + 3
+    left = normal(gen, rows, k, dtype=torch.bfloat16, device=cuda_device)
+    shape = (len(counts), n, k) if transposed else (len(counts), k, n)
+    right = normal(gen, *shape, dtype=torch.bfloat16, device=cuda_device, scale=0.1)
+    if transposed:
+        right = right.transpose(1, 2)
+    left[sum(counts):] = float("nan")  # rows that nobody owns stay out
+    runs = [ops.grouped_gemm(left, right, ends_of(counts, cuda_device), out_dtype=out_dtype) for _ in range(3)]
+    assert torch.equal(runs[0], runs[1]) and torch.equal(runs[0], runs[2])
+    left[sum(counts):] = 0
+    exact, magnitude = by_group(left, right, counts)
+    assert_close(runs[0], exact, magnitude, k)
+    assert not runs[0][sum(counts):].any()
+
+
 @pytest.mark.parametrize("counts", COUNTS)
 @pytest.mark.parametrize("m,n", [(128, 64), (8, 8), (264, 200), (130, 520), (33, 7)])
 @pytest.mark.parametrize("out_dtype", [None, torch.float32])
