@@ -614,12 +614,14 @@ extern "C" int gns_adamw_states_step(int count, void* const* params, const void*
   if (rc != GNS_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const StateScalars k{beta1, one_minus_beta1, beta2, one_minus_beta2, epsilon, decay, grad_scale};
-  // Long chunks keep a warp's ring going; short ones give every SM work. Elements are
-  // divided into 32 chunks an SM (about eleven turns of its three CTAs) where there are enough.
+  // Long chunks keep a warp's ring going; short ones give every SM work. 8-bit states:
+  // up to 8 chunks an SM of the shortest kind, then longer ones (7.8M bf16 elements 34.7
+  // us with up to 32, 25.0 with 8 or 12; 3M: 17.2, 14.2; 16M: 40.3, 33.6). 32-bit states
+  // have no ring: up to 32 (16M: 61.8 us with 8, 56.6 with 32).
   int64_t total = 0;
   for (int i = 0; i < count; ++i) total += numel[i];
   int chunk = kChunkMin;
-  while (chunk < kChunkMax && total / chunk > 32 * static_cast<int64_t>(device_sm_count())) chunk *= 2;
+  while (chunk < kChunkMax && total / chunk > (state_bits == 8 ? 8 : 32) * static_cast<int64_t>(device_sm_count())) chunk *= 2;
   // 8-bit states: the tensors whose rows all start on 16 bytes, then the others.
   auto is_aligned = [&](int i) {
     const uintptr_t all = reinterpret_cast<uintptr_t>(params[i]) | reinterpret_cast<uintptr_t>(grads[i]) |
