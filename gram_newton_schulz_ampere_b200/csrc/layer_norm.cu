@@ -13,11 +13,14 @@
 // written once per CTA and joined by a second kernel in a fixed order (no
 // atomics, the same bits on every run).
 //
-// Rows reach the registers in one of two ways. Aligned rows of more than 512
-// elements come through a ring of rows in shared memory, filled by bulk copies
-// several rows ahead (ring kernels); the bytes in flight do not depend on
-// registers or occupancy. Other rows are loaded directly, the next row before the
-// current row's reduction (direct kernels).
+// Rows reach the registers in one of two ways. Rows of more than 512 elements come
+// through a ring of rows in shared memory, filled by bulk copies several rows ahead
+// (ring kernels); the bytes in flight do not depend on registers or occupancy. Rows
+// that start anywhere are copied from the multiple of 16 bytes before them and read
+// out of the ring element by element (read directly from global memory, 20157 bf16
+// rows of 2337 took 166 us forward and 424 backward, now 93 and 99; fp32 rows 104 and
+// 162, now 86 and 92). Shorter rows are loaded directly, a row a warp, the next row
+// before the current row's reduction (direct kernels).
 // Statistics, sums and all arithmetic are fp32; y, dx, dw and db are rounded
 // once, at their stores. Bound by HBM: 2 elements moved forward, 3 backward.
 #include <algorithm>
@@ -384,8 +387,23 @@ struct Ring {
   }
 };
 
+// Bytes of a row behind a multiple of 16.
+template <int XD, bool VEC>
+__device__ __forceinline__ uint32_t row_shift(const void* base, int64_t row, int64_t stride) {
+  constexpr int es = XD == kF32 ? 4 : 2;
+  return VEC ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base) + row * stride * es) & 15u;
+}
+
+// A row into its slot. A row that starts anywhere is copied from the multiple of 16
+// before it to the one behind it: every 16 bytes read hold one of the row.
+template <int XD, bool VEC>
+__device__ __forceinline__ uint32_t row_span(const NormArgs& a, uint32_t shift) {
+  const uint32_t bytes = static_cast<uint32_t>(a.cols) * (XD == kF32 ? 4u : 2u);
+  return VEC ? bytes : (bytes + shift + 15u) & ~15u;
+}
+
 // One row of each tensor into a stage, by one thread of each group.
-template <int XD, int TENSORS>
+template <int XD, int TENSORS, bool VEC>
 __device__ __forceinline__ void fetch(Ring& ring, int st, int group, const NormArgs& a, int64_t row) {
   constexpr int es = XD == kF32 ? 4 : 2;
   if (row >= a.rows) {
@@ -393,11 +411,19 @@ __device__ __forceinline__ void fetch(Ring& ring, int st, int group, const NormA
     return;
   }
   uint8_t* slot = ring.slot(st, group, TENSORS);
-  mbar_arrive_expect_tx(&ring.full[st], TENSORS * ring.row_bytes);
-  bulk_load(slot, static_cast<const uint8_t*>(a.x) + row * a.x_stride * es, ring.row_bytes, &ring.full[st]);
+  const uint32_t x_shift = row_shift<XD, VEC>(a.x, row, a.x_stride);
+  const uint32_t dy_shift = TENSORS == 2 ? row_shift<XD, VEC>(a.dy, row, a.dy_stride) : 0u;
+  const uint32_t x_span = row_span<XD, VEC>(a, x_shift), dy_span = row_span<XD, VEC>(a, dy_shift);
+  mbar_arrive_expect_tx(&ring.full[st], x_span + (TENSORS == 2 ? dy_span : 0u));
+  bulk_load(slot, static_cast<const uint8_t*>(a.x) + row * a.x_stride * es - x_shift, x_span, &ring.full[st]);
   if (TENSORS == 2)
-    bulk_load(slot + ring.row_bytes, static_cast<const uint8_t*>(a.dy) + row * a.dy_stride * es, ring.row_bytes,
+    bulk_load(slot + ring.row_bytes, static_cast<const uint8_t*>(a.dy) + row * a.dy_stride * es - dy_shift, dy_span,
               &ring.full[st]);
+}
+
+// Slot of a row in a ring.
+__host__ __device__ constexpr uint32_t slot_bytes(bool vec, int64_t cols, int es) {
+  return static_cast<uint32_t>(vec ? cols * es : (cols * es + 15) / 16 * 16 + 16);
 }
 
 // Elements of a row per thread in the forward ring kernel: a reduction over a row
@@ -416,13 +442,14 @@ __device__ __forceinline__ float warp_total(float v) {
 // squared deviations from its own mean, S_w and Q_w, and over the warps
 //   mu = sum S_w / n,   n var = sum Q_w + n_w (S_w / n_w - mu)^2,
 // which loses nothing to cancellation, unlike sums of squares.
-template <int XD, int TPR>
+template <int XD, int TPR, bool VEC>
 __global__ void __launch_bounds__(threads_of<TPR>()) norm_forward_ring_kernel(const NormArgs a, int stages) {
   constexpr int kThreads = threads_of<TPR>();
   constexpr int kGroups = kThreads / TPR;
   constexpr int kW = TPR / 32;
   constexpr int E = kFwdPer;
-  using P = Piece<XD, TPR, true, E>;
+  using P = Piece<XD, TPR, VEC, E>;
+  constexpr int kStep = VEC ? P::kV : 1;  // columns that are in or out together
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float2 slots[2][kThreads / 32];  // S_w, Q_w
   __shared__ float2 sizes[kThreads / 32];     // n_w, 1 / n_w
@@ -432,15 +459,15 @@ __global__ void __launch_bounds__(threads_of<TPR>()) norm_forward_ring_kernel(co
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int mine = 0;
 #pragma unroll
-  for (int i = 0; i < E; i += P::kV) mine += P::col(t, i) < a.cols ? P::kV : 0;
+  for (int i = 0; i < E; i += kStep) mine += P::col(t, i) < a.cols ? kStep : 0;
   const float n_w = warp_total(static_cast<float>(mine));
   const float inv_w = n_w > 0.0f ? 1.0f / n_w : 0.0f;
   if (lane == 0) sizes[warp] = make_float2(n_w, inv_w);
-  Ring ring(smem, stages, kGroups, 1, static_cast<uint32_t>(a.cols) * (XD == kF32 ? 4 : 2));
+  Ring ring(smem, stages, kGroups, 1, slot_bytes(VEC, a.cols, XD == kF32 ? 4 : 2));
   const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
   const int64_t base = static_cast<int64_t>(blockIdx.x) * kGroups;
   if (t == 0)
-    for (int i = 0; i < stages; ++i) fetch<XD, 1>(ring, i, group, a, base + group + i * step);
+    for (int i = 0; i < stages; ++i) fetch<XD, 1, VEC>(ring, i, group, a, base + group + i * step);
   float w[E], b[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) {
@@ -453,7 +480,7 @@ __global__ void __launch_bounds__(threads_of<TPR>()) norm_forward_ring_kernel(co
     const int64_t row = first + group;
     ring.wait();
     P p;
-    p.load(ring.slot(ring.stage, group, 1), 0, 0, t, a.cols, true);
+    p.load(ring.slot(ring.stage, group, 1) + row_shift<XD, VEC>(a.x, row, a.x_stride), 0, 0, t, a.cols, true);
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < E; ++i) sum += p.get(i);
@@ -461,10 +488,10 @@ __global__ void __launch_bounds__(threads_of<TPR>()) norm_forward_ring_kernel(co
     const float mean_w = sum * inv_w;
     float sq = 0.0f;
 #pragma unroll
-    for (int i = 0; i < E; i += P::kV) {
+    for (int i = 0; i < E; i += kStep) {
       if (P::col(t, i) >= a.cols) continue;
 #pragma unroll
-      for (int q = 0; q < P::kV; ++q) {
+      for (int q = 0; q < kStep; ++q) {
         const float d = p.get(i + q) - mean_w;
         sq = fmaf(d, d, sq);
       }
@@ -501,7 +528,7 @@ __global__ void __launch_bounds__(threads_of<TPR>()) norm_forward_ring_kernel(co
       __syncwarp();
     }
     // Every thread of the group has read the slot: it is filled again.
-    if (t == 0) fetch<XD, 1>(ring, ring.stage, group, a, row + stages * step);
+    if (t == 0) fetch<XD, 1, VEC>(ring, ring.stage, group, a, row + stages * step);
     ring.advance();
     const float r = rsqrtf(fmaf(var, inv_n, a.eps));
     const float shift = -mu * r;
@@ -509,7 +536,7 @@ __global__ void __launch_bounds__(threads_of<TPR>()) norm_forward_ring_kernel(co
       float v[E];
 #pragma unroll
       for (int i = 0; i < E; ++i) v[i] = fmaf(fmaf(p.get(i), r, shift), w[i], b[i]);
-      store_row<XD, TPR, true, E>(a.y, row, a.cols, t, v);
+      store_row<XD, TPR, VEC, E>(a.y, row, a.cols, t, v);
       if (t == 0) {
         a.mean[row] = mu;
         a.rstd[row] = r;
@@ -519,29 +546,29 @@ __global__ void __launch_bounds__(threads_of<TPR>()) norm_forward_ring_kernel(co
   ring.finish();
 }
 
-template <int XD, int TPR>
+template <int XD, int TPR, bool VEC>
 __global__ void __launch_bounds__(threads_of<TPR>()) norm_backward_ring_kernel(const NormArgs a, int stages) {
   pdl_launch_dependents();
   constexpr int kThreads = threads_of<TPR>();
   constexpr int kGroups = kThreads / TPR;
-  using P = Piece<XD, TPR, true>;
+  using P = Piece<XD, TPR, VEC>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float2 slots[2][kThreads / 32];
   int slot = 0;
   const int t = threadIdx.x % TPR;
   const int group = threadIdx.x / TPR;
-  Ring ring(smem, stages, kGroups, 2, static_cast<uint32_t>(a.cols) * (XD == kF32 ? 4 : 2));
+  Ring ring(smem, stages, kGroups, 2, slot_bytes(VEC, a.cols, XD == kF32 ? 4 : 2));
   const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
   const int64_t base = static_cast<int64_t>(blockIdx.x) * kGroups;
   if (t == 0)
-    for (int i = 0; i < stages; ++i) fetch<XD, 2>(ring, i, group, a, base + group + i * step);
+    for (int i = 0; i < stages; ++i) fetch<XD, 2, VEC>(ring, i, group, a, base + group + i * step);
   // Elements go two to an instruction (one at a time the kernel took 77 us for 16384
   // bf16 rows of 4096).
   Pair w[kPer / 2], dw[kPer / 2], db[kPer / 2];
 #pragma unroll
   for (int i = 0; i < kPer; i += 2) {
-    const int c = P::col(t, i);  // rows are multiples of 16 bytes: both columns are in or out
-    w[i / 2] = c < a.cols ? Pair(load_as_float(a.w, c, a.w_dt), load_as_float(a.w, c + 1, a.w_dt)) : Pair(0.0f);
+    const int c = P::col(t, i), d = P::col(t, i + 1);
+    w[i / 2] = Pair(c < a.cols ? load_as_float(a.w, c, a.w_dt) : 0.0f, d < a.cols ? load_as_float(a.w, d, a.w_dt) : 0.0f);
     dw[i / 2] = Pair(0.0f);
     db[i / 2] = Pair(0.0f);
   }
@@ -563,8 +590,8 @@ __global__ void __launch_bounds__(threads_of<TPR>()) norm_backward_ring_kernel(c
     ring.wait();
     const uint8_t* at = ring.slot(ring.stage, group, 2);
     P px, pg;
-    px.load(at, 0, 0, t, a.cols, live);
-    pg.load(at + ring.row_bytes, 0, 0, t, a.cols, live);
+    px.load(at + row_shift<XD, VEC>(a.x, row, a.x_stride), 0, 0, t, a.cols, live);
+    pg.load(at + ring.row_bytes + row_shift<XD, VEC>(a.dy, row, a.dy_stride), 0, 0, t, a.cols, live);
     Pair h[kPer / 2], g[kPer / 2], s1(0.0f), s2(0.0f);
 #pragma unroll
     for (int i = 0; i < kPer / 2; ++i) {
@@ -580,13 +607,13 @@ __global__ void __launch_bounds__(threads_of<TPR>()) norm_backward_ring_kernel(c
     s1.get(s1a, s1b);
     s2.get(s2a, s2b);
     const float2 c = group_sum<TPR, kThreads>(s1a + s1b, s2a + s2b, slots, slot);
-    if (t == 0) fetch<XD, 2>(ring, ring.stage, group, a, row + stages * step);
+    if (t == 0) fetch<XD, 2, VEC>(ring, ring.stage, group, a, row + stages * step);
     ring.advance();
     const Pair c1(-c.x * inv_n), c2(-c.y * inv_n);
     float out[kPer];
 #pragma unroll
     for (int i = 0; i < kPer / 2; ++i) mul2(add2(fma2(h[i], c1, c2), g[i]), Pair(r)).get(out[2 * i], out[2 * i + 1]);
-    if (live) store_row<XD, TPR, true, kPer>(a.y, row, a.cols, t, out);
+    if (live) store_row<XD, TPR, VEC, kPer>(a.y, row, a.cols, t, out);
   }
   float dws[kPer], dbs[kPer];
 #pragma unroll
@@ -700,8 +727,8 @@ int threads_per_row(int64_t cols, int per) {
   return t;
 }
 
-// How a call runs: `stages` > 0, the ring kernels; else the direct kernels, or the
-// wide ones for rows that no CTA's registers hold.
+// How a call runs: `stages` > 0, the ring kernels; else the direct kernels for rows of
+// up to 512 elements, or the wide ones for rows that no CTA's registers or ring hold.
 struct Plan {
   bool wide;
   int stages, grid, tpr;
@@ -714,7 +741,7 @@ constexpr int kRingBytes = 200 * 1024;
 
 Plan plan_norm(bool backward, bool vec, int x_dt, int64_t rows, int64_t cols) {
   Plan p{};
-  const bool ring = vec && cols > 32 * kPer && cols <= static_cast<int64_t>(kMaxTPR) * kPer;
+  const bool ring = cols > 32 * kPer && cols <= static_cast<int64_t>(kMaxTPR) * kPer;
   const int tpr = threads_per_row(cols, ring && !backward ? kFwdPer : kPer);
   const int threads = tpr < 256 ? 256 : tpr;
   const int groups = threads / tpr;
@@ -723,7 +750,7 @@ Plan plan_norm(bool backward, bool vec, int x_dt, int64_t rows, int64_t cols) {
   p.tpr = tpr;
   if (ring) {
     const int ctas = threads > 256 ? 1 : 2;  // per SM: what the registers allow
-    const int64_t stage = cols * dtype_size(x_dt) * groups * (backward ? 2 : 1);
+    const int64_t stage = static_cast<int64_t>(slot_bytes(vec, cols, dtype_size(x_dt))) * groups * (backward ? 2 : 1);
     const int64_t stages = kRingBytes / ctas / stage;
     if (stages >= 2) {
       p.stages = static_cast<int>(stages < kMaxStages ? stages : kMaxStages);
@@ -735,7 +762,7 @@ Plan plan_norm(bool backward, bool vec, int x_dt, int64_t rows, int64_t cols) {
     }
   }
   p.tpr = threads_per_row(cols, kPer);
-  p.wide = p.tpr == kMaxTPR;
+  p.wide = p.tpr > 32;
   if (p.wide) {
     const int64_t most = 2 * static_cast<int64_t>(sms);
     p.grid = static_cast<int>(rows < most ? rows : most);
@@ -761,20 +788,21 @@ bool is_lone(const Plan& p, int64_t rows) {
 int backward_parts(const Plan& p, int64_t rows) { return p.wide ? static_cast<int>(rows < 64 ? rows : 64) : p.grid; }
 
 std::mutex g_mutex;
-bool g_ready[64][64] = {};
+bool g_ready[64][128] = {};
 
-template <int XD, int TPR>
+template <int XD, int TPR, bool VEC>
 int launch_ring(bool backward, const Plan& p, int slot, cudaStream_t st, const NormArgs& a) {
   // The forward kernel's 32 elements a thread need no more than 512 threads, and the
   // backward kernel's 16 no fewer than 64.
-  auto kernel = backward ? norm_backward_ring_kernel<XD, (TPR < 64 ? 64 : TPR)> : norm_forward_ring_kernel<XD, (TPR > 512 ? 512 : TPR)>;
+  auto kernel = backward ? norm_backward_ring_kernel<XD, (TPR < 64 ? 64 : TPR), VEC>
+                         : norm_forward_ring_kernel<XD, (TPR > 512 ? 512 : TPR), VEC>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
   if (dev < 0 || dev >= 64) return fail(GNS_ERR_DEVICE, "device index out of range");
   {
     std::lock_guard<std::mutex> lock(g_mutex);
-    bool& ready = g_ready[dev][slot + (backward ? 32 : 0)];
+    bool& ready = g_ready[dev][slot + (backward ? 32 : 0) + (VEC ? 0 : 64)];
     if (!ready) {
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes + 1024);
       if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(smem)");
@@ -785,41 +813,37 @@ int launch_ring(bool backward, const Plan& p, int slot, cudaStream_t st, const N
   return GNS_OK;
 }
 
-template <int XD, int TPR, bool VEC>
+template <int XD, bool VEC>
 int launch_direct(bool backward, const Plan& p, cudaStream_t st, const NormArgs& a) {
   if (backward)
-    norm_backward_kernel<XD, TPR, VEC><<<p.grid, threads_of<TPR>(), 0, st>>>(a);
+    norm_backward_kernel<XD, 32, VEC><<<p.grid, threads_of<32>(), 0, st>>>(a);
   else
-    norm_forward_kernel<XD, TPR, VEC><<<p.grid, threads_of<TPR>(), 0, st>>>(a);
+    norm_forward_kernel<XD, 32, VEC><<<p.grid, threads_of<32>(), 0, st>>>(a);
   return GNS_OK;
 }
 
-template <int XD>
-int launch_type(bool backward, bool vec, const Plan& p, cudaStream_t st, const NormArgs& a) {
-  if (p.stages > 0) {
-    switch (p.tpr) {
-      case 32: return launch_ring<XD, 32>(backward, p, 8 * XD + 5, st, a);
-      case 64: return launch_ring<XD, 64>(backward, p, 8 * XD, st, a);
-      case 128: return launch_ring<XD, 128>(backward, p, 8 * XD + 1, st, a);
-      case 256: return launch_ring<XD, 256>(backward, p, 8 * XD + 2, st, a);
-      case 512: return launch_ring<XD, 512>(backward, p, 8 * XD + 3, st, a);
-      default: return launch_ring<XD, 1024>(backward, p, 8 * XD + 4, st, a);
-    }
-  }
-  if (vec && p.tpr == 32) return launch_direct<XD, 32, true>(backward, p, st, a);
+template <int XD, bool VEC>
+int launch_type(bool backward, const Plan& p, cudaStream_t st, const NormArgs& a) {
+  if (p.stages == 0) return launch_direct<XD, VEC>(backward, p, st, a);
   switch (p.tpr) {
-    case 32: return launch_direct<XD, 32, false>(backward, p, st, a);
-    case 64: return launch_direct<XD, 64, false>(backward, p, st, a);
-    case 128: return launch_direct<XD, 128, false>(backward, p, st, a);
-    case 256: return launch_direct<XD, 256, false>(backward, p, st, a);
-    default: return launch_direct<XD, 512, false>(backward, p, st, a);
+    case 32: return launch_ring<XD, 32, VEC>(backward, p, 8 * XD + 5, st, a);
+    case 64: return launch_ring<XD, 64, VEC>(backward, p, 8 * XD, st, a);
+    case 128: return launch_ring<XD, 128, VEC>(backward, p, 8 * XD + 1, st, a);
+    case 256: return launch_ring<XD, 256, VEC>(backward, p, 8 * XD + 2, st, a);
+    case 512: return launch_ring<XD, 512, VEC>(backward, p, 8 * XD + 3, st, a);
+    default: return launch_ring<XD, 1024, VEC>(backward, p, 8 * XD + 4, st, a);
   }
 }
 
+template <int XD>
+int launch_rows(bool backward, bool vec, const Plan& p, cudaStream_t st, const NormArgs& a) {
+  return vec ? launch_type<XD, true>(backward, p, st, a) : launch_type<XD, false>(backward, p, st, a);
+}
+
 int launch_any(bool backward, bool vec, int x_dt, const Plan& p, cudaStream_t st, const NormArgs& a) {
-  if (x_dt == kBF16) return launch_type<kBF16>(backward, vec, p, st, a);
-  if (x_dt == kF16) return launch_type<kF16>(backward, vec, p, st, a);
-  return launch_type<kF32>(backward, vec, p, st, a);
+  if (x_dt == kBF16) return launch_rows<kBF16>(backward, vec, p, st, a);
+  if (x_dt == kF16) return launch_rows<kF16>(backward, vec, p, st, a);
+  return launch_rows<kF32>(backward, vec, p, st, a);
 }
 
 // Rows that 16-byte pieces can be read from: every piece aligned and none past the end.

@@ -98,6 +98,22 @@ def test_shapes_strides_and_no_bias(cuda_device):
     check_norm(x[0], weight, bias, grad[0])
 
 
+@pytest.mark.parametrize("rows", [2, 1500])
+@pytest.mark.parametrize("columns", [513, 1024, 1027, 2053, 5003, 8200, 16381])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_rows_that_start_anywhere(cuda_device, rows, columns, dtype):
+    """Rows of x and of its gradient at different offsets, between rows of NaN."""
+    gen = torch.Generator(device=cuda_device).manual_seed(7)
+    values, weight, bias, grads = inputs(gen, rows, columns, dtype, torch.float32, cuda_device)
+    nan = float("nan")
+    wide = torch.full((rows + 2, columns + 6), nan, dtype=dtype, device=cuda_device)
+    grad = torch.full((rows + 2, columns + 11), nan, dtype=dtype, device=cuda_device)
+    x, dy = wide[1:-1, 1:columns + 1], grad[1:-1, 3:columns + 3]
+    x.copy_(values)
+    dy.copy_(grads)
+    check_norm(x, weight, bias, dy)
+
+
 def test_constant_and_large_rows(cuda_device):
     """Rows of one value (variance zero), rows far from zero, rows of large values."""
     gen = torch.Generator(device=cuda_device).manual_seed(4)
