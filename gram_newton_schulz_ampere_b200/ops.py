@@ -1160,7 +1160,8 @@ def grouped_gemm(left: Tensor, right: Tensor, ends: Tensor, out_dtype: torch.dty
     group e owns the rows ``ends[e - 1] <= r < ends[e]``. They are read on the device, without
     a synchronisation, and are clamped to [0, T] and to ascending order. Rows that no group
     owns (from ``ends[-1]`` on) come out zero. Sums are fp32, rounded once to ``out_dtype``
-    (default: the inputs' type).
+    (default: the inputs' type); their order depends on the sizes of the call (few rows with
+    a long k are summed in parts), never on the run.
 
     With an expert layer's weights W [E, n, k], the layer is
     ``grouped_gemm(x, W.transpose(1, 2), ends)``, its gradient for the rows
