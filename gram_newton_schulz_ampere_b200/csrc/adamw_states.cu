@@ -349,7 +349,7 @@ struct Slot {
 // without a register held for it, and no barrier between warps. Loads into
 // registers kept 41 KB in flight and moved 2.9 TB/s, or 4.5 TB/s with the next
 // block prefetched; the ring moves 6.3 TB/s, 0.98 of the measured copy rate (323M
-// bf16 elements in 1129, 717 and 515 us; four CTAs an SM at 64 registers instead of
+// bf16 elements in 1129, 717 and 508 us; four CTAs an SM at 64 registers instead of
 // three: 553). The scales of the warp's blocks are read and written once, a lane
 // for each.
 //
