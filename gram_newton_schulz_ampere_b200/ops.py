@@ -969,7 +969,7 @@ class AdamWStates:
         def scales(given: Sequence[Tensor] | None) -> list[Tensor]:
             counts = [(p.numel() + STATE_BLOCK - 1) // STATE_BLOCK for p in self.parameters]
             if given is None:
-                return [torch.zeros(n, dtype=torch.float32, device=self.device) for n in counts]
+                return [torch.zeros(n, dtype=torch.float32, device=p.device) for n, p in zip(counts, self.parameters)]
             return self._checked(given, torch.float32, counts, "scales")
 
         self.exp_avgs = moments(exp_avgs)
@@ -978,11 +978,7 @@ class AdamWStates:
         self.exp_avg_sq_scales = scales(exp_avg_sq_scales) if bits == 8 else []
         self._numel = [p.numel() for p in self.parameters]
         self._sizes = (ctypes.c_int64 * max(len(self._numel), 1))(*self._numel)
-        self._states = (
-            _ptr_array(self.exp_avgs), _ptr_array(self.exp_avg_sqs),
-            _ptr_array(self.exp_avg_scales) if bits == 8 else None,
-            _ptr_array(self.exp_avg_sq_scales) if bits == 8 else None,
-        )
+        self._note(*self._tensors_now())
 
     def _checked(self, given: Sequence[Tensor], dtype: torch.dtype, counts: list[int], what: str) -> list[Tensor]:
         if len(given) != len(counts):
@@ -997,6 +993,44 @@ class AdamWStates:
             if t.device != self.device:
                 raise ValueError("all tensors must be on the same CUDA device")
         return list(given)
+
+    def _tensors_now(self) -> tuple[array.array, list[int]]:
+        """Addresses and bytes of the parameters, moments and scales."""
+        held = [*self.parameters, *self.exp_avgs, *self.exp_avg_sqs, *self.exp_avg_scales, *self.exp_avg_sq_scales]
+        return array.array("Q", map(Tensor.data_ptr, held)), [t.nbytes for t in held]
+
+    def _note(self, places: array.array, extents: list[int]) -> None:
+        """Keeps what was checked, and each list's addresses as the native call takes them."""
+        self._places, self._bytes = places, extents
+        row = ctypes.c_void_p * len(self._numel)
+        self._rows = tuple(
+            row.from_buffer(places, i * ctypes.sizeof(row)) if row._length_ and (i < 3 or self.bits == 8) else None
+            for i in range(5)
+        )
+
+    def _look_at_tensors(self) -> None:
+        """Brings ``_rows`` up to date with the tensors in the lists. Between two steps any of
+        them may be replaced, or moved by an assignment to its ``.data``, so their addresses are
+        read on every step. All else is checked again only where an address or the bytes behind
+        it are new (checked on every step it would cost twice the rest of a small step)."""
+        places, extents = self._tensors_now()
+        if places == self._places and extents == self._bytes:
+            return
+        for p, n in zip(self.parameters, self._numel, strict=True):
+            if p.numel() != n:
+                raise ValueError("a parameter's size is not that of its moments")
+            if p.dtype != self.parameters[0].dtype:
+                raise TypeError("all parameters of one call must share a dtype")
+            if p.device != self.device:
+                raise ValueError("parameters must stay on the device of their moments")
+        dtype = torch.float8_e4m3fn if self.bits == 8 else torch.float32
+        self._checked(self.exp_avgs, dtype, self._numel, "moments")
+        self._checked(self.exp_avg_sqs, dtype, self._numel, "moments")
+        if self.bits == 8:
+            counts = [(n + STATE_BLOCK - 1) // STATE_BLOCK for n in self._numel]
+            self._checked(self.exp_avg_scales, torch.float32, counts, "scales")
+            self._checked(self.exp_avg_sq_scales, torch.float32, counts, "scales")
+        self._note(places, extents)
 
     def step(
         self,
@@ -1021,7 +1055,7 @@ class AdamWStates:
         if not epsilon > 0.0:
             raise ValueError(f"epsilon must be positive, got {epsilon}")
         try:
-            dtypes = {cast(Tensor, g).dtype for g in gradients}
+            dtypes = {g.dtype for g in gradients}  # type: ignore[union-attr]
             whole = True
         except AttributeError:  # None among them
             whole = False
@@ -1040,8 +1074,9 @@ class AdamWStates:
         if not (all(map(Tensor.is_contiguous, given)) and all(map(Tensor.is_contiguous, places))):
             raise ValueError("gradients and parameters must be contiguous")
         index = cast(torch.device, self.device).index
-        if set(map(Tensor.get_device, given)) != {index} or set(map(Tensor.get_device, places)) != {index}:
+        if set(map(Tensor.get_device, given)) != {index}:
             raise ValueError("gradients must be on the parameters' device")
+        self._look_at_tensors()
         if gradient_scale is not None:
             if gradient_scale.dtype != torch.float32 or gradient_scale.numel() != 1:
                 raise ValueError("gradient_scale must be one float32 value")
@@ -1058,15 +1093,15 @@ class AdamWStates:
                 raise ValueError("step must be one value or one for each parameter")
             pairs = [self._bias_corrections(step[i], learning_rate, beta1, beta2) for i in present]
             corrections = tuple(floats.from_buffer(array.array("f", values)) for values in zip(*pairs))
-        states, sizes = self._states, self._sizes
+        rows, sizes = self._rows, self._sizes
         if not whole:
             sizes = (ctypes.c_int64 * len(given))(*numel)
-            roles = (self.exp_avgs, self.exp_avg_sqs, self.exp_avg_scales, self.exp_avg_sq_scales)
-            states = tuple(_ptr_array([role[i] for i in present]) if role else None for role in roles)
+            roles = (self.parameters, self.exp_avgs, self.exp_avg_sqs, self.exp_avg_scales, self.exp_avg_sq_scales)
+            rows = tuple(_ptr_array([role[i] for i in present]) if role else None for role in roles)
         lib = nat.load()
         with nat.on_device(index) as stream:
             rc = lib.gns_adamw_states_step(
-                len(given), _pointers(places), _pointers(given), *states, sizes,
+                len(given), rows[0], _pointers(given), *rows[1:], sizes,
                 nat.dtype_code(places[0].dtype), nat.dtype_code(g_dtype), self.bits, *corrections,
                 beta1, 1 - beta1, beta2, 1 - beta2, epsilon, 1 - learning_rate * weight_decay,
                 nat.ptr(gradient_scale), stream,
