@@ -531,11 +531,15 @@ __global__ void __launch_bounds__(threads_of<TPR>()) norm_forward_ring_kernel(co
     if (t == 0) fetch<XD, 1, VEC>(ring, ring.stage, group, a, row + stages * step);
     ring.advance();
     const float r = rsqrtf(fmaf(var, inv_n, a.eps));
-    const float shift = -mu * r;
     if (row < a.rows) {
+      // The mean is taken off before the scaling: x r - mu r would round mu r, which shows
+      // where the mean is large beside the deviations (a row of 1000s came out 0.01 off).
       float v[E];
 #pragma unroll
-      for (int i = 0; i < E; ++i) v[i] = fmaf(fmaf(p.get(i), r, shift), w[i], b[i]);
+      for (int i = 0; i < E; i += 2) {
+        const Pair h = mul2(add2(Pair(p.get(i), p.get(i + 1)), Pair(-mu)), Pair(r));
+        fma2(h, Pair(w[i], w[i + 1]), Pair(b[i], b[i + 1])).get(v[i], v[i + 1]);
+      }
       store_row<XD, TPR, VEC, E>(a.y, row, a.cols, t, v);
       if (t == 0) {
         a.mean[row] = mu;
