@@ -34,6 +34,7 @@ namespace gns {
 namespace {
 
 constexpr int kPer = 16;        // elements of a row per thread
+constexpr int kDirectTPR = 32;  // the direct kernels: a row a warp
 constexpr int kMaxTPR = 1024;   // threads of a row; wider rows are read twice (the wide kernels)
 constexpr int kWideThreads = 1024;
 constexpr int kColThreads = 256;
@@ -184,8 +185,9 @@ constexpr int threads_of() {
   return TPR < 256 ? 256 : TPR;
 }
 
-template <int XD, int TPR, bool VEC>
-__global__ void __launch_bounds__(threads_of<TPR>()) norm_forward_kernel(const NormArgs a) {
+template <int XD, bool VEC>
+__global__ void __launch_bounds__(threads_of<kDirectTPR>()) norm_forward_kernel(const NormArgs a) {
+  constexpr int TPR = kDirectTPR;
   constexpr int kThreads = threads_of<TPR>();
   constexpr int kGroups = kThreads / TPR;
   using P = Piece<XD, TPR, VEC>;
@@ -278,8 +280,9 @@ __device__ __forceinline__ void write_partial(const NormArgs& a, const float (&d
   }
 }
 
-template <int XD, int TPR, bool VEC>
-__global__ void __launch_bounds__(threads_of<TPR>()) norm_backward_kernel(const NormArgs a) {
+template <int XD, bool VEC>
+__global__ void __launch_bounds__(threads_of<kDirectTPR>()) norm_backward_kernel(const NormArgs a) {
+  constexpr int TPR = kDirectTPR;
   pdl_launch_dependents();
   constexpr int kThreads = threads_of<TPR>();
   constexpr int kGroups = kThreads / TPR;
@@ -798,8 +801,10 @@ template <int XD, int TPR, bool VEC>
 int launch_ring(bool backward, const Plan& p, int slot, cudaStream_t st, const NormArgs& a) {
   // The forward kernel's 32 elements a thread need no more than 512 threads, and the
   // backward kernel's 16 no fewer than 64.
-  auto kernel = backward ? norm_backward_ring_kernel<XD, (TPR < 64 ? 64 : TPR), VEC>
-                         : norm_forward_ring_kernel<XD, (TPR > 512 ? 512 : TPR), VEC>;
+  constexpr int kForward = TPR > 512 ? 512 : TPR, kBackward = TPR < 64 ? 64 : TPR;
+  auto kernel = backward ? norm_backward_ring_kernel<XD, kBackward, VEC> : norm_forward_ring_kernel<XD, kForward, VEC>;
+  const int threads = backward ? threads_of<kBackward>() : threads_of<kForward>();
+  if (p.tpr != (backward ? kBackward : kForward)) return fail(GNS_ERR_UNSUPPORTED, "no ring kernel has these threads a row");
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
@@ -813,16 +818,16 @@ int launch_ring(bool backward, const Plan& p, int slot, cudaStream_t st, const N
       ready = true;
     }
   }
-  kernel<<<p.grid, threads_of<TPR>(), p.smem, st>>>(a, p.stages);
+  kernel<<<p.grid, threads, p.smem, st>>>(a, p.stages);
   return GNS_OK;
 }
 
 template <int XD, bool VEC>
 int launch_direct(bool backward, const Plan& p, cudaStream_t st, const NormArgs& a) {
   if (backward)
-    norm_backward_kernel<XD, 32, VEC><<<p.grid, threads_of<32>(), 0, st>>>(a);
+    norm_backward_kernel<XD, VEC><<<p.grid, threads_of<kDirectTPR>(), 0, st>>>(a);
   else
-    norm_forward_kernel<XD, 32, VEC><<<p.grid, threads_of<32>(), 0, st>>>(a);
+    norm_forward_kernel<XD, VEC><<<p.grid, threads_of<kDirectTPR>(), 0, st>>>(a);
   return GNS_OK;
 }
 
