@@ -5,9 +5,9 @@
 //   backward  h = (x - mu) r,  a = w dy,  c1 = mean(a h),  c2 = mean(a)
 //             dx = r (a - c2 - h c1);  dw = sum over rows of dy h;  db = sum of dy
 //
-// A row is held in the registers of TPR threads, 16 elements each, so x (and dy)
-// are read once: the mean is subtracted before the squares are summed, which
-// costs a second reduction but no second read. Rows go to the groups of a
+// A row is held in the registers of TPR threads, 16 elements each (32 in the forward
+// ring kernel), so x (and dy) are read once: the mean is subtracted before the squares
+// are summed, which costs a second reduction but no second read. Rows go to the groups of a
 // persistent grid round robin. Each thread keeps the same columns for all its
 // rows: w and b stay in registers, and dw and db are summed there over the rows,
 // written once per CTA and joined by a second kernel in a fixed order (no
@@ -20,7 +20,12 @@
 // out of the ring element by element (read directly from global memory, 20157 bf16
 // rows of 2337 took 166 us forward and 424 backward, now 93 and 99; fp32 rows 104 and
 // 162, now 86 and 92). Shorter rows are loaded directly, a row a warp, the next row
-// before the current row's reduction (direct kernels).
+// before the current row's reduction (direct kernels). Rows that have no place there go
+// to the wide kernels, element by element from global memory in three passes: rows of
+// more than 16384 elements, and in the backward pass fp32 rows from 12801 elements on
+// (fewer by a few where they start anywhere), of which a stage of x and dy does not fit a
+// ring twice (4096 fp32 rows backward: 12800 elements 183 us through the ring, 12808
+// elements 339 without; 20480 bf16 elements 283 us forward and 472 backward).
 // Statistics, sums and all arithmetic are fp32; y, dx, dw and db are rounded
 // once, at their stores. Bound by HBM: 2 elements moved forward, 3 backward.
 #include <algorithm>
@@ -35,7 +40,7 @@ namespace {
 
 constexpr int kPer = 16;        // elements of a row per thread
 constexpr int kDirectTPR = 32;  // the direct kernels: a row a warp
-constexpr int kMaxTPR = 1024;   // threads of a row; wider rows are read twice (the wide kernels)
+constexpr int kMaxTPR = 1024;   // threads of a row; wider rows have kernels of their own
 constexpr int kWideThreads = 1024;
 constexpr int kColThreads = 256;
 
@@ -632,7 +637,8 @@ __global__ void __launch_bounds__(threads_of<TPR>()) norm_backward_ring_kernel(c
   write_partial<TPR, P>(a, dws, dbs, reinterpret_cast<float*>(ring.rows), t, group);
 }
 
-// Rows too wide for the registers of a CTA: a CTA per row, read again for each pass.
+// Rows that no ring holds: a CTA per row. Forward x is read three times (sum, squares,
+// result), backward x and dy twice for dx and once more for the sums over the rows.
 __device__ __forceinline__ float2 cta_sum(float a, float b, float2 (*slots)[kWideThreads / 32], int& slot) {
   return group_sum<kWideThreads, kWideThreads>(a, b, slots, slot);
 }
@@ -735,7 +741,7 @@ int threads_per_row(int64_t cols, int per) {
 }
 
 // How a call runs: `stages` > 0, the ring kernels; else the direct kernels for rows of
-// up to 512 elements, or the wide ones for rows that no CTA's registers or ring hold.
+// up to 512 elements, or the wide ones for rows that no ring holds in two stages.
 struct Plan {
   bool wide;
   int stages, grid, tpr;
