@@ -897,17 +897,22 @@ class Muon(Optimizer):
         for entries in members.values():
             steps = [state["step"] for _, _, state in entries]
             values = self._host_step_values(steps)
-            torch._foreach_add_(steps, 1)
             writeback: list[tuple[Tensor, Tensor]] = []
-            held = {name: [state[name] for _, _, state in entries] for name in ADAMW_STATES if name in entries[0][2]}
-            states = ops.AdamWStates(
-                [_contiguous_in_place(p.detach(), writeback) for p, _, _ in entries], bits,
-                held["exp_avg"], held["exp_avg_sq"], held.get("exp_avg_scale"), held.get("exp_avg_sq_scale"),
-            )
-            states.step(
-                [g.contiguous() for _, g, _ in entries], float(cast(LearningRate, group["lr"])), beta1, beta2,
-                cast(float, group["epsilon"]), float(cast(LearningRate, group["weight_decay"])), values,
-            )
+            try:
+                held = {name: [state[name] for _, _, state in entries] for name in ADAMW_STATES if name in entries[0][2]}
+                states = ops.AdamWStates(
+                    [_contiguous_in_place(p.detach(), writeback) for p, _, _ in entries], bits,
+                    held["exp_avg"], held["exp_avg_sq"], held.get("exp_avg_scale"), held.get("exp_avg_sq_scale"),
+                )
+                states.step(
+                    [g.contiguous() for _, g, _ in entries], float(cast(LearningRate, group["lr"])), beta1, beta2,
+                    cast(float, group["epsilon"]), float(cast(LearningRate, group["weight_decay"])), values,
+                )
+            except Exception:  # no step was taken: the counts stay, and are read back before the next one
+                for t in steps:
+                    self.__dict__["_adamw_host_steps"].pop(id(t), None)
+                raise
+            torch._foreach_add_(steps, 1)
             for original, copy in writeback:
                 original.copy_(copy)
 
