@@ -202,8 +202,9 @@ class Muon(Optimizer):
             raise ValueError(f"Unknown Newton--Schulz algorithm: {self.ns_algorithm}")
 
     def load_state_dict(self, state_dict: StateDict) -> None:
+        configured = [cast("int | None", group.get("state_bits")) for group in self.param_groups]
         super().load_state_dict(state_dict)
-        self._restore_adamw_states(state_dict)
+        self._restore_adamw_states(state_dict, configured)
         first = self.param_groups[0]
         self.ns_algorithm = cast(NewtonSchulzAlgorithm, first.get("ns_algorithm", self.ns_algorithm))
         self.ns_epsilon = cast(float, first.get("ns_epsilon", self.ns_epsilon))
@@ -225,17 +226,38 @@ class Muon(Optimizer):
         self.validate_cuda_configuration()
         self.configure_newton_schulz()
 
-    def _restore_adamw_states(self, state_dict: StateDict) -> None:
-        """Moments, scales and step counts of the groups with ``state_bits`` as they were saved,
-        in tensors of their own: torch's loading casts every state tensor to its parameter's
+    def _restore_adamw_states(self, state_dict: StateDict, configured: Sequence[int | None]) -> None:
+        """Moments, scales and step counts of the adamw groups that are, or were when they were
+        saved, held with ``state_bits``. A group keeps the ``state_bits`` it was configured with
+        (torch's loading takes the saved group's settings): moments saved in another form are
+        brought into it, the others stay as they were saved, bit for bit. Either way they get
+        tensors of their own: torch's loading casts every state tensor to its parameter's
         type, which would round them, and shares those that need no cast with the source."""
-        for group, saved in zip(self.param_groups, state_dict["param_groups"], strict=True):
-            if group["algorithm"] != "adamw" or group.get("state_bits") is None:
+        for group, saved, bits in zip(self.param_groups, state_dict["param_groups"], configured, strict=True):
+            was = saved.get("state_bits")
+            if group["algorithm"] != "adamw" or (bits is None and was is None):
                 continue
+            group["state_bits"] = bits
             for parameter, key in zip(cast(list[Tensor], group["params"]), saved["params"], strict=True):
-                for name, value in state_dict["state"].get(key, {}).items():
-                    if name in ADAMW_STATES or name == "step":
-                        self.state[parameter][name] = value.detach().to(parameter.device, copy=True)
+                held = {
+                    name: value.detach().to(parameter.device, copy=True)
+                    for name, value in state_dict["state"].get(key, {}).items()
+                    if name in ADAMW_STATES or name == "step"
+                }
+                if bits != was and "exp_avg" in held:
+                    if isinstance(parameter, DTensor):
+                        raise ValueError("moments saved with state_bits cannot be loaded for a DTensor parameter")
+                    for name in ADAMW_STATES[:2]:
+                        moment, scale = held[name], held.pop(f"{name}_scale", None)
+                        if scale is not None:
+                            moment = ops.moment_from_8_bits(moment, scale)
+                        if bits == 8:
+                            held[name], held[f"{name}_scale"] = ops.moment_in_8_bits(moment, name == "exp_avg_sq")
+                        else:
+                            held[name] = moment.to(torch.float32 if bits == 32 else parameter.dtype)
+                for name in ADAMW_STATES:
+                    self.state[parameter].pop(name, None)
+                self.state[parameter].update(held)
 
     def add_param_group(self, param_group: ParameterGroupInput) -> None:
         group_count = len(self.param_groups)

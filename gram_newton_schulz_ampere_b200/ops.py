@@ -916,6 +916,25 @@ def _pointers(tensors: Sequence[Tensor]) -> ctypes.Array:
     return (ctypes.c_void_p * len(places)).from_buffer(places)
 
 
+def moment_in_8_bits(moment: Tensor, second: bool) -> tuple[Tensor, Tensor]:
+    """A moment as ``AdamWStates`` holds it in 8 bits: e4m3 values of its shape and one fp32 scale
+    for each ``STATE_BLOCK`` elements. ``second``: values above zero stay above it."""
+    flat = moment.detach().reshape(-1).float()
+    blocks = torch.nn.functional.pad(flat, (0, -flat.numel() % STATE_BLOCK)).view(-1, STATE_BLOCK)
+    top = blocks.abs().amax(1) if blocks.numel() else blocks.new_zeros(0)
+    codes = blocks * torch.where(top > 1e-30, 448.0 / top, 0.0)[:, None]
+    if second:
+        codes = torch.where(blocks > 0, codes.clamp_min(2.0**-9), codes)
+    held = codes.clamp(-448.0, 448.0).to(torch.float8_e4m3fn).reshape(-1)[:flat.numel()]
+    return held.clone().view(moment.shape), top * (1 / 448)
+
+
+def moment_from_8_bits(codes: Tensor, scales: Tensor) -> Tensor:
+    """The fp32 values of a moment that ``AdamWStates`` holds in 8 bits."""
+    each = scales.repeat_interleave(STATE_BLOCK)[:codes.numel()]
+    return (codes.reshape(-1).float() * each).view(codes.shape)
+
+
 class AdamWStates:
     """The AdamW moments of a list of parameters, in 32 bits or in 8, and the step over them.
 
