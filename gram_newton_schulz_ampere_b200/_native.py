@@ -147,6 +147,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [c_int, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _I64, _I64, _P, c_int, _P, c_int, _I64, _P],
     ),
+    "gns_grouped_gemm_plan": (c_int, [_I64, _I64, _I64, _I64, ctypes.POINTER(c_int), ctypes.POINTER(c_int)]),
     "gns_align_rows": (c_int, [_I64, _I64, _I64, _P, _I64, _I64, _P, c_int, _P, _I64, _I64, _P]),
     "gns_grouped_gemm_reduce": (
         c_int,

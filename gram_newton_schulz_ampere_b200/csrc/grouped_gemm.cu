@@ -1391,6 +1391,19 @@ int gns_grouped_gemm(int ab_dtype, int64_t rows, int64_t n, int64_t k, int64_t g
   return launch_rows_any<512, true>(!k_major, f32, c, 12, st);
 }
 
+int gns_grouped_gemm_plan(int64_t rows, int64_t n, int64_t k, int64_t groups, int* tile_rows, int* split) {
+  clear_error();
+  int rc = check_groups(kBF16, 32, groups, rows, n, k, kBF16);
+  if (rc != GNS_OK) return rc;
+  if (rows == 0 || n == 0 || k == 0 || groups == 0) return fail(GNS_ERR_UNSUPPORTED, "an empty product has no plan");
+  if (tile_rows == nullptr || split == nullptr) return fail(GNS_ERR_ARGUMENT, "null result");
+  rc = check_device();
+  if (rc != GNS_OK) return rc;
+  *tile_rows = rows_tile_choice(rows, n, k, groups);
+  *split = *tile_rows == 64 ? rows_split(rows, n, (k + kBK - 1) / kBK, groups) : 1;
+  return GNS_OK;
+}
+
 int gns_align_rows(int64_t batch, int64_t rows, int64_t cols, const void* src, int64_t src_bstride, int64_t src_rstride,
                    const void* ends, int ends_bits, void* dst, int64_t dst_bstride, int64_t dst_rstride,
                    gns_stream_t stream) {

@@ -1248,6 +1248,15 @@ def grouped_gemm(left: Tensor, right: Tensor, ends: Tensor, out_dtype: torch.dty
     return out
 
 
+def grouped_gemm_plan(rows: int, n: int, k: int, groups: int) -> tuple[int, int]:
+    """How ``grouped_gemm`` runs [rows, k] by [groups, k, n] on the current device: the rows of a
+    tile, and the CTAs that share a tile's contraction."""
+    tile, split = ctypes.c_int(), ctypes.c_int()
+    rc = nat.load().gns_grouped_gemm_plan(rows, n, k, groups, ctypes.byref(tile), ctypes.byref(split))
+    nat.check(rc, "gns_grouped_gemm_plan")
+    return tile.value, split.value
+
+
 def grouped_gemm_reduce(left: Tensor, right: Tensor, ends: Tensor, out_dtype: torch.dtype | None = None) -> Tensor:
     """``out[e] = left[rows of e].T @ right[rows of e]`` for each group of rows, on tcgen05
     tensor cores: [E, m, n] from left [T, m] and right [T, n], zero for a group without rows.

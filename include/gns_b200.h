@@ -370,6 +370,10 @@ GNS_API int gns_grouped_gemm(int ab_dtype, int64_t rows, int64_t n, int64_t k, i
                              int64_t left_rstride, const void* right, int64_t right_gstride, int64_t right_rstride,
                              int64_t right_cstride, const void* ends, int ends_bits, void* out, int out_dtype,
                              int64_t out_rstride, gns_stream_t stream);
+/* How gns_grouped_gemm runs a product of these sizes on the current device: the rows of
+ * a tile (64, 128: a CTA; 256, 512: a pair) and the CTAs that share a tile's contraction
+ * (1, 2, 4 or 8). */
+GNS_API int gns_grouped_gemm_plan(int64_t rows, int64_t n, int64_t k, int64_t groups, int* tile_rows, int* split);
 /* Copies [batch][rows][cols] of a 16-bit type with unit column stride, wherever its
  * rows start, to rows that start on 16 bytes (dst and its strides in 16-byte
  * multiples, a row of dst holding cols rounded up to 8): operands that the TMA rule
