@@ -54,6 +54,7 @@ def train(steps: int = 60, width: int = 256, experts: int = 8, tokens: int = 204
                 "algorithm": "adamw",
                 "lr": 3e-3,
                 "state_bits": 8,
+                "state_rounding": "unbiased",
             },
         ],
         lr=0.01,

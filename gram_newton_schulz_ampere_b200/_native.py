@@ -143,6 +143,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [c_int, _PP, _PP, _PP, _PP, _PP, _PP, _PI64, c_int, c_int, c_int, _PF, _PF, c_float, c_float, c_float, c_float,
          c_float, c_float, _P, _P],
     ),
+    "gns_adamw_states_step_unbiased": (
+        c_int,
+        [c_int, _PP, _PP, _PP, _PP, _PP, _PP, _PI64, c_int, c_int, ctypes.POINTER(ctypes.c_uint32), _PF, _PF, c_float,
+         c_float, c_float, c_float, c_float, c_float, _P, _P],
+    ),
     "gns_grouped_gemm": (
         c_int,
         [c_int, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _I64, _I64, _P, c_int, _P, c_int, _I64, _P],

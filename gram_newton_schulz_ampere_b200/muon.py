@@ -22,7 +22,8 @@ momentum kernel shrink to the owned 1/W share.
 AdamW and Lion groups (vectors and scalars) are one fused multi-tensor kernel
 per dtype combination. An AdamW group with ``"state_bits": 8`` (or 32) holds its
 moments in 8 bits (or fp32) whatever the parameters' type and steps in fp32
-arithmetic (``ops.AdamWStates``; no counterpart in the reference). Under DistributedDataParallel, ``momentum_comm_hook()``
+arithmetic (``ops.AdamWStates``; no counterpart in the reference); 8-bit moments round to
+nearest, or with ``"state_rounding": "unbiased"`` so that their mean is right over long runs. Under DistributedDataParallel, ``momentum_comm_hook()``
 moves stage 1 into the backward pass: each gradient bucket's momentum runs as
 soon as its all-reduce has landed.
 """
@@ -202,7 +203,7 @@ class Muon(Optimizer):
             raise ValueError(f"Unknown Newton--Schulz algorithm: {self.ns_algorithm}")
 
     def load_state_dict(self, state_dict: StateDict) -> None:
-        configured = [cast("int | None", group.get("state_bits")) for group in self.param_groups]
+        configured = [(group.get("state_bits"), group.get("state_rounding")) for group in self.param_groups]
         super().load_state_dict(state_dict)
         self._restore_adamw_states(state_dict, configured)
         first = self.param_groups[0]
@@ -226,18 +227,18 @@ class Muon(Optimizer):
         self.validate_cuda_configuration()
         self.configure_newton_schulz()
 
-    def _restore_adamw_states(self, state_dict: StateDict, configured: Sequence[int | None]) -> None:
+    def _restore_adamw_states(self, state_dict: StateDict, configured: Sequence[tuple]) -> None:
         """Moments, scales and step counts of the adamw groups that are, or were when they were
-        saved, held with ``state_bits``. A group keeps the ``state_bits`` it was configured with
-        (torch's loading takes the saved group's settings): moments saved in another form are
+        saved, held with ``state_bits``. A group keeps the ``state_bits`` and ``state_rounding`` it was
+        configured with (torch's loading takes the saved group's settings): moments saved in another form are
         brought into it, the others stay as they were saved, bit for bit. Either way they get
         tensors of their own: torch's loading casts every state tensor to its parameter's
         type, which would round them, and shares those that need no cast with the source."""
-        for group, saved, bits in zip(self.param_groups, state_dict["param_groups"], configured, strict=True):
+        for group, saved, (bits, rounding) in zip(self.param_groups, state_dict["param_groups"], configured, strict=True):
             was = saved.get("state_bits")
             if group["algorithm"] != "adamw" or (bits is None and was is None):
                 continue
-            group["state_bits"] = bits
+            group["state_bits"], group["state_rounding"] = bits, rounding
             for parameter, key in zip(cast(list[Tensor], group["params"]), saved["params"], strict=True):
                 held = {
                     name: value.detach().to(parameter.device, copy=True)
@@ -353,6 +354,12 @@ class Muon(Optimizer):
                 raise ValueError("state_bits is a setting of adamw groups")
             if any(isinstance(p, DTensor) for p in cast(list[Tensor], group["params"])):
                 raise ValueError("state_bits requires parameters that are not DTensors")
+        state_rounding = group.get("state_rounding")
+        if state_rounding is not None:
+            if state_rounding not in ops.STATE_ROUNDINGS:
+                raise ValueError(f"state_rounding must be one of {ops.STATE_ROUNDINGS}, got {state_rounding!r}")
+            if state_bits != 8:
+                raise ValueError("state_rounding is a setting of groups with state_bits 8")
         self.validate_nonnegative_group_scalar(group, "lr")
         self.validate_nonnegative_group_scalar(group, "weight_decay")
         momentum = group["momentum"]
@@ -925,6 +932,7 @@ class Muon(Optimizer):
                 states = ops.AdamWStates(
                     [_contiguous_in_place(p.detach(), writeback) for p, _, _ in entries], bits,
                     held["exp_avg"], held["exp_avg_sq"], held.get("exp_avg_scale"), held.get("exp_avg_sq_scale"),
+                    cast(str, group.get("state_rounding") or "nearest"),
                 )
                 states.step(
                     [g.contiguous() for _, g, _ in entries], float(cast(LearningRate, group["lr"])), beta1, beta2,

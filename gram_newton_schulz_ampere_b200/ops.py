@@ -907,6 +907,7 @@ def lion_step(
 
 
 # ------------------------------------------------- AdamW states in 8 or 32 bits
+STATE_ROUNDINGS = ("nearest", "unbiased")  # of the 8-bit states
 STATE_BLOCK = 256  # consecutive elements of a tensor that share a scale of the 8-bit states
 
 
@@ -947,6 +948,19 @@ class AdamWStates:
 
     Unlike ``adamw_step``, which rounds after every operation as the torch sequence it
     replaces does, the arithmetic is fp32 throughout with one rounding at the end.
+
+    ``rounding`` says how 8-bit moments round. ``"nearest"``: each step's values are as near
+    as they can be, but a value that decays by less than half a code a step stays where it
+    is. With a ``beta2`` of 0.95 that is 1.125 or 1.25 times a power of two, with 0.999 every
+    code, so an element's second moment may stay above its exact value (and its steps too
+    small) until its block's scale comes down: over 3000 steps at 0.95 the root of the second
+    moment grew to 1.45 times the exact one where elements were a tenth of their block's
+    largest (1.41 at 0.99, 1.19 at 0.999), and an element whose gradient stopped kept
+    it. ``"unbiased"`` rounds up or down with the probabilities that make the mean right
+    (0.994 to 0.998 of the exact root in all of these), for any ``beta2`` and long runs;
+    single values are then up to a whole code off. The random bits follow from the step
+    number, the tensor's place in the call and the element's place in the tensor, so equal
+    runs give equal bits. Unbiased second moments still never round to zero.
     """
 
     def __init__(
@@ -957,10 +971,16 @@ class AdamWStates:
         exp_avg_sqs: Sequence[Tensor] | None = None,
         exp_avg_scales: Sequence[Tensor] | None = None,
         exp_avg_sq_scales: Sequence[Tensor] | None = None,
+        rounding: str = "nearest",
     ) -> None:
         if bits not in (8, 32):
             raise ValueError(f"bits must be 8 or 32, got {bits}")
+        if rounding not in STATE_ROUNDINGS:
+            raise ValueError(f"rounding must be one of {STATE_ROUNDINGS}, got {rounding!r}")
+        if rounding != "nearest" and bits != 8:
+            raise ValueError("rounding is a setting of 8-bit moments")
         self.bits = bits
+        self.rounding = rounding
         self.parameters = list(parameters)
         if (exp_avgs is None) != (exp_avg_sqs is None):
             raise ValueError("give both moments or neither")
@@ -1117,11 +1137,15 @@ class AdamWStates:
             sizes = (ctypes.c_int64 * len(given))(*numel)
             roles = (self.parameters, self.exp_avgs, self.exp_avg_sqs, self.exp_avg_scales, self.exp_avg_sq_scales)
             rows = tuple(_ptr_array([role[i] for i in present]) if role else None for role in roles)
-        lib = nat.load()
+        call, form = nat.load().gns_adamw_states_step, (self.bits,)
+        if self.rounding == "unbiased":
+            numbers = [step] * len(given) if isinstance(step, (int, float)) else [step[i] for i in present]
+            seeds = array.array("I", [int(number) & 0xFFFFFFFF for number in numbers])
+            call, form = nat.load().gns_adamw_states_step_unbiased, ((ctypes.c_uint32 * len(seeds)).from_buffer(seeds),)
         with nat.on_device(index) as stream:
-            rc = lib.gns_adamw_states_step(
+            rc = call(
                 len(given), rows[0], _pointers(given), *rows[1:], sizes,
-                nat.dtype_code(places[0].dtype), nat.dtype_code(g_dtype), self.bits, *corrections,
+                nat.dtype_code(places[0].dtype), nat.dtype_code(g_dtype), *form, *corrections,
                 beta1, 1 - beta1, beta2, 1 - beta2, epsilon, 1 - learning_rate * weight_decay,
                 nat.ptr(gradient_scale), stream,
             )

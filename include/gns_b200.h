@@ -349,6 +349,19 @@ GNS_API int gns_adamw_states_step(int count, void* const* params, const void* co
                                   int state_bits, const float* lr_bc1, const float* inv_bc2, float beta1,
                                   float one_minus_beta1, float beta2, float one_minus_beta2, float epsilon,
                                   float decay, const float* grad_scale, gns_stream_t stream);
+/* The same with 8-bit states whose values round up or down with the probabilities that
+ * make their mean right, instead of to nearest. To nearest, a value that decays by less
+ * than half a code a step stays where it is: a second moment above its exact value comes
+ * down only as its block's scale does. The random bits follow from steps[i] (the tensor's
+ * step number), the tensor's place i and the element's place in it: equal calls give equal
+ * bits (for tensors that start on 16 bytes and that do not, different ones). */
+GNS_API int gns_adamw_states_step_unbiased(int count, void* const* params, const void* const* grads,
+                                           void* const* exp_avgs, void* const* exp_avg_sqs,
+                                           float* const* exp_avg_scales, float* const* exp_avg_sq_scales,
+                                           const int64_t* numel, int p_dtype, int g_dtype, const uint32_t* steps,
+                                           const float* lr_bc1, const float* inv_bc2, float beta1,
+                                           float one_minus_beta1, float beta2, float one_minus_beta2, float epsilon,
+                                           float decay, const float* grad_scale, gns_stream_t stream);
 
 /* ------------------------------------------------ products grouped by expert
  * Rows are sorted by group: group e owns the rows [ends[e - 1], ends[e]) (from 0
