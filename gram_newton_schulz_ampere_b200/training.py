@@ -6,6 +6,10 @@ layer's weights [experts, out, in] are a batch of matrices as the orthogonaliser
 so ``Muon`` steps them in one call; the norms, routers and embeddings beside them go to
 an ``adamw`` group, whose moments may be held in 8 bits (``"state_bits": 8``). The
 reference has no layers; these are what its optimizers are used next to.
+
+They run eagerly and in captured CUDA graphs. ``torch.compile`` breaks its graph at each of
+them (``fullgraph=True`` refuses), there is no forward mode and no ``vmap``, and they do not
+cast under autocast: ``grouped_linear`` refuses fp32 inputs there as elsewhere.
 """
 
 from __future__ import annotations
