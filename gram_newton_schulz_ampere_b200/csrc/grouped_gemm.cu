@@ -1360,6 +1360,7 @@ int gns_grouped_gemm(int ab_dtype, int64_t rows, int64_t n, int64_t k, int64_t g
   if (rows == 0 || n == 0) return GNS_OK;
   if (groups == 0 || k == 0) return fail(GNS_ERR_UNSUPPORTED, "a grouped product needs a group and k > 0");
   if (left == nullptr || right == nullptr || ends == nullptr || out == nullptr) return fail(GNS_ERR_ARGUMENT, "null tensor");
+  if (rows > 1 && out_rstride < n) return fail(GNS_ERR_LAYOUT, "rows of the output overlap");
   const bool k_unit = right_rstride == 1 || k == 1;  // right is [group][k][n]
   const bool n_unit = right_cstride == 1 || n == 1;
   const bool k_major = k_unit && ((right_cstride * 2) % 16 == 0 || n == 1);
@@ -1450,6 +1451,8 @@ int gns_grouped_gemm_reduce(int ab_dtype, int64_t rows, int64_t m, int64_t n, in
   if (groups == 0 || m == 0 || n == 0) return GNS_OK;
   if (rows == 0) return fail(GNS_ERR_UNSUPPORTED, "a reduced product needs rows");
   if (left == nullptr || right == nullptr || ends == nullptr || out == nullptr) return fail(GNS_ERR_ARGUMENT, "null tensor");
+  if ((m > 1 && out_rstride < n) || (groups > 1 && out_gstride < (m > 1 ? (m - 1) * out_rstride : 0) + n))
+    return fail(GNS_ERR_LAYOUT, "rows or groups of the output overlap");
   const bool pair = m > kBM;
   const int64_t tiles_m = (m + (pair ? 2 * kBM : kBM) - 1) / (pair ? 2 * kBM : kBM);
   const int64_t tiles_n = (n + kReduceN - 1) / kReduceN;

@@ -373,7 +373,7 @@ GNS_API int gns_adamw_states_step_unbiased(int count, void* const* params, const
  * past the last end come out zero. left is [rows][k] with unit column stride,
  * right [group][k][n] with a unit stride along k or along n, out [rows][n] with
  * unit column stride. Base addresses 16-byte aligned and the other strides
- * multiples of 16 bytes (a TMA rule; out may have any row stride).
+ * multiples of 16 bytes (a TMA rule; out may have any row stride that keeps its rows apart).
  *
  * gns_grouped_gemm_reduce: out[e] = left[rows of e]^T . right[rows of e], zero for
  * a group without rows. left is [rows][m], right [rows][n], both with unit column
