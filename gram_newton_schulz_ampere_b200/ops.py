@@ -1022,7 +1022,12 @@ class AdamWStates:
     def _checked(self, given: Sequence[Tensor], dtype: torch.dtype, counts: list[int], what: str) -> list[Tensor]:
         if len(given) != len(counts):
             raise ValueError("tensor lists must have equal lengths")
-        for t, n in zip(given, counts, strict=True):
+        if self.device is not None and (
+            list(map(Tensor.numel, given)) == counts and all(map(Tensor.is_contiguous, given))
+            and {t.dtype for t in given} == {dtype} and set(map(Tensor.get_device, given)) == {self.device.index}
+        ):
+            return list(given)
+        for t, n in zip(given, counts, strict=True):  # which of them it is
             if t.dtype != dtype:
                 raise TypeError(f"{self.bits}-bit AdamW {what} must be {dtype}, got {t.dtype}")
             if t.numel() != n:
