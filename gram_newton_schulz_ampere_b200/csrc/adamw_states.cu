@@ -391,7 +391,7 @@ struct Slot {
 // registers kept 41 KB in flight and moved 2.9 TB/s, or 4.5 TB/s with the next
 // block prefetched; the ring moves 6.3 TB/s, 0.98 of the measured copy rate (323M
 // bf16 elements in 1129, 717 and 508 us; four CTAs an SM at 64 registers instead of
-// three: 553). The scales of the warp's blocks are read and written once, a lane
+// three: 553; a sustained run under the power cap takes 580). The scales of the warp's blocks are read and written once, a lane
 // for each.
 //
 // ALIGNED: all rows start on multiples of 16 bytes. Otherwise the copies start at the
