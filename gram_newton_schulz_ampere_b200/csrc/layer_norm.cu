@@ -450,8 +450,14 @@ __device__ __forceinline__ float warp_total(float v) {
 // squared deviations from its own mean, S_w and Q_w, and over the warps
 //   mu = sum S_w / n,   n var = sum Q_w + n_w (S_w / n_w - mu)^2,
 // which loses nothing to cancellation, unlike sums of squares.
+//
+// The grid has two CTAs of 256 threads an SM, so registers are held to 128: left alone, the
+// compiler takes up to 148 for 256 threads a row, and the second CTA waits (8192 rows of
+// 8192 bf16 elements 68 us, now 51; 5001 fp16 elements 98, now 78). Not so for aligned
+// fp32 rows, whose longer pieces then spill (8192 elements 90 us against 98).
 template <int XD, int TPR, bool VEC>
-__global__ void __launch_bounds__(threads_of<TPR>()) norm_forward_ring_kernel(const NormArgs a, int stages) {
+__global__ void __launch_bounds__(threads_of<TPR>(), threads_of<TPR>() > 256 || (XD == kF32 && VEC) ? 0 : 2)
+    norm_forward_ring_kernel(const NormArgs a, int stages) {
   constexpr int kThreads = threads_of<TPR>();
   constexpr int kGroups = kThreads / TPR;
   constexpr int kW = TPR / 32;
