@@ -116,10 +116,11 @@ def _quantized(x, block_rows):
     padded = torch.nn.functional.pad(x, (0, -cols % BLOCK, 0, tall - rows))
     blocks = padded.view(tall // block_rows, block_rows, -1, BLOCK)
     top = blocks.abs().amax((1, 3)).clamp_min(LEAST)
-    scaled = (blocks * (TOP / top)[:, None, :, None]).clamp(-TOP, TOP).view(tall, -1)
+    whole = torch.full_like(top, TOP)  # a tensor: a plain number over one is divided with two roundings
+    scaled = (blocks * (whole / top)[:, None, :, None]).clamp(-TOP, TOP).view(tall, -1)
     codes = torch.zeros((rows, _round_up(cols, 16)), dtype=torch.float8_e4m3fn, device=x.device)[:, :cols]
     codes.copy_(scaled[:rows, :cols].to(torch.float8_e4m3fn))
-    return codes, (top / torch.full_like(top, TOP)).t().contiguous().t()
+    return codes, (top / whole).t().contiguous().t()
 
 
 def prepare(case, seed):
