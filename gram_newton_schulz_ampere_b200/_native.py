@@ -167,6 +167,28 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [c_int, c_int, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, c_size_t, _P],
     ),
+    "gns_gemm_8bit": (
+        c_int,
+        [_I64, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, c_int, _I64, _P],
+    ),
+    "gns_quantize_8bit": (c_int, [c_int, c_int, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _P]),
+    "gns_rms_norm_forward": (
+        c_int,
+        [c_int, c_int, _I64, _I64, _P, _I64, _P, _I64, _P, c_float, _P, _P, _P, _P],
+    ),
+    "gns_rms_norm_forward_8bit": (
+        c_int,
+        [c_int, c_int, _I64, _I64, _P, _I64, _P, _I64, _P, c_float, _P, _I64, _P, _I64, _I64, _P, _P, _P],
+    ),
+    "gns_rms_norm_backward_workspace_size": (c_size_t, [_I64, _I64]),
+    "gns_rms_norm_backward": (
+        c_int,
+        [c_int, c_int, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _P, _I64, _P, _P, _P, c_size_t, _P],
+    ),
+    "gns_distillation_loss": (
+        c_int,
+        [c_int, _I64, _I64, _I64, _P, _I64, _P, c_int, _I64, _P, c_int, _I64, c_float, _P, _P, _P, _P, _I64, _P],
+    ),
 }
 
 _lock = threading.Lock()

@@ -24,6 +24,7 @@ INCLUDE_DIR = PACKAGE_DIR.parent / "include"
 SOURCES = (
     "gemm_launch.cu", "ns_chain.cu", "optim_kernels.cu", "small_chain.cu",
     "adamw_states.cu", "grouped_gemm.cu", "layer_norm.cu",
+    "gemm_8bit.cu", "quantize.cu", "rms_norm.cu", "distillation.cu",
 )
 ARCH_FLAGS = ("-gencode", "arch=compute_100a,code=sm_100a")
 NVCC_FLAGS = (

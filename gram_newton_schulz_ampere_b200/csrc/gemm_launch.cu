@@ -138,6 +138,27 @@ int make_map(CUtensorMap* map, int dtype, const void* ptr, int64_t inner, int64_
   return GNS_OK;
 }
 
+// Encodes a map of a matrix [outer][inner] whose box has 128 bytes of `inner` and `box_outer`
+// rows, with 128-byte swizzle.
+int make_matrix_map(CUtensorMap* map, CUtensorMapDataType type, int64_t es, const void* ptr, int64_t inner,
+                    int64_t outer, int64_t outer_stride, int box_outer) {
+  EncodeTiledFn enc = encode_fn();
+  if (enc == nullptr) return fail(GNS_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
+  if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0)
+    return fail(GNS_ERR_LAYOUT, "operand base address must be 16-byte aligned");
+  if (outer == 1) outer_stride = round_up(inner, 16);
+  if ((outer_stride * es) % 16 != 0) return fail(GNS_ERR_LAYOUT, "operand strides must be multiples of 16 bytes");
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer), 1u};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(outer_stride * es),
+                           static_cast<cuuint64_t>(round_up(outer_stride * outer * es, 16))};
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / es), static_cast<cuuint32_t>(box_outer), 1u};
+  cuuint32_t estr[3] = {1u, 1u, 1u};
+  CUresult r = enc(map, type, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(GNS_ERR_LAYOUT, "cuTensorMapEncodeTiled rejected operand layout");
+  return GNS_OK;
+}
+
 // Decides whether a logical [rows, k] operand (A-style: rows = M) is K-major.
 // Returns 0 = K-major, 1 = MN-major, -1 = unsupported.
 int operand_major(int64_t rows, int64_t k, int64_t rstride, int64_t cstride) {
@@ -397,6 +418,16 @@ int encode_f16_tiles(CUtensorMap* map, const void* ptr, int64_t inner, int64_t o
                      int64_t outer_stride, int64_t batch_stride, int box_outer) {
   return make_map(map, kF16, ptr, inner, outer, batch, outer_stride, batch_stride, box_outer);
 }
+
+int encode_byte_tiles(CUtensorMap* map, const void* ptr, int64_t inner, int64_t outer, int64_t outer_stride, int box_outer) {
+  return make_matrix_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, ptr, inner, outer, outer_stride, box_outer);
+}
+
+int encode_store_tiles(CUtensorMap* map, int dtype, const void* ptr, int64_t inner, int64_t outer, int64_t outer_stride,
+                       int box_outer) {
+  return make_matrix_map(map, dtype == kF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : tma_dtype(dtype), dtype_size(dtype), ptr,
+                         inner, outer, outer_stride, box_outer);
+}
 }  // namespace gns
 
 extern "C" {
@@ -479,6 +510,14 @@ int gns_device_status(int* status, int clear) {
   rc = gns::states_status(&states, clear);
   if (rc != GNS_OK) return rc;
   if (*status == 0) *status = states;
+  int gemm8 = 0;
+  rc = gns::gemm8_status(&gemm8, clear);
+  if (rc != GNS_OK) return rc;
+  if (*status == 0) *status = gemm8;
+  int rms = 0;
+  rc = gns::rms_status(&rms, clear);
+  if (rc != GNS_OK) return rc;
+  if (*status == 0) *status = rms;
   return GNS_OK;
 }
 

@@ -103,11 +103,20 @@ int encode_f16_tiles(CUtensorMap* map, const void* ptr, int64_t inner, int64_t o
 int encode_tiles(CUtensorMap* map, int dtype, const void* ptr, int64_t inner, int64_t outer, int64_t batch,
                  int64_t outer_stride, int64_t batch_stride, int box_outer);
 
+// Maps of 8-bit matrices and of matrices to be stored: boxes of 128 bytes and `box_outer`
+// rows with 128-byte swizzle.
+int encode_byte_tiles(CUtensorMap* map, const void* ptr, int64_t inner, int64_t outer, int64_t outer_stride, int box_outer);
+int encode_store_tiles(CUtensorMap* map, int dtype, const void* ptr, int64_t inner, int64_t outer, int64_t outer_stride,
+                       int box_outer);
+
 // Status word of the grouped products (0 = ok); optionally cleared.
 int grouped_status(int* status, int clear);
 // The same of the layer norm kernels and of the AdamW kernel for 8-bit states.
 int norm_status(int* status, int clear);
 int states_status(int* status, int clear);
+// The same of the 8-bit products and of the RMS norm.
+int gemm8_status(int* status, int clear);
+int rms_status(int* status, int clear);
 
 // Fused single-kernel Gram Newton-Schulz chain for matrices whose short side is
 // at most 128 (small_chain.cu). x0 holds the normalised fp16 X and x1 is the

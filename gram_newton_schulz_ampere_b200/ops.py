@@ -1398,3 +1398,308 @@ def layer_norm_backward(
         )
     nat.check(rc, "gns_layer_norm_backward")
     return dx, dweight, dbias
+
+
+# ------------------------------------------------------ 8 bits, blocks of 128
+_BLOCK = 128
+
+
+def _code_buffers(like: Tensor, rows: int, columns: int, block_rows: int = 1) -> tuple[Tensor, Tensor]:
+    """Buffers for the codes [rows, columns] and scales of a matrix: rows of codes start on 16
+    bytes, the scales of one block column follow one another."""
+    pitch = (columns + 15) // 16 * 16
+    codes = like.new_empty((rows, pitch), dtype=torch.float8_e4m3fn)
+    scales = like.new_empty(((columns + _BLOCK - 1) // _BLOCK, (rows + block_rows - 1) // block_rows), dtype=torch.float32)
+    return codes if pitch == columns else codes[:, :columns], scales.t()
+
+
+def quantize_8bit(x: Tensor, block_rows: int = 1) -> tuple[Tensor, Tensor]:
+    """A matrix [rows, columns] as e4m3 codes with an fp32 scale for each block of ``block_rows``
+    (1 or 128) rows and 128 columns: ``scale = top / 448`` and ``code = e4m3(x * (448 / top))``,
+    rounded to nearest even, with top the block's largest magnitude (at least 448 * 2^-126).
+
+    Returns the codes (``float8_e4m3fn``, x's shape, rows starting on multiples of 16 bytes) and
+    the scales [ceil(rows / block_rows), ceil(columns / 128)]. ``gemm_8bit`` takes activations
+    and gradients in blocks of 1 x 128, weights in blocks of 128 x 128. x is float16, bfloat16 or
+    float32. A NaN keeps a code of NaN; an infinity makes its block's scale infinite and the
+    block's products NaN."""
+    index = _device_index(x)
+    if x.ndim != 2:
+        raise ValueError("expected a matrix")
+    if block_rows not in (1, _BLOCK):
+        raise ValueError(f"a block has 1 or 128 rows, got {block_rows}")
+    code = nat.dtype_code(x.dtype)
+    rows, columns = x.shape
+    codes, scales = _code_buffers(x, rows, columns, block_rows)
+    if rows == 0 or columns == 0:
+        return codes, scales
+    held = _norm_rows(x, columns)
+    with nat.on_device(index) as stream:
+        rc = nat.load().gns_quantize_8bit(
+            code, block_rows, rows, columns, held.data_ptr(), held.stride(0), codes.data_ptr(), codes.stride(0),
+            scales.data_ptr(), *scales.stride(), stream,
+        )
+    nat.check(rc, "gns_quantize_8bit")
+    return codes, scales
+
+
+def _byte_layout(t: Tensor) -> tuple[Tensor, int, int]:
+    """(owner, row stride, column stride) of the 8-bit matrix `t` or of a copy of it, in the same
+    order, that TMA can read: a unit stride, the other one a multiple of 16 bytes."""
+    rows, columns = t.shape
+    sr, sc = t.stride()
+    sound = t.data_ptr() % 16 == 0
+    if sound and (sc == 1 or columns == 1) and ((sr % 16 == 0 and sr >= columns) or rows == 1):
+        return t, sr if rows > 1 else 0, 1
+    if sound and (sr == 1 or rows == 1) and ((sc % 16 == 0 and sc >= rows) or columns == 1):
+        return t, 1, sc if columns > 1 else 0
+    if sr == 1 and sc != 1:
+        held, stride, _ = _byte_layout(t.t())
+        return held, 1, stride
+    pitch = (columns + 15) // 16 * 16
+    copy = t.new_empty((rows, pitch))
+    copy.view(torch.uint8)[:, :columns].copy_(t.view(torch.uint8))
+    return copy, pitch, 1
+
+
+def gemm_8bit(
+    left: Tensor, left_scales: Tensor, right: Tensor, right_scales: Tensor, out_dtype: torch.dtype = torch.bfloat16
+) -> Tensor:
+    """``left @ right`` of e4m3 matrices with fp32 scales, on tcgen05 tensor cores.
+
+    left [m, k] has a scale for each row and each 128 of k: left_scales [m, ceil(k / 128)].
+    right [k, n] has one for each 128 x 128 block: right_scales [ceil(k / 128), ceil(n / 128)];
+    it may be stored by rows or by columns. Both come from ``quantize_8bit`` (left also from
+    ``rms_norm_8bit``). With a layer's weights W [n, k] in blocks of 128 x 128, codes w and
+    scales s, the layer is ``gemm_8bit(x, xs, w.T, s.T)`` and the gradient of its input
+    ``gemm_8bit(dy, dys, w, s)``.
+
+    The sum over a block of 128 is the tensor cores' with fp32 accumulators; it is scaled by the
+    fp32 product of its two scales and added up in fp32, and rounded once to ``out_dtype``
+    (float16, bfloat16 or float32). The order of the sums depends on the sizes of the call (few
+    rows with a long k are summed in parts), never on the run. Operands that TMA cannot read (rows
+    that do not start on 16 bytes) are copied first."""
+    index = _device_index(left, left_scales, right, right_scales)
+    if left.ndim != 2 or right.ndim != 2 or left.shape[1] != right.shape[0]:
+        raise ValueError(f"incompatible shapes {tuple(left.shape)} @ {tuple(right.shape)}")
+    if left.dtype != torch.float8_e4m3fn or right.dtype != torch.float8_e4m3fn:
+        raise TypeError("left and right must be float8_e4m3fn")
+    if left_scales.dtype != torch.float32 or right_scales.dtype != torch.float32:
+        raise TypeError("scales must be float32")
+    m, k = left.shape
+    n = right.shape[1]
+    blocks = (k + _BLOCK - 1) // _BLOCK
+    if tuple(left_scales.shape) != (m, blocks):
+        raise ValueError(f"left_scales must be {(m, blocks)}, got {tuple(left_scales.shape)}")
+    if tuple(right_scales.shape) != (blocks, (n + _BLOCK - 1) // _BLOCK):
+        raise ValueError(f"right_scales must be {(blocks, (n + _BLOCK - 1) // _BLOCK)}, got {tuple(right_scales.shape)}")
+    code = nat.dtype_code(out_dtype)
+    if m == 0 or n == 0 or k == 0:
+        return torch.zeros((m, n), dtype=out_dtype, device=left.device)
+    left_held, left_pitch, unit = _byte_layout(left)
+    if unit != 1 and k > 1:
+        left_held, left_pitch, _ = _byte_layout(left.contiguous())
+    right_held, *right_strides = _byte_layout(right)
+    out = left.new_empty((m, n), dtype=out_dtype)
+    with nat.on_device(index) as stream:
+        rc = nat.load().gns_gemm_8bit(
+            m, n, k, left_held.data_ptr(), left_pitch, left_scales.data_ptr(), *left_scales.stride(),
+            right_held.data_ptr(), *right_strides, right_scales.data_ptr(), *right_scales.stride(),
+            out.data_ptr(), code, n, stream,
+        )
+    nat.check(rc, "gns_gemm_8bit")
+    return out
+
+
+# --------------------------------------------------------------------- RMS norm
+def _rms_check(x: Tensor, weight: Tensor, residual: Tensor | None) -> int:
+    columns = _norm_check(x, weight, None)
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError("x and residual shapes differ")
+    if residual is not None and residual.dtype != x.dtype:
+        raise TypeError("x and residual must share a dtype")
+    return columns
+
+
+def rms_norm(
+    x: Tensor, weight: Tensor, residual: Tensor | None = None, epsilon: float = 1e-5
+) -> tuple[Tensor, Tensor, Tensor]:
+    """Root-mean-square norm of a residual stream: ``total = x + residual`` and
+    ``y = total * rstd * weight`` with ``rstd = 1 / sqrt(mean(total^2) + epsilon)`` over the last
+    dimension.
+
+    Returns y and total (x's type, contiguous; total is x itself without a residual) and the
+    fp32 rstd of each row. total is rounded to x's type before the norm; all arithmetic is fp32.
+    weight has a floating type of its own."""
+    index = _device_index(x, weight, residual)
+    columns = _rms_check(x, weight, residual)
+    flat = _norm_rows(x, columns)
+    other = _norm_rows(residual, columns) if residual is not None else None
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    total = torch.empty_like(y) if other is not None else x
+    rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    w = weight.contiguous()
+    with nat.on_device(index) as stream:
+        rc = nat.load().gns_rms_norm_forward(
+            nat.dtype_code(x.dtype), nat.dtype_code(w.dtype), flat.shape[0], columns, flat.data_ptr(), flat.stride(0),
+            nat.ptr(other), other.stride(0) if other is not None else 0, w.data_ptr(), float(epsilon), y.data_ptr(),
+            total.data_ptr(), rstd.data_ptr(), stream,
+        )
+    nat.check(rc, "gns_rms_norm_forward")
+    return y, total, rstd
+
+
+def rms_norm_8bit(
+    x: Tensor, weight: Tensor, residual: Tensor | None = None, epsilon: float = 1e-5
+) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """``rms_norm`` whose y comes as e4m3 codes with a scale for each 128 columns of a row, as
+    ``quantize_8bit`` makes them of the unrounded y: the left factor of ``gemm_8bit``.
+
+    Returns the codes [rows, columns] and scales [rows, ceil(columns / 128)] (rows: all dimensions
+    of x but the last), total and rstd as ``rms_norm``."""
+    index = _device_index(x, weight, residual)
+    columns = _rms_check(x, weight, residual)
+    flat = _norm_rows(x, columns)
+    other = _norm_rows(residual, columns) if residual is not None else None
+    rows = flat.shape[0]
+    codes, scales = _code_buffers(x, rows, columns)
+    total = torch.empty_like(x, memory_format=torch.contiguous_format) if other is not None else x
+    rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    w = weight.contiguous()
+    with nat.on_device(index) as stream:
+        rc = nat.load().gns_rms_norm_forward_8bit(
+            nat.dtype_code(x.dtype), nat.dtype_code(w.dtype), rows, columns, flat.data_ptr(), flat.stride(0),
+            nat.ptr(other), other.stride(0) if other is not None else 0, w.data_ptr(), float(epsilon), codes.data_ptr(),
+            codes.stride(0), scales.data_ptr(), *scales.stride(), total.data_ptr(), rstd.data_ptr(), stream,
+        )
+    nat.check(rc, "gns_rms_norm_forward_8bit")
+    return codes, scales, total, rstd
+
+
+def rms_norm_backward(
+    grad: Tensor, total: Tensor, weight: Tensor, rstd: Tensor, grad_total: Tensor | None = None
+) -> tuple[Tensor, Tensor]:
+    """Gradients (dx, dweight) of ``rms_norm`` from the gradients of y and of total (which may be
+    None). dx is the gradient of x and of the residual alike, of total's type; dweight has the
+    weight's type, its sum over the rows is fp32 in a fixed order."""
+    index = _device_index(grad, total, weight, rstd, grad_total)
+    columns = _rms_check(total, weight, grad_total)
+    if grad.shape != total.shape:
+        raise ValueError("grad and total shapes differ")
+    if grad.dtype != total.dtype:
+        raise TypeError("grad and total must share a dtype")
+    rows = total.numel() // columns
+    if rstd.dtype != torch.float32 or rstd.numel() != rows or not rstd.is_contiguous():
+        raise ValueError("rstd must be contiguous float32 with one entry per row")
+    flat, g = _norm_rows(total, columns), _norm_rows(grad, columns)
+    more = _norm_rows(grad_total, columns) if grad_total is not None else None
+    w = weight.contiguous()
+    dx = torch.empty_like(total, memory_format=torch.contiguous_format)
+    dweight = torch.empty_like(w)
+    lib = nat.load()
+    nbytes = lib.gns_rms_norm_backward_workspace_size(rows, columns)
+    ws = total.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    with nat.on_device(index) as stream:
+        rc = lib.gns_rms_norm_backward(
+            nat.dtype_code(total.dtype), nat.dtype_code(w.dtype), rows, columns, g.data_ptr(), g.stride(0),
+            flat.data_ptr(), flat.stride(0), w.data_ptr(), rstd.data_ptr(), nat.ptr(more),
+            more.stride(0) if more is not None else 0, dx.data_ptr(), dweight.data_ptr(), nat.ptr(ws), nbytes, stream,
+        )
+    nat.check(rc, "gns_rms_norm_backward")
+    return dx, dweight
+
+
+# ---------------------------------------------------- distillation from top logits
+def _distillation_rows(logits: Tensor, indices: Tensor, teacher: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+    if logits.ndim != 2 or logits.shape[1] == 0:
+        raise ValueError("expected logits [rows, vocabulary]")
+    if indices.ndim != 2 or indices.shape != teacher.shape or indices.shape[0] != logits.shape[0]:
+        raise ValueError("expected indices and teacher [rows, top], a row for each row of the logits")
+    if indices.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"indices must be int32 or int64, got {indices.dtype}")
+    nat.dtype_code(logits.dtype)
+    nat.dtype_code(teacher.dtype)
+    top = indices.shape[1]
+
+    def rows(t: Tensor) -> Tensor:
+        return t if t.stride(1) == 1 or top <= 1 else t.contiguous()
+
+    return _norm_rows(logits, logits.shape[1]), rows(indices), rows(teacher)
+
+
+def _row_values(t: Tensor, rows: int, name: str) -> Tensor:
+    if t.dtype != torch.float32 or t.shape != (rows,):
+        raise ValueError(f"{name} must be float32 with one value for each row")
+    return t.contiguous()
+
+
+def _distillation(
+    z: Tensor, indices: Tensor, teacher: Tensor, temperature: float, grad: Tensor | None, loss: Tensor | None,
+    stats: Tensor | None, dlogits: Tensor | None,
+) -> None:
+    rows, vocabulary = z.shape
+    with nat.on_device(z.get_device()) as stream:
+        rc = nat.load().gns_distillation_loss(
+            nat.dtype_code(z.dtype), rows, vocabulary, indices.shape[1], z.data_ptr(), z.stride(0), indices.data_ptr(),
+            8 * indices.element_size(), indices.stride(0), teacher.data_ptr(), nat.dtype_code(teacher.dtype),
+            teacher.stride(0), float(temperature), nat.ptr(grad), nat.ptr(loss), nat.ptr(stats), nat.ptr(dlogits),
+            vocabulary, stream,
+        )
+    nat.check(rc, "gns_distillation_loss")
+
+
+def distillation_loss(
+    logits: Tensor, indices: Tensor, teacher: Tensor, temperature: float = 1.0
+) -> tuple[Tensor, Tensor]:
+    """The loss of each row against a teacher's top logits:
+    ``T^2 * sum_j p_j (log p_j - log q[i_j])`` with p the softmax over the row's entries of
+    ``teacher / T`` and q that of ``logits / T`` over the whole vocabulary.
+
+    logits [rows, vocabulary] and teacher [rows, top] are float16, bfloat16 or float32, indices
+    [rows, top] int32 or int64; top is at most 1024. An entry whose index is outside the vocabulary
+    (-1) has no part in its row; an index may come more than once. A row without entries, or
+    whose entries' logits are all -inf, has a loss of zero whatever its logits hold. Where they
+    count, logits of -inf have a q of zero, and a NaN, a +inf or a row of -inf alone makes
+    the row's loss and gradient NaN.
+
+    Returns the fp32 loss [rows] and the statistics [rows, 2] that
+    ``distillation_loss_backward`` takes."""
+    _device_index(logits, indices, teacher)
+    z, index, t = _distillation_rows(logits, indices, teacher)
+    loss = z.new_empty(z.shape[0], dtype=torch.float32)
+    stats = z.new_empty((z.shape[0], 2), dtype=torch.float32)
+    _distillation(z, index, t, temperature, None, loss, stats, None)
+    return loss, stats
+
+
+def distillation_loss_backward(
+    grad: Tensor, logits: Tensor, indices: Tensor, teacher: Tensor, statistics: Tensor, temperature: float = 1.0
+) -> Tensor:
+    """The gradient of the logits, ``grad * T * (q - p)``, from the gradient of each row's loss
+    (fp32) and the statistics that ``distillation_loss`` returned. Of the logits' type; rows
+    without entries get zeros."""
+    _device_index(grad, logits, indices, teacher, statistics)
+    z, index, t = _distillation_rows(logits, indices, teacher)
+    g = _row_values(grad, z.shape[0], "grad")
+    if statistics.dtype != torch.float32 or statistics.shape != (z.shape[0], 2) or not statistics.is_contiguous():
+        raise ValueError("statistics must be contiguous float32 [rows, 2]")
+    dlogits = torch.empty_like(z, memory_format=torch.contiguous_format)
+    _distillation(z, index, t, temperature, g, None, statistics, dlogits)
+    return dlogits
+
+
+def distillation_loss_gradient(
+    grad: Tensor, logits: Tensor, indices: Tensor, teacher: Tensor, temperature: float = 1.0
+) -> tuple[Tensor, Tensor]:
+    """``distillation_loss`` and the gradient of the logits in one call, which reads the logits from
+    memory once: for a loop that knows each row's weight in its loss beforehand (``grad``, fp32, a
+    mask over the number of tokens for a mean) and goes on with ``logits.backward(dlogits)``.
+
+    Returns the loss [rows] and dlogits."""
+    _device_index(grad, logits, indices, teacher)
+    z, index, t = _distillation_rows(logits, indices, teacher)
+    g = _row_values(grad, z.shape[0], "grad")
+    loss = z.new_empty(z.shape[0], dtype=torch.float32)
+    dlogits = torch.empty_like(z, memory_format=torch.contiguous_format)
+    _distillation(z, index, t, temperature, g, loss, None, dlogits)
+    return loss, dlogits

@@ -419,6 +419,68 @@ GNS_API int gns_layer_norm_backward(int x_dtype, int w_dtype, int64_t rows, int6
                                     const float* mean, const float* rstd, void* dx, void* dweight, void* dbias,
                                     void* workspace, size_t workspace_bytes, gns_stream_t stream);
 
+/* -------------------------------------------------- products of 8-bit matrices
+ * out = left . right with e4m3 operands and fp32 scales for blocks of 128 of the
+ * contraction: left [m][k] (unit column stride) has a scale for each row and block
+ * [m][ceil(k / 128)], right [k][n] (unit stride along k or along n) one for each 128 x 128
+ * block [ceil(k / 128)][ceil(n / 128)]; both arrays of scales have strides of their own.
+ * Operands start on 16 bytes and their other strides are multiples of 16 (a TMA rule); out
+ * [m][n] is F16, BF16 or F32 with unit column stride. Sums are fp32, rounded once; a block's
+ * sum is multiplied by the fp32 product of its two scales.
+ * No counterpart in the reference. */
+GNS_API int gns_gemm_8bit(int64_t m, int64_t n, int64_t k, const void* left, int64_t left_rstride,
+                          const float* left_scales, int64_t left_scale_rstride, int64_t left_scale_cstride,
+                          const void* right, int64_t right_rstride, int64_t right_cstride, const float* right_scales,
+                          int64_t right_scale_rstride, int64_t right_scale_cstride, void* out, int out_dtype,
+                          int64_t out_rstride, gns_stream_t stream);
+/* Codes and scales of x [rows][cols] (unit column stride, any row stride of at least cols):
+ * blocks of block_rows (1 or 128) x 128, top = max(largest magnitude, 448 * 2^-126), scale =
+ * top / 448, code = e4m3(x * (448 / top)) to nearest even. Rows of codes start on 16 bytes
+ * (codes_rstride a multiple of 16) and are written up to cols rounded up to 16, zeros behind
+ * the last column. scales [ceil(rows / block_rows)][ceil(cols / 128)] has strides of its own. */
+GNS_API int gns_quantize_8bit(int x_dtype, int block_rows, int64_t rows, int64_t cols, const void* x, int64_t x_rstride,
+                              void* codes, int64_t codes_rstride, float* scales, int64_t scale_rstride,
+                              int64_t scale_cstride, gns_stream_t stream);
+
+/* ----------------------------------------------------- root-mean-square norm
+ * total = x + residual, rounded to x's type (x itself where residual is NULL; total is then
+ * not written), y = total * rstd * weight, rstd = 1 / sqrt(mean(total^2) + eps). x and residual
+ * share x_dtype and have unit column stride; y and total are contiguous; rstd is fp32.
+ * The 8-bit form writes codes and scales (blocks of 1 x 128, as gns_quantize_8bit) of the
+ * unrounded y in its place.
+ * Backward: dx = the gradient through the norm + grad_total (NULL: none), of x and of the
+ * residual alike; dweight sums over the rows in fp32, in a fixed order. rows may be 0.
+ * No counterpart in the reference. */
+GNS_API int gns_rms_norm_forward(int x_dtype, int w_dtype, int64_t rows, int64_t cols, const void* x, int64_t x_rstride,
+                                 const void* residual, int64_t residual_rstride, const void* weight, float eps, void* y,
+                                 void* total, float* rstd, gns_stream_t stream);
+GNS_API int gns_rms_norm_forward_8bit(int x_dtype, int w_dtype, int64_t rows, int64_t cols, const void* x,
+                                      int64_t x_rstride, const void* residual, int64_t residual_rstride,
+                                      const void* weight, float eps, void* codes, int64_t codes_rstride, float* scales,
+                                      int64_t scale_rstride, int64_t scale_cstride, void* total, float* rstd,
+                                      gns_stream_t stream);
+GNS_API size_t gns_rms_norm_backward_workspace_size(int64_t rows, int64_t cols);
+GNS_API int gns_rms_norm_backward(int x_dtype, int w_dtype, int64_t rows, int64_t cols, const void* grad,
+                                  int64_t grad_rstride, const void* total, int64_t total_rstride, const void* weight,
+                                  const float* rstd, const void* grad_total, int64_t grad_total_rstride, void* dx,
+                                  void* dweight, void* workspace, size_t workspace_bytes, gns_stream_t stream);
+
+/* ------------------------------------------------------- distillation loss
+ * loss = T^2 sum_j p_j (log p_j - log q[i_j]) of each row: p is the softmax of the row's
+ * teacher logits over T, q that of its logits over T and the whole vocabulary. Entries whose
+ * index is outside [0, vocabulary) have no part; a row without entries (or with -inf teacher
+ * logits only) has a loss and a gradient of zero. top <= 1024, T in [1e-4, 1e4].
+ * With grad (fp32, one value a row) and dlogits: dlogits = grad T (q - p), of the logits' type.
+ * stats (fp32, two values a row: the largest logit and the sum of exponentials) is written
+ * with the loss where it is not NULL; with loss NULL the gradient is formed from it.
+ * logits, indices, teacher and dlogits have unit column stride.
+ * No counterpart in the reference. */
+GNS_API int gns_distillation_loss(int z_dtype, int64_t rows, int64_t vocabulary, int64_t top, const void* logits,
+                                  int64_t logits_rstride, const void* indices, int index_bits, int64_t indices_rstride,
+                                  const void* teacher, int teacher_dtype, int64_t teacher_rstride, float temperature,
+                                  const float* grad, float* loss, float* stats, void* dlogits, int64_t dlogits_rstride,
+                                  gns_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
