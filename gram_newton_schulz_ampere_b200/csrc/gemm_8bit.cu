@@ -84,34 +84,33 @@ __device__ __forceinline__ uint64_t tile_desc(const uint8_t* tile) { return make
 constexpr uint64_t step_of(bool mn) { return mn ? 32 * 128 / 16 : 32 / 16; }
 constexpr int kSteps = kBlock / 32;
 
+// Barriers. `done` says both that a stage may be filled again and that its partial sum is in
+// its accumulator: one commit a block, which the producer and the summing warps wait for (a
+// commit costs the issuing thread about 60 cycles, a block's products take 512). In a pair
+// the `full` and `read` barriers of CTA 0 serve both CTAs, and each CTA has its own `done`.
 template <int S, bool PAIR>
 struct Pipe {
-  uint64_t* full;    // a stage has landed
-  uint64_t* empty;   // its products are done
-  uint64_t* tfull;   // a block's partial sum is in its accumulator
-  uint64_t* tempty;  // the accumulator has been read
+  uint64_t* full;  // a stage has landed
+  uint64_t* done;  // its products are done
+  uint64_t* read;  // the accumulator has been read
   uint32_t* tmem_slot;
   volatile int* abort_flag;
-  static constexpr uint32_t kBytes = (2 * S + 4) * 8 + 8;
+  static constexpr uint32_t kBytes = (2 * S + 2) * 8 + 8;
 
   __device__ __forceinline__ explicit Pipe(uint8_t* at) {
     full = reinterpret_cast<uint64_t*>(at);
-    empty = full + S;
-    tfull = empty + S;
-    tempty = tfull + 2;
-    tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+    done = full + S;
+    read = done + S;
+    tmem_slot = reinterpret_cast<uint32_t*>(read + 2);
     abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   }
 
   __device__ __forceinline__ void init() const {
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&done[s], 1);
     }
-    for (int a = 0; a < 2; ++a) {
-      mbar_init(&tfull[a], 1);
-      mbar_init(&tempty[a], (PAIR ? 2 : 1) * kEpiWarps);
-    }
+    for (int a = 0; a < 2; ++a) mbar_init(&read[a], (PAIR ? 2 : 1) * kEpiWarps);
     *abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async_smem();
@@ -121,11 +120,11 @@ struct Pipe {
     return mbar_wait_bounded(bar, parity, abort_flag, &g_gemm8_status, code);
   }
 
-  // The producer's end: every stage that it filled has been released, so that no arrival
-  // is on its way when the CTA leaves.
+  // The producer's end: the products of every stage that it filled are done, so that no
+  // arrival is on its way when the CTA leaves.
   __device__ __forceinline__ void drain(int st, uint32_t ph, bool ok) const {
     for (int i = 0; i < S && ok; ++i) {
-      ok = wait(&empty[st], ph ^ 1u, kStatusProducerTimeout);
+      ok = wait(&done[st], ph ^ 1u, kStatusProducerTimeout);
       if (++st == S) {
         st = 0;
         ph ^= 1u;
@@ -133,6 +132,16 @@ struct Pipe {
     }
   }
 };
+
+// Arrives on the barrier at the same place in both CTAs of the pair once every earlier pair
+// MMA of this thread has completed.
+__device__ __forceinline__ void commit_to_both(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
 
 template <bool CLUSTER>
 __device__ __forceinline__ void meet() {
@@ -142,7 +151,49 @@ __device__ __forceinline__ void meet() {
     __syncthreads();
 }
 
+// 32 columns of a thread's TMEM lane on their way to registers: they hold nothing of use
+// until land(), which waits for every load that the thread has issued.
+struct TmemPiece {
+  uint32_t r[32];
+
+  __device__ __forceinline__ void issue(uint32_t at) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at)
+        : "memory");
+  }
+
+  // The registers are operands, so that nothing that reads them moves above the wait.
+  __device__ __forceinline__ void land() {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                   "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                   "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+  }
+
+  __device__ __forceinline__ void add_to(Pair* sum, Pair scale) const {
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      sum[e] = fma2(Pair(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), scale, sum[e]);
+  }
+};
+
 // ------------------------------------------------------------------ many rows
+// Warps 0 to 3 load and issue (two of them idle), 4 to 11 sum. The sums take 128 registers of a
+// thread and two pieces on their way another 64, so the four leave registers to the eight:
+// 40 and twice 232 of the 168 a thread at launch (3 x 168 = 40 + 2 x 232).
+constexpr int kPairThreads = 32 * (4 + kEpiWarps);
+
 template <bool OUT_F32>
 struct PairConfig {
   static constexpr int kStages = 5;
@@ -168,7 +219,7 @@ struct Tiling {
 };
 
 template <bool B_MN, bool OUT_F32>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kPairThreads, 1)
     gemm8_pair_kernel(const __grid_constant__ CUtensorMap map_left, const __grid_constant__ CUtensorMap map_right,
                       const __grid_constant__ CUtensorMap map_out, const Scales scales, const Shape8 shape,
                       const Tiling tiling, const Out8 out) {
@@ -199,9 +250,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_launch_dependents();
   pdl_wait_predecessor();
   const uint32_t tmem = *pipe.tmem_slot;
-
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 0 && lane == 0) {
       const uint32_t full0 = cluster_addr(&pipe.full[0], 0);
       int st = 0;
       uint32_t ph = 0;
@@ -211,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tiling.place(t, i, j);
         const int row = i * kTile + static_cast<int>(rank) * 128, col = j * kTile + static_cast<int>(rank) * 128;
         for (int b = 0; b < shape.blocks; ++b) {
-          ok = pipe.wait(&pipe.empty[st], ph ^ 1u, kStatusProducerTimeout);
+          ok = pipe.wait(&pipe.done[st], ph ^ 1u, kStatusProducerTimeout);
           if (!ok) break;
           uint8_t* at = smem + st * Cfg::kStageBytes;
           if (rank == 0) mbar_arrive_expect_tx(&pipe.full[st], 2 * Cfg::kStageBytes);
@@ -229,50 +280,47 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       pipe.drain(st, ph, ok);
     }
-  } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    // Two warps issue the products, one the even blocks into the first accumulator, the other
+    // the odd ones into the second: what a block costs its thread beside the products (two
+    // waits and a commit, 300 cycles; 512 for the products, of which few are queued ahead)
+    // passes while the other's run.
+    if ((warp == 1 || warp == 2) && lane == 0 && rank == 0) {
       const uint32_t idesc = idesc_8bit(false, B_MN, kTile, kTile);
-      uint32_t empty[2], tfull[2];
-      for (uint32_t r = 0; r < 2; ++r) {
-        empty[r] = cluster_addr(&pipe.empty[0], r);
-        tfull[r] = cluster_addr(&pipe.tfull[0], r);
-      }
-      int st = 0, acc = 0;
+      const int acc = warp - 1;
+      const int mine = first < tiles ? (tiles - first + step - 1) / step : 0;
+      const int64_t count = static_cast<int64_t>(mine) * shape.blocks;
+      int st = acc;
       uint32_t ph = 0, acc_ph = 0;
-      bool ok = true;
-      for (int t = first; t < tiles && ok; t += step) {
-        for (int b = 0; b < shape.blocks; ++b) {
-          ok = pipe.wait(&pipe.tempty[acc], acc_ph ^ 1u, kStatusMmaTimeout) &&
-               pipe.wait(&pipe.full[st], ph, kStatusMmaTimeout);
-          if (!ok) break;
-          tc_fence_after();
-          const uint8_t* at = smem + st * Cfg::kStageBytes;
-          const uint64_t left = tile_desc(at), right = tile_desc(at + kTileBytes);
+      for (int64_t i = acc; i < count; i += 2) {
+        if (!pipe.wait(&pipe.full[st], ph, kStatusMmaTimeout) ||
+            !pipe.wait(&pipe.read[acc], acc_ph ^ 1u, kStatusMmaTimeout))
+          break;
+        tc_fence_after();
+        const uint8_t* at = smem + st * Cfg::kStageBytes;
+        const uint64_t left = tile_desc(at), right = tile_desc(at + kTileBytes);
 #pragma unroll
-          for (int k = 0; k < kSteps; ++k)
-            mma_8bit_pair(tmem + static_cast<uint32_t>(acc * kTile), left + k * step_of(false), right + k * step_of(B_MN),
-                          idesc, k > 0 ? 1u : 0u);
-          for (int r = 0; r < 2; ++r) tc_commit_pair(empty[r] + static_cast<uint32_t>(st) * 8u);
-          // Last, so that a CTA that has seen it has seen every earlier arrival on its barriers.
-          for (int r = 0; r < 2; ++r) tc_commit_pair(tfull[r] + static_cast<uint32_t>(acc) * 8u);
-          if (++st == S) {
-            st = 0;
-            ph ^= 1u;
-          }
-          acc ^= 1;
-          if (acc == 0) acc_ph ^= 1u;
+        for (int k = 0; k < kSteps; ++k)
+          mma_8bit_pair(tmem + static_cast<uint32_t>(acc * kTile), left + k * step_of(false), right + k * step_of(B_MN),
+                        idesc, k > 0 ? 1u : 0u);
+        commit_to_both(&pipe.done[st]);
+        acc_ph ^= 1u;
+        st += 2;
+        if (st >= S) {
+          st -= S;
+          ph ^= 1u;
         }
       }
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     // A warp has 32 rows (its quarter of the TMEM lanes) and 128 columns of the CTA's tile:
     // 128 fp32 sums a thread, and one scale a block.
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
-    uint8_t* slot = smem_out + (warp - 2) * Cfg::kSlotBytes;
-    const uint32_t tempty0 = cluster_addr(&pipe.tempty[0], 0);
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    uint8_t* slot = smem_out + (warp - 4) * Cfg::kSlotBytes;
+    const uint32_t read0 = cluster_addr(&pipe.read[0], 0);
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(128 * half);
-    int acc = 0;
-    uint32_t acc_ph = 0;
+    int st = 0, acc = 0;
+    uint32_t ph = 0;
     bool ok = true;
     for (int t = first; t < tiles && ok; t += step) {
       int i, j;
@@ -300,21 +348,33 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int next = min(b0 + q + kAhead, shape.blocks - 1);
           l[q] = ls[next * scales.left_cstride];
           r[q] = rs[next * scales.right_rstride];
-          ok = __all_sync(0xffffffffu, pipe.wait(&pipe.tfull[acc], acc_ph, kStatusEpilogueTimeout));
+          ok = __all_sync(0xffffffffu, pipe.wait(&pipe.done[st], ph, kStatusEpilogueTimeout));
           if (!ok) continue;
           tc_fence_after();
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float v[32];
-            tmem_load_32cols(lanes + static_cast<uint32_t>(acc * kTile + 32 * c), v);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) sum[16 * c + e] = fma2(Pair(v[2 * e], v[2 * e + 1]), scale, sum[16 * c + e]);
-          }
+          // Two pieces are on their way at a time, and the accumulator is handed back as soon
+          // as the last two have landed: their additions run beside the next products.
+          const uint32_t at = lanes + static_cast<uint32_t>(acc * kTile);
+          TmemPiece even, odd;
+          even.issue(at);
+          odd.issue(at + 32);
+          even.land();
+          odd.land();
+          even.add_to(sum, scale);
+          even.issue(at + 64);
+          odd.add_to(sum + 16, scale);
+          odd.issue(at + 96);
+          even.land();
+          odd.land();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(tempty0 + static_cast<uint32_t>(acc) * 8u);
+          if (lane == 0) mbar_arrive_cluster(read0 + static_cast<uint32_t>(acc) * 8u);
+          even.add_to(sum + 32, scale);
+          odd.add_to(sum + 48, scale);
           acc ^= 1;
-          if (acc == 0) acc_ph ^= 1u;
+          if (++st == S) {
+            st = 0;
+            ph ^= 1u;
+          }
         }
       }
       if (!ok) break;
@@ -467,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t ph = 0;
       bool ok = true;
       for (int b = b_begin; b < b_end; ++b) {
-        ok = pipe.wait(&pipe.empty[st], ph ^ 1u, kStatusProducerTimeout);
+        ok = pipe.wait(&pipe.done[st], ph ^ 1u, kStatusProducerTimeout);
         if (!ok) break;
         uint8_t* at = smem + st * Cfg::kStageBytes;
         mbar_arrive_expect_tx(&pipe.full[st], Cfg::kStageBytes);
@@ -489,8 +549,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       int st = 0, acc = 0;
       uint32_t ph = 0, acc_ph = 0;
       for (int b = b_begin; b < b_end; ++b) {
-        if (!pipe.wait(&pipe.tempty[acc], acc_ph ^ 1u, kStatusMmaTimeout) ||
-            !pipe.wait(&pipe.full[st], ph, kStatusMmaTimeout))
+        if (!pipe.wait(&pipe.full[st], ph, kStatusMmaTimeout) ||
+            !pipe.wait(&pipe.read[acc], acc_ph ^ 1u, kStatusMmaTimeout))
           break;
         tc_fence_after();
         const uint8_t* at = smem + st * Cfg::kStageBytes;
@@ -499,8 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int k = 0; k < kSteps; ++k)
           mma_8bit(tmem + static_cast<uint32_t>(acc * TOK), features + k * step_of(M_MN), tokens + k * step_of(false), idesc,
                    k > 0 ? 1u : 0u);
-        tc_commit(&pipe.empty[st]);
-        tc_commit(&pipe.tfull[acc]);
+        tc_commit(&pipe.done[st]);
         if (++st == S) {
           st = 0;
           ph ^= 1u;
@@ -530,8 +589,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 #pragma unroll
     for (int q = 0; q < Cfg::kHalf / 2; ++q) sum[q] = Pair(0.0f);
-    int acc = 0;
-    uint32_t acc_ph = 0;
+    int st = 0, acc = 0;
+    uint32_t ph = 0;
     bool ok = true;
     for (int b0 = b_begin; b0 < b_end && ok; b0 += kAhead) {
 #pragma unroll
@@ -545,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         r[q] = rs[next * scales.right_rstride];
 #pragma unroll
         for (int e = 0; e < kEach; ++e) l[q][e] = ls[e][next * scales.left_cstride];
-        ok = __all_sync(0xffffffffu, pipe.wait(&pipe.tfull[acc], acc_ph, kStatusEpilogueTimeout));
+        ok = __all_sync(0xffffffffu, pipe.wait(&pipe.done[st], ph, kStatusEpilogueTimeout));
         if (!ok) continue;
         tc_fence_after();
 #pragma unroll
@@ -561,9 +620,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&pipe.tempty[acc]);
+        if (lane == 0) mbar_arrive(&pipe.read[acc]);
         acc ^= 1;
-        if (acc == 0) acc_ph ^= 1u;
+        if (++st == S) {
+          st = 0;
+          ph ^= 1u;
+        }
       }
     }
   }
@@ -649,7 +711,7 @@ int prepare_kernel(void (*kernel)(Params...), int slot, size_t smem, bool pair, 
       attr[0].val.clusterDim.x = 2;
       attr[0].val.clusterDim.y = 1;
       attr[0].val.clusterDim.z = 1;
-      cfg.blockDim = dim3(kThreads, 1, 1);
+      cfg.blockDim = dim3(kPairThreads, 1, 1);
       cfg.gridDim = dim3(static_cast<unsigned>(n / 2 * 2), 1, 1);
       cfg.dynamicSmemBytes = smem;
       cfg.attrs = attr;
@@ -672,11 +734,11 @@ struct Call8 {
 };
 
 template <typename... Params, typename... Args>
-int launch8(void (*kernel)(Params...), dim3 grid, int cluster, size_t smem, cudaStream_t stream, const Args&... args) {
+int launch8(void (*kernel)(Params...), dim3 grid, int threads, int cluster, size_t smem, cudaStream_t stream, const Args&... args) {
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -701,7 +763,7 @@ int launch_pair(const Call8& c, cudaStream_t stream) {
   if (rc != GNS_OK) return rc;
   const Tiling tiling{(c.shape.m + kTile - 1) / kTile, (c.shape.n + kTile - 1) / kTile};
   const int tiles = tiling.rows * tiling.cols;
-  return launch8(kernel, dim3(2u * static_cast<unsigned>(std::min(tiles, resident))), 2, smem, stream, c.left, c.right,
+  return launch8(kernel, dim3(2u * static_cast<unsigned>(std::min(tiles, resident))), kPairThreads, 2, smem, stream, c.left, c.right,
                  c.out_map, c.scales, c.shape, tiling, c.out);
 }
 
@@ -714,7 +776,7 @@ int launch_rows(const Call8& c, int parts, int slot, cudaStream_t stream) {
   if (rc != GNS_OK) return rc;
   const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>((c.shape.n + 127) / 128),
                   static_cast<unsigned>((c.shape.m + TOK - 1) / TOK));
-  return launch8(kernel, grid, parts, smem, stream, c.left, c.right, c.scales, c.shape, c.out);
+  return launch8(kernel, grid, kThreads, parts, smem, stream, c.left, c.right, c.scales, c.shape, c.out);
 }
 
 template <bool MN, bool F32>
