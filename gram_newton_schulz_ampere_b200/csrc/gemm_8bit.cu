@@ -331,50 +331,50 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       Pair sum[64];
 #pragma unroll
       for (int q = 0; q < 64; ++q) sum[q] = Pair(0.0f);
-      // Scales are loaded four blocks ahead of their use.
-      constexpr int kAhead = 4;
-      float l[kAhead], r[kAhead];
-#pragma unroll
-      for (int q = 0; q < kAhead; ++q) {
-        const int b = min(q, shape.blocks - 1);
-        l[q] = ls[b * scales.left_cstride];
-        r[q] = rs[b * scales.right_rstride];
+      // Scales are loaded two blocks ahead of their use.
+      float l0 = *ls, r0 = *rs, l1 = l0, r1 = r0;
+      if (shape.blocks > 1) {
+        ls += scales.left_cstride;
+        rs += scales.right_rstride;
+        l1 = *ls;
+        r1 = *rs;
       }
-      for (int b0 = 0; b0 < shape.blocks && ok; b0 += kAhead) {
-#pragma unroll
-        for (int q = 0; q < kAhead; ++q) {
-          if (b0 + q >= shape.blocks || !ok) continue;
-          const Pair scale(l[q] * r[q]);
-          const int next = min(b0 + q + kAhead, shape.blocks - 1);
-          l[q] = ls[next * scales.left_cstride];
-          r[q] = rs[next * scales.right_rstride];
-          ok = __all_sync(0xffffffffu, pipe.wait(&pipe.done[st], ph, kStatusEpilogueTimeout));
-          if (!ok) continue;
-          tc_fence_after();
-          // Two pieces are on their way at a time, and the accumulator is handed back as soon
-          // as the last two have landed: their additions run beside the next products.
-          const uint32_t at = lanes + static_cast<uint32_t>(acc * kTile);
-          TmemPiece even, odd;
-          even.issue(at);
-          odd.issue(at + 32);
-          even.land();
-          odd.land();
-          even.add_to(sum, scale);
-          even.issue(at + 64);
-          odd.add_to(sum + 16, scale);
-          odd.issue(at + 96);
-          even.land();
-          odd.land();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(read0 + static_cast<uint32_t>(acc) * 8u);
-          even.add_to(sum + 32, scale);
-          odd.add_to(sum + 48, scale);
-          acc ^= 1;
-          if (++st == S) {
-            st = 0;
-            ph ^= 1u;
-          }
+      for (int b = 0; b < shape.blocks; ++b) {
+        const Pair scale(l0 * r0);
+        l0 = l1;
+        r0 = r1;
+        if (b + 2 < shape.blocks) {
+          ls += scales.left_cstride;
+          rs += scales.right_rstride;
+          l1 = *ls;
+          r1 = *rs;
+        }
+        ok = __all_sync(0xffffffffu, pipe.wait(&pipe.done[st], ph, kStatusEpilogueTimeout));
+        if (!ok) break;
+        tc_fence_after();
+        // Two pieces are on their way at a time, and the accumulator is handed back as soon
+        // as the last two have landed: their additions run beside the next products.
+        const uint32_t at = lanes + static_cast<uint32_t>(acc * kTile);
+        TmemPiece even, odd;
+        even.issue(at);
+        odd.issue(at + 32);
+        even.land();
+        odd.land();
+        even.add_to(sum, scale);
+        even.issue(at + 64);
+        odd.add_to(sum + 16, scale);
+        odd.issue(at + 96);
+        even.land();
+        odd.land();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(read0 + static_cast<uint32_t>(acc) * 8u);
+        even.add_to(sum + 32, scale);
+        odd.add_to(sum + 48, scale);
+        acc ^= 1;
+        if (++st == S) {
+          st = 0;
+          ph ^= 1u;
         }
       }
       if (!ok) break;
