@@ -8,11 +8,24 @@
 // registers, while the tensor cores work on the next block in the other accumulator.
 // Rounded once, at the store.
 //
-// Two kernels. Many rows: a CTA pair computes 256 x 256 tiles of the output, rows of left
+// Three kernels. Many rows: a CTA pair computes 256 x 256 tiles of the output, rows of left
 // on the MMA's M side, so that a thread's scale is one number a block (its row's, times
-// the right block's). Few rows: right's columns (a layer's features) are the M side and up
-// to 128 rows of left the N side, whose width follows the rows; a cluster of CTAs shares a
-// tile's contraction and joins the fp32 sums out of shared memory in a fixed order.
+// the right block's). Fewer rows: 128 x 128 tiles of a CTA, alike. Up to 32 rows: right's
+// columns (a layer's features) are the M side and the rows of left the N side, whose width
+// follows them. In the last two a cluster of CTAs may share a tile's contraction; it joins the
+// fp32 sums out of shared memory in a fixed order.
+//
+// The pair kernel, 16384 x 4096 x 14336: 861 us, 2.23 PFLOP/s, at the power cap (1.67 GHz; in a
+// run of seconds 1030 us at 1.44 GHz); 717 us, 2.68 PFLOP/s, with operands of zeros, which leave
+// the clock at 1.965 GHz: 900 cycles a block of 256 x 256 x 128 a pair, where its products
+// take 512. A block's way from its last product to the first one that may overwrite its
+// accumulator is 980 cycles of signals between the CTAs and 310 of reading, with two
+// accumulators (all of TMEM) under way: (512 + 980 + 310) / 2. Without the summing it is 750.
+// Measured and not kept: halves of 128 columns with four accumulators (950 without the summing:
+// products 128 wide read the left operand twice as often), sixteen summing warps of 64
+// columns (1046 against 962 under the profiler: twice the instructions beside the sums), sums
+// one at a time instead of in pairs (1106). A library product with one scale for all, which
+// adds nothing up outside of TMEM: 670 us.
 //
 // Every wait is bounded.
 #include <algorithm>
@@ -48,7 +61,7 @@ struct Out8 {
   void* d;
   int64_t ldd;
   int bf16;  // 16-bit outputs: 1 = bf16, 0 = fp16
-  int tma;   // the output's rows can be written by TMA
+  int whole; // the output's rows start on 16 bytes (few rows: on words)
 };
 
 // D (+)= A . B, 8-bit floating point operands (e4m3: format 0 in the instruction descriptor).
@@ -88,29 +101,30 @@ constexpr int kSteps = kBlock / 32;
 // its accumulator: one commit a block, which the producer and the summing warps wait for (a
 // commit costs the issuing thread about 60 cycles, a block's products take 512). In a pair
 // the `full` and `read` barriers of CTA 0 serve both CTAs, and each CTA has its own `done`.
-template <int S, bool PAIR>
+template <int S, int ACC>
 struct Pipe {
   uint64_t* full;  // a stage has landed
   uint64_t* done;  // its products are done
   uint64_t* read;  // the accumulator has been read
   uint32_t* tmem_slot;
   volatile int* abort_flag;
-  static constexpr uint32_t kBytes = (2 * S + 2) * 8 + 8;
+  static constexpr uint32_t kBytes = (2 * S + ACC) * 8 + 8;
 
   __device__ __forceinline__ explicit Pipe(uint8_t* at) {
     full = reinterpret_cast<uint64_t*>(at);
     done = full + S;
     read = done + S;
-    tmem_slot = reinterpret_cast<uint32_t*>(read + 2);
+    tmem_slot = reinterpret_cast<uint32_t*>(read + ACC);
     abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   }
 
-  __device__ __forceinline__ void init() const {
+  // readers: the warps that read an accumulator.
+  __device__ __forceinline__ void init(uint32_t readers) const {
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&done[s], 1);
     }
-    for (int a = 0; a < 2; ++a) mbar_init(&read[a], (PAIR ? 2 : 1) * kEpiWarps);
+    for (int a = 0; a < ACC; ++a) mbar_init(&read[a], readers);
     *abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async_smem();
@@ -201,7 +215,7 @@ struct PairConfig {
   // A warp's part of the output on its way to memory: 32 rows in two boxes of 128 bytes a row.
   static constexpr uint32_t kBoxBytes = 32 * 128;
   static constexpr uint32_t kSlotBytes = 2 * kBoxBytes;
-  static constexpr size_t kSmemBytes = 1024 + kStages * kStageBytes + kEpiWarps * kSlotBytes + Pipe<kStages, true>::kBytes;
+  static constexpr size_t kSmemBytes = 1024 + kStages * kStageBytes + kEpiWarps * kSlotBytes + Pipe<kStages, 2>::kBytes;
 };
 
 // Tiles in bands of eight rows of tiles, column by column: the tiles that run at one time
@@ -233,12 +247,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* smem_out = smem + S * Cfg::kStageBytes;
-  const Pipe<S, true> pipe(smem_out + kEpiWarps * Cfg::kSlotBytes);
+  const Pipe<S, 2> pipe(smem_out + kEpiWarps * Cfg::kSlotBytes);
 
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&map_left);
     tma_prefetch_desc(&map_right);
-    pipe.init();
+    pipe.init(2 * kEpiWarps);
   }
   if (warp == 1) {
     tmem_alloc_pair(pipe.tmem_slot, 512);
@@ -339,11 +353,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         l1 = *ls;
         r1 = *rs;
       }
-      for (int b = 0; b < shape.blocks; ++b) {
+      for (int left = shape.blocks; left > 0; --left) {
         const Pair scale(l0 * r0);
         l0 = l1;
         r0 = r1;
-        if (b + 2 < shape.blocks) {
+        if (left > 2) {
           ls += scales.left_cstride;
           rs += scales.right_rstride;
           l1 = *ls;
@@ -404,7 +418,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           *reinterpret_cast<uint4*>(at + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
         const int col = col0 + box * kCols;
-        if (out.tma) {
+        if (out.whole) {
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
@@ -414,14 +428,18 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         } else {
           __syncwarp();
           constexpr int es = OUT_F32 ? 4 : 2;
-          for (int q = 0; q < min(32, shape.m - row0); ++q) {
-            const int64_t to = static_cast<int64_t>(row0 + q) * out.ldd + col;
-            for (int c = lane; c < min(kCols, shape.n - col); c += 32) {
+          const int rows = min(32, shape.m - row0), cols = shape.n - col;
+          uint8_t* to = static_cast<uint8_t*>(out.d) + (static_cast<int64_t>(row0) * out.ldd + col + lane) * es;
+#pragma unroll 8
+          for (int q = 0; q < rows; ++q, to += out.ldd * es) {
+#pragma unroll
+            for (int c = lane; c < lane + kCols; c += 32) {
+              if (c >= cols) continue;
               const uint8_t* from = at + q * 128 + (((c * es / 16) ^ (q & 7)) << 4) + c * es % 16;
               if (OUT_F32)
-                static_cast<uint32_t*>(out.d)[to + c] = *reinterpret_cast<const uint32_t*>(from);
+                *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
               else
-                static_cast<uint16_t*>(out.d)[to + c] = *reinterpret_cast<const uint16_t*>(from);
+                *reinterpret_cast<uint16_t*>(to + (c - lane) * es) = *reinterpret_cast<const uint16_t*>(from);
             }
           }
           __syncwarp();
@@ -443,17 +461,249 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   }
 }
 
+// ---------------------------------------------------------------- some rows
+// Tiles of 128 rows of left and 128 columns of right, a CTA each, for products whose pair
+// tiles would leave SMs idle. As above a thread sums a row of left, 64 columns of it, with one
+// scale a block. A cluster of up to 8 CTAs shares a tile's contraction: the partial sums
+// are left in shared memory and added up, by rows, in the parts' order.
+struct TileConfig {
+  static constexpr int kStages = 6;
+  static constexpr uint32_t kStageBytes = 2 * kTileBytes;
+  // Four accumulators: a block's way from its products through the summing warps and back
+  // takes longer than the next one's products.
+  static constexpr int kAcc = 4;
+  static constexpr size_t kSmemBytes = 1024 + kStages * kStageBytes + Pipe<kStages, kAcc>::kBytes;
+  static_assert(kStages * kStageBytes >= 128 * 128 * 4, "the partial sums take the stages' place");
+};
+
+constexpr int kTileThreads = kThreads + 32;
+
+template <bool B_MN, bool OUT_F32>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    gemm8_tile_kernel(const __grid_constant__ CUtensorMap map_left, const __grid_constant__ CUtensorMap map_right,
+                      const Scales scales, const Shape8 shape, const Out8 out) {
+  using Cfg = TileConfig;
+  constexpr int S = Cfg::kStages;
+  // blockIdx.x: the CTA's part of the contraction; y: columns of right; z: rows of left.
+  const int parts = static_cast<int>(gridDim.x), part = static_cast<int>(blockIdx.x);
+  const int row0 = static_cast<int>(blockIdx.z) * 128, col0 = static_cast<int>(blockIdx.y) * 128;
+  const int b_begin = static_cast<int>(static_cast<int64_t>(part) * shape.blocks / parts);
+  const int b_end = static_cast<int>(static_cast<int64_t>(part + 1) * shape.blocks / parts);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const Pipe<S, Cfg::kAcc> pipe(smem + S * Cfg::kStageBytes);
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&map_left);
+    tma_prefetch_desc(&map_right);
+    pipe.init(kEpiWarps);
+  }
+  if (warp == 1) {
+    tmem_alloc(pipe.tmem_slot, Cfg::kAcc * 128);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_dependents();
+  pdl_wait_predecessor();
+  const uint32_t tmem = *pipe.tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int st = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int b = b_begin; b < b_end; ++b) {
+        ok = pipe.wait(&pipe.done[st], ph ^ 1u, kStatusProducerTimeout);
+        if (!ok) break;
+        uint8_t* at = smem + st * Cfg::kStageBytes;
+        mbar_arrive_expect_tx(&pipe.full[st], Cfg::kStageBytes);
+        tma_load_3d(at, &map_left, &pipe.full[st], b * kBlock, row0, 0);
+        if (B_MN)
+          tma_load_3d(at + kTileBytes, &map_right, &pipe.full[st], col0, b * kBlock, 0);
+        else
+          tma_load_3d(at + kTileBytes, &map_right, &pipe.full[st], b * kBlock, col0, 0);
+        if (++st == S) {
+          st = 0;
+          ph ^= 1u;
+        }
+      }
+      pipe.drain(st, ph, ok);
+    }
+  } else if (warp == 1 || warp == 2 + kEpiWarps) {
+    // Two warps issue the blocks' products in turn.
+    if (lane == 0) {
+      const uint32_t idesc = idesc_8bit(false, B_MN, 128, 128);
+      const int turn = warp == 1 ? 0 : 1;
+      int st = turn, acc = turn;
+      uint32_t ph = 0, acc_ph = 0;
+      for (int b = b_begin + turn; b < b_end; b += 2) {
+        if (!pipe.wait(&pipe.full[st], ph, kStatusMmaTimeout) ||
+            !pipe.wait(&pipe.read[acc], acc_ph ^ 1u, kStatusMmaTimeout))
+          break;
+        tc_fence_after();
+        const uint8_t* at = smem + st * Cfg::kStageBytes;
+        const uint64_t left = tile_desc(at), right = tile_desc(at + kTileBytes);
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+          mma_8bit(tmem + static_cast<uint32_t>(acc * 128), left + k * step_of(false), right + k * step_of(B_MN), idesc,
+                   k > 0 ? 1u : 0u);
+        tc_commit(&pipe.done[st]);
+        st += 2;
+        if (st >= S) {
+          st -= S;
+          ph ^= 1u;
+        }
+        acc += 2;
+        if (acc >= Cfg::kAcc) {
+          acc -= Cfg::kAcc;
+          acc_ph ^= 1u;
+        }
+      }
+    }
+  } else {
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(64 * half);
+    const int mine = quarter * 32 + lane;
+    const float* ls = scales.left + min(row0 + mine, shape.m - 1) * scales.left_rstride + b_begin * scales.left_cstride;
+    const float* rs = scales.right + col0 / kBlock * scales.right_cstride + b_begin * scales.right_rstride;
+    Pair sum[32];
+#pragma unroll
+    for (int q = 0; q < 32; ++q) sum[q] = Pair(0.0f);
+    // Scales are loaded two blocks ahead of their use.
+    float l0 = *ls, r0 = *rs, l1 = l0, r1 = r0;
+    if (b_end - b_begin > 1) {
+      ls += scales.left_cstride;
+      rs += scales.right_rstride;
+      l1 = *ls;
+      r1 = *rs;
+    }
+    int st = 0, acc = 0;
+    uint32_t ph = 0;
+    for (int left = b_end - b_begin; left > 0; --left) {
+      const Pair scale(l0 * r0);
+      l0 = l1;
+      r0 = r1;
+      if (left > 2) {
+        ls += scales.left_cstride;
+        rs += scales.right_rstride;
+        l1 = *ls;
+        r1 = *rs;
+      }
+      if (!__all_sync(0xffffffffu, pipe.wait(&pipe.done[st], ph, kStatusEpilogueTimeout))) break;
+      tc_fence_after();
+      const uint32_t at = lanes + static_cast<uint32_t>(acc * 128);
+      TmemPiece even, odd;
+      even.issue(at);
+      odd.issue(at + 32);
+      even.land();
+      odd.land();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&pipe.read[acc]);
+      even.add_to(sum, scale);
+      odd.add_to(sum + 16, scale);
+      if (++acc == Cfg::kAcc) acc = 0;
+      if (++st == S) {
+        st = 0;
+        ph ^= 1u;
+      }
+    }
+    // Every stage has been multiplied: the sums take their place, rows of 512 bytes whose
+    // 16-byte pieces are turned by the row within each 128 bytes.
+    uint8_t* to = smem + mine * 512 + half * 256;
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+      float v[4];
+      sum[2 * c].get(v[0], v[1]);
+      sum[2 * c + 1].get(v[2], v[3]);
+      *reinterpret_cast<float4*>(to + (c / 8) * 128 + (((c % 8) ^ (lane & 7)) << 4)) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (*pipe.abort_flag) settle_for_ns(2000000ull);
+  cluster_sync_all();
+  tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc(tmem, Cfg::kAcc * 128);
+  }
+  // The cluster's CTAs take the rows in turn, a warp a row, four rows on their way together.
+  if (warp >= 2 && warp < 2 + kEpiWarps) {
+    const int rows = min(128, shape.m - row0);
+    const int col = col0 + lane * 4, left = shape.n - col;
+    constexpr int kDeep = 4;
+    for (int r0 = part + parts * (warp - 2); r0 < rows; r0 += parts * kEpiWarps * kDeep) {
+      float4 v[kDeep];
+#pragma unroll
+      for (int q = 0; q < kDeep; ++q) v[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int p = 0; p < parts; ++p) {
+        float4 u[kDeep];
+#pragma unroll
+        for (int q = 0; q < kDeep; ++q) {
+          const int r = r0 + q * parts * kEpiWarps;
+          u[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (r >= rows) continue;
+          const uint8_t* at = smem + r * 512 + (lane / 8) * 128 + (((lane % 8) ^ (r & 7)) << 4);
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(u[q].x), "=f"(u[q].y), "=f"(u[q].z), "=f"(u[q].w)
+                       : "r"(cluster_addr(at, static_cast<uint32_t>(p)))
+                       : "memory");
+        }
+#pragma unroll
+        for (int q = 0; q < kDeep; ++q)
+          v[q] = make_float4(v[q].x + u[q].x, v[q].y + u[q].y, v[q].z + u[q].z, v[q].w + u[q].w);
+      }
+#pragma unroll
+      for (int q = 0; q < kDeep; ++q) {
+        const int r = r0 + q * parts * kEpiWarps;
+        if (r >= rows) continue;
+        const int64_t at = static_cast<int64_t>(row0 + r) * out.ldd + col;
+        const float one[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+        if (OUT_F32) {
+          float* d = static_cast<float*>(out.d) + at;
+          if (out.whole && left >= 4) {
+            *reinterpret_cast<float4*>(d) = v[q];
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (e < left) d[e] = one[e];
+          }
+        } else {
+          uint16_t* d = static_cast<uint16_t*>(out.d) + at;
+          if (out.whole && left >= 4) {
+            *reinterpret_cast<uint2*>(d) = make_uint2(pack_pair(one[0], one[1], out.bf16), pack_pair(one[2], one[3], out.bf16));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (e < left) d[e] = float_to_half_bits(one[e], out.bf16);
+          }
+        }
+      }
+    }
+  }
+  cluster_sync_all();  // no CTA leaves while another reads its sums
+}
+
 // ------------------------------------------------------------------- few rows
 // A tile: 128 features and up to TOK rows of left.
 template <int TOK>
 struct RowConfig {
   static constexpr uint32_t kRowBytes = TOK * kBlock;
   static constexpr uint32_t kStageBytes = kTileBytes + kRowBytes;
-  static constexpr int kStages = 6 * 32768 / kStageBytes;
+  static constexpr int kStages = 3 * 32768 / kStageBytes;  // two CTAs on an SM
   static constexpr int kHalf = TOK / 2;  // rows of left that a warp sums
-  static constexpr uint32_t kTmemCols = 2 * TOK < 32 ? 32 : 2 * TOK;
+  // Four accumulators: a block's way from its products through the summing warps and back
+  // takes longer than the next one's products.
+  static constexpr int kAcc = 4;
+  static constexpr uint32_t kTmemCols = kAcc * TOK;
   static constexpr uint32_t kScaleBytes = kEpiWarps * 2 * kHalf * 4;
-  static constexpr size_t kSmemBytes = 1024 + kStages * kStageBytes + kScaleBytes + Pipe<kStages, false>::kBytes;
+  static constexpr size_t kSmemBytes = 1024 + kStages * kStageBytes + kScaleBytes + Pipe<kStages, kAcc>::kBytes;
   static_assert(kStages * kStageBytes >= TOK * 128 * 4, "the partial sums take the stages' place");
 };
 
@@ -484,7 +734,7 @@ __device__ __forceinline__ void tmem_load(uint32_t at, float (&v)[N]) {
 }
 
 template <bool M_MN, int TOK, bool OUT_F32>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, 2)
     gemm8_rows_kernel(const __grid_constant__ CUtensorMap map_left, const __grid_constant__ CUtensorMap map_right,
                       const Scales scales, const Shape8 shape, const Out8 out) {
   using Cfg = RowConfig<TOK>;
@@ -500,12 +750,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* smem_scales = reinterpret_cast<float*>(smem + S * Cfg::kStageBytes);
-  const Pipe<S, false> pipe(smem + S * Cfg::kStageBytes + Cfg::kScaleBytes);
+  const Pipe<S, Cfg::kAcc> pipe(smem + S * Cfg::kStageBytes + Cfg::kScaleBytes);
 
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&map_left);
     tma_prefetch_desc(&map_right);
-    pipe.init();
+    pipe.init(kEpiWarps);
   }
   if (warp == 1) {
     tmem_alloc(pipe.tmem_slot, Cfg::kTmemCols);
@@ -564,8 +814,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           st = 0;
           ph ^= 1u;
         }
-        acc ^= 1;
-        if (acc == 0) acc_ph ^= 1u;
+        if (++acc == Cfg::kAcc) {
+          acc = 0;
+          acc_ph ^= 1u;
+        }
       }
     }
   } else {
@@ -606,6 +858,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < kEach; ++e) l[q][e] = ls[e][next * scales.left_cstride];
         ok = __all_sync(0xffffffffu, pipe.wait(&pipe.done[st], ph, kStatusEpilogueTimeout));
         if (!ok) continue;
+        __syncwarp();
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < Cfg::kHalf; c += kPiece) {
@@ -621,7 +874,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&pipe.read[acc]);
-        acc ^= 1;
+        if (++acc == Cfg::kAcc) acc = 0;
         if (++st == S) {
           st = 0;
           ph ^= 1u;
@@ -675,7 +928,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {
         uint16_t* d = static_cast<uint16_t*>(out.d) + at;
         const uint32_t two = pack_pair(x, y, out.bf16);
-        if (out.tma && left > 1) {
+        if (out.whole && left > 1) {
           *reinterpret_cast<uint32_t*>(d) = two;
         } else {
           if (left > 0) d[0] = static_cast<uint16_t>(two);
@@ -763,8 +1016,8 @@ int launch_pair(const Call8& c, cudaStream_t stream) {
   if (rc != GNS_OK) return rc;
   const Tiling tiling{(c.shape.m + kTile - 1) / kTile, (c.shape.n + kTile - 1) / kTile};
   const int tiles = tiling.rows * tiling.cols;
-  return launch8(kernel, dim3(2u * static_cast<unsigned>(std::min(tiles, resident))), kPairThreads, 2, smem, stream, c.left, c.right,
-                 c.out_map, c.scales, c.shape, tiling, c.out);
+  return launch8(kernel, dim3(2u * static_cast<unsigned>(std::min(tiles, resident))), kPairThreads, 2, smem, stream, c.left,
+                 c.right, c.out_map, c.scales, c.shape, tiling, c.out);
 }
 
 template <bool M_MN, int TOK, bool OUT_F32>
@@ -772,7 +1025,7 @@ int launch_rows(const Call8& c, int parts, int slot, cudaStream_t stream) {
   auto kernel = gemm8_rows_kernel<M_MN, TOK, OUT_F32>;
   constexpr size_t smem = RowConfig<TOK>::kSmemBytes;
   int resident = 0;
-  const int rc = prepare_kernel(kernel, 4 + slot + (M_MN ? 8 : 0) + (OUT_F32 ? 16 : 0), smem, false, &resident);
+  const int rc = prepare_kernel(kernel, 4 + slot + (M_MN ? 4 : 0) + (OUT_F32 ? 8 : 0), smem, false, &resident);
   if (rc != GNS_OK) return rc;
   const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>((c.shape.n + 127) / 128),
                   static_cast<unsigned>((c.shape.m + TOK - 1) / TOK));
@@ -782,24 +1035,51 @@ int launch_rows(const Call8& c, int parts, int slot, cudaStream_t stream) {
 template <bool MN, bool F32>
 int launch_rows_any(const Call8& c, int tok, int parts, cudaStream_t stream) {
   if (tok == 16) return launch_rows<MN, 16, F32>(c, parts, 0, stream);
-  if (tok == 32) return launch_rows<MN, 32, F32>(c, parts, 1, stream);
-  if (tok == 64) return launch_rows<MN, 64, F32>(c, parts, 2, stream);
-  return launch_rows<MN, 128, F32>(c, parts, 3, stream);
+  return launch_rows<MN, 32, F32>(c, parts, 1, stream);
+}
+
+template <bool B_MN, bool OUT_F32>
+int launch_tiles(const Call8& c, int parts, cudaStream_t stream) {
+  auto kernel = gemm8_tile_kernel<B_MN, OUT_F32>;
+  constexpr size_t smem = TileConfig::kSmemBytes;
+  int resident = 0;
+  const int rc = prepare_kernel(kernel, 20 + (B_MN ? 2 : 0) + (OUT_F32 ? 1 : 0), smem, false, &resident);
+  if (rc != GNS_OK) return rc;
+  const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>((c.shape.n + 127) / 128),
+                  static_cast<unsigned>((c.shape.m + 127) / 128));
+  return launch8(kernel, grid, kTileThreads, parts, smem, stream, c.left, c.right, c.scales, c.shape, c.out);
 }
 
 struct Plan8 {
-  int tok;    // rows of left of a tile of the few-rows kernel; 0: the many-rows kernel
+  int rows;   // of left in a tile: 16, 32 (few rows), 128 (a CTA) or 256 (a pair)
   int parts;  // CTAs that share a tile's contraction
 };
 
+// Which kernel, and how many CTAs share a tile. Microseconds measured on one B200, captured
+// calls whose weights come from HBM, m x k x n:
+//   up to 32 rows, parts 1 / 2 / 4 / 8: doubled while the CTAs are at most two an SM and each
+//   part has two blocks
+//     1 x 4096 x 14336   17.1 / 13.5 / 17.6 / 24.4     1 x 14336 x 4096   44.2 / 24.7 / 15.8 / 13.5
+//     1 x 1024 x 4096    5.7 / 4.7 / 4.1 / 5.0         32 x 8192 x 512    27.6 / 15.8 / 9.6 / 6.8
+//   128-row tiles where there is an SM for each, parts 1 / 2 / 4 against pair tiles: doubled
+//   while there are SMs, to four (clusters of 8 leave SMs of a GPC unused, and the join reads
+//   the sums at 17 bytes a cycle), and each part has eight blocks
+//     96 x 14336 x 4096  53.9 / 31.3 / 21.5, 52.2      96 x 4096 x 14336  20.6 / 25.9 / -, 19.8
+//     256 x 4096 x 4096  19.7 / 13.2 / 20.5, 19.0      256 x 1024 x 4096  7.3 / 7.0 / 14.9, 8.1
+//     96 x 2048 x 512    8.3 / 7.1 / 7.3, 10.8         1024 x 2048 x 2048 9.7 / 15.7 / -, 11.8
+//     1024 x 4096 x 4096 40.2, 19.7
 Plan8 plan8(int64_t m, int64_t n, int64_t blocks) {
-  if (m > 128) return {0, 1};
-  const int tok = m <= 16 ? 16 : (m <= 32 ? 32 : (m <= 64 ? 64 : 128));
-  const int64_t tiles = (n + 127) / 128;
   const int sms = device_sm_count();
+  const int64_t tiles = (n + 127) / 128;
   int parts = 1;
-  while (parts < 8 && tiles * parts * 2 <= sms && blocks >= 2 * parts) parts *= 2;
-  return {tok, parts};
+  if (m <= 32) {
+    while (parts < 8 && tiles * parts * 2 <= 2 * sms && blocks >= 4 * parts) parts *= 2;
+    return {m <= 16 ? 16 : 32, parts};
+  }
+  const int64_t all = tiles * ((m + 127) / 128);
+  if (all > sms) return {256, 1};
+  while (parts < 4 && all * parts * 2 <= sms && blocks >= 16 * parts) parts *= 2;
+  return {128, parts};
 }
 
 }  // namespace
@@ -842,7 +1122,7 @@ int gns_gemm_8bit(int64_t m, int64_t n, int64_t k, const void* left, int64_t lef
   c.shape = {static_cast<int>(m), static_cast<int>(n), static_cast<int>((k + kBlock - 1) / kBlock)};
   c.out = {out, out_rstride, out_dtype == kBF16 ? 1 : 0, 0};
   const Plan8 plan = plan8(m, n, c.shape.blocks);
-  rc = encode_byte_tiles(&c.left, left, k, m, left_rstride, plan.tok > 0 ? plan.tok : 128);
+  rc = encode_byte_tiles(&c.left, left, k, m, left_rstride, std::min(plan.rows, 128));
   if (rc == GNS_OK)
     rc = k_major ? encode_byte_tiles(&c.right, right, k, n, right_cstride, 128)
                  : encode_byte_tiles(&c.right, right, n, k, right_rstride, 128);
@@ -850,14 +1130,18 @@ int gns_gemm_8bit(int64_t m, int64_t n, int64_t k, const void* left, int64_t lef
   const int es = dtype_size(out_dtype);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool f32 = out_dtype == kF32;
-  if (plan.tok > 0) {
+  if (plan.rows <= 32) {
     // Pairs of 16-bit values are stored as one word where rows start on words.
-    c.out.tma = reinterpret_cast<uintptr_t>(out) % 4 == 0 && (out_rstride * es) % 4 == 0;
-    if (k_major) return f32 ? launch_rows_any<false, true>(c, plan.tok, plan.parts, st) : launch_rows_any<false, false>(c, plan.tok, plan.parts, st);
-    return f32 ? launch_rows_any<true, true>(c, plan.tok, plan.parts, st) : launch_rows_any<true, false>(c, plan.tok, plan.parts, st);
+    c.out.whole = reinterpret_cast<uintptr_t>(out) % 4 == 0 && (out_rstride * es) % 4 == 0;
+    if (k_major) return f32 ? launch_rows_any<false, true>(c, plan.rows, plan.parts, st) : launch_rows_any<false, false>(c, plan.rows, plan.parts, st);
+    return f32 ? launch_rows_any<true, true>(c, plan.rows, plan.parts, st) : launch_rows_any<true, false>(c, plan.rows, plan.parts, st);
   }
-  c.out.tma = reinterpret_cast<uintptr_t>(out) % 16 == 0 && (out_rstride * es) % 16 == 0;
-  if (c.out.tma) {
+  c.out.whole = reinterpret_cast<uintptr_t>(out) % 16 == 0 && (out_rstride * es) % 16 == 0;
+  if (plan.rows == 128) {
+    if (k_major) return f32 ? launch_tiles<false, true>(c, plan.parts, st) : launch_tiles<false, false>(c, plan.parts, st);
+    return f32 ? launch_tiles<true, true>(c, plan.parts, st) : launch_tiles<true, false>(c, plan.parts, st);
+  }
+  if (c.out.whole) {
     rc = encode_store_tiles(&c.out_map, out_dtype, out, n, m, out_rstride, 32);
     if (rc != GNS_OK) return rc;
   }
