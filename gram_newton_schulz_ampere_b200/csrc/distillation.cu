@@ -15,9 +15,15 @@
 // through shared memory. z - m is formed before it is scaled: z / T would lose the digits
 // that large logits have in common.
 //
+// Logits reach the registers through rings in shared memory, one of each warp, that bulk
+// copies fill three slots of two kilobytes ahead, over the ends of passes and rows: 190 KB under
+// way on an SM whatever the warps wait for.
+//
 // The gradient at the row's entries is written over the dense one behind a barrier, the
 // entries of one index added up by the first of them in the list's order: no atomics.
 #include <algorithm>
+#include <mutex>
+#include <type_traits>
 
 #include "../../include/gns_b200.h"
 #include "gns_common.cuh"
@@ -26,11 +32,15 @@
 namespace gns {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
+__device__ int g_loss_status = 0;
+
 constexpr int kMaxTop = 1024;
-constexpr int kDeep = 4;  // pieces that a thread loads at once
 constexpr int kMaxCluster = 8;
+constexpr int kSlots = 3;                      // of a warp's ring
+constexpr int kSlotPieces = 128;               // 16-byte pieces of a slot
+constexpr int kEach = kSlotPieces / 32;        // of a lane
+constexpr uint32_t kSlotBytes = kSlotPieces * 16;
+constexpr int kWarpsPerSm = 32;
 
 struct LossArgs {
   const void* z;
@@ -72,14 +82,42 @@ template <int XD>
 struct Logits {
   static constexpr int kN = XD == kF32 ? 4 : 8;
   uint4 u;
-  __device__ __forceinline__ float get(int i) const {
+
+  __device__ __forceinline__ Pair pair(int q) const {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    if (XD == kF32) return __uint_as_float(w[i % 4]);
-    const uint32_t two = w[i / 2 % 4];
-    if (XD == kBF16) return __uint_as_float((i & 1) ? (two & 0xffff0000u) : (two << 16));
-    return __half2float(__ushort_as_half(static_cast<uint16_t>((i & 1) ? (two >> 16) : two)));
+    if (XD == kF32) return Pair(__uint_as_float(w[2 * q % 4]), __uint_as_float(w[(2 * q + 1) % 4]));
+    const uint32_t two = w[q % 4];
+    if (XD == kBF16) return Pair(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two));
+    return Pair(f.x, f.y);
+  }
+
+  static __device__ __forceinline__ uint4 minus_infinity() {
+    const uint32_t w = XD == kF32 ? 0xff800000u : (XD == kBF16 ? 0xff80ff80u : 0xfc00fc00u);
+    return make_uint4(w, w, w, w);
   }
 };
+
+// The largest of K pieces' elements that is not a NaN.
+template <int XD, int K>
+__device__ __forceinline__ float largest(const Logits<XD> (&p)[K]) {
+  if (XD == kF32) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < K; ++q)
+      m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(p[q].u.x), __uint_as_float(p[q].u.y)),
+                         fmaxf(__uint_as_float(p[q].u.z), __uint_as_float(p[q].u.w))));
+    return m;
+  }
+  using Two = typename std::conditional<XD == kBF16, __nv_bfloat162, __half2>::type;
+  Two m = *reinterpret_cast<const Two*>(&p[0].u.x);
+#pragma unroll
+  for (int q = 0; q < K; ++q) {
+    const Two* h = reinterpret_cast<const Two*>(&p[q].u);
+    m = __hmax2(m, __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+  }
+  return fmaxf(static_cast<float>(m.x), static_cast<float>(m.y));
+}
 
 template <int XD>
 __device__ __forceinline__ uint4 packed(const float (&v)[XD == kF32 ? 4 : 8]) {
@@ -114,14 +152,18 @@ __device__ __forceinline__ float warp_add(float v) {
 
 // A row's entries in shared memory: the index (-1: left out) and its share p.
 struct Entries {
-  int index[kMaxTop];
-  float p[kMaxTop];
-  float top, log_sum;  // largest t, log of the sum of exp((t - top) / T)
-  int some;            // whether any entry counts
+  int* index;
+  float* p;
+  float* log_sum;  // of exp((t - top) / T); behind it the largest t and whether any entry counts
+  static __host__ __device__ constexpr uint32_t bytes(int top) { return static_cast<uint32_t>((top * 8 + 12 + 15) / 16 * 16); }
+  __device__ __forceinline__ Entries(uint8_t* at, int top)
+      : index(reinterpret_cast<int*>(at)), p(reinterpret_cast<float*>(at) + top), log_sum(reinterpret_cast<float*>(at) + 2 * top) {}
+  __device__ __forceinline__ float& top() const { return log_sum[1]; }
+  __device__ __forceinline__ int& some() const { return reinterpret_cast<int*>(log_sum)[2]; }
 };
 
 // One warp fills a row's entries.
-__device__ __forceinline__ void fill_entries(Entries& e, const LossArgs& a, int64_t row, int lane) {
+__device__ __forceinline__ void fill_entries(const Entries& e, const LossArgs& a, int64_t row, int lane) {
   float top = -INFINITY;
   bool some = false;
   for (int j = lane; j < a.top; j += 32) {
@@ -146,95 +188,213 @@ __device__ __forceinline__ void fill_entries(Entries& e, const LossArgs& a, int6
     e.p[j] = exp2_approx((e.p[j] - at) * a.scale) * inv;
   }
   if (lane == 0) {
-    e.top = at;
-    e.log_sum = logf(sum);
-    e.some = some ? 1 : 0;
+    e.top() = at;
+    *e.log_sum = logf(sum);
+    e.some() = some ? 1 : 0;
   }
 }
 
-// MODE 1: loss. 2: gradient from the statistics of an earlier call. 3: both.
-template <int XD, int MODE>
-__global__ void __launch_bounds__(kThreads, 2) distillation_kernel(const LossArgs a) {
+// What a CTA has of a row: `head` elements up to a multiple of 16 bytes (CTA 0), the pieces
+// [lo, hi) behind them, and what is left at the end (the last CTA).
+template <int XD>
+struct Share {
+  static constexpr int es = XD == kF32 ? 4 : 2;
+  const uint8_t* z;
+  int head, pieces, lo, hi;
+
+  __device__ __forceinline__ Share(const LossArgs& a, int64_t row, uint32_t rank, uint32_t ctas) {
+    z = static_cast<const uint8_t*>(a.z) + row * a.z_stride * es;
+    head = min(a.vocabulary, static_cast<int>((16u - (reinterpret_cast<uintptr_t>(z) & 15u)) & 15u) / es);
+    pieces = (a.vocabulary - head) / (16 / es);
+    lo = static_cast<int>(static_cast<int64_t>(rank) * pieces / ctas);
+    hi = static_cast<int>(static_cast<int64_t>(rank + 1) * pieces / ctas);
+  }
+  __device__ __forceinline__ const uint8_t* body() const { return z + head * es; }
+  __device__ __forceinline__ int slots() const { return (hi - lo + kSlotPieces - 1) / kSlotPieces; }
+};
+
+// A warp's ring. It asks for what the warp will read, in that order: its slots of a row (every
+// W-th), as often as there are passes, then the next row's.
+template <int XD, int W, int PASSES>
+struct WarpRing {
+  uint64_t* full;
+  uint8_t* slots;
+  volatile int* abort_flag;
+  int next = 0, last = 0, under_way = 0;  // slot to be read, slot to be filled, copies not yet read
+  uint32_t phase = 0;
+  // What is asked for next.
+  int64_t row, step;
+  int pass = 0, at, count;
+  const uint8_t* from;
+  int left;  // pieces from `from` on to the end of the CTA's share
+
+  __device__ __forceinline__ void enter(const LossArgs& a, uint32_t rank, uint32_t ctas, int warp) {
+    pass = 0;
+    at = warp;
+    count = 0;
+    if (row >= a.rows) return;
+    const Share<XD> s(a, row, rank, ctas);
+    count = s.slots();
+    from = s.body() + static_cast<int64_t>(s.lo) * 16;
+    left = s.hi - s.lo;
+  }
+
+  // Asks for the next slot; every lane keeps count, the first one copies.
+  __device__ __forceinline__ void fetch(const LossArgs& a, uint32_t rank, uint32_t ctas, int warp, int lane) {
+    while (row < a.rows && at >= count) {
+      at = warp;
+      if (++pass == PASSES || count <= warp) {
+        row += step;
+        enter(a, rank, ctas, warp);
+      }
+    }
+    if (row >= a.rows) return;
+    if (lane == 0) {
+      const uint32_t bytes = static_cast<uint32_t>(min(kSlotPieces, left - at * kSlotPieces)) * 16u;
+      mbar_arrive_expect_tx(&full[last], bytes);
+      bulk_load(slots + last * kSlotBytes, from + static_cast<int64_t>(at) * kSlotBytes, bytes, &full[last]);
+    }
+    last = last + 1 == kSlots ? 0 : last + 1;
+    ++under_way;
+    at += W;
+  }
+
+  __device__ __forceinline__ void wait() const {
+    mbar_wait_bounded(&full[next], (phase >> next) & 1u, abort_flag, &g_loss_status, kStatusProducerTimeout);
+  }
+
+  // The lane's pieces of the slot, of which the first `live` are the row's: the others -inf.
+  __device__ __forceinline__ void read(Logits<XD> (&p)[kEach], int live, int lane) const {
+    wait();
+    const uint4* slot = reinterpret_cast<const uint4*>(slots + next * kSlotBytes);
+    if (live >= kSlotPieces) {
+#pragma unroll
+      for (int q = 0; q < kEach; ++q) p[q].u = slot[lane + 32 * q];
+    } else {
+#pragma unroll
+      for (int q = 0; q < kEach; ++q) p[q].u = lane + 32 * q < live ? slot[lane + 32 * q] : Logits<XD>::minus_infinity();
+    }
+    __syncwarp();
+  }
+
+  __device__ __forceinline__ void done() {
+    phase ^= 1u << next;
+    next = next + 1 == kSlots ? 0 : next + 1;
+    --under_way;
+  }
+
+  // Leaves a row out: what has come of it is thrown away, what has not been asked for is not.
+  __device__ __forceinline__ void skip(const LossArgs& a, int64_t of, int slots_of_row, uint32_t rank, uint32_t ctas, int warp,
+                                       int lane) {
+    int mine = PASSES * (slots_of_row > warp ? (slots_of_row - warp + W - 1) / W : 0);
+    const bool here = row == of;
+    if (here) mine = under_way;
+    for (int i = 0; i < mine; ++i) {
+      wait();
+      done();
+      __syncwarp();
+      if (!here) fetch(a, rank, ctas, warp, lane);
+    }
+    if (here) {
+      row += step;
+      enter(a, rank, ctas, warp);
+      for (int i = 0; i < kSlots; ++i) fetch(a, rank, ctas, warp, lane);
+    }
+  }
+};
+
+// MODE 1: loss. 2: gradient from the statistics of an earlier call. 3: both. W: warps of a CTA.
+template <int XD, int MODE, int W>
+__global__ void __launch_bounds__(32 * W, kWarpsPerSm / W) distillation_kernel(const LossArgs a) {
   constexpr bool kLoss = (MODE & 1) != 0, kGrad = (MODE & 2) != 0;
+  constexpr int kPasses = MODE == 3 ? 2 : 1, kThreads = 32 * W;
   using L = Logits<XD>;
   constexpr int N = L::kN;
   constexpr int es = XD == kF32 ? 4 : 2;
-  __shared__ Entries entries[2];
-  __shared__ float2 warps[2][kWarps];
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float2 warps[2][W];
   __shared__ float2 parts[2][kMaxCluster];
+  __shared__ int aborted;
   const uint32_t rank = cluster_ctarank(), ctas = cluster_nctarank();
-  const int64_t step = gridDim.x / ctas;
+  const int64_t step = gridDim.x / ctas, first = blockIdx.x / ctas;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  uint64_t* barriers = reinterpret_cast<uint64_t*>(smem + W * kSlots * kSlotBytes);
+  uint8_t* lists = smem + W * kSlots * kSlotBytes + (W * kSlots * 8 + 15) / 16 * 16;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < W * kSlots; ++i) mbar_init(&barriers[i], 1);
+    aborted = 0;
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  __syncthreads();
+  WarpRing<XD, W, kPasses> ring;
+  ring.full = barriers + warp * kSlots;
+  ring.slots = smem + warp * kSlots * kSlotBytes;
+  ring.abort_flag = &aborted;
+  ring.row = first;
+  ring.step = step;
+  ring.enter(a, rank, ctas, warp);
+  for (int i = 0; i < kSlots; ++i) ring.fetch(a, rank, ctas, warp, lane);
   int turn = 0, exchange = 0;
-  for (int64_t row = blockIdx.x / ctas; row < a.rows; row += step, turn ^= 1) {
-    const uint8_t* z = static_cast<const uint8_t*>(a.z) + row * a.z_stride * es;
-    // The row: `head` elements up to a multiple of 16 bytes, pieces of 16 bytes, the rest.
-    const int head = min(a.vocabulary, static_cast<int>((16u - (reinterpret_cast<uintptr_t>(z) & 15u)) & 15u) / es);
-    const int pieces = (a.vocabulary - head) / N;
-    const int lo = static_cast<int>(static_cast<int64_t>(rank) * pieces / ctas), hi = static_cast<int>(static_cast<int64_t>(rank + 1) * pieces / ctas);
-    const uint4* body = reinterpret_cast<const uint4*>(z + head * es);
+  if (warp == 0 && first < a.rows) fill_entries(Entries(lists, a.top), a, first, lane);
+  for (int64_t row = first; row < a.rows; row += step, turn ^= 1) {
+    const Share<XD> share(a, row, rank, ctas);
+    const uint8_t* z = share.z;
+    const int slots = share.slots();
     // This thread's element outside the pieces: of the head (CTA 0) or the rest (the last CTA).
-    const int rest = head + pieces * N + static_cast<int>(threadIdx.x) - 32;
-    const int lone = rank == 0 && threadIdx.x < static_cast<unsigned>(head) ? static_cast<int>(threadIdx.x)
+    const int rest = share.head + share.pieces * N + static_cast<int>(threadIdx.x) - 32;
+    const int lone = rank == 0 && threadIdx.x < static_cast<unsigned>(share.head) ? static_cast<int>(threadIdx.x)
                      : rank + 1 == ctas && threadIdx.x >= 32 && rest < a.vocabulary ? rest
                                                                                     : -1;
-    Entries& e = entries[turn];
-    L first[kDeep];
-    if (kLoss) {
-#pragma unroll
-      for (int q = 0; q < kDeep; ++q) {
-        const int i = lo + q * kThreads + static_cast<int>(threadIdx.x);
-        if (i < hi) first[q].u = body[i];
-      }
-    }
-    if (warp == 0) fill_entries(e, a, row, lane);
+    const float alone = lone >= 0 ? load_as_float(z, lone, XD) : 0.0f;
+    const float2 known = kLoss ? make_float2(0.0f, 0.0f) : a.stats[row];
+    const Entries e(lists + turn * Entries::bytes(a.top), a.top);
     __syncthreads();
-    const bool some = e.some != 0;
+    const bool some = e.some() != 0;
     Stat st{-INFINITY, 0.0f};
     if (!some) {
       if (kLoss && rank == 0 && threadIdx.x == 0) {
         a.loss[row] = 0.0f;
         if (a.stats != nullptr) a.stats[row] = make_float2(0.0f, 0.0f);
       }
+      ring.skip(a, row, slots, rank, ctas, warp, lane);
     } else if (kLoss) {
-      for (int i0 = lo; i0 < hi; i0 += kDeep * kThreads) {
-        L now[kDeep];
-#pragma unroll
-        for (int q = 0; q < kDeep; ++q) {
-          now[q] = first[q];
-          const int i = i0 + (kDeep + q) * kThreads + static_cast<int>(threadIdx.x);
-          if (i < hi) first[q].u = body[i];
+      for (int c = warp; c < slots; c += W) {
+        L now[kEach];
+        ring.read(now, share.hi - share.lo - c * kSlotPieces, lane);
+        ring.done();
+        ring.fetch(a, rank, ctas, warp, lane);
+        const float top = largest<XD, kEach>(now);
+        if (top > st.m) {
+          st.s *= exp2_approx((st.m - top) * a.scale);
+          st.m = top;
         }
+        const Pair at(-st.base());
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int q = 0; q < kDeep; ++q) {
-          if (i0 + q * kThreads + static_cast<int>(threadIdx.x) >= hi) continue;
-          float top = now[q].get(0);
+        for (int q = 0; q < kEach; ++q)
 #pragma unroll
-          for (int k = 1; k < N; ++k) top = fmaxf(top, now[q].get(k));
-          if (top > st.m) {
-            st.s *= exp2_approx((st.m - top) * a.scale);
-            st.m = top;
+          for (int k = 0; k < N / 2; ++k) {
+            float x, y;
+            mul2(add2(now[q].pair(k), at), Pair(a.scale)).get(x, y);
+            sum[2 * (q % 2)] += exp2_approx(x);
+            sum[2 * (q % 2) + 1] += exp2_approx(y);
           }
-          const float at = st.base();
-#pragma unroll
-          for (int k = 0; k < N; ++k) st.s += exp2_approx((now[q].get(k) - at) * a.scale);
-        }
+        st.s += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       }
-      if (lone >= 0) {
-        const float v = load_as_float(z, lone, XD);
-        // A NaN leaves the maximum and makes the sum one.
-        st.join(v == v ? v : -INFINITY, v == v ? 1.0f : v, a.scale);
-      }
+      // A NaN leaves the maximum and makes the sum one.
+      if (lone >= 0) st.join(alone == alone ? alone : -INFINITY, alone == alone ? 1.0f : alone, a.scale);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1)
         st.join(__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), a.scale);
       if (lane == 0) warps[turn][warp] = make_float2(st.m, st.s);
       __syncthreads();
-      const float2 one = lane < kWarps ? warps[turn][lane] : make_float2(-INFINITY, 0.0f);
+      const float2 one = lane < W ? warps[turn][lane] : make_float2(-INFINITY, 0.0f);
       st = {one.x, one.y};
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1)
+      for (int o = W / 2; o > 0; o >>= 1)
         st.join(__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), a.scale);
+      st = {__shfl_sync(0xffffffffu, st.m, 0), __shfl_sync(0xffffffffu, st.s, 0)};
       if (ctas > 1) {
         // Two buffers in turn: a CTA writes to one again only behind the barrier of the other's
         // exchange, which every reader of it has passed.
@@ -256,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 2) distillation_kernel(const LossArg
           const int i = e.index[j];
           if (i < 0) continue;
           const float t = load_as_float(a.teacher, row * a.teacher_stride + j, a.teacher_dt);
-          const float log_p = (t - e.top) * inv_t - e.log_sum;
+          const float log_p = (t - e.top()) * inv_t - *e.log_sum;
           const float log_q = (load_as_float(z, i, XD) - st.m) * inv_t - log_s;
           if (e.p[j] != 0.0f) sum = fmaf(e.p[j], log_p - log_q, sum);
         }
@@ -267,43 +427,61 @@ __global__ void __launch_bounds__(kThreads, 2) distillation_kernel(const LossArg
         }
       }
     } else {
-      const float2 known = a.stats[row];
       st = {known.x, known.y};
     }
+    // The next row's entries, while the other warps work on. Everybody is through with the
+    // row before, whose place they take.
+    if (warp == 0 && row + step < a.rows) fill_entries(Entries(lists + (turn ^ 1) * Entries::bytes(a.top), a.top), a, row + step, lane);
     if (!kGrad) continue;
     uint8_t* dz = static_cast<uint8_t*>(a.dz) + row * a.dz_stride * es;
     const float g = some ? a.grad[row] * a.temperature : 0.0f;
-    const float at = st.base(), share = some ? __fdiv_rn(1.0f, st.s) : 0.0f, factor = share * g;
-    auto value = [&](float v) { return exp2_approx((v - at) * a.scale) * factor; };
+    const float at = st.base(), inverse = some ? __fdiv_rn(1.0f, st.s) : 0.0f, factor = inverse * g;
     // Pieces of the gradient lie on 16 bytes where its rows start as the logits' do.
     const bool alike = ((reinterpret_cast<uintptr_t>(dz) ^ reinterpret_cast<uintptr_t>(z)) & 15u) == 0;
-    for (int i0 = lo; i0 < hi; i0 += kDeep * kThreads) {
-      L now[kDeep];
+    for (int c = warp; c < slots; c += W) {
+      const int live = share.hi - share.lo - c * kSlotPieces;
+      uint8_t* to = dz + share.head * es + (static_cast<int64_t>(share.lo) + c * kSlotPieces + lane) * 16;
+      if (!some) {
 #pragma unroll
-      for (int q = 0; q < kDeep; ++q) {
-        const int i = i0 + q * kThreads + static_cast<int>(threadIdx.x);
-        if (i < hi && some) now[q].u = body[i];
+        for (int q = 0; q < kEach; ++q) {
+          if (lane + 32 * q >= live) continue;
+          if (alike) {
+            __stcs(reinterpret_cast<uint4*>(to + 512 * q), make_uint4(0u, 0u, 0u, 0u));
+          } else {
+#pragma unroll
+            for (int k = 0; k < N; ++k) store_from_float(to + 512 * q, k, XD, 0.0f);
+          }
+        }
+        continue;
       }
+      L now[kEach];
+      ring.read(now, live, lane);
+      ring.done();
+      ring.fetch(a, rank, ctas, warp, lane);
 #pragma unroll
-      for (int q = 0; q < kDeep; ++q) {
-        const int i = i0 + q * kThreads + static_cast<int>(threadIdx.x);
-        if (i >= hi) continue;
+      for (int q = 0; q < kEach; ++q) {
         float v[N];
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[k] = some ? value(now[q].get(k)) : 0.0f;
+        for (int k = 0; k < N; k += 2) {
+          float x, y;
+          mul2(add2(now[q].pair(k / 2), Pair(-at)), Pair(a.scale)).get(x, y);
+          mul2(Pair(exp2_approx(x), exp2_approx(y)), Pair(factor)).get(v[k], v[k + 1]);
+        }
+        if (lane + 32 * q >= live) continue;
         if (alike) {
-          *reinterpret_cast<uint4*>(dz + head * es + static_cast<int64_t>(i) * 16) = packed<XD>(v);
+          // Written for a later kernel: the rows that are read again are to stay in L2.
+          __stcs(reinterpret_cast<uint4*>(to + 512 * q), packed<XD>(v));
         } else {
 #pragma unroll
-          for (int k = 0; k < N; ++k) store_from_float(dz, head + static_cast<int64_t>(i) * N + k, XD, v[k]);
+          for (int k = 0; k < N; ++k) store_from_float(to + 512 * q, k, XD, v[k]);
         }
       }
     }
-    if (lone >= 0) store_from_float(dz, lone, XD, some ? value(load_as_float(z, lone, XD)) : 0.0f);
+    if (lone >= 0) store_from_float(dz, lone, XD, some ? exp2_approx((alone - at) * a.scale) * factor : 0.0f);
     __syncthreads();
     if (!some) continue;
     // Entries of this CTA's stretch, each by its first place in the list.
-    const int begin = rank == 0 ? 0 : head + lo * N, end = rank + 1 == ctas ? a.vocabulary : head + hi * N;
+    const int begin = rank == 0 ? 0 : share.head + share.lo * N, end = rank + 1 == ctas ? a.vocabulary : share.head + share.hi * N;
     for (int j = threadIdx.x; j < a.top; j += kThreads) {
       const int i = e.index[j];
       if (i < begin || i >= end) continue;
@@ -315,11 +493,19 @@ __global__ void __launch_bounds__(kThreads, 2) distillation_kernel(const LossArg
         p += e.p[k];
       }
       if (is_first) {
-        const float q = exp2_approx((load_as_float(z, i, XD) - at) * a.scale) * share;
+        const float q = exp2_approx((load_as_float(z, i, XD) - at) * a.scale) * inverse;
         store_from_float(dz, i, XD, (q - p) * g);
       }
     }
   }
+  __syncthreads();
+  if (aborted) settle_for_ns(2000000ull);
+}
+
+constexpr int kManyWarps = 16, kFewWarps = 4;
+
+bool short_rows(int64_t rows, int64_t vocabulary, int dt) {
+  return vocabulary * dtype_size(dt) <= 65536 && rows > 2 * device_sm_count();
 }
 
 // CTAs that share a row: with rows for all SMs, one; else up to eight, each with 8 KB of it at least.
@@ -331,33 +517,70 @@ int row_cluster(int64_t rows, int64_t vocabulary, int dt) {
   return c;
 }
 
-template <int XD, int MODE>
+std::mutex g_mutex;
+
+template <int XD, int MODE, int W>
 int launch(const LossArgs& a, cudaStream_t stream) {
-  const int cluster = row_cluster(a.rows, a.vocabulary, XD);
+  auto kernel = distillation_kernel<XD, MODE, W>;
+  constexpr size_t rings = W * kSlots * kSlotBytes + (W * kSlots * 8 + 15) / 16 * 16;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  if (dev < 0 || dev >= 64) return fail(GNS_ERR_DEVICE, "device index out of range");
+  {
+    static bool ready[64] = {};
+    std::lock_guard<std::mutex> lock(g_mutex);
+    if (!ready[dev]) {
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(rings + 2 * Entries::bytes(kMaxTop)));
+      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(smem)");
+      ready[dev] = true;
+    }
+  }
+  const int cluster = W == kManyWarps ? row_cluster(a.rows, a.vocabulary, XD) : 1;
+  const int resident = kWarpsPerSm / W * device_sm_count() / cluster;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(static_cast<unsigned>(cluster * std::min<int64_t>(a.rows, std::max(1, 2 * device_sm_count() / cluster))));
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3(static_cast<unsigned>(cluster * std::min<int64_t>(a.rows, std::max(1, resident))));
+  cfg.blockDim = dim3(32 * W);
+  cfg.dynamicSmemBytes = rings + 2 * Entries::bytes(a.top);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, distillation_kernel<XD, MODE>, a);
+  e = cudaLaunchKernelEx(&cfg, kernel, a);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? GNS_OK : cuda_fail(e, "distillation loss kernel");
 }
 
+// Warps of a CTA: sixteen for long rows or few of them, four for many short ones.
+template <int XD, int MODE>
+int launch_rows(const LossArgs& a, cudaStream_t stream) {
+  const bool few = short_rows(a.rows, a.vocabulary, XD);
+  return few ? launch<XD, MODE, kFewWarps>(a, stream) : launch<XD, MODE, kManyWarps>(a, stream);
+}
+
 template <int MODE>
 int launch_any(int dt, const LossArgs& a, cudaStream_t stream) {
-  if (dt == kBF16) return launch<kBF16, MODE>(a, stream);
-  if (dt == kF16) return launch<kF16, MODE>(a, stream);
-  return launch<kF32, MODE>(a, stream);
+  if (dt == kBF16) return launch_rows<kBF16, MODE>(a, stream);
+  if (dt == kF16) return launch_rows<kF16, MODE>(a, stream);
+  return launch_rows<kF32, MODE>(a, stream);
 }
 
 }  // namespace
+
+int loss_status(int* status, int clear) {
+  cudaError_t e = cudaMemcpyFromSymbol(status, g_loss_status, sizeof(int));
+  if (e == cudaSuccess && clear && *status != 0) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_loss_status, &zero, sizeof(int));
+  }
+  return e == cudaSuccess ? GNS_OK : cuda_fail(e, "distillation loss status");
+}
+
 }  // namespace gns
 
 using namespace gns;

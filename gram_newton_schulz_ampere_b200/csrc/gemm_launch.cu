@@ -518,6 +518,10 @@ int gns_device_status(int* status, int clear) {
   rc = gns::rms_status(&rms, clear);
   if (rc != GNS_OK) return rc;
   if (*status == 0) *status = rms;
+  int loss = 0;
+  rc = gns::loss_status(&loss, clear);
+  if (rc != GNS_OK) return rc;
+  if (*status == 0) *status = loss;
   return GNS_OK;
 }
 

@@ -114,9 +114,10 @@ int grouped_status(int* status, int clear);
 // The same of the layer norm kernels and of the AdamW kernel for 8-bit states.
 int norm_status(int* status, int clear);
 int states_status(int* status, int clear);
-// The same of the 8-bit products and of the RMS norm.
+// The same of the 8-bit products, of the RMS norm and of the distillation loss.
 int gemm8_status(int* status, int clear);
 int rms_status(int* status, int clear);
+int loss_status(int* status, int clear);
 
 // Fused single-kernel Gram Newton-Schulz chain for matrices whose short side is
 // at most 128 (small_chain.cu). x0 holds the normalised fp16 X and x1 is the
