@@ -36,7 +36,7 @@ __device__ int g_loss_status = 0;
 
 constexpr int kMaxTop = 1024;
 constexpr int kMaxCluster = 8;
-constexpr int kSlots = 3;                      // of a warp's ring
+constexpr int kSlots = 2;                      // of a warp's ring
 constexpr int kSlotPieces = 128;               // 16-byte pieces of a slot
 constexpr int kEach = kSlotPieces / 32;        // of a lane
 constexpr uint32_t kSlotBytes = kSlotPieces * 16;
@@ -150,48 +150,80 @@ __device__ __forceinline__ float warp_add(float v) {
   return v;
 }
 
-// A row's entries in shared memory: the index (-1: left out) and its share p.
+// A row's entries in shared memory: the index (-1: left out), the share p, d = t - the largest
+// t, and the logit z. The gradient at the entries takes the places of d and z once the loss
+// is formed: its index (-1: none to be written) and its value.
 struct Entries {
   int* index;
   float* p;
-  float* log_sum;  // of exp((t - top) / T); behind it the largest t and whether any entry counts
-  static __host__ __device__ constexpr uint32_t bytes(int top) { return static_cast<uint32_t>((top * 8 + 12 + 15) / 16 * 16); }
+  float* d;
+  float* z;
+  float* log_sum;  // of exp(d / T); behind it whether any entry counts
+  static __host__ __device__ constexpr int padded(int top) { return (top + 3) / 4 * 4; }
+  static __host__ __device__ constexpr uint32_t bytes(int top) { return static_cast<uint32_t>(padded(top) * 16 + 16); }
   __device__ __forceinline__ Entries(uint8_t* at, int top)
-      : index(reinterpret_cast<int*>(at)), p(reinterpret_cast<float*>(at) + top), log_sum(reinterpret_cast<float*>(at) + 2 * top) {}
-  __device__ __forceinline__ float& top() const { return log_sum[1]; }
-  __device__ __forceinline__ int& some() const { return reinterpret_cast<int*>(log_sum)[2]; }
+      : index(reinterpret_cast<int*>(at)),
+        p(reinterpret_cast<float*>(at) + padded(top)),
+        d(p + padded(top)),
+        z(d + padded(top)),
+        log_sum(z + padded(top)) {}
+  __device__ __forceinline__ int& some() const { return reinterpret_cast<int*>(log_sum)[1]; }
+  __device__ __forceinline__ int* where() const { return reinterpret_cast<int*>(d); }
 };
 
-// One warp fills a row's entries.
+// One warp fills a row's entries, four of a lane's on their way together.
+template <int XD>
 __device__ __forceinline__ void fill_entries(const Entries& e, const LossArgs& a, int64_t row, int lane) {
+  constexpr int kTogether = 4;
+  const uint8_t* z = static_cast<const uint8_t*>(a.z) + row * a.z_stride * (XD == kF32 ? 4 : 2);
   float top = -INFINITY;
   bool some = false;
-  for (int j = lane; j < a.top; j += 32) {
-    const int64_t at = row * a.index_stride + j;
-    const int64_t i = a.index64 ? static_cast<const int64_t*>(a.index)[at] : static_cast<const int32_t*>(a.index)[at];
-    const bool there = i >= 0 && i < a.vocabulary;
-    const float t = there ? load_as_float(a.teacher, row * a.teacher_stride + j, a.teacher_dt) : -INFINITY;
-    e.index[j] = there ? static_cast<int>(i) : -1;
-    e.p[j] = t;
-    top = fmaxf(top, t);
-    some |= !(t == -INFINITY);  // a NaN counts
+  for (int j0 = lane; j0 < e.padded(a.top); j0 += 32 * kTogether) {
+    int index[kTogether];
+    float t[kTogether], at[kTogether];
+#pragma unroll
+    for (int q = 0; q < kTogether; ++q) {
+      const int j = j0 + 32 * q;
+      index[q] = -1;
+      if (j >= a.top) continue;
+      const int64_t place = row * a.index_stride + j;
+      const int64_t i = a.index64 ? static_cast<const int64_t*>(a.index)[place] : static_cast<const int32_t*>(a.index)[place];
+      if (i >= 0 && i < a.vocabulary) index[q] = static_cast<int>(i);
+    }
+#pragma unroll
+    for (int q = 0; q < kTogether; ++q) {
+      t[q] = index[q] >= 0 ? load_as_float(a.teacher, row * a.teacher_stride + j0 + 32 * q, a.teacher_dt) : -INFINITY;
+      at[q] = index[q] >= 0 ? load_as_float(z, index[q], XD) : 0.0f;
+    }
+#pragma unroll
+    for (int q = 0; q < kTogether; ++q) {
+      const int j = j0 + 32 * q;
+      if (j >= e.padded(a.top)) continue;
+      e.index[j] = t[q] == -INFINITY ? -1 : index[q];  // a share of zero
+      e.d[j] = t[q];
+      e.z[j] = at[q];
+      top = fmaxf(top, t[q]);
+      some |= !(t[q] == -INFINITY);  // a NaN counts
+    }
   }
   top = warp_max(top);
   some = __any_sync(0xffffffffu, some);
-  const float at = top == -INFINITY ? 0.0f : top;
+  const float base = top == -INFINITY ? 0.0f : top;
   float sum = 0.0f;
-  for (int j = lane; j < a.top; j += 32) sum += exp2_approx((e.p[j] - at) * a.scale);
+  for (int j = lane; j < e.padded(a.top); j += 32) {
+    const float d = e.d[j] - base, p = exp2_approx(d * a.scale);
+    e.d[j] = d;
+    e.p[j] = p;
+    sum += p;
+  }
   sum = warp_add(sum);
   const float inv = __fdiv_rn(1.0f, sum);
-  for (int j = lane; j < a.top; j += 32) {
-    if (!some || e.p[j] == -INFINITY) e.index[j] = -1;  // a share of zero
-    e.p[j] = exp2_approx((e.p[j] - at) * a.scale) * inv;
-  }
+  for (int j = lane; j < e.padded(a.top); j += 32) e.p[j] *= inv;
   if (lane == 0) {
-    e.top() = at;
     *e.log_sum = logf(sum);
     e.some() = some ? 1 : 0;
   }
+  __syncwarp();
 }
 
 // What a CTA has of a row: `head` elements up to a multiple of 16 bytes (CTA 0), the pieces
@@ -206,16 +238,17 @@ struct Share {
     z = static_cast<const uint8_t*>(a.z) + row * a.z_stride * es;
     head = min(a.vocabulary, static_cast<int>((16u - (reinterpret_cast<uintptr_t>(z) & 15u)) & 15u) / es);
     pieces = (a.vocabulary - head) / (16 / es);
-    lo = static_cast<int>(static_cast<int64_t>(rank) * pieces / ctas);
-    hi = static_cast<int>(static_cast<int64_t>(rank + 1) * pieces / ctas);
+    // At most 2^26 pieces and 8 CTAs.
+    lo = ctas == 1 ? 0 : static_cast<int>(rank * static_cast<uint32_t>(pieces) / ctas);
+    hi = ctas == 1 ? pieces : static_cast<int>((rank + 1) * static_cast<uint32_t>(pieces) / ctas);
   }
   __device__ __forceinline__ const uint8_t* body() const { return z + head * es; }
   __device__ __forceinline__ int slots() const { return (hi - lo + kSlotPieces - 1) / kSlotPieces; }
 };
 
 // A warp's ring. It asks for what the warp will read, in that order: its slots of a row (every
-// W-th), as often as there are passes, then the next row's.
-template <int XD, int W, int PASSES>
+// S-th), as often as there are passes, then the next row's.
+template <int XD, int S, int PASSES>
 struct WarpRing {
   uint64_t* full;
   uint8_t* slots;
@@ -256,7 +289,7 @@ struct WarpRing {
     }
     last = last + 1 == kSlots ? 0 : last + 1;
     ++under_way;
-    at += W;
+    at += S;
   }
 
   __device__ __forceinline__ void wait() const {
@@ -286,7 +319,7 @@ struct WarpRing {
   // Leaves a row out: what has come of it is thrown away, what has not been asked for is not.
   __device__ __forceinline__ void skip(const LossArgs& a, int64_t of, int slots_of_row, uint32_t rank, uint32_t ctas, int warp,
                                        int lane) {
-    int mine = PASSES * (slots_of_row > warp ? (slots_of_row - warp + W - 1) / W : 0);
+    int mine = PASSES * (slots_of_row > warp ? (slots_of_row - warp + S - 1) / S : 0);
     const bool here = row == of;
     if (here) mine = under_way;
     for (int i = 0; i < mine; ++i) {
@@ -303,217 +336,267 @@ struct WarpRing {
   }
 };
 
-// MODE 1: loss. 2: gradient from the statistics of an earlier call. 3: both. W: warps of a CTA.
+// Barrier `id` of the CTA's named ones: both halves, or the arrival alone.
+template <int THREADS>
+__device__ __forceinline__ void named_sync(int id) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(THREADS) : "memory");
+}
+template <int THREADS>
+__device__ __forceinline__ void named_arrive(int id) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(THREADS) : "memory");
+}
+
+// MODE 1: loss. 2: gradient from the statistics of an earlier call. 3: both.
+// W: warps of a CTA. All but the last stream the logits; the last one has the rows' entries: it
+// reads those of the row after the next, forms the loss, and corrects the gradient at the
+// entries, while the others are at work. They meet once a row, between its passes (kMeet):
+// there the row's statistics are complete, and the next row's entries in place. The streaming
+// warps do not wait for the corrections; they tell when a row's gradient is written (kWritten),
+// and the next meeting comes after its corrections.
 template <int XD, int MODE, int W>
 __global__ void __launch_bounds__(32 * W, kWarpsPerSm / W) distillation_kernel(const LossArgs a) {
   constexpr bool kLoss = (MODE & 1) != 0, kGrad = (MODE & 2) != 0;
-  constexpr int kPasses = MODE == 3 ? 2 : 1, kThreads = 32 * W;
+  constexpr int kPasses = MODE == 3 ? 2 : 1, S = W - 1, kThreads = 32 * W;
+  constexpr int kMeet = 1, kWritten = 2;
   using L = Logits<XD>;
   constexpr int N = L::kN;
   constexpr int es = XD == kF32 ? 4 : 2;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float2 warps[2][W];
+  __shared__ float2 warps[2][S];
   __shared__ float2 parts[2][kMaxCluster];
   __shared__ int aborted;
   const uint32_t rank = cluster_ctarank(), ctas = cluster_nctarank();
   const int64_t step = gridDim.x / ctas, first = blockIdx.x / ctas;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  uint64_t* barriers = reinterpret_cast<uint64_t*>(smem + W * kSlots * kSlotBytes);
-  uint8_t* lists = smem + W * kSlots * kSlotBytes + (W * kSlots * 8 + 15) / 16 * 16;
+  uint64_t* barriers = reinterpret_cast<uint64_t*>(smem + S * kSlots * kSlotBytes);
+  uint8_t* lists = smem + S * kSlots * kSlotBytes + (S * kSlots * 8 + 15) / 16 * 16;
+  auto list = [&](int which) { return Entries(lists + which * Entries::bytes(a.top), a.top); };
   if (threadIdx.x == 0) {
-    for (int i = 0; i < W * kSlots; ++i) mbar_init(&barriers[i], 1);
+    for (int i = 0; i < S * kSlots; ++i) mbar_init(&barriers[i], 1);
     aborted = 0;
     fence_barrier_init();
     fence_proxy_async_smem();
   }
   __syncthreads();
-  WarpRing<XD, W, kPasses> ring;
-  ring.full = barriers + warp * kSlots;
-  ring.slots = smem + warp * kSlots * kSlotBytes;
-  ring.abort_flag = &aborted;
-  ring.row = first;
-  ring.step = step;
-  ring.enter(a, rank, ctas, warp);
-  for (int i = 0; i < kSlots; ++i) ring.fetch(a, rank, ctas, warp, lane);
-  int turn = 0, exchange = 0;
-  if (warp == 0 && first < a.rows) fill_entries(Entries(lists, a.top), a, first, lane);
-  for (int64_t row = first; row < a.rows; row += step, turn ^= 1) {
-    const Share<XD> share(a, row, rank, ctas);
-    const uint8_t* z = share.z;
-    const int slots = share.slots();
-    // This thread's element outside the pieces: of the head (CTA 0) or the rest (the last CTA).
-    const int rest = share.head + share.pieces * N + static_cast<int>(threadIdx.x) - 32;
-    const int lone = rank == 0 && threadIdx.x < static_cast<unsigned>(share.head) ? static_cast<int>(threadIdx.x)
-                     : rank + 1 == ctas && threadIdx.x >= 32 && rest < a.vocabulary ? rest
-                                                                                    : -1;
-    const float alone = lone >= 0 ? load_as_float(z, lone, XD) : 0.0f;
-    const float2 known = kLoss ? make_float2(0.0f, 0.0f) : a.stats[row];
-    const Entries e(lists + turn * Entries::bytes(a.top), a.top);
-    __syncthreads();
-    const bool some = e.some() != 0;
-    Stat st{-INFINITY, 0.0f};
-    if (!some) {
-      if (kLoss && rank == 0 && threadIdx.x == 0) {
-        a.loss[row] = 0.0f;
-        if (a.stats != nullptr) a.stats[row] = make_float2(0.0f, 0.0f);
-      }
-      ring.skip(a, row, slots, rank, ctas, warp, lane);
-    } else if (kLoss) {
-      for (int c = warp; c < slots; c += W) {
-        L now[kEach];
-        ring.read(now, share.hi - share.lo - c * kSlotPieces, lane);
-        ring.done();
-        ring.fetch(a, rank, ctas, warp, lane);
-        const float top = largest<XD, kEach>(now);
-        if (top > st.m) {
-          st.s *= exp2_approx((st.m - top) * a.scale);
-          st.m = top;
+  WarpRing<XD, S, kPasses> ring;
+  if (warp == S) {
+    if (first < a.rows) fill_entries<XD>(list(0), a, first, lane);
+  } else {
+    ring.full = barriers + warp * kSlots;
+    ring.slots = smem + warp * kSlots * kSlotBytes;
+    ring.abort_flag = &aborted;
+    ring.row = first;
+    ring.step = step;
+    ring.enter(a, rank, ctas, warp);
+    for (int i = 0; i < kSlots; ++i) ring.fetch(a, rank, ctas, warp, lane);
+  }
+  __syncthreads();
+  int turn = 0, which = 0, exchange = 0;
+  // A row's statistics from the streaming warps' and, in a cluster, the CTAs'.
+  auto joined = [&]() {
+    const float2 one = lane < S ? warps[turn][lane] : make_float2(-INFINITY, 0.0f);
+    Stat st{one.x, one.y};
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      st.join(__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), a.scale);
+    if (ctas > 1) {
+      // Two buffers in turn: a CTA writes to one again only behind the barrier of the other's
+      // exchange, which every reader of it has passed.
+      if (threadIdx.x < ctas)
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(cluster_addr(&parts[exchange][rank], threadIdx.x)),
+                     "f"(st.m), "f"(st.s)
+                     : "memory");
+      __syncwarp();
+      cluster_sync_all();
+      st = {-INFINITY, 0.0f};
+      for (uint32_t c = 0; c < ctas; ++c) st.join(parts[exchange][c].x, parts[exchange][c].y, a.scale);
+      exchange ^= 1;
+    }
+    return st;
+  };
+
+  if (warp == S) {
+    if (first + step < a.rows) fill_entries<XD>(list(1), a, first + step, lane);
+    for (int64_t row = first; row < a.rows; row += step, turn ^= 1, which = which == 2 ? 0 : which + 1) {
+      const Share<XD> share(a, row, rank, ctas);
+      const Entries e = list(which);
+      const bool some = e.some() != 0;
+      Stat st{-INFINITY, 0.0f};
+      const float2 known = !kLoss && some ? a.stats[row] : make_float2(0.0f, 0.0f);
+      const float g = kGrad && some ? a.grad[row] * a.temperature : 0.0f;
+      named_sync<kThreads>(kMeet);
+      if (!some) {
+        if (kLoss && rank == 0 && lane == 0) {
+          a.loss[row] = 0.0f;
+          if (a.stats != nullptr) a.stats[row] = make_float2(0.0f, 0.0f);
         }
-        const Pair at(-st.base());
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int q = 0; q < kEach; ++q)
-#pragma unroll
-          for (int k = 0; k < N / 2; ++k) {
-            float x, y;
-            mul2(add2(now[q].pair(k), at), Pair(a.scale)).get(x, y);
-            sum[2 * (q % 2)] += exp2_approx(x);
-            sum[2 * (q % 2) + 1] += exp2_approx(y);
+      } else if (kLoss) {
+        st = joined();
+        if (rank == 0) {
+          // log2(e) / T times T is log2(e): exponents are differences over T.
+          const float inv_t = 1.0f / a.temperature, log_s = logf(st.s);
+          float sum = 0.0f;
+          for (int j = lane; j < a.top; j += 32) {
+            if (e.index[j] < 0) continue;
+            const float log_p = e.d[j] * inv_t - *e.log_sum;
+            const float log_q = (e.z[j] - st.m) * inv_t - log_s;
+            if (e.p[j] != 0.0f) sum = fmaf(e.p[j], log_p - log_q, sum);
           }
-        st.s += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          sum = warp_add(sum);
+          if (lane == 0) {
+            a.loss[row] = a.temperature * a.temperature * sum;
+            if (a.stats != nullptr) a.stats[row] = make_float2(st.m, st.s);
+          }
+        }
+      } else {
+        st = {known.x, known.y};
       }
-      // A NaN leaves the maximum and makes the sum one.
-      if (lone >= 0) st.join(alone == alone ? alone : -INFINITY, alone == alone ? 1.0f : alone, a.scale);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1)
-        st.join(__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), a.scale);
-      if (lane == 0) warps[turn][warp] = make_float2(st.m, st.s);
-      __syncthreads();
-      const float2 one = lane < W ? warps[turn][lane] : make_float2(-INFINITY, 0.0f);
-      st = {one.x, one.y};
-#pragma unroll
-      for (int o = W / 2; o > 0; o >>= 1)
-        st.join(__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), a.scale);
-      st = {__shfl_sync(0xffffffffu, st.m, 0), __shfl_sync(0xffffffffu, st.s, 0)};
-      if (ctas > 1) {
-        // Two buffers in turn: a CTA writes to one again only behind the barrier of the other's
-        // exchange, which every reader of it has passed.
-        if (threadIdx.x < ctas)
-          asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(cluster_addr(&parts[exchange][rank], threadIdx.x)),
-                       "f"(st.m), "f"(st.s)
-                       : "memory");
+      if (kGrad && some) {
+        // The gradient at the entries of this CTA's stretch, each by its first place in the list.
         __syncwarp();
-        cluster_sync_all();
-        st = {-INFINITY, 0.0f};
-        for (uint32_t c = 0; c < ctas; ++c) st.join(parts[exchange][c].x, parts[exchange][c].y, a.scale);
-        exchange ^= 1;
-      }
-      if (rank == 0 && warp == 0) {
-        // log2(e) / T times T is log2(e): exponents are differences over T.
-        const float inv_t = 1.0f / a.temperature, log_s = logf(st.s);
-        float sum = 0.0f;
+        const float at = st.base(), inverse = __fdiv_rn(1.0f, st.s);
+        const int begin = rank == 0 ? 0 : share.head + share.lo * N;
+        const int end = rank + 1 == ctas ? a.vocabulary : share.head + share.hi * N;
         for (int j = lane; j < a.top; j += 32) {
           const int i = e.index[j];
-          if (i < 0) continue;
-          const float t = load_as_float(a.teacher, row * a.teacher_stride + j, a.teacher_dt);
-          const float log_p = (t - e.top()) * inv_t - *e.log_sum;
-          const float log_q = (load_as_float(z, i, XD) - st.m) * inv_t - log_s;
-          if (e.p[j] != 0.0f) sum = fmaf(e.p[j], log_p - log_q, sum);
-        }
-        sum = warp_add(sum);
-        if (lane == 0) {
-          a.loss[row] = a.temperature * a.temperature * sum;
-          if (a.stats != nullptr) a.stats[row] = make_float2(st.m, st.s);
+          const bool mine = i >= begin && i < end;
+          int first_place = j;
+          float p = 0.0f;
+          for (int k = 0; k < e.padded(a.top); k += 4) {
+            const int4 four = *reinterpret_cast<const int4*>(e.index + k);
+            if (four.x != i && four.y != i && four.z != i && four.w != i) continue;
+            const int other[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              if (other[q] != i) continue;
+              first_place = min(first_place, k + q);
+              p += e.p[k + q];
+            }
+          }
+          const float q = exp2_approx((e.z[j] - at) * a.scale) * inverse;
+          e.where()[j] = mine && first_place == j ? i : -1;
+          e.z[j] = (q - p) * g;
         }
       }
-    } else {
-      st = {known.x, known.y};
+      if (row + 2 * step < a.rows) fill_entries<XD>(list(which == 0 ? 2 : which - 1), a, row + 2 * step, lane);
+      if (!kGrad) continue;
+      named_sync<kThreads>(kWritten);
+      if (!some) continue;
+      uint8_t* dz = static_cast<uint8_t*>(a.dz) + row * a.dz_stride * es;
+      for (int j = lane; j < a.top; j += 32)
+        if (e.where()[j] >= 0) store_from_float(dz, e.where()[j], XD, e.z[j]);
     }
-    // The next row's entries, while the other warps work on. Everybody is through with the
-    // row before, whose place they take.
-    if (warp == 0 && row + step < a.rows) fill_entries(Entries(lists + (turn ^ 1) * Entries::bytes(a.top), a.top), a, row + step, lane);
-    if (!kGrad) continue;
-    uint8_t* dz = static_cast<uint8_t*>(a.dz) + row * a.dz_stride * es;
-    const float g = some ? a.grad[row] * a.temperature : 0.0f;
-    const float at = st.base(), inverse = some ? __fdiv_rn(1.0f, st.s) : 0.0f, factor = inverse * g;
-    // Pieces of the gradient lie on 16 bytes where its rows start as the logits' do.
-    const bool alike = ((reinterpret_cast<uintptr_t>(dz) ^ reinterpret_cast<uintptr_t>(z)) & 15u) == 0;
-    for (int c = warp; c < slots; c += W) {
-      const int live = share.hi - share.lo - c * kSlotPieces;
-      uint8_t* to = dz + share.head * es + (static_cast<int64_t>(share.lo) + c * kSlotPieces + lane) * 16;
-      if (!some) {
+  } else {
+    for (int64_t row = first; row < a.rows; row += step, turn ^= 1, which = which == 2 ? 0 : which + 1) {
+      const Share<XD> share(a, row, rank, ctas);
+      const uint8_t* z = share.z;
+      const int slots = share.slots();
+      // This thread's element outside the pieces: of the head (CTA 0) or the rest (the last CTA).
+      const int rest = share.head + share.pieces * N + static_cast<int>(threadIdx.x) - 32;
+      const int lone = rank == 0 && threadIdx.x < static_cast<unsigned>(share.head) ? static_cast<int>(threadIdx.x)
+                       : rank + 1 == ctas && threadIdx.x >= 32 && rest < a.vocabulary ? rest
+                                                                                      : -1;
+      const float alone = lone >= 0 ? load_as_float(z, lone, XD) : 0.0f;
+      const float grad = kGrad ? a.grad[row] : 0.0f;
+      const bool some = list(which).some() != 0;
+      Stat st{-INFINITY, 0.0f};
+      if (!kLoss) {
+        const float2 known = a.stats[row];
+        st = {known.x, known.y};
+      }
+      if (!some) ring.skip(a, row, slots, rank, ctas, warp, lane);
+      if (kLoss && some) {
+        for (int c = warp; c < slots; c += S) {
+          L now[kEach];
+          ring.read(now, share.hi - share.lo - c * kSlotPieces, lane);
+          ring.done();
+          ring.fetch(a, rank, ctas, warp, lane);
+          const float top = largest<XD, kEach>(now);
+          if (top > st.m) {
+            st.s *= exp2_approx((st.m - top) * a.scale);
+            st.m = top;
+          }
+          const Pair at(-st.base());
+          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int q = 0; q < kEach; ++q)
+#pragma unroll
+            for (int k = 0; k < N / 2; ++k) {
+              float x, y;
+              mul2(add2(now[q].pair(k), at), Pair(a.scale)).get(x, y);
+              sum[2 * (q % 2)] += exp2_approx(x);
+              sum[2 * (q % 2) + 1] += exp2_approx(y);
+            }
+          st.s += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        }
+        // A NaN leaves the maximum and makes the sum one.
+        if (lone >= 0) st.join(alone == alone ? alone : -INFINITY, alone == alone ? 1.0f : alone, a.scale);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+          st.join(__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), a.scale);
+        if (lane == 0) warps[turn][warp] = make_float2(st.m, st.s);
+      }
+      named_sync<kThreads>(kMeet);
+      if (kLoss && some) st = joined();
+      if (!kGrad) continue;
+      uint8_t* dz = static_cast<uint8_t*>(a.dz) + row * a.dz_stride * es;
+      const float at = st.base(), factor = some ? __fdiv_rn(1.0f, st.s) * (grad * a.temperature) : 0.0f;
+      // Pieces of the gradient lie on 16 bytes where its rows start as the logits' do.
+      const bool alike = ((reinterpret_cast<uintptr_t>(dz) ^ reinterpret_cast<uintptr_t>(z)) & 15u) == 0;
+      for (int c = warp; c < slots; c += S) {
+        const int live = share.hi - share.lo - c * kSlotPieces;
+        uint8_t* to = dz + share.head * es + (static_cast<int64_t>(share.lo) + c * kSlotPieces + lane) * 16;
+        if (!some) {
+#pragma unroll
+          for (int q = 0; q < kEach; ++q) {
+            if (lane + 32 * q >= live) continue;
+            if (alike) {
+              __stcs(reinterpret_cast<uint4*>(to + 512 * q), make_uint4(0u, 0u, 0u, 0u));
+            } else {
+#pragma unroll
+              for (int k = 0; k < N; ++k) store_from_float(to + 512 * q, k, XD, 0.0f);
+            }
+          }
+          continue;
+        }
+        L now[kEach];
+        ring.read(now, live, lane);
+        ring.done();
+        ring.fetch(a, rank, ctas, warp, lane);
 #pragma unroll
         for (int q = 0; q < kEach; ++q) {
+          float v[N];
+#pragma unroll
+          for (int k = 0; k < N; k += 2) {
+            float x, y;
+            mul2(add2(now[q].pair(k / 2), Pair(-at)), Pair(a.scale)).get(x, y);
+            mul2(Pair(exp2_approx(x), exp2_approx(y)), Pair(factor)).get(v[k], v[k + 1]);
+          }
           if (lane + 32 * q >= live) continue;
           if (alike) {
-            __stcs(reinterpret_cast<uint4*>(to + 512 * q), make_uint4(0u, 0u, 0u, 0u));
+            // Written for a later kernel: the rows that are read again are to stay in L2.
+            __stcs(reinterpret_cast<uint4*>(to + 512 * q), packed<XD>(v));
           } else {
 #pragma unroll
-            for (int k = 0; k < N; ++k) store_from_float(to + 512 * q, k, XD, 0.0f);
+            for (int k = 0; k < N; ++k) store_from_float(to + 512 * q, k, XD, v[k]);
           }
         }
-        continue;
       }
-      L now[kEach];
-      ring.read(now, live, lane);
-      ring.done();
-      ring.fetch(a, rank, ctas, warp, lane);
-#pragma unroll
-      for (int q = 0; q < kEach; ++q) {
-        float v[N];
-#pragma unroll
-        for (int k = 0; k < N; k += 2) {
-          float x, y;
-          mul2(add2(now[q].pair(k / 2), Pair(-at)), Pair(a.scale)).get(x, y);
-          mul2(Pair(exp2_approx(x), exp2_approx(y)), Pair(factor)).get(v[k], v[k + 1]);
-        }
-        if (lane + 32 * q >= live) continue;
-        if (alike) {
-          // Written for a later kernel: the rows that are read again are to stay in L2.
-          __stcs(reinterpret_cast<uint4*>(to + 512 * q), packed<XD>(v));
-        } else {
-#pragma unroll
-          for (int k = 0; k < N; ++k) store_from_float(to + 512 * q, k, XD, v[k]);
-        }
-      }
-    }
-    if (lone >= 0) store_from_float(dz, lone, XD, some ? exp2_approx((alone - at) * a.scale) * factor : 0.0f);
-    __syncthreads();
-    if (!some) continue;
-    // Entries of this CTA's stretch, each by its first place in the list.
-    const int begin = rank == 0 ? 0 : share.head + share.lo * N, end = rank + 1 == ctas ? a.vocabulary : share.head + share.hi * N;
-    for (int j = threadIdx.x; j < a.top; j += kThreads) {
-      const int i = e.index[j];
-      if (i < begin || i >= end) continue;
-      float p = 0.0f;
-      bool is_first = true;
-      for (int k = 0; k < a.top; ++k) {
-        if (e.index[k] != i) continue;
-        is_first &= k >= j;
-        p += e.p[k];
-      }
-      if (is_first) {
-        const float q = exp2_approx((load_as_float(z, i, XD) - at) * a.scale) * inverse;
-        store_from_float(dz, i, XD, (q - p) * g);
-      }
+      if (lone >= 0) store_from_float(dz, lone, XD, some ? exp2_approx((alone - at) * a.scale) * factor : 0.0f);
+      __threadfence_block();
+      named_arrive<kThreads>(kWritten);
     }
   }
   __syncthreads();
   if (aborted) settle_for_ns(2000000ull);
 }
 
-constexpr int kManyWarps = 16, kFewWarps = 4;
-
-bool short_rows(int64_t rows, int64_t vocabulary, int dt) {
-  return vocabulary * dtype_size(dt) <= 65536 && rows > 2 * device_sm_count();
-}
-
-// CTAs that share a row: with rows for all SMs, one; else up to eight, each with 8 KB of it at least.
-int row_cluster(int64_t rows, int64_t vocabulary, int dt) {
-  const int sms = device_sm_count();
+// CTAs that share a row: one where there are rows for all CTAs that fit; else up to eight, each
+// with 8 KB of it at least.
+int row_cluster(int64_t rows, int64_t vocabulary, int dt, int ctas) {
   const int64_t bytes = vocabulary * dtype_size(dt);
   int c = 1;
-  while (c < kMaxCluster && rows * c * 2 <= 2 * sms && bytes / (2 * c) >= 8192) c *= 2;
+  while (c < kMaxCluster && rows * c * 2 <= ctas && bytes / (2 * c) >= 8192) c *= 2;
   return c;
 }
 
@@ -522,7 +605,7 @@ std::mutex g_mutex;
 template <int XD, int MODE, int W>
 int launch(const LossArgs& a, cudaStream_t stream) {
   auto kernel = distillation_kernel<XD, MODE, W>;
-  constexpr size_t rings = W * kSlots * kSlotBytes + (W * kSlots * 8 + 15) / 16 * 16;
+  constexpr size_t rings = (W - 1) * kSlots * kSlotBytes + ((W - 1) * kSlots * 8 + 15) / 16 * 16;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
@@ -532,13 +615,14 @@ int launch(const LossArgs& a, cudaStream_t stream) {
     std::lock_guard<std::mutex> lock(g_mutex);
     if (!ready[dev]) {
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               static_cast<int>(rings + 2 * Entries::bytes(kMaxTop)));
+                               static_cast<int>(rings + 3 * Entries::bytes(kMaxTop)));
       if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(smem)");
       ready[dev] = true;
     }
   }
-  const int cluster = W == kManyWarps ? row_cluster(a.rows, a.vocabulary, XD) : 1;
-  const int resident = kWarpsPerSm / W * device_sm_count() / cluster;
+  const int ctas = kWarpsPerSm / W * device_sm_count();
+  const int cluster = W == 4 ? 1 : row_cluster(a.rows, a.vocabulary, XD, ctas);
+  const int resident = ctas / cluster;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -547,7 +631,7 @@ int launch(const LossArgs& a, cudaStream_t stream) {
   attr[0].val.clusterDim.z = 1;
   cfg.gridDim = dim3(static_cast<unsigned>(cluster * std::min<int64_t>(a.rows, std::max(1, resident))));
   cfg.blockDim = dim3(32 * W);
-  cfg.dynamicSmemBytes = rings + 2 * Entries::bytes(a.top);
+  cfg.dynamicSmemBytes = rings + 3 * Entries::bytes(a.top);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
@@ -556,11 +640,11 @@ int launch(const LossArgs& a, cudaStream_t stream) {
   return e == cudaSuccess ? GNS_OK : cuda_fail(e, "distillation loss kernel");
 }
 
-// Warps of a CTA: sixteen for long rows or few of them, four for many short ones.
 template <int XD, int MODE>
 int launch_rows(const LossArgs& a, cudaStream_t stream) {
-  const bool few = short_rows(a.rows, a.vocabulary, XD);
-  return few ? launch<XD, MODE, kFewWarps>(a, stream) : launch<XD, MODE, kManyWarps>(a, stream);
+  if (a.vocabulary * dtype_size(XD) <= 65536 && a.rows > 2 * device_sm_count()) return launch<XD, MODE, 4>(a, stream);
+  if (MODE == 3 && a.vocabulary * dtype_size(XD) > 160 * 1024) return launch<XD, MODE, 32>(a, stream);
+  return launch<XD, MODE, 16>(a, stream);
 }
 
 template <int MODE>

@@ -66,14 +66,15 @@ def check(logits, indices, teacher, temperature=1.0, grad=None):
     loss, statistics = ops.distillation_loss(logits, indices, teacher, temperature)
     both, dlogits = ops.distillation_loss_gradient(grad, logits, indices, teacher, temperature)
     apart = ops.distillation_loss_backward(grad, logits, indices, teacher, statistics, temperature)
-    assert torch.equal(loss, both) and torch.equal(dlogits, apart)
     assert loss.shape == (rows,) and dlogits.shape == logits.shape and dlogits.dtype == logits.dtype
-    excess = ((loss.double() - want).abs() - error).max().item()
-    assert excess <= 0.0, f"loss: largest excess {excess}"
+    # The calls share a row among different numbers of warps, so their sums differ in order.
     rounding = torch.finfo(logits.dtype).eps / 2
     bound = e_dz + rounding * (dz.abs() + e_dz) + (2.0**-25 if logits.dtype == torch.float16 else 1e-37)
-    excess = ((dlogits.double() - dz).abs() - bound).max().item()
-    assert excess <= 0.0, f"gradient: largest excess {excess}"
+    for values, gradient in ((loss, dlogits), (both, apart)):
+        excess = ((values.double() - want).abs() - error).max().item()
+        assert excess <= 0.0, f"loss: largest excess {excess}"
+        excess = ((gradient.double() - dz).abs() - bound).max().item()
+        assert excess <= 0.0, f"gradient: largest excess {excess}"
     return loss, dlogits
 
 
@@ -113,7 +114,8 @@ def test_rows_that_leave_nothing(cuda_device):
     finite = torch.where(torch.isfinite(logits), logits, 0.0)
     grad = torch.rand(8, device=cuda_device) + 0.5
     loss, dlogits = ops.distillation_loss_gradient(grad, logits, indices, teacher, 2.0)
-    want, want_dlogits = check(finite, indices, teacher, 2.0, grad)
+    check(finite, indices, teacher, 2.0, grad)
+    want, want_dlogits = ops.distillation_loss_gradient(grad, finite, indices, teacher, 2.0)
     assert torch.equal(loss, want) and torch.equal(dlogits, want_dlogits)
     for r in (0, 1, 3):
         assert loss[r] == 0 and not dlogits[r].any()
