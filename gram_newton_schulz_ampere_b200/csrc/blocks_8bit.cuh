@@ -32,7 +32,11 @@ struct BlockScale {
   float scale, factor;
   __device__ __forceinline__ explicit BlockScale(float largest) {
     const float top = fmaxf(largest, kLeastTop);
-    scale = __fdiv_rn(top, kE4m3Top);
+    // top / 448 correctly rounded (Markstein's correction of a product with the reciprocal); the
+    // remainder of an infinity is a NaN.
+    constexpr float kInverse = 1.0f / kE4m3Top;
+    const float q = top * kInverse;
+    scale = top == INFINITY ? top : fmaf(fmaf(-q, kE4m3Top, top), kInverse, q);
     factor = __fdiv_rn(kE4m3Top, top);
   }
 };

@@ -4,6 +4,8 @@
 // Sixteen lanes hold a row's block of 128, eight elements each, so that a block's largest
 // magnitude takes four shuffles and the codes of a lane are one store of 8 bytes. Read once,
 // written once: bound by HBM (3 bytes an element for 16-bit inputs).
+#include <type_traits>
+
 #include "../../include/gns_b200.h"
 #include "blocks_8bit.cuh"
 #include "gns_host.h"
@@ -20,78 +22,103 @@ struct QuantArgs {
   int64_t stride;
   int64_t rows;
   int cols, blocks;
+  uint32_t tile_cols;  // row kernel: tiles of 2^shift blocks side by side
+  int shift;
   CodesOut out;
 };
 
-// Eight elements from column c on, zeros past the end.
-template <int XD, bool VEC>
-__device__ __forceinline__ void load8(const QuantArgs& a, int64_t row, int c, float (&v)[8]) {
-  constexpr int es = XD == kF32 ? 4 : 2;
-  const uint8_t* p = static_cast<const uint8_t*>(a.x) + (row * a.stride + c) * es;
-  if (VEC && c + 8 <= a.cols) {
-    uint32_t w[XD == kF32 ? 8 : 4];
+// Eight elements as loaded.
+template <int XD>
+struct Eight {
+  static constexpr int kWords = XD == kF32 ? 8 : 4;
+  uint32_t w[kWords];
+
+  // From column c on, zeros past the end.
+  template <bool VEC>
+  __device__ __forceinline__ void load(const QuantArgs& a, int64_t row, int c) {
+    constexpr int es = XD == kF32 ? 4 : 2;
+    const uint8_t* p = static_cast<const uint8_t*>(a.x) + (row * a.stride + c) * es;
+    if (VEC && c + 8 <= a.cols) {
 #pragma unroll
-    for (int q = 0; q < (XD == kF32 ? 2 : 1); ++q) {
-      const uint4 u = reinterpret_cast<const uint4*>(p)[q];
-      w[4 * q] = u.x; w[4 * q + 1] = u.y; w[4 * q + 2] = u.z; w[4 * q + 3] = u.w;
-    }
+      for (int q = 0; q < kWords / 4; ++q) {
+        const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p) + q);
+        w[4 * q] = u.x; w[4 * q + 1] = u.y; w[4 * q + 2] = u.z; w[4 * q + 3] = u.w;
+      }
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (XD == kF32) {
-        v[i] = __uint_as_float(w[i % (XD == kF32 ? 8 : 4)]);
-      } else if (XD == kBF16) {
-        v[i] = __uint_as_float((i & 1) ? (w[i / 2] & 0xffff0000u) : (w[i / 2] << 16));
-      } else {
-        v[i] = __half2float(__ushort_as_half(static_cast<uint16_t>((i & 1) ? (w[i / 2] >> 16) : w[i / 2])));
+      for (int i = 0; i < 8; ++i) {
+        if (XD == kF32) {
+          w[i % kWords] = c + i < a.cols ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
+        } else {
+          const uint32_t one = c + i < a.cols ? reinterpret_cast<const uint16_t*>(p)[i] : 0u;
+          w[i / 2 % kWords] = i & 1 ? w[i / 2 % kWords] | one << 16 : one;
+        }
       }
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < a.cols ? load_as_float(p, i, XD) : 0.0f;
   }
-}
 
-__device__ __forceinline__ float largest8(const float (&v)[8]) {
-  float top = 0.0f;
+  __device__ __forceinline__ float get(int i) const {
+    if (XD == kF32) return __uint_as_float(w[i % kWords]);
+    const uint32_t two = w[i / 2 % kWords];
+    if (XD == kBF16) return __uint_as_float((i & 1) ? (two & 0xffff0000u) : (two << 16));
+    return __half2float(__ushort_as_half(static_cast<uint16_t>((i & 1) ? (two >> 16) : two)));
+  }
+
+  // The largest magnitude that is not a NaN.
+  __device__ __forceinline__ float largest() const {
+    if (XD != kF32) {
+      using Two = typename std::conditional<XD == kBF16, __nv_bfloat162, __half2>::type;
+      uint32_t m[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
-  return top;
-}
+      for (int q = 0; q < 4; ++q) m[q] = w[q % kWords] & 0x7fff7fffu;
+      const Two* h = reinterpret_cast<const Two*>(m);
+      const Two top = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+      return fmaxf(fmaxf(static_cast<float>(top.x), static_cast<float>(top.y)), 0.0f);
+    }
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(get(i)));
+    return top;
+  }
 
-__device__ __forceinline__ void store8(const QuantArgs& a, int64_t row, int c, const float (&v)[8], float factor) {
-  if (c >= a.out.width) return;
-  uint2 codes;
-  codes.x = e4m3_four(v[0] * factor, v[1] * factor, v[2] * factor, v[3] * factor);
-  codes.y = e4m3_four(v[4] * factor, v[5] * factor, v[6] * factor, v[7] * factor);
-  *reinterpret_cast<uint2*>(a.out.codes + row * a.out.ld + c) = codes;
-}
+  __device__ __forceinline__ void store(const CodesOut& out, int64_t row, int c, float factor) const {
+    if (c >= out.width) return;
+    uint2 codes;
+    codes.x = e4m3_four(get(0) * factor, get(1) * factor, get(2) * factor, get(3) * factor);
+    codes.y = e4m3_four(get(4) * factor, get(5) * factor, get(6) * factor, get(7) * factor);
+    *reinterpret_cast<uint2*>(out.codes + row * out.ld + c) = codes;
+  }
+};
 
+// 64 blocks a CTA: as many of a row as fit 1024 columns, and the rows below them, so that rows
+// are read in stretches of 2 KB and the scales of a block column written in sectors.
 template <int XD, bool VEC>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantArgs a) {
   const int lane16 = threadIdx.x & 15;
-  const int64_t items = a.rows * a.blocks;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kHalves * kRowItems) + threadIdx.x / 16;
-  float v[kRowItems][8];
-  int64_t row[kRowItems];
-  int block[kRowItems];
+  const uint32_t down = blockIdx.x / a.tile_cols, across = blockIdx.x - down * a.tile_cols;
+  const int64_t row0 = static_cast<int64_t>(down) * ((kHalves * kRowItems) >> a.shift);
+  const int block0 = static_cast<int>(across) << a.shift;
+  Eight<XD> v[kRowItems];
 #pragma unroll
   for (int q = 0; q < kRowItems; ++q) {
-    const int64_t item = first + q * kHalves;
-    row[q] = item / a.blocks;
-    block[q] = static_cast<int>(item - row[q] * a.blocks);
-    if (item >= items) continue;
-    load8<XD, VEC>(a, row[q], block[q] * kScaleBlock + lane16 * 8, v[q]);
+    const int item = q * kHalves + static_cast<int>(threadIdx.x / 16);
+    const int64_t row = row0 + (item >> a.shift);
+    const int block = block0 + (item & ((1 << a.shift) - 1));
+    if (row < a.rows && block < a.blocks) v[q].template load<VEC>(a, row, block * kScaleBlock + lane16 * 8);
   }
 #pragma unroll
   for (int q = 0; q < kRowItems; ++q) {
-    const bool live = first + q * kHalves < items;
-    float top = live ? largest8(v[q]) : 0.0f;
+    const int item = q * kHalves + static_cast<int>(threadIdx.x / 16);
+    const int64_t row = row0 + (item >> a.shift);
+    const int block = block0 + (item & ((1 << a.shift) - 1));
+    const bool live = row < a.rows && block < a.blocks;
+    float top = live ? v[q].largest() : 0.0f;
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (!live) continue;
     const BlockScale s(top);
-    store8(a, row[q], block[q] * kScaleBlock + lane16 * 8, v[q], s.factor);
-    if (lane16 == 0) a.out.scales[row[q] * a.out.srow + block[q] * a.out.scol] = s.scale;
+    v[q].store(a.out, row, block * kScaleBlock + lane16 * 8, s.factor);
+    if (lane16 == 0) a.out.scales[row * a.out.srow + block * a.out.scol] = s.scale;
   }
 }
 
@@ -103,17 +130,16 @@ __global__ void __launch_bounds__(kThreads) quantize_blocks_kernel(const QuantAr
   const int64_t row0 = static_cast<int64_t>(blockIdx.x / static_cast<unsigned>(a.blocks)) * kScaleBlock;
   const int block = static_cast<int>(blockIdx.x % static_cast<unsigned>(a.blocks));
   const int c = block * kScaleBlock + (threadIdx.x & 15) * 8;
-  float v[kRows][8];
+  Eight<XD> v[kRows];
   float top = 0.0f;
 #pragma unroll
   for (int q = 0; q < kRows; ++q) {
     const int64_t row = row0 + q * kHalves + threadIdx.x / 16;
-    if (row >= a.rows) continue;
-    load8<XD, VEC>(a, row, c, v[q]);
+    if (row < a.rows) v[q].template load<VEC>(a, row, c);
   }
 #pragma unroll
   for (int q = 0; q < kRows; ++q)
-    if (row0 + q * kHalves + threadIdx.x / 16 < a.rows) top = fmaxf(top, largest8(v[q]));
+    if (row0 + q * kHalves + threadIdx.x / 16 < a.rows) top = fmaxf(top, v[q].largest());
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if ((threadIdx.x & 31) == 0) tops[threadIdx.x / 32] = top;
@@ -124,7 +150,7 @@ __global__ void __launch_bounds__(kThreads) quantize_blocks_kernel(const QuantAr
 #pragma unroll
   for (int q = 0; q < kRows; ++q) {
     const int64_t row = row0 + q * kHalves + threadIdx.x / 16;
-    if (row < a.rows) store8(a, row, c, v[q], s.factor);
+    if (row < a.rows) v[q].store(a.out, row, c, s.factor);
   }
   if (threadIdx.x == 0) a.out.scales[row0 / kScaleBlock * a.out.srow + block * a.out.scol] = s.scale;
 }
@@ -164,14 +190,17 @@ extern "C" int gns_quantize_8bit(int x_dtype, int block_rows, int64_t rows, int6
     return fail(GNS_ERR_LAYOUT, "rows of codes must start on 16 bytes and hold a row");
   const int rc = check_device();
   if (rc != GNS_OK) return rc;
-  const QuantArgs a{x, x_rstride, rows, static_cast<int>(cols), static_cast<int>((cols + kScaleBlock - 1) / kScaleBlock),
-              {static_cast<uint8_t*>(codes), codes_rstride, static_cast<int>(round_up(cols, 16)), scales, scale_rstride,
-               scale_cstride}};
+  const int blocks = static_cast<int>((cols + kScaleBlock - 1) / kScaleBlock);
+  int shift = 0;
+  while (shift < 3 && (1 << shift) < blocks) ++shift;
+  const int64_t tile_cols = (blocks + (1 << shift) - 1) >> shift, tile_rows = (kHalves * kRowItems) >> shift;
+  const QuantArgs a{x, x_rstride, rows, static_cast<int>(cols), blocks, static_cast<uint32_t>(tile_cols), shift,
+                    {static_cast<uint8_t*>(codes), codes_rstride, static_cast<int>(round_up(cols, 16)), scales,
+                     scale_rstride, scale_cstride}};
   const int es = dtype_size(x_dtype);
   const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (x_rstride * es) % 16 == 0;
   const bool square = block_rows != 1;
-  const int64_t ctas = square ? (rows + kScaleBlock - 1) / kScaleBlock * a.blocks
-                              : (rows * a.blocks + kHalves * kRowItems - 1) / (kHalves * kRowItems);
+  const int64_t ctas = square ? (rows + kScaleBlock - 1) / kScaleBlock * blocks : (rows + tile_rows - 1) / tile_rows * tile_cols;
   if (ctas > (1ll << 31) - 1) return fail(GNS_ERR_UNSUPPORTED, "matrix beyond kernel limits");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const unsigned grid = static_cast<unsigned>(ctas);
