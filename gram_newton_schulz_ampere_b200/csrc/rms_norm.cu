@@ -681,9 +681,9 @@ int gns_rms_norm_forward(int x_dtype, int w_dtype, int64_t rows, int64_t cols, c
   clear_error();
   int rc = check_rms(x_dtype, w_dtype, rows, cols);
   if (rc != GNS_OK || rows == 0) return rc;
+  if (y == nullptr) return fail(GNS_ERR_ARGUMENT, "null tensor");
   rc = check_inputs(rows, cols, x, x_rstride, residual, residual_rstride, weight, total, rstd);
   if (rc != GNS_OK) return rc;
-  if (y == nullptr) return fail(GNS_ERR_ARGUMENT, "null tensor");
   RmsArgs a{};
   a.x = x;
   a.x_stride = x_rstride;
