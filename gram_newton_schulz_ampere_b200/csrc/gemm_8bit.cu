@@ -130,8 +130,18 @@ struct Pipe {
     fence_proxy_async_smem();
   }
 
+  // Waits that are not over at once are left to the hardware first, for up to 100 us: lanes that
+  // poll take power and issue slots from those that work (operands of zeros 720 -> 705 us).
   __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int code) const {
-    return mbar_wait_bounded(bar, parity, abort_flag, &g_gemm8_status, code);
+    uint32_t over;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(over)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(100000u)
+        : "memory");
+    return over != 0 || mbar_wait_bounded(bar, parity, abort_flag, &g_gemm8_status, code);
   }
 
   // The producer's end: the products of every stage that it filled are done, so that no
@@ -487,8 +497,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   // blockIdx.x: the CTA's part of the contraction; y: columns of right; z: rows of left.
   const int parts = static_cast<int>(gridDim.x), part = static_cast<int>(blockIdx.x);
   const int row0 = static_cast<int>(blockIdx.z) * 128, col0 = static_cast<int>(blockIdx.y) * 128;
-  const int b_begin = static_cast<int>(static_cast<int64_t>(part) * shape.blocks / parts);
-  const int b_end = static_cast<int>(static_cast<int64_t>(part + 1) * shape.blocks / parts);
+  // Its blocks are every parts-th, so that what the cluster reads at a time lies together in
+  // memory, and tiles begin at different ones, so that not all of them read the same columns
+  // of right, which lie in few of the memory's channels.
+  const int count = (shape.blocks - part + parts - 1) / parts;
+  const int turned = static_cast<int>(blockIdx.y * static_cast<unsigned>(count) / gridDim.y);
+  auto block = [&](int i) {
+    i += turned;
+    return part + (i < count ? i : i - count) * parts;
+  };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   extern __shared__ uint8_t smem_raw[];
@@ -516,7 +533,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       int st = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int b = b_begin; b < b_end; ++b) {
+      for (int i = 0; i < count; ++i) {
+        const int b = block(i);
         ok = pipe.wait(&pipe.done[st], ph ^ 1u, kStatusProducerTimeout);
         if (!ok) break;
         uint8_t* at = smem + st * Cfg::kStageBytes;
@@ -540,7 +558,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const int turn = warp == 1 ? 0 : 1;
       int st = turn, acc = turn;
       uint32_t ph = 0, acc_ph = 0;
-      for (int b = b_begin + turn; b < b_end; b += 2) {
+      for (int i = turn; i < count; i += 2) {
         if (!pipe.wait(&pipe.full[st], ph, kStatusMmaTimeout) ||
             !pipe.wait(&pipe.read[acc], acc_ph ^ 1u, kStatusMmaTimeout))
           break;
@@ -568,30 +586,26 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(64 * half);
     const int mine = quarter * 32 + lane;
-    const float* ls = scales.left + min(row0 + mine, shape.m - 1) * scales.left_rstride + b_begin * scales.left_cstride;
-    const float* rs = scales.right + col0 / kBlock * scales.right_cstride + b_begin * scales.right_rstride;
+    const float* ls = scales.left + min(row0 + mine, shape.m - 1) * scales.left_rstride;
+    const float* rs = scales.right + col0 / kBlock * scales.right_cstride;
     Pair sum[32];
 #pragma unroll
     for (int q = 0; q < 32; ++q) sum[q] = Pair(0.0f);
     // Scales are loaded two blocks ahead of their use.
-    float l0 = *ls, r0 = *rs, l1 = l0, r1 = r0;
-    if (b_end - b_begin > 1) {
-      ls += scales.left_cstride;
-      rs += scales.right_rstride;
-      l1 = *ls;
-      r1 = *rs;
+    float l0 = ls[block(0) * scales.left_cstride], r0 = rs[block(0) * scales.right_rstride], l1 = l0, r1 = r0;
+    if (count > 1) {
+      l1 = ls[block(1) * scales.left_cstride];
+      r1 = rs[block(1) * scales.right_rstride];
     }
     int st = 0, acc = 0;
     uint32_t ph = 0;
-    for (int left = b_end - b_begin; left > 0; --left) {
+    for (int i = 0; i < count; ++i) {
       const Pair scale(l0 * r0);
       l0 = l1;
       r0 = r1;
-      if (left > 2) {
-        ls += scales.left_cstride;
-        rs += scales.right_rstride;
-        l1 = *ls;
-        r1 = *rs;
+      if (i + 2 < count) {
+        l1 = ls[block(i + 2) * scales.left_cstride];
+        r1 = rs[block(i + 2) * scales.right_rstride];
       }
       if (!__all_sync(0xffffffffu, pipe.wait(&pipe.done[st], ph, kStatusEpilogueTimeout))) break;
       tc_fence_after();
@@ -743,8 +757,15 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int parts = static_cast<int>(gridDim.x), part = static_cast<int>(blockIdx.x);
   const int f0 = static_cast<int>(blockIdx.y) * 128, row0 = static_cast<int>(blockIdx.z) * TOK;
   const int rows = min(TOK, shape.m - row0);
-  const int b_begin = static_cast<int>(static_cast<int64_t>(part) * shape.blocks / parts);
-  const int b_end = static_cast<int>(static_cast<int64_t>(part + 1) * shape.blocks / parts);
+  // Its blocks are every parts-th, so that what the cluster reads at a time lies together in
+  // memory, and tiles begin at different ones, so that not all of them read the same columns
+  // of right, which lie in few of the memory's channels.
+  const int count = (shape.blocks - part + parts - 1) / parts;
+  const int turned = static_cast<int>(blockIdx.y * static_cast<unsigned>(count) / gridDim.y);
+  auto block = [&](int i) {
+    i += turned;
+    return part + (i < count ? i : i - count) * parts;
+  };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   extern __shared__ uint8_t smem_raw[];
@@ -776,7 +797,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       int st = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int b = b_begin; b < b_end; ++b) {
+      for (int i = 0; i < count; ++i) {
+        const int b = block(i);
         ok = pipe.wait(&pipe.done[st], ph ^ 1u, kStatusProducerTimeout);
         if (!ok) break;
         uint8_t* at = smem + st * Cfg::kStageBytes;
@@ -798,7 +820,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       const uint32_t idesc = idesc_8bit(M_MN, false, 128, (rows + 15) / 16 * 16);
       int st = 0, acc = 0;
       uint32_t ph = 0, acc_ph = 0;
-      for (int b = b_begin; b < b_end; ++b) {
+      for (int i = 0; i < count; ++i) {
         if (!pipe.wait(&pipe.full[st], ph, kStatusMmaTimeout) ||
             !pipe.wait(&pipe.read[acc], acc_ph ^ 1u, kStatusMmaTimeout))
           break;
@@ -834,7 +856,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     float l[kAhead][kEach], r[kAhead];
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) {
-      const int b = min(b_begin + q, shape.blocks - 1);
+      const int b = block(min(q, count - 1));
       r[q] = rs[b * scales.right_rstride];
 #pragma unroll
       for (int e = 0; e < kEach; ++e) l[q][e] = ls[e][b * scales.left_cstride];
@@ -844,15 +866,15 @@ __global__ void __launch_bounds__(kThreads, 2)
     int st = 0, acc = 0;
     uint32_t ph = 0;
     bool ok = true;
-    for (int b0 = b_begin; b0 < b_end && ok; b0 += kAhead) {
+    for (int i0 = 0; i0 < count && ok; i0 += kAhead) {
 #pragma unroll
       for (int q = 0; q < kAhead; ++q) {
-        if (b0 + q >= b_end || !ok) continue;
+        if (i0 + q >= count || !ok) continue;
         float* now = mine + (q & 1) * Cfg::kHalf;
 #pragma unroll
         for (int e = 0; e < kEach; ++e)
           if (32 * e + lane < Cfg::kHalf) now[32 * e + lane] = l[q][e] * r[q];
-        const int next = min(b0 + q + kAhead, shape.blocks - 1);
+        const int next = block(min(i0 + q + kAhead, count - 1));
         r[q] = rs[next * scales.right_rstride];
 #pragma unroll
         for (int e = 0; e < kEach; ++e) l[q][e] = ls[e][next * scales.left_cstride];
