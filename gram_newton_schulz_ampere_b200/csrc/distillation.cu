@@ -377,7 +377,11 @@ __global__ void __launch_bounds__(32 * W, kWarpsPerSm / W) distillation_kernel(c
     fence_barrier_init();
     fence_proxy_async_smem();
   }
-  __syncthreads();
+  // In a cluster, every CTA has begun before another writes to its shared memory.
+  if (ctas > 1)
+    cluster_sync_all();
+  else
+    __syncthreads();
   WarpRing<XD, S, kPasses> ring;
   if (warp == S) {
     if (first < a.rows) fill_entries<XD>(list(0), a, first, lane);

@@ -1081,15 +1081,15 @@ struct Plan8 {
 // calls whose weights come from HBM, m x k x n:
 //   up to 32 rows, parts 1 / 2 / 4 / 8: doubled while the CTAs are at most two an SM and each
 //   part has two blocks
-//     1 x 4096 x 14336   17.1 / 13.5 / 17.6 / 24.4     1 x 14336 x 4096   44.2 / 24.7 / 15.8 / 13.5
-//     1 x 1024 x 4096    5.7 / 4.7 / 4.1 / 5.0         32 x 8192 x 512    27.6 / 15.8 / 9.6 / 6.8
+//     1 x 4096 x 14336   19.0 / 13.3 / 17.8 / 24.5     1 x 14336 x 4096   49.8 / 27.8 / 17.2 / 14.1
+//     1 x 1024 x 4096    6.2 / 4.9 / 4.2 / 5.0         32 x 8192 x 512    30.9 / 17.4 / 10.5 / 7.3
 //   128-row tiles where there is an SM for each, parts 1 / 2 / 4 against pair tiles: doubled
 //   while there are SMs, to four (clusters of 8 leave SMs of a GPC unused, and the join reads
-//   the sums at 17 bytes a cycle), and each part has eight blocks
-//     96 x 14336 x 4096  53.9 / 31.3 / 21.5, 52.2      96 x 4096 x 14336  20.6 / 25.9 / -, 19.8
-//     256 x 4096 x 4096  19.7 / 13.2 / 20.5, 19.0      256 x 1024 x 4096  7.3 / 7.0 / 14.9, 8.1
-//     96 x 2048 x 512    8.3 / 7.1 / 7.3, 10.8         1024 x 2048 x 2048 9.7 / 15.7 / -, 11.8
-//     1024 x 4096 x 4096 40.2, 19.7
+//   the sums at 17 bytes a cycle), and each part has four blocks
+//     96 x 14336 x 4096  42.9 / 25.0 / 17.4, 51.7      96 x 4096 x 14336  17.8 / 24.5 / -, 20.2
+//     256 x 4096 x 4096  16.8 / 12.2 / 19.6, 18.9      256 x 1024 x 4096  7.9 / 7.2 / 14.4, 8.0
+//     96 x 2048 x 512    9.6 / 7.4 / 6.4, 10.4         1024 x 2048 x 2048 11.3 / 16.5 / -, 11.5
+//     1024 x 4096 x 4096 34.1 / - / -, 20.2
 Plan8 plan8(int64_t m, int64_t n, int64_t blocks) {
   const int sms = device_sm_count();
   const int64_t tiles = (n + 127) / 128;
@@ -1100,7 +1100,7 @@ Plan8 plan8(int64_t m, int64_t n, int64_t blocks) {
   }
   const int64_t all = tiles * ((m + 127) / 128);
   if (all > sms) return {256, 1};
-  while (parts < 4 && all * parts * 2 <= sms && blocks >= 16 * parts) parts *= 2;
+  while (parts < 4 && all * parts * 2 <= sms && blocks >= 8 * parts) parts *= 2;
   return {128, parts};
 }
 
@@ -1128,7 +1128,9 @@ int gns_gemm_8bit(int64_t m, int64_t n, int64_t k, const void* left, int64_t lef
   clear_error();
   if (out_dtype < 0 || out_dtype > 2) return fail(GNS_ERR_ARGUMENT, "bad output dtype");
   if (m < 0 || n < 0 || k < 0) return fail(GNS_ERR_ARGUMENT, "negative dimension");
-  if (m > (1 << 30) || n > (1 << 24) || k > (1 << 24)) return fail(GNS_ERR_UNSUPPORTED, "dimension beyond kernel limits");
+  // A grid has at most 65535 tiles of 128 columns.
+  if (m > (1 << 30) || n > 65535 * 128 || k > (1 << 24) || (m + 255) / 256 * ((n + 255) / 256) > (1 << 30))
+    return fail(GNS_ERR_UNSUPPORTED, "dimension beyond kernel limits");
   if (m == 0 || n == 0) return GNS_OK;
   if (k == 0) return fail(GNS_ERR_UNSUPPORTED, "an 8-bit product needs k > 0");
   if (left == nullptr || right == nullptr || left_scales == nullptr || right_scales == nullptr || out == nullptr)

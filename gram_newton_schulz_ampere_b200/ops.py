@@ -1443,6 +1443,14 @@ def quantize_8bit(x: Tensor, block_rows: int = 1) -> tuple[Tensor, Tensor]:
     return codes, scales
 
 
+def _byte_rows(t: Tensor) -> Tensor:
+    """A copy of the 8-bit matrix `t` whose rows start on multiples of 16 bytes."""
+    rows, columns = t.shape
+    copy = t.new_empty((rows, (columns + 15) // 16 * 16))
+    copy.view(torch.uint8)[:, :columns].copy_(t.view(torch.uint8))
+    return copy
+
+
 def _byte_layout(t: Tensor) -> tuple[Tensor, int, int]:
     """(owner, row stride, column stride) of the 8-bit matrix `t` or of a copy of it, in the same
     order, that TMA can read: a unit stride, the other one a multiple of 16 bytes."""
@@ -1456,10 +1464,8 @@ def _byte_layout(t: Tensor) -> tuple[Tensor, int, int]:
     if sr == 1 and sc != 1:
         held, stride, _ = _byte_layout(t.t())
         return held, 1, stride
-    pitch = (columns + 15) // 16 * 16
-    copy = t.new_empty((rows, pitch))
-    copy.view(torch.uint8)[:, :columns].copy_(t.view(torch.uint8))
-    return copy, pitch, 1
+    copy = _byte_rows(t)
+    return copy, copy.stride(0), 1
 
 
 def gemm_8bit(
@@ -1497,8 +1503,9 @@ def gemm_8bit(
     if m == 0 or n == 0 or k == 0:
         return torch.zeros((m, n), dtype=out_dtype, device=left.device)
     left_held, left_pitch, unit = _byte_layout(left)
-    if unit != 1 and k > 1:
-        left_held, left_pitch, _ = _byte_layout(left.contiguous())
+    if unit != 1:  # held by columns
+        left_held = _byte_rows(left)
+        left_pitch = left_held.stride(0)
     right_held, *right_strides = _byte_layout(right)
     out = left.new_empty((m, n), dtype=out_dtype)
     with nat.on_device(index) as stream:

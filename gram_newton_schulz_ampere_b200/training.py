@@ -112,8 +112,8 @@ def rms_norm(
 
 
 def _check_16_bits(x: Tensor, weight: Tensor) -> None:
-    if weight.ndim != 2 or x.ndim < 1 or x.shape[-1] != weight.shape[1]:
-        raise ValueError("expected x [..., in] and weight [out, in]")
+    if weight.ndim != 2 or weight.numel() == 0 or x.ndim < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError("expected x [..., in] and weight [out, in], neither size zero")
     if x.dtype != weight.dtype or x.dtype not in (torch.float16, torch.bfloat16):
         raise TypeError("x and weight must share dtype float16 or bfloat16")
 

@@ -150,6 +150,21 @@ def test_product_of_operands_anywhere(cuda_device, m):
     assert torch.equal(ops.gemm_8bit(wide.view(torch.float8_e4m3fn), xs, wc.t(), ws.t()), want)
 
 
+@pytest.mark.parametrize("m,k,n", [(5, 1, 7), (1, 1, 1), (200, 1, 1), (1, 20, 1), (40, 3, 1), (300, 16, 300)])
+def test_product_of_thin_operands(cuda_device, m, k, n):
+    """Without padding between rows, by rows and by columns: sizes of one leave strides undetermined."""
+    x = torch.randn(m, k, device=cuda_device)
+    w = torch.randn(n, k, device=cuda_device)
+    xc, xs = ops.quantize_8bit(x)
+    wc, ws = ops.quantize_8bit(w, BLOCK)
+    want = ops.gemm_8bit(xc, xs, wc.t(), ws.t(), out_dtype=torch.float32)
+    left, right = (c.view(torch.uint8).contiguous() for c in (xc, wc))
+    f8 = torch.float8_e4m3fn
+    for a in (left, left.t().contiguous().t()):
+        for b in (right.t(), right.t().contiguous()):
+            assert torch.equal(ops.gemm_8bit(a.view(f8), xs, b.view(f8), ws.t(), out_dtype=torch.float32), want)
+
+
 def test_same_bits_on_every_run(cuda_device):
     for m, k, n in ((1, 4096, 512), (50, 4096, 256), (300, 1024, 600)):
         outs = [product(cuda_device, m, k, n, torch.float32, False, seed=7) for _ in range(3)]

@@ -52,6 +52,8 @@ def test_layers_check_their_arguments():
         training.rms_norm_linear_8bit(x.half(), x[0], x.bfloat16())
     with pytest.raises(ValueError, match="out, in"):
         training.linear_8bit(x.half(), x[:, :64].half())
+    with pytest.raises(ValueError, match="size zero"):
+        training.linear_8bit(x[:, :0].half(), x[:, :0].half())
     index, teacher = torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, 2)
     with pytest.raises(ValueError, match="no gradient"):
         training.distillation_loss(x, index, teacher.requires_grad_())
@@ -68,7 +70,9 @@ def test_native_products_check_their_arguments(library):
     assert "dtype" in failure(library, gemm(dt=3))
     assert "negative" in failure(library, gemm(m=-1))
     assert "k > 0" in failure(library, gemm(k=0))
-    assert "limits" in failure(library, gemm(n=1 << 25))
+    assert "limits" in failure(library, gemm(n=1 << 23, ldd=1 << 23))
+    assert "limits" in failure(library, gemm(k=1 << 25))
+    assert "limits" in failure(library, gemm(m=1 << 30, n=1 << 20, ldd=1 << 20))
     for name in ("left", "ls", "right", "rs", "out"):
         assert "null" in failure(library, gemm(**{name: None}))
     assert "overlap" in failure(library, gemm(ldd=3))
