@@ -1,9 +1,9 @@
 // A matrix in 8 bits with a scale for each block: 1 x 128 (activations and gradients, as the
 // left factor of gns_gemm_8bit) or 128 x 128 (weights, as the right one).
 //
-// Sixteen lanes hold a row's block of 128, eight elements each, so that a block's largest
-// magnitude takes four shuffles and the codes of a lane are one store of 8 bytes. Read once,
-// written once: bound by HBM (3 bytes an element for 16-bit inputs).
+// Read once, written once: bound by HBM (3 bytes an element for 16-bit inputs) and, near it, by
+// the instructions beside the conversions. So eight lanes hold a row's block of 128, twice eight
+// elements each: three shuffles and one pair of divisions serve 16 elements.
 #include <type_traits>
 
 #include "../../include/gns_b200.h"
@@ -15,7 +15,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kHalves = kThreads / 16;
-constexpr int kRowItems = 4;  // blocks of a row kernel's half-warp, loaded together
+constexpr int kRowLanes = 8;                    // of a block in the row kernel
+constexpr int kRowGroups = kThreads / kRowLanes;
+constexpr int kRowItems = 2;                    // blocks of such a group, loaded together
+constexpr int kRowPieces = 16 / kRowLanes;      // of eight elements, in each
 
 struct QuantArgs {
   const void* x;
@@ -94,31 +97,38 @@ struct Eight {
 // are read in stretches of 2 KB and the scales of a block column written in sectors.
 template <int XD, bool VEC>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantArgs a) {
-  const int lane16 = threadIdx.x & 15;
+  const int lane8 = threadIdx.x & (kRowLanes - 1);
   const uint32_t down = blockIdx.x / a.tile_cols, across = blockIdx.x - down * a.tile_cols;
-  const int64_t row0 = static_cast<int64_t>(down) * ((kHalves * kRowItems) >> a.shift);
+  const int64_t row0 = static_cast<int64_t>(down) * ((kRowGroups * kRowItems) >> a.shift);
   const int block0 = static_cast<int>(across) << a.shift;
-  Eight<XD> v[kRowItems];
+  Eight<XD> v[kRowItems][kRowPieces];
 #pragma unroll
   for (int q = 0; q < kRowItems; ++q) {
-    const int item = q * kHalves + static_cast<int>(threadIdx.x / 16);
+    const int item = q * kRowGroups + static_cast<int>(threadIdx.x / kRowLanes);
     const int64_t row = row0 + (item >> a.shift);
     const int block = block0 + (item & ((1 << a.shift) - 1));
-    if (row < a.rows && block < a.blocks) v[q].template load<VEC>(a, row, block * kScaleBlock + lane16 * 8);
+    if (row >= a.rows || block >= a.blocks) continue;
+#pragma unroll
+    for (int i = 0; i < kRowPieces; ++i) v[q][i].template load<VEC>(a, row, block * kScaleBlock + (lane8 + kRowLanes * i) * 8);
   }
 #pragma unroll
   for (int q = 0; q < kRowItems; ++q) {
-    const int item = q * kHalves + static_cast<int>(threadIdx.x / 16);
+    const int item = q * kRowGroups + static_cast<int>(threadIdx.x / kRowLanes);
     const int64_t row = row0 + (item >> a.shift);
     const int block = block0 + (item & ((1 << a.shift) - 1));
     const bool live = row < a.rows && block < a.blocks;
-    float top = live ? v[q].largest() : 0.0f;
+    float top = 0.0f;
+    if (live) {
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      for (int i = 0; i < kRowPieces; ++i) top = fmaxf(top, v[q][i].largest());
+    }
+#pragma unroll
+    for (int o = kRowLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (!live) continue;
     const BlockScale s(top);
-    v[q].store(a.out, row, block * kScaleBlock + lane16 * 8, s.factor);
-    if (lane16 == 0) a.out.scales[row * a.out.srow + block * a.out.scol] = s.scale;
+#pragma unroll
+    for (int i = 0; i < kRowPieces; ++i) v[q][i].store(a.out, row, block * kScaleBlock + (lane8 + kRowLanes * i) * 8, s.factor);
+    if (lane8 == 0) a.out.scales[row * a.out.srow + block * a.out.scol] = s.scale;
   }
 }
 
@@ -193,7 +203,7 @@ extern "C" int gns_quantize_8bit(int x_dtype, int block_rows, int64_t rows, int6
   const int blocks = static_cast<int>((cols + kScaleBlock - 1) / kScaleBlock);
   int shift = 0;
   while (shift < 3 && (1 << shift) < blocks) ++shift;
-  const int64_t tile_cols = (blocks + (1 << shift) - 1) >> shift, tile_rows = (kHalves * kRowItems) >> shift;
+  const int64_t tile_cols = (blocks + (1 << shift) - 1) >> shift, tile_rows = (kRowGroups * kRowItems) >> shift;
   const QuantArgs a{x, x_rstride, rows, static_cast<int>(cols), blocks, static_cast<uint32_t>(tile_cols), shift,
                     {static_cast<uint8_t*>(codes), codes_rstride, static_cast<int>(round_up(cols, 16)), scales,
                      scale_rstride, scale_cstride}};

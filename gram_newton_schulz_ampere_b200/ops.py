@@ -165,7 +165,7 @@ def _gemm_eager(
     symmetric: bool = False,
     out_dtype: torch.dtype | None = None,
 ) -> Tensor:
-    device = _require_cuda(left, right, accumulator)
+    index = _device_index(left, right, accumulator)
     squeeze = left.ndim == 2
     a = _as_batched(left)
     b = _as_batched(right)
@@ -178,7 +178,7 @@ def _gemm_eager(
     if symmetric and m != n:
         raise ValueError("a symmetric product must be square")
     dtype = out_dtype or a.dtype
-    out = torch.empty((batch, m, n), dtype=dtype, device=device)
+    out = left.new_empty((batch, m, n), dtype=dtype)
     if batch == 0 or m == 0 or n == 0:
         return out[0] if squeeze else out
     if k == 0:
@@ -198,7 +198,7 @@ def _gemm_eager(
         if c.stride(-1) != 1 or (batch > 1 and c.stride(0) == 0):
             c = c.contiguous()
     lib = nat.load()
-    with torch.cuda.device(device):
+    with nat.on_device(index) as stream:
         rc = lib.gns_gemm(
             nat.dtype_code(a.dtype), batch, m, n, k,
             a.data_ptr(), a.stride(0), a.stride(1), a.stride(2),
@@ -207,7 +207,7 @@ def _gemm_eager(
             c.stride(0) if c is not None else 0, c.stride(1) if c is not None else 0,
             out.data_ptr(), nat.dtype_code(dtype), out.stride(0), out.stride(1),
             float(alpha), float(beta) if c is not None else 0.0, 1 if symmetric else 0,
-            nat.stream_handle(device),
+            stream,
         )
     nat.check(rc, "gns_gemm")
     return out[0] if squeeze else out
