@@ -6,18 +6,31 @@
 //
 // An entry whose index is not in the vocabulary has no part in a row; a row without entries
 // (or whose entries' logits are all -inf) has a loss and a gradient of zero, whatever its
-// logits hold, and they are not read.
+// logits hold.
 //
 // One pass over a row finds its largest logit m and s = sum exp((z - m) / T) together (each
-// thread rescales its sum when its maximum grows); a second one writes the gradient. A CTA
-// has a row, so that both passes of a call with a gradient run while the row is in L2: it
-// comes from memory once. Few rows: a cluster of CTAs shares a row and exchanges (m, s)
-// through shared memory. z - m is formed before it is scaled: z / T would lose the digits
-// that large logits have in common.
+// thread rescales its sum when its maximum grows); a second one writes the gradient. z - m is
+// formed before it is scaled: z / T would lose the digits that large logits have in common.
+//
+// A CTA has a row, so that both passes of a call with a gradient run while the row is in L2 and
+// it comes from memory once. Rows of more than 160 KB then have an SM each, of 32 warps: with
+// two CTAs an SM, 296 rows on their way, a third of the logits came from memory twice (4096 x
+// 131072 bf16 499 us against 434; 4096 x 65536 the other way round: 233 against 270). Many rows of
+// up to 64 KB have CTAs of four warps (8192 x 8192 bf16 39 us; eight warps 54, sixteen 88).
+// Few rows: a cluster of CTAs shares a row and exchanges (m, s) through shared memory (1 x
+// 131072 bf16: 7 us).
 //
 // Logits reach the registers through rings in shared memory, one of each warp, that bulk
-// copies fill three slots of two kilobytes ahead, over the ends of passes and rows: 190 KB under
-// way on an SM whatever the warps wait for.
+// copies fill two slots of two kilobytes ahead, over the ends of passes and rows: 124 KB under
+// way on an SM whatever the warps wait for. (Loaded to registers four pieces ahead: 4096 x
+// 131072 551 us. Three slots instead of two: 2368 x 131072 fp32, loss alone, 210 us against 181.)
+//
+// What a row's entries ask for is a warp's own work, beside the other warps' passes: read and
+// turned into shares two rows ahead, the loss, and the gradient's corrections (with the teacher
+// and the logits at the entries read when they are needed: 475 us against 434).
+//
+// Bound by HBM: loss alone 5.6 TB/s (bf16) to 7 (fp32), 4096 x 131072 with the gradient 434 us
+// (2.15 GB, 4.95 TB/s): between its two passes a row's SM has less than the rings hold to wait for.
 //
 // The gradient at the row's entries is written over the dense one behind a barrier, the
 // entries of one index added up by the first of them in the list's order: no atomics.
@@ -644,6 +657,7 @@ int launch(const LossArgs& a, cudaStream_t stream) {
   return e == cudaSuccess ? GNS_OK : cuda_fail(e, "distillation loss kernel");
 }
 
+// Warps of a CTA by the row's length (measured at the top of this file).
 template <int XD, int MODE>
 int launch_rows(const LossArgs& a, cudaStream_t stream) {
   if (a.vocabulary * dtype_size(XD) <= 65536 && a.rows > 2 * device_sm_count()) return launch<XD, MODE, 4>(a, stream);

@@ -3,7 +3,9 @@
 //
 // Read once, written once: bound by HBM (3 bytes an element for 16-bit inputs) and, near it, by
 // the instructions beside the conversions. So eight lanes hold a row's block of 128, twice eight
-// elements each: three shuffles and one pair of divisions serve 16 elements.
+// elements each: three shuffles and one division serve 16 elements. 16384 x 4096 bf16: 33 us
+// (6.1 TB/s; with sixteen lanes 43, a block at a time with its place found by divisions 81);
+// 14336 x 4096 in blocks of 128 x 128 29 us (6.1 TB/s); rows that start anywhere 57.
 #include <type_traits>
 
 #include "../../include/gns_b200.h"
