@@ -10,8 +10,8 @@
 // are held in the registers of a group of threads: 32 elements each forward, 16 backward. A
 // row costs one reduction and one barrier of its group; groups of a CTA do not wait for one
 // another. The backward pass sums dw in registers over a group's rows; the sums are joined in
-// a fixed order by a second kernel. Rows that the rings do not hold go to a kernel that
-// reads them from global memory element by element.
+// a fixed order by a second kernel. Rows of more than 16384 elements go to kernels that read
+// them from global memory element by element.
 //
 // Rows that start on 16 bytes are read in pieces of 16 bytes: thread t of a group has the
 // pieces t, t + T, ... of its row, so that a scale's 128 columns lie in 16 neighbouring lanes
@@ -539,7 +539,10 @@ __global__ void __launch_bounds__(32 * kJoinRows) rms_join_kernel(const float* p
   store_from_float(dw, c, dt, s);
 }
 
-// How a call runs: with `stages` >= 2 through rings, else by the wide kernels.
+// How a call runs: with stages through rings, else by the wide kernels. A single stage hides
+// little, but the wide kernels read twice and element by element (4096 fp32 rows with a
+// residual or the stream's gradient, one stage against none: 8192 elements forward 94 us and
+// 252, 14336 forward 151 and 458, backward 222 and 470).
 struct Plan {
   int stages, grid, threads;
   size_t smem;
@@ -555,7 +558,7 @@ Plan plan_rms(int per, int tensors, bool vec, int dt, int64_t rows, int64_t cols
     const int ctas = threads > 256 ? 1 : 2;  // of an SM
     const int64_t stage = static_cast<int64_t>(slot_bytes(vec, cols, dtype_size(dt))) * groups * tensors;
     const int64_t stages = kRingBytes / ctas / stage;
-    if (stages >= 2) {
+    if (stages > 0) {
       p.threads = t;
       p.stages = static_cast<int>(std::min<int64_t>(stages, kMaxStages));
       p.grid = static_cast<int>(std::min<int64_t>((rows + groups - 1) / groups, static_cast<int64_t>(sms) * ctas));
@@ -643,7 +646,7 @@ int forward(int x_dtype, int w_dtype, const RmsArgs& given, int64_t rows, int64_
   const bool vec = vector_rows(a.x, a.x_stride, cols, x_dtype) && vector_rows(a.second, a.second_stride, cols, x_dtype) &&
                    vector_rows(a.total, cols, cols, x_dtype) && vector_rows(a.y, cols, cols, x_dtype);
   const Plan plan = plan_rms(kFwd, a.second != nullptr ? 2 : 1, vec, x_dtype, rows, cols);
-  if (plan.stages >= 2) {
+  if (plan.stages > 0) {
     const int rc = launch_any(false, vec, x_dtype, plan, st, a);
     if (rc != GNS_OK) return rc;
   } else if (a.out8.codes != nullptr) {
@@ -736,7 +739,7 @@ size_t gns_rms_norm_backward_workspace_size(int64_t rows, int64_t cols) {
     for (bool vec : {false, true})
       for (int tensors : {2, 3}) {
         const Plan p = plan_rms(kBwd, tensors, vec, dt, rows, cols);
-        parts = std::max(parts, p.stages >= 2 ? p.grid : wide_parts(rows));
+        parts = std::max(parts, p.stages > 0 ? p.grid : wide_parts(rows));
       }
   return static_cast<size_t>(parts) * static_cast<size_t>(cols) * sizeof(float);
 }
@@ -777,7 +780,7 @@ int gns_rms_norm_backward(int x_dtype, int w_dtype, int64_t rows, int64_t cols, 
     const bool vec = vector_rows(total, total_rstride, cols, x_dtype) && vector_rows(grad, grad_rstride, cols, x_dtype) &&
                      vector_rows(grad_total, grad_total_rstride, cols, x_dtype) && vector_rows(dx, cols, cols, x_dtype);
     const Plan plan = plan_rms(kBwd, grad_total != nullptr ? 3 : 2, vec, x_dtype, rows, cols);
-    if (plan.stages >= 2) {
+    if (plan.stages > 0) {
       parts = plan.grid;
       rc = launch_any(true, vec, x_dtype, plan, st, a);
       if (rc != GNS_OK) return rc;
