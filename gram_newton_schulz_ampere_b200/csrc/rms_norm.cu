@@ -326,6 +326,7 @@ __global__ void __launch_bounds__(threads_of<T>(), threads_of<T>() > 256 ? 1 : 2
 #pragma unroll
     for (int j = 0; j < E / kPer; ++j) {
       const int c0 = P::col(t, j * kPer);  // of the thread's first element in this block
+      if (P::col(t & ~31, j * kPer) >= a.out8.width) continue;  // the warp has none
       float v[kPer];
       float top = 0.0f;
 #pragma unroll
