@@ -84,8 +84,7 @@ struct Stat {
   __device__ __forceinline__ void join(float m2, float s2, float scale) {
     const float top = fmaxf(m, m2);
     const float at = top == -INFINITY ? 0.0f : top;
-    // Not fused, so that both sides of an exchange come to the same bits.
-    s = __fadd_rn(__fmul_rn(s, exp2_approx((m - at) * scale)), __fmul_rn(s2, exp2_approx((m2 - at) * scale)));
+    s = s * exp2_approx((m - at) * scale) + s2 * exp2_approx((m2 - at) * scale);
     m = top;
   }
 };
@@ -161,6 +160,13 @@ __device__ __forceinline__ float warp_add(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
+}
+
+// The lanes' statistics as one: the largest value first, then the sums relative to it. The
+// product is rounded before it is added, so that all lanes come to the same bits.
+__device__ __forceinline__ Stat warp_join(Stat st, float scale) {
+  const Stat all{warp_max(st.m), 0.0f};
+  return {all.m, warp_add(__fmul_rn(st.s, exp2_approx((st.m - all.base()) * scale)))};
 }
 
 // A row's entries in shared memory: the index (-1: left out), the share p, d = t - the largest
@@ -412,10 +418,7 @@ __global__ void __launch_bounds__(32 * W, kWarpsPerSm / W) distillation_kernel(c
   // A row's statistics from the streaming warps' and, in a cluster, the CTAs'.
   auto joined = [&]() {
     const float2 one = lane < S ? warps[turn][lane] : make_float2(-INFINITY, 0.0f);
-    Stat st{one.x, one.y};
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-      st.join(__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), a.scale);
+    Stat st = warp_join(Stat{one.x, one.y}, a.scale);
     if (ctas > 1) {
       // Two buffers in turn: a CTA writes to one again only behind the barrier of the other's
       // exchange, which every reader of it has passed.
@@ -548,9 +551,7 @@ __global__ void __launch_bounds__(32 * W, kWarpsPerSm / W) distillation_kernel(c
         }
         // A NaN leaves the maximum and makes the sum one.
         if (lone >= 0) st.join(alone == alone ? alone : -INFINITY, alone == alone ? 1.0f : alone, a.scale);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-          st.join(__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), a.scale);
+        st = warp_join(st, a.scale);
         if (lane == 0) warps[turn][warp] = make_float2(st.m, st.s);
       }
       named_sync<kThreads>(kMeet);
