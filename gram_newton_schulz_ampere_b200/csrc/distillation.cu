@@ -265,9 +265,20 @@ struct Share {
   __device__ __forceinline__ int slots() const { return (hi - lo + kSlotPieces - 1) / kSlotPieces; }
 };
 
+// A bulk load of what is not read again: the first to leave L2.
+__device__ __forceinline__ void bulk_load_last(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .b64 policy;\n\t"
+      "createpolicy.fractional.L2::evict_first.b64 policy, 1.0;\n\t"
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], policy;\n\t"
+      "}\n" ::"r"(smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
 // A warp's ring. It asks for what the warp will read, in that order: its slots of a row (every
 // S-th), as often as there are passes, then the next row's.
-template <int XD, int S, int PASSES>
+template <int XD, int S, int PASSES, bool LEAVE>
 struct WarpRing {
   uint64_t* full;
   uint8_t* slots;
@@ -304,7 +315,11 @@ struct WarpRing {
     if (lane == 0) {
       const uint32_t bytes = static_cast<uint32_t>(min(kSlotPieces, left - at * kSlotPieces)) * 16u;
       mbar_arrive_expect_tx(&full[last], bytes);
-      bulk_load(slots + last * kSlotBytes, from + static_cast<int64_t>(at) * kSlotBytes, bytes, &full[last]);
+      const uint8_t* piece = from + static_cast<int64_t>(at) * kSlotBytes;
+      if (LEAVE && pass == 1)
+        bulk_load_last(slots + last * kSlotBytes, piece, bytes, &full[last]);
+      else
+        bulk_load(slots + last * kSlotBytes, piece, bytes, &full[last]);
     }
     last = last + 1 == kSlots ? 0 : last + 1;
     ++under_way;
@@ -366,13 +381,14 @@ __device__ __forceinline__ void named_arrive(int id) {
 }
 
 // MODE 1: loss. 2: gradient from the statistics of an earlier call. 3: both.
+// LEAVE: what the second pass has read leaves L2 first.
 // W: warps of a CTA. All but the last stream the logits; the last one has the rows' entries: it
 // reads those of the row after the next, forms the loss, and corrects the gradient at the
 // entries, while the others are at work. They meet once a row, between its passes (kMeet):
 // there the row's statistics are complete, and the next row's entries in place. The streaming
 // warps do not wait for the corrections; they tell when a row's gradient is written (kWritten),
 // and the next meeting comes after its corrections.
-template <int XD, int MODE, int W>
+template <int XD, int MODE, int W, bool LEAVE>
 __global__ void __launch_bounds__(32 * W, kWarpsPerSm / W) distillation_kernel(const LossArgs a) {
   constexpr bool kLoss = (MODE & 1) != 0, kGrad = (MODE & 2) != 0;
   constexpr int kPasses = MODE == 3 ? 2 : 1, S = W - 1, kThreads = 32 * W;
@@ -401,7 +417,7 @@ __global__ void __launch_bounds__(32 * W, kWarpsPerSm / W) distillation_kernel(c
     cluster_sync_all();
   else
     __syncthreads();
-  WarpRing<XD, S, kPasses> ring;
+  WarpRing<XD, S, kPasses, LEAVE> ring;
   if (warp == S) {
     if (first < a.rows) fill_entries<XD>(list(0), a, first, lane);
   } else {
@@ -618,11 +634,17 @@ int row_cluster(int64_t rows, int64_t vocabulary, int dt, int ctas) {
   return c;
 }
 
+// Bytes of rows under way at one time: beyond this L2 has too little room for their gradients,
+// unless what the second pass has read goes first. 2000 x 131072 fp32 (76 MB under way) 458 -> 403
+// us, 2000 x 100000 320 -> 295, 5000 x 32000 bf16 (76 MB) 162 -> 143; below it the hint costs: 4000
+// x 65536 fp32 (38 MB) 377 us, with it 388, 4096 x 131072 bf16 (38 MB) 428 and 434.
+constexpr int64_t kUnderWay = 48ll << 20;
+
 std::mutex g_mutex;
 
-template <int XD, int MODE, int W>
-int launch(const LossArgs& a, cudaStream_t stream) {
-  auto kernel = distillation_kernel<XD, MODE, W>;
+template <int XD, int MODE, int W, bool LEAVE>
+int launch_kernel(const LossArgs& a, int ctas, int cluster, cudaStream_t stream) {
+  auto kernel = distillation_kernel<XD, MODE, W, LEAVE>;
   constexpr size_t rings = (W - 1) * kSlots * kSlotBytes + ((W - 1) * kSlots * 8 + 15) / 16 * 16;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -638,8 +660,6 @@ int launch(const LossArgs& a, cudaStream_t stream) {
       ready[dev] = true;
     }
   }
-  const int ctas = kWarpsPerSm / W * device_sm_count();
-  const int cluster = W == 4 ? 1 : row_cluster(a.rows, a.vocabulary, XD, ctas);
   const int resident = ctas / cluster;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
@@ -656,6 +676,17 @@ int launch(const LossArgs& a, cudaStream_t stream) {
   e = cudaLaunchKernelEx(&cfg, kernel, a);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? GNS_OK : cuda_fail(e, "distillation loss kernel");
+}
+
+template <int XD, int MODE, int W>
+int launch(const LossArgs& a, cudaStream_t stream) {
+  const int ctas = kWarpsPerSm / W * device_sm_count();
+  const int cluster = W == 4 ? 1 : row_cluster(a.rows, a.vocabulary, XD, ctas);
+  if constexpr (MODE == 3) {
+    if (std::min<int64_t>(a.rows, ctas / cluster) * a.vocabulary * dtype_size(XD) > kUnderWay)
+      return launch_kernel<XD, MODE, W, true>(a, ctas, cluster, stream);
+  }
+  return launch_kernel<XD, MODE, W, false>(a, ctas, cluster, stream);
 }
 
 // Warps of a CTA by the row's length (measured at the top of this file).
