@@ -15,8 +15,8 @@
 // A CTA has a row, so that both passes of a call with a gradient run while the row is in L2 and
 // it comes from memory once. Rows of more than 160 KB then have an SM each, of 32 warps: with
 // two CTAs an SM, 296 rows on their way, a third of the logits came from memory twice (4096 x
-// 131072 bf16 499 us against 434; 4096 x 65536 the other way round: 233 against 270). Many rows of
-// up to 64 KB have CTAs of four warps (8192 x 8192 bf16 39 us; eight warps 54, sixteen 88).
+// 131072 bf16 499 us against 434 then; 4096 x 65536 the other way round: 233 against 270). Many rows of
+// up to 64 KB have CTAs of four warps (8192 x 8192 bf16, loss alone, 37 us; eight warps 54, sixteen 88).
 // Few rows: a cluster of CTAs shares a row and exchanges (m, s) through shared memory (1 x
 // 131072 bf16: 7 us).
 //
@@ -27,10 +27,11 @@
 //
 // What a row's entries ask for is a warp's own work, beside the other warps' passes: read and
 // turned into shares two rows ahead, the loss, and the gradient's corrections (with the teacher
-// and the logits at the entries read when they are needed: 475 us against 434).
+// and the logits at the entries read when they are needed: 475 us against 434 then).
 //
-// Bound by HBM: loss alone 5.6 TB/s (bf16) to 7 (fp32), 4096 x 131072 with the gradient 434 us
-// (2.15 GB, 4.95 TB/s): between its two passes a row's SM has less than the rings hold to wait for.
+// Bound by HBM: loss alone 5.6 TB/s (bf16) to 7 (fp32), 4096 x 131072 with the gradient 428 us
+// (2.15 GB, 5.0 TB/s): between its two passes a row's SM has less than the rings hold to wait
+// for. (The next row brought into L2 during the second pass: 474 us.)
 //
 // The gradient at the row's entries is written over the dense one behind a barrier, the
 // entries of one index added up by the first of them in the list's order: no atomics.

@@ -1518,6 +1518,83 @@ def gemm_8bit(
     return out
 
 
+def _quantized(lib, x: Tensor, block_rows: int, stream: int) -> tuple[Tensor, int, int, int, int]:  # type: ignore[no-untyped-def]
+    """``quantize_8bit`` of a 16-bit matrix into one buffer, scales behind the codes, for the calls
+    below, whose host time counts: (buffer, and of codes and scales address and stride)."""
+    rows, columns = x.shape
+    pitch, tall = (columns + 15) // 16 * 16, (rows + block_rows - 1) // block_rows
+    buffer = x.new_empty(rows * pitch + 4 * tall * ((columns + _BLOCK - 1) // _BLOCK), dtype=torch.uint8)
+    codes = buffer.data_ptr()
+    scales = codes + rows * pitch
+    rc = lib.gns_quantize_8bit(
+        nat.DTYPE_CODES[x.dtype], block_rows, rows, columns, x.data_ptr(), x.stride(0), codes, pitch, scales, 1, tall,
+        stream,
+    )
+    nat.check(rc, "gns_quantize_8bit")
+    return buffer, codes, pitch, scales, tall
+
+
+def _linear_8bit(x: Tensor, weight: Tensor) -> tuple[Tensor, Tensor]:
+    """``x @ weight.T`` with both in 8 bits, and the weight's codes and scales for the gradient: the
+    same calls as ``quantize_8bit`` and ``gemm_8bit`` make, with a look at the device and the
+    arguments (16-bit matrices of one type) for all of them."""
+    index = _device_index(x, weight)
+    n, k = weight.shape
+    x, weight = _norm_rows(x, k), _norm_rows(weight, k)
+    m = x.shape[0]
+    y = x.new_empty((m, n))
+    lib = nat.load()
+    with nat.on_device(index) as stream:
+        kept, right, pitch, right_scales, tall = _quantized(lib, weight, _BLOCK, stream)
+        if m > 0:
+            held, left, left_pitch, left_scales, left_tall = _quantized(lib, x, 1, stream)
+            rc = lib.gns_gemm_8bit(
+                m, n, k, left, left_pitch, left_scales, 1, left_tall, right, 1, pitch, right_scales, tall, 1,
+                y.data_ptr(), nat.DTYPE_CODES[x.dtype], n, stream,
+            )
+            nat.check(rc, "gns_gemm_8bit")
+    return y, kept
+
+
+def _linear_8bit_gradient(grad: Tensor, kept: Tensor, n: int, k: int) -> Tensor:
+    """The gradient [m, k] of x in ``_linear_8bit`` from that of its output [m, n]."""
+    index = _device_index(grad, kept)
+    grad = _norm_rows(grad, n)
+    m = grad.shape[0]
+    dx = grad.new_empty((m, k))
+    if m == 0:
+        return dx
+    pitch = (k + 15) // 16 * 16
+    right = kept.data_ptr()
+    lib = nat.load()
+    with nat.on_device(index) as stream:
+        held, left, left_pitch, left_scales, left_tall = _quantized(lib, grad, 1, stream)
+        rc = lib.gns_gemm_8bit(
+            m, k, n, left, left_pitch, left_scales, 1, left_tall, right, pitch, 1, right + n * pitch, 1,
+            (n + _BLOCK - 1) // _BLOCK, dx.data_ptr(), nat.DTYPE_CODES[grad.dtype], k, stream,
+        )
+        nat.check(rc, "gns_gemm_8bit")
+    return dx
+
+
+def _rows_product(left: Tensor, right: Tensor) -> Tensor:
+    """``gemm(left.t(), right)`` of 16-bit matrices [rows, a] and [rows, b], rows > 0, as the
+    gradients of linear layers have them."""
+    index = _device_index(left, right)
+    (rows, a), b = left.shape, right.shape[1]
+    left, left_place, left_pitch = _row_layout(left)
+    right, right_place, right_pitch = _row_layout(right)
+    out = left.new_empty((a, b))
+    code = nat.DTYPE_CODES[left.dtype]
+    with nat.on_device(index) as stream:
+        rc = nat.load().gns_gemm(
+            code, 1, a, b, rows, left_place, rows * left_pitch, 1, left_pitch, right_place, rows * right_pitch,
+            right_pitch, 1, None, 0, 0, 0, out.data_ptr(), code, a * b, b, 1.0, 0.0, 0, stream,
+        )
+    nat.check(rc, "gns_gemm")
+    return out
+
+
 # --------------------------------------------------------------------- RMS norm
 def _rms_check(x: Tensor, weight: Tensor, residual: Tensor | None) -> int:
     columns = _norm_check(x, weight, None)

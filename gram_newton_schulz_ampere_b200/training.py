@@ -122,28 +122,28 @@ def _weight_gradient(grad: Tensor, x: Tensor) -> Tensor:
     """``grad.T @ x`` of 16-bit matrices [rows, out] and [rows, in]."""
     if grad.shape[0] == 0:
         return grad.new_zeros((grad.shape[1], x.shape[1]))
-    return ops.gemm(ops.row_operand(grad).t(), ops.row_operand(x))
+    return ops._rows_product(grad, x)
 
 
 class _Linear8bit(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, weight: Tensor) -> Tensor:  # type: ignore[no-untyped-def]
-        rows = x.reshape(-1, weight.shape[1])
-        codes, scales = ops.quantize_8bit(weight, 128)
-        ctx.save_for_backward(x, codes, scales)
-        y = ops.gemm_8bit(*ops.quantize_8bit(rows), codes.t(), scales.t(), out_dtype=x.dtype)
-        return y.view(*x.shape[:-1], weight.shape[0])
+        y, kept = ops._linear_8bit(x, weight)
+        ctx.save_for_backward(x, kept)
+        ctx.shape = n, _ = weight.shape
+        return y if x.ndim == 2 else y.view(*x.shape[:-1], n)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad: Tensor):  # type: ignore[no-untyped-def]
-        x, codes, scales = ctx.saved_tensors
-        grad = grad.reshape(-1, codes.shape[0])
+        x, kept = ctx.saved_tensors
+        n, k = ctx.shape
+        grad = grad.reshape(-1, n)
         dx = dweight = None
         if ctx.needs_input_grad[0]:
-            dx = ops.gemm_8bit(*ops.quantize_8bit(grad), codes, scales, out_dtype=x.dtype).view(x.shape)
+            dx = ops._linear_8bit_gradient(grad, kept, n, k).view(x.shape)
         if ctx.needs_input_grad[1]:
-            dweight = _weight_gradient(grad, x.reshape(-1, codes.shape[1]))
+            dweight = _weight_gradient(grad, x.reshape(-1, k))
         return dx, dweight
 
 

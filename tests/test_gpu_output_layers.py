@@ -109,6 +109,36 @@ def test_linear_8bit_views_and_frozen_factors(gen):
     assert empty.shape == (0, 70)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,k,n", [(1, 1, 1), (1, 5, 130), (37, 129, 1), (300, 1, 70), (65, 257, 131), (129, 512, 384)])
+def test_linear_8bit_is_its_parts(gen, rows, k, n, dtype):
+    """The layer makes the calls that a user may make one by one: the same bits."""
+    x = normal(gen, rows, k).to(dtype).requires_grad_()
+    w = normal(gen, n, k).to(dtype).requires_grad_()
+    dy = normal(gen, rows, n).to(dtype)
+    y = linear_8bit(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    codes, scales = ops.quantize_8bit(w.detach(), BLOCK)
+    assert torch.equal(y, ops.gemm_8bit(*ops.quantize_8bit(x.detach()), codes.t(), scales.t(), out_dtype=dtype))
+    assert torch.equal(dx, ops.gemm_8bit(*ops.quantize_8bit(dy), codes, scales, out_dtype=dtype))
+    assert torch.equal(dw, ops.gemm(ops.row_operand(dy).t(), ops.row_operand(x.detach())))
+
+
+def test_linear_8bit_rows_that_start_anywhere(gen):
+    """One row with an odd stride, rows from an odd address, a weight's columns out of a wider matrix."""
+    wide = normal(gen, 9, 141).bfloat16()
+    w = normal(gen, 50, 300).bfloat16()[:, 7:136].requires_grad_()
+    for x in (wide[3:4, 5:134], wide[:, 1:130], wide.t()[:129].t()):
+        x = x.detach().requires_grad_()
+        assert not x.is_contiguous() or x.shape[0] == 1
+        y = linear_8bit(x, w)
+        got = torch.autograd.grad(y, (x, w), torch.ones_like(y))
+        x2, w2 = x.detach().clone().requires_grad_(), w.detach().contiguous().requires_grad_()
+        y2 = linear_8bit(x2, w2)
+        want = torch.autograd.grad(y2, (x2, w2), torch.ones_like(y2))
+        assert torch.equal(y, y2) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_rms_norm_linear_8bit(gen):
     """The norm and the product in one, against the same of the operators and the gradients' formulas."""
     x, r = (normal(gen, 130, 384).bfloat16().requires_grad_() for _ in range(2))
