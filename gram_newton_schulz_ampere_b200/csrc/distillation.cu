@@ -737,6 +737,8 @@ extern "C" int gns_distillation_loss(int z_dtype, int64_t rows, int64_t vocabula
   if (loss == nullptr && (dlogits == nullptr || stats == nullptr))
     return fail(GNS_ERR_ARGUMENT, "a call returns a loss, or a gradient from an earlier call's statistics");
   if ((dlogits == nullptr) != (grad == nullptr)) return fail(GNS_ERR_ARGUMENT, "grad and dlogits come together");
+  // A row's pair is one access.
+  if (reinterpret_cast<uintptr_t>(stats) % 8 != 0) return fail(GNS_ERR_LAYOUT, "statistics must start on 8 bytes");
   if (rows > 1 && (logits_rstride < vocabulary || (dlogits != nullptr && dlogits_rstride < vocabulary)))
     return fail(GNS_ERR_LAYOUT, "row stride below the row length");
   const int rc = check_device();

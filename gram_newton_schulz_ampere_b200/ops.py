@@ -1767,6 +1767,8 @@ def distillation_loss_backward(
     g = _row_values(grad, z.shape[0], "grad")
     if statistics.dtype != torch.float32 or statistics.shape != (z.shape[0], 2) or not statistics.is_contiguous():
         raise ValueError("statistics must be contiguous float32 [rows, 2]")
+    if statistics.data_ptr() % 8 != 0:  # the kernel reads a row's pair at once
+        statistics = statistics.clone()
     dlogits = torch.empty_like(z, memory_format=torch.contiguous_format)
     _distillation(z, index, t, temperature, g, None, statistics, dlogits)
     return dlogits

@@ -472,7 +472,8 @@ GNS_API int gns_rms_norm_backward(int x_dtype, int w_dtype, int64_t rows, int64_
  * logits only) has a loss and a gradient of zero. top <= 1024, T in [1e-4, 1e4].
  * With grad (fp32, one value a row) and dlogits: dlogits = grad T (q - p), of the logits' type.
  * stats (fp32, two values a row: the largest logit and the sum of exponentials) is written
- * with the loss where it is not NULL; with loss NULL the gradient is formed from it.
+ * with the loss where it is not NULL; with loss NULL the gradient is formed from it. It starts
+ * on 8 bytes.
  * logits, indices, teacher and dlogits have unit column stride.
  * No counterpart in the reference. */
 GNS_API int gns_distillation_loss(int z_dtype, int64_t rows, int64_t vocabulary, int64_t top, const void* logits,
