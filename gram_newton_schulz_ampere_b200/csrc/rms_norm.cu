@@ -156,12 +156,18 @@ __device__ __forceinline__ void group_barrier(int group) {
     asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(T) : "memory");
 }
 
-// The sum over a group, in each of its threads. `slot` alternates between two buffers, so
-// that one barrier is enough: a buffer is written again only behind the other's barrier.
+// The sum over a group, in each of its threads, behind a barrier of the group, on which the
+// refilling of the ring relies. `slot` alternates between two buffers, so that one barrier is
+// enough: a buffer is written again only behind the other's barrier.
 template <int T>
 __device__ __forceinline__ float group_sum(float v, float* slots, int group, int& slot) {
   v = warp_sum(v);
-  if (T == 32) return v;
+  if (T == 32) {
+    // Shuffles order no accesses to shared memory, and the backward pass reads a third row of
+    // the slot that does not enter the sum: every lane has read the slot only behind this.
+    group_barrier<T>(group);
+    return v;
+  }
   constexpr int kW = T / 32;
   float* buf = slots + slot * 32 + group * kW;
   slot ^= 1;
