@@ -129,7 +129,10 @@ class _Linear8bit(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, weight: Tensor) -> Tensor:  # type: ignore[no-untyped-def]
         y, kept = ops._linear_8bit(x, weight)
-        ctx.save_for_backward(x, kept)
+        # x serves the weight's gradient, the weight's codes that of x.
+        needs_x, needs_weight = ctx.needs_input_grad
+        ctx.save_for_backward(x if needs_weight else None, kept if needs_x else None)
+        ctx.x_shape = x.shape
         ctx.shape = n, _ = weight.shape
         return y if x.ndim == 2 else y.view(*x.shape[:-1], n)
 
@@ -141,7 +144,7 @@ class _Linear8bit(torch.autograd.Function):
         grad = grad.reshape(-1, n)
         dx = dweight = None
         if ctx.needs_input_grad[0]:
-            dx = ops._linear_8bit_gradient(grad, kept, n, k).view(x.shape)
+            dx = ops._linear_8bit_gradient(grad, kept, n, k).view(ctx.x_shape)
         if ctx.needs_input_grad[1]:
             dweight = _weight_gradient(grad, x.reshape(-1, k))
         return dx, dweight
@@ -165,9 +168,13 @@ class _RmsNormLinear8bit(torch.autograd.Function):
         normed, scale, total, rstd = ops.rms_norm_8bit(x, norm_weight, residual, epsilon)
         codes, scales = ops.quantize_8bit(weight, 128)
         y = ops.gemm_8bit(normed, scale, codes.t(), scales.t(), out_dtype=x.dtype)
-        ctx.save_for_backward(total, norm_weight, rstd, codes, scales)
+        # The weight's gradient takes the stream and the norm's weight; all others pass through the product.
+        needs = ctx.needs_input_grad
+        through = (rstd, codes, scales) if needs[0] or needs[1] or needs[3] else (None, None, None)
+        ctx.save_for_backward(total, norm_weight, *through)
         ctx.set_materialize_grads(False)
         ctx.epsilon = epsilon
+        ctx.shape = weight.shape
         y = y.view(*x.shape[:-1], weight.shape[0])
         return y if residual is None else (y, total)
 
@@ -176,16 +183,17 @@ class _RmsNormLinear8bit(torch.autograd.Function):
     def backward(ctx, grad, grad_total=None):  # type: ignore[no-untyped-def]
         total, norm_weight, rstd, codes, scales = ctx.saved_tensors
         needs = ctx.needs_input_grad
+        n, k = ctx.shape
         dx, dnorm, dweight = grad_total, None, None
         if grad is not None:
-            grad = grad.reshape(-1, codes.shape[0])
+            grad = grad.reshape(-1, n)
             if needs[0] or needs[1] or needs[3]:
                 inner = ops.gemm_8bit(*ops.quantize_8bit(grad), codes, scales, out_dtype=total.dtype)
                 dx, dnorm = ops.rms_norm_backward(inner.view(total.shape), total, norm_weight, rstd, grad_total)
             if needs[2]:
                 # The norm is made again in 16 bits: cheaper than keeping it.
                 normed = ops.rms_norm(total, norm_weight, None, ctx.epsilon)[0]
-                dweight = _weight_gradient(grad, normed.view(-1, codes.shape[1]))
+                dweight = _weight_gradient(grad, normed.view(-1, k))
         return dx if needs[0] else None, dnorm if needs[1] else None, dweight, dx if needs[3] else None, None
 
 
