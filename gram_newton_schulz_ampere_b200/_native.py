@@ -171,6 +171,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [_I64, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, c_int, _I64, _P],
     ),
+    "gns_gemm_8bit_plan": (c_int, [_I64, _I64, _I64, ctypes.POINTER(c_int), ctypes.POINTER(c_int)]),
     "gns_quantize_8bit": (c_int, [c_int, c_int, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _P]),
     "gns_rms_norm_forward": (
         c_int,

@@ -1104,6 +1104,14 @@ Plan8 plan8(int64_t m, int64_t n, int64_t blocks) {
   return {128, parts};
 }
 
+int check_sizes(int64_t m, int64_t n, int64_t k) {
+  if (m < 0 || n < 0 || k < 0) return fail(GNS_ERR_ARGUMENT, "negative dimension");
+  // A grid has at most 65535 tiles of 128 columns.
+  if (m > (1 << 30) || n > 65535 * 128 || k > (1 << 24) || (m + 255) / 256 * ((n + 255) / 256) > (1 << 30))
+    return fail(GNS_ERR_UNSUPPORTED, "dimension beyond kernel limits");
+  return GNS_OK;
+}
+
 }  // namespace
 
 int gemm8_status(int* status, int clear) {
@@ -1121,17 +1129,28 @@ using namespace gns;
 
 extern "C" {
 
+int gns_gemm_8bit_plan(int64_t m, int64_t n, int64_t k, int* tile_rows, int* parts) {
+  clear_error();
+  int rc = check_sizes(m, n, k);
+  if (rc != GNS_OK) return rc;
+  if (m == 0 || n == 0 || k == 0) return fail(GNS_ERR_UNSUPPORTED, "an empty product has no plan");
+  if (tile_rows == nullptr || parts == nullptr) return fail(GNS_ERR_ARGUMENT, "null result");
+  rc = check_device();
+  if (rc != GNS_OK) return rc;
+  const Plan8 plan = plan8(m, n, (k + kBlock - 1) / kBlock);
+  *tile_rows = plan.rows;
+  *parts = plan.parts;
+  return GNS_OK;
+}
+
 int gns_gemm_8bit(int64_t m, int64_t n, int64_t k, const void* left, int64_t left_rstride, const float* left_scales,
                   int64_t left_scale_rstride, int64_t left_scale_cstride, const void* right, int64_t right_rstride,
                   int64_t right_cstride, const float* right_scales, int64_t right_scale_rstride,
                   int64_t right_scale_cstride, void* out, int out_dtype, int64_t out_rstride, gns_stream_t stream) {
   clear_error();
   if (out_dtype < 0 || out_dtype > 2) return fail(GNS_ERR_ARGUMENT, "bad output dtype");
-  if (m < 0 || n < 0 || k < 0) return fail(GNS_ERR_ARGUMENT, "negative dimension");
-  // A grid has at most 65535 tiles of 128 columns.
-  if (m > (1 << 30) || n > 65535 * 128 || k > (1 << 24) || (m + 255) / 256 * ((n + 255) / 256) > (1 << 30))
-    return fail(GNS_ERR_UNSUPPORTED, "dimension beyond kernel limits");
-  if (m == 0 || n == 0) return GNS_OK;
+  int rc = check_sizes(m, n, k);
+  if (rc != GNS_OK || m == 0 || n == 0) return rc;
   if (k == 0) return fail(GNS_ERR_UNSUPPORTED, "an 8-bit product needs k > 0");
   if (left == nullptr || right == nullptr || left_scales == nullptr || right_scales == nullptr || out == nullptr)
     return fail(GNS_ERR_ARGUMENT, "null tensor");
@@ -1139,7 +1158,7 @@ int gns_gemm_8bit(int64_t m, int64_t n, int64_t k, const void* left, int64_t lef
   const bool k_major = (right_rstride == 1 || k == 1) && (right_cstride % 16 == 0 || n == 1);
   if (!k_major && !((right_cstride == 1 || n == 1) && (right_rstride % 16 == 0 || k == 1)))
     return fail(GNS_ERR_LAYOUT, "right needs a unit stride along rows or columns and 16-byte multiples along the other");
-  int rc = check_device();
+  rc = check_device();
   if (rc != GNS_OK) return rc;
   Call8 c{};
   c.scales = {left_scales, right_scales, left_scale_rstride, left_scale_cstride, right_scale_rstride, right_scale_cstride};

@@ -1518,6 +1518,15 @@ def gemm_8bit(
     return out
 
 
+def gemm_8bit_plan(m: int, n: int, k: int) -> tuple[int, int]:
+    """How ``gemm_8bit`` runs [m, k] by [k, n] on the current device: the rows of a tile, and the
+    CTAs that share a tile's contraction."""
+    tile, parts = ctypes.c_int(), ctypes.c_int()
+    rc = nat.load().gns_gemm_8bit_plan(m, n, k, ctypes.byref(tile), ctypes.byref(parts))
+    nat.check(rc, "gns_gemm_8bit_plan")
+    return tile.value, parts.value
+
+
 def _quantized(lib, x: Tensor, block_rows: int, stream: int) -> tuple[Tensor, int, int, int, int]:  # type: ignore[no-untyped-def]
     """``quantize_8bit`` of a 16-bit matrix into one buffer, scales behind the codes, for the calls
     below, whose host time counts: (buffer, and of codes and scales address and stride)."""

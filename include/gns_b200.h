@@ -433,7 +433,11 @@ GNS_API int gns_gemm_8bit(int64_t m, int64_t n, int64_t k, const void* left, int
                           const void* right, int64_t right_rstride, int64_t right_cstride, const float* right_scales,
                           int64_t right_scale_rstride, int64_t right_scale_cstride, void* out, int out_dtype,
                           int64_t out_rstride, gns_stream_t stream);
-/* Codes and scales of x [rows][cols] (unit column stride, any row stride of at least cols):
+/* How gns_gemm_8bit runs a product of these sizes on the current device: the rows of left in a
+ * tile (16, 32, 128: a CTA; 256: a pair of CTAs) and the CTAs that share a tile's contraction
+ * (1, 2, 4 or 8). */
+GNS_API int gns_gemm_8bit_plan(int64_t m, int64_t n, int64_t k, int* tile_rows, int* parts);
+/* Codes and scales of x [rows][cols] (unit column stride, any row stride of at least cols, or 0):
  * blocks of block_rows (1 or 128) x 128, top = max(largest magnitude, 448 * 2^-126), scale =
  * top / 448, code = e4m3(x * (448 / top)) to nearest even. Rows of codes start on 16 bytes
  * (codes_rstride a multiple of 16) and are written up to cols rounded up to 16, zeros behind
