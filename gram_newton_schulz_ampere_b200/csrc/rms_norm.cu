@@ -15,8 +15,10 @@
 //
 // Rows that start on 16 bytes are read in pieces of 16 bytes: thread t of a group has the
 // pieces t, t + T, ... of its row, so that a scale's 128 columns lie in 16 neighbouring lanes
-// (32 with fp32). Rows that start anywhere are copied from the multiple of 16 before them,
-// and a warp has a stretch of the row, its lanes neighbouring elements.
+// (32 with fp32). Rows that start anywhere are copied from the multiple of 16 before them to
+// the one behind them: every 16 bytes read hold an element of the row, so none lie in another
+// page, and the others are not used. A warp has a stretch of such a row, its lanes neighbouring
+// elements.
 //
 // Sums, statistics and all arithmetic are fp32. Bound by HBM: 16384 rows of 4096 bf16 elements with
 // a residual and 8-bit output take 71 us forward (470 MB, 6.6 TB/s) and, with the stream's

@@ -409,6 +409,9 @@ GNS_API int gns_grouped_gemm_reduce(int ab_dtype, int64_t rows, int64_t m, int64
  * Backward: dx (contiguous, x's type), and dweight / dbias (w_dtype), the sums
  * over all rows of grad * (x - mean) * rstd and of grad, in fp32 and in a fixed
  * order; dbias may be NULL. rows may be 0 (the sums are then zero).
+ * Rows that do not start and end on 16 bytes are read in whole multiples of 16 bytes: up
+ * to 15 bytes on either side of a row, in the same 16 as one of its elements, are read
+ * and not used.
  * No counterpart in the reference. */
 GNS_API int gns_layer_norm_forward(int x_dtype, int w_dtype, int64_t rows, int64_t cols, const void* x,
                                    int64_t x_rstride, const void* weight, const void* bias, float eps, void* y,
@@ -454,6 +457,8 @@ GNS_API int gns_quantize_8bit(int x_dtype, int block_rows, int64_t rows, int64_t
  * unrounded y in its place.
  * Backward: dx = the gradient through the norm + grad_total (NULL: none), of x and of the
  * residual alike; dweight sums over the rows in fp32, in a fixed order. rows may be 0.
+ * x, residual, total, grad and grad_total are read in whole multiples of 16 bytes, as the
+ * layer norm's rows are.
  * No counterpart in the reference. */
 GNS_API int gns_rms_norm_forward(int x_dtype, int w_dtype, int64_t rows, int64_t cols, const void* x, int64_t x_rstride,
                                  const void* residual, int64_t residual_rstride, const void* weight, float eps, void* y,
