@@ -21,9 +21,11 @@
 // 131072 bf16: 7 us).
 //
 // Logits reach the registers through rings in shared memory, one of each warp, that bulk
-// copies fill two slots of two kilobytes ahead, over the ends of passes and rows: 124 KB under
-// way on an SM whatever the warps wait for. (Loaded to registers four pieces ahead: 4096 x
-// 131072 551 us. Three slots instead of two: 2368 x 131072 fp32, loss alone, 210 us against 181.)
+// copies fill two slots of two kilobytes ahead, over the ends of passes and rows. Under way on an
+// SM, whatever the warps wait for: 124 KB with a CTA of thirty-two warps, 120 with two of sixteen,
+// 96 with eight of four (of which the lists of 1024 entries a row, 48 KB a CTA, leave room for
+// three: 36). Loaded to registers four pieces ahead: 4096 x 131072 551 us. Three slots instead of
+// two: 2368 x 131072 fp32, loss alone, 210 us against 181.
 //
 // What a row's entries ask for is a warp's own work, beside the other warps' passes: read and
 // turned into shares two rows ahead, the loss, and the gradient's corrections (with the teacher
@@ -399,7 +401,7 @@ __global__ void __launch_bounds__(32 * W, kWarpsPerSm / W) distillation_kernel(c
   constexpr int es = XD == kF32 ? 4 : 2;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float2 warps[2][S];
-  __shared__ float2 parts[2][kMaxCluster];
+  __shared__ float2 parts[kMaxCluster];
   __shared__ int aborted;
   const uint32_t rank = cluster_ctarank(), ctas = cluster_nctarank();
   const int64_t step = gridDim.x / ctas, first = blockIdx.x / ctas;
@@ -431,23 +433,21 @@ __global__ void __launch_bounds__(32 * W, kWarpsPerSm / W) distillation_kernel(c
     for (int i = 0; i < kSlots; ++i) ring.fetch(a, rank, ctas, warp, lane);
   }
   __syncthreads();
-  int turn = 0, which = 0, exchange = 0;
-  // A row's statistics from the streaming warps' and, in a cluster, the CTAs'.
+  int turn = 0, which = 0;
+  // A row's statistics from the streaming warps' and, in a cluster, the CTAs'. A cluster has one
+  // row (row_cluster), so the exchange is made once.
   auto joined = [&]() {
     const float2 one = lane < S ? warps[turn][lane] : make_float2(-INFINITY, 0.0f);
     Stat st = warp_join(Stat{one.x, one.y}, a.scale);
     if (ctas > 1) {
-      // Two buffers in turn: a CTA writes to one again only behind the barrier of the other's
-      // exchange, which every reader of it has passed.
       if (threadIdx.x < ctas)
-        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(cluster_addr(&parts[exchange][rank], threadIdx.x)),
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(cluster_addr(&parts[rank], threadIdx.x)),
                      "f"(st.m), "f"(st.s)
                      : "memory");
       __syncwarp();
       cluster_sync_all();
       st = {-INFINITY, 0.0f};
-      for (uint32_t c = 0; c < ctas; ++c) st.join(parts[exchange][c].x, parts[exchange][c].y, a.scale);
-      exchange ^= 1;
+      for (uint32_t c = 0; c < ctas; ++c) st.join(parts[c].x, parts[c].y, a.scale);
     }
     return st;
   };
@@ -627,7 +627,7 @@ __global__ void __launch_bounds__(32 * W, kWarpsPerSm / W) distillation_kernel(c
 }
 
 // CTAs that share a row: one where there are rows for all CTAs that fit; else up to eight, each
-// with 8 KB of it at least.
+// with 8 KB of it at least. Where more than one shares a row, every row has a cluster of its own.
 int row_cluster(int64_t rows, int64_t vocabulary, int dt, int ctas) {
   const int64_t bytes = vocabulary * dtype_size(dt);
   int c = 1;
@@ -683,7 +683,8 @@ template <int XD, int MODE, int W>
 int launch(const LossArgs& a, cudaStream_t stream) {
   const int ctas = kWarpsPerSm / W * device_sm_count();
   const int cluster = W == 4 ? 1 : row_cluster(a.rows, a.vocabulary, XD, ctas);
-  if constexpr (MODE == 3) {
+  // Two CTAs of sixteen warps an SM, with rows of at most 160 KB, stay below on 148 SMs (46 MB).
+  if constexpr (MODE == 3 && W != 16) {
     if (std::min<int64_t>(a.rows, ctas / cluster) * a.vocabulary * dtype_size(XD) > kUnderWay)
       return launch_kernel<XD, MODE, W, true>(a, ctas, cluster, stream);
   }
@@ -694,7 +695,9 @@ int launch(const LossArgs& a, cudaStream_t stream) {
 template <int XD, int MODE>
 int launch_rows(const LossArgs& a, cudaStream_t stream) {
   if (a.vocabulary * dtype_size(XD) <= 65536 && a.rows > 2 * device_sm_count()) return launch<XD, MODE, 4>(a, stream);
-  if (MODE == 3 && a.vocabulary * dtype_size(XD) > 160 * 1024) return launch<XD, MODE, 32>(a, stream);
+  if constexpr (MODE == 3) {
+    if (a.vocabulary * dtype_size(XD) > 160 * 1024) return launch<XD, MODE, 32>(a, stream);
+  }
   return launch<XD, MODE, 16>(a, stream);
 }
 

@@ -17,10 +17,12 @@
 //
 // The pair kernel, 16384 x 4096 x 14336: 861 us, 2.23 PFLOP/s, at the power cap (1.67 GHz; in a
 // run of seconds 1030 us at 1.44 GHz); 717 us, 2.68 PFLOP/s, with operands of zeros, which leave
-// the clock at 1.965 GHz: 900 cycles a block of 256 x 256 x 128 a pair, where its products
-// take 512. A block's way from its last product to the first one that may overwrite its
-// accumulator is 980 cycles of signals between the CTAs and 310 of reading, with two
-// accumulators (all of TMEM) under way: (512 + 980 + 310) / 2. Without the summing it is 750.
+// the clock at 1.965 GHz: 900 cycles a block of 256 x 256 x 128 a pair. Without the summing it is
+// 750, near the 730 that twice the measured rate of a bf16 library product gives (the nominal rate
+// gives 512; what keeps either product from it was not found). The other 150 are the hand-over:
+// a block's way from its last product to the first one that may overwrite its accumulator is
+// 980 cycles of signals between the CTAs and 310 of reading, more than the one block that the
+// second accumulator (all of TMEM is two) gives time for.
 // Measured and not kept: halves of 128 columns with four accumulators (950 without the summing:
 // products 128 wide read the left operand twice as often), sixteen summing warps of 64
 // columns (1046 against 962 under the profiler: twice the instructions beside the sums), sums
@@ -167,14 +169,6 @@ __device__ __forceinline__ void commit_to_both(uint64_t* bar) {
       : "memory");
 }
 
-template <bool CLUSTER>
-__device__ __forceinline__ void meet() {
-  if (CLUSTER)
-    cluster_sync_all();
-  else
-    __syncthreads();
-}
-
 // 32 columns of a thread's TMEM lane on their way to registers: they hold nothing of use
 // until land(), which waits for every load that the thread has issued.
 struct TmemPiece {
@@ -218,7 +212,6 @@ struct TmemPiece {
 // 40 and twice 232 of the 168 a thread at launch (3 x 168 = 40 + 2 x 232).
 constexpr int kPairThreads = 32 * (4 + kEpiWarps);
 
-template <bool OUT_F32>
 struct PairConfig {
   static constexpr int kStages = 5;
   static constexpr uint32_t kStageBytes = 2 * kTileBytes;
@@ -247,7 +240,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     gemm8_pair_kernel(const __grid_constant__ CUtensorMap map_left, const __grid_constant__ CUtensorMap map_right,
                       const __grid_constant__ CUtensorMap map_out, const Scales scales, const Shape8 shape,
                       const Tiling tiling, const Out8 out) {
-  using Cfg = PairConfig<OUT_F32>;
+  using Cfg = PairConfig;
   constexpr int S = Cfg::kStages;
   const uint32_t rank = cluster_ctarank();
   const int first = static_cast<int>(blockIdx.x) / 2, step = static_cast<int>(gridDim.x) / 2;
@@ -721,30 +714,26 @@ struct RowConfig {
   static_assert(kStages * kStageBytes >= TOK * 128 * 4, "the partial sums take the stages' place");
 };
 
-// Columns of the thread's TMEM lane, 8, 16 or 32.
+// Columns of the thread's TMEM lane, 8 or 16.
 template <int N>
 __device__ __forceinline__ void tmem_load(uint32_t at, float (&v)[N]) {
-  static_assert(N == 8 || N == 16 || N == 32, "");
+  static_assert(N == 8 || N == 16, "");
   uint32_t r[N];
   if constexpr (N == 8)
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "r"(at)
                  : "memory");
-  else if constexpr (N == 16)
+  else
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(at)
         : "memory");
-  if constexpr (N < 32) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = __uint_as_float(r[i]);
-  } else {
-    tmem_load_32cols(at, v);
-  }
+  for (int i = 0; i < N; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 template <bool M_MN, int TOK, bool OUT_F32>
@@ -789,8 +778,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   pdl_wait_predecessor();
   const uint32_t tmem = *pipe.tmem_slot;
   const int quarter = warp & 3, half = (warp - 2) >> 2;
-  constexpr int kPiece = Cfg::kHalf < 32 ? Cfg::kHalf : 32;  // columns of one TMEM load
-  Pair sum[Cfg::kHalf / 2];
+  constexpr int kHalf = Cfg::kHalf;
+  Pair sum[kHalf / 2];
 
   if (warp == 0) {
     if (lane == 0) {
@@ -845,24 +834,20 @@ __global__ void __launch_bounds__(kThreads, 2)
   } else {
     // A thread sums a feature for half of the tile's rows of left. The scales of those rows
     // (times the block's own) go to the warp's threads through shared memory.
-    float* mine = smem_scales + (warp - 2) * 2 * Cfg::kHalf;
-    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(Cfg::kHalf * half);
+    float* mine = smem_scales + (warp - 2) * 2 * kHalf;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(kHalf * half);
     const float* rs = scales.right + f0 / kBlock * scales.right_cstride;
-    constexpr int kEach = (Cfg::kHalf + 31) / 32, kAhead = 4;
-    const float* ls[kEach];
-#pragma unroll
-    for (int e = 0; e < kEach; ++e)
-      ls[e] = scales.left + min(row0 + half * Cfg::kHalf + min(32 * e + lane, Cfg::kHalf - 1), shape.m - 1) * scales.left_rstride;
-    float l[kAhead][kEach], r[kAhead];
+    constexpr int kAhead = 4;
+    const float* ls = scales.left + min(row0 + half * kHalf + min(lane, kHalf - 1), shape.m - 1) * scales.left_rstride;
+    float l[kAhead], r[kAhead];
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) {
       const int b = block(min(q, count - 1));
       r[q] = rs[b * scales.right_rstride];
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) l[q][e] = ls[e][b * scales.left_cstride];
+      l[q] = ls[b * scales.left_cstride];
     }
 #pragma unroll
-    for (int q = 0; q < Cfg::kHalf / 2; ++q) sum[q] = Pair(0.0f);
+    for (int q = 0; q < kHalf / 2; ++q) sum[q] = Pair(0.0f);
     int st = 0, acc = 0;
     uint32_t ph = 0;
     bool ok = true;
@@ -870,28 +855,22 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int q = 0; q < kAhead; ++q) {
         if (i0 + q >= count || !ok) continue;
-        float* now = mine + (q & 1) * Cfg::kHalf;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e)
-          if (32 * e + lane < Cfg::kHalf) now[32 * e + lane] = l[q][e] * r[q];
+        float* now = mine + (q & 1) * kHalf;
+        if (lane < kHalf) now[lane] = l[q] * r[q];
         const int next = block(min(i0 + q + kAhead, count - 1));
         r[q] = rs[next * scales.right_rstride];
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) l[q][e] = ls[e][next * scales.left_cstride];
+        l[q] = ls[next * scales.left_cstride];
         ok = __all_sync(0xffffffffu, pipe.wait(&pipe.done[st], ph, kStatusEpilogueTimeout));
         if (!ok) continue;
         __syncwarp();
         tc_fence_after();
+        float v[kHalf];
+        tmem_load<kHalf>(lanes + static_cast<uint32_t>(acc * TOK), v);
 #pragma unroll
-        for (int c = 0; c < Cfg::kHalf; c += kPiece) {
-          float v[kPiece];
-          tmem_load<kPiece>(lanes + static_cast<uint32_t>(acc * TOK + c), v);
-#pragma unroll
-          for (int e = 0; e < kPiece; e += 4) {
-            const float4 s = *reinterpret_cast<const float4*>(now + c + e);
-            sum[(c + e) / 2] = fma2(Pair(v[e], v[e + 1]), Pair(s.x, s.y), sum[(c + e) / 2]);
-            sum[(c + e) / 2 + 1] = fma2(Pair(v[e + 2], v[e + 3]), Pair(s.z, s.w), sum[(c + e) / 2 + 1]);
-          }
+        for (int e = 0; e < kHalf; e += 4) {
+          const float4 s = *reinterpret_cast<const float4*>(now + e);
+          sum[e / 2] = fma2(Pair(v[e], v[e + 1]), Pair(s.x, s.y), sum[e / 2]);
+          sum[e / 2 + 1] = fma2(Pair(v[e + 2], v[e + 3]), Pair(s.z, s.w), sum[e / 2 + 1]);
         }
         tc_fence_before();
         __syncwarp();
@@ -913,15 +892,15 @@ __global__ void __launch_bounds__(kThreads, 2)
   float* joined = reinterpret_cast<float*>(smem);
   if (warp >= 2) {
 #pragma unroll
-    for (int q = 0; q < Cfg::kHalf / 2; ++q) {
+    for (int q = 0; q < kHalf / 2; ++q) {
       float x, y;
       sum[q].get(x, y);
-      float* to = joined + (half * Cfg::kHalf + 2 * q) * 128 + quarter * 32 + lane;
+      float* to = joined + (half * kHalf + 2 * q) * 128 + quarter * 32 + lane;
       to[0] = x;
       to[128] = y;
     }
   }
-  meet<true>();
+  cluster_sync_all();
   if (warp == 1) {
     __syncwarp();
     tmem_dealloc(tmem, Cfg::kTmemCols);
@@ -959,7 +938,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
   }
-  meet<true>();  // no CTA leaves while another reads its sums
+  cluster_sync_all();  // no CTA leaves while another reads its sums
 }
 
 // -------------------------------------------------------------------- launch
@@ -1032,7 +1011,7 @@ int launch8(void (*kernel)(Params...), dim3 grid, int threads, int cluster, size
 template <bool B_MN, bool OUT_F32>
 int launch_pair(const Call8& c, cudaStream_t stream) {
   auto kernel = gemm8_pair_kernel<B_MN, OUT_F32>;
-  constexpr size_t smem = PairConfig<OUT_F32>::kSmemBytes;
+  constexpr size_t smem = PairConfig::kSmemBytes;
   int resident = 0;
   const int rc = prepare_kernel(kernel, (B_MN ? 2 : 0) + (OUT_F32 ? 1 : 0), smem, true, &resident);
   if (rc != GNS_OK) return rc;
