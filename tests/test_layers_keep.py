@@ -1,6 +1,6 @@
-"""What the differentiable 8-bit layers keep for their backward pass, and that it is what the pass reads.
-
-On the CPU, with the kernels' calls replaced by plain ones of the same results' shapes."""
+"""What the differentiable 8-bit layers keep for their backward pass, and that it is what the pass
+reads: on the CPU with the kernels' calls replaced by plain ones of the same results' shapes, and on
+the kernels."""
 
 from __future__ import annotations
 
@@ -92,3 +92,31 @@ def test_norm_and_linear(plain, x_needs, norm_needs, w_needs, r_needs):
     for t, needs in ((x, x_needs), (nw, norm_needs), (w, w_needs), (r, bool(r_needs))):
         if t is not None:
             assert (t.grad is not None) == needs and (not needs or t.grad.shape == t.shape)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("residual", [False, True])
+def test_gradients_of_any_subset_are_those_of_all(cuda_device, residual):
+    """The kernels' layers with every choice of frozen inputs: the same bits as with none frozen."""
+    gen = torch.Generator(device=cuda_device).manual_seed(1)
+    shapes = [(3, 50, 136), (136,), (200, 136)] + ([(3, 50, 136)] if residual else [])
+    values = [torch.randn(shape, generator=gen, device=cuda_device).bfloat16() for shape in shapes]
+    dy = torch.randn(3, 50, 200, generator=gen, device=cuda_device).bfloat16()
+
+    def gradients(call, needs):
+        leaves = [v.clone().requires_grad_(n) for v, n in zip(values, needs)]
+        out = call(leaves)
+        (out[0] if isinstance(out, tuple) else out).backward(dy)
+        return [t.grad for t in leaves]
+
+    places = range(len(shapes))
+    for call, inputs in ((lambda t: training.rms_norm_linear_8bit(*t), set(places)),
+                         (lambda t: training.linear_8bit(t[0], t[2]), {0, 2})):
+        whole = gradients(call, [True for _ in places])
+        for bits in range(1, 2 ** len(shapes)):
+            needs = [bool(bits >> i & 1) for i in places]
+            if not any(needs[i] for i in inputs):
+                continue
+            for i, (got, want) in enumerate(zip(gradients(call, needs), whole)):
+                assert (got is not None) == (needs[i] and i in inputs)
+                assert got is None or torch.equal(got, want)
