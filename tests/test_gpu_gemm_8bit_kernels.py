@@ -5,6 +5,8 @@ scaling and an addition a block (and a part), one rounding to the output's type.
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
@@ -59,6 +61,15 @@ def factors(device, m, k, n, turned):
 def test_every_kernel_has_a_case():
     assert {kernel for kernel, *_ in CASES} == {(rows, parts) for rows in (16, 32) for parts in (1, 2, 4, 8)} | {
         (128, 1), (128, 2), (128, 4), (256, 1)}
+
+
+def test_plan_refusals(native_lib):
+    tile, parts = ctypes.c_int(), ctypes.c_int()
+    for arguments, words in (((-1, 1, 1), b"negative"), ((4, 1 << 23, 128), b"limits"), ((0, 4, 4), b"no plan"), ((4, 4, 0), b"no plan")):
+        assert native_lib.gns_gemm_8bit_plan(*arguments, ctypes.byref(tile), ctypes.byref(parts)) < 0
+        assert words in native_lib.gns_last_error()
+    assert native_lib.gns_gemm_8bit_plan(4, 4, 4, None, ctypes.byref(parts)) < 0
+    assert b"null" in native_lib.gns_last_error()
 
 
 @pytest.mark.parametrize("kernel,m,k,n", CASES)
